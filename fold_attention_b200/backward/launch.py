@@ -17,7 +17,7 @@ from dataclasses import dataclass
 import torch
 
 from .. import _lib
-from ..utils import Launch, check_status
+from ..utils import Launch, check_status, check_window
 from .plan import Plan, plan_dense, plan_varlen, tile_config
 
 P, I, F, Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
@@ -31,9 +31,16 @@ _lib.register(
     "fold_bwd_run_phases",
     [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, P, Z, I, I, I, I, P],
 )
+_lib.register(
+    "fold_bwd_window",
+    [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, P, Z, I, I, I, I, P],
+)
+_lib.register("fold_bwd_window_layout", [I, I, I, I, I, I, I, I, I, P])
 _lib.register("fold_bwd_counters", [P, I])
 _lib.register("fold_wait_probe", [ctypes.c_longlong, P, P, P])
 _lib.register("fold_fwd_run", [P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, P])
+_lib.register("fold_fwd_window", [P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, I, P, I, P])
+_lib.register("fold_fwd_window_sm100", [P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, I, P, I, P, P])
 _lib.register("fold_fwd_sm100_supported", [I, I])
 _lib.register("fold_fwd_run_sm100", [P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, P, P])
 
@@ -78,6 +85,8 @@ def prepare_backward(
     out_dtype=None,
     plan: Plan | None = None,
     kernel: str = "auto",
+    window=None,
+    sinks=0,
 ):
     """Bind dQ, dK and dV of causal or full self-attention to one call's
     tensors, and return the launch that computes them.
@@ -88,7 +97,15 @@ def prepare_backward(
     "mma" or "sm100". `plan` cuts the work (`plan_dense` / `plan_varlen` by
     default): the tcgen05 main loop takes any `Plan`, the mma.sync one only
     whole groups over whole query ranges.
+
+    `window` and `sinks` (causal calls): query i sees key j when `i - j <
+    window` or `j < sinks`. A windowed call cuts its own work and takes no
+    `plan`: key blocks past the sinks stay private to a CTA, the sinks' blocks
+    meet every later query and fold on the integer grids.
     """
+    window, sinks = check_window(window, sinks, causal)
+    if window and plan is not None:
+        raise NotImplementedError("a windowed backward cuts its own work: it takes no plan")
     varlen = cu_seqlens is not None
     if varlen:
         total, H, D = q.shape
@@ -133,7 +150,9 @@ def prepare_backward(
         raise ValueError(f"kernel is one of {tuple(KERNELS)}")
     G = H // H_KV
     cfg = tile_config(D, kernel)
-    if plan is None:
+    if window:
+        plan = Plan(G, 0)
+    elif plan is None:
         plan = plan_varlen(H, H_KV, cfg) if varlen else plan_dense(B, H, H_KV, S, D, bool(causal), cfg)
     if plan.subgroup < 1 or G % plan.subgroup or plan.record < 0:
         raise ValueError(f"a plan of {plan.subgroup} heads per work item for groups of {G}")
@@ -144,10 +163,14 @@ def prepare_backward(
     if lse.dtype != torch.float32:
         raise ValueError("lse must be fp32")
     dq, dk, dv = (torch.empty_like(x) for x in (q, k, v))
-    nbytes = _lib.lib.fold_bwd_workspace_bytes(B, H, H_KV, S, total, D, int(varlen), plan.subgroup, plan.record)
+    lay = (ctypes.c_int64 * 12)()
+    if window:
+        _lib.call("fold_bwd_window_layout", B, H, H_KV, S, total, D, int(varlen), window, sinks, lay)
+        nbytes = lay[11]
+    else:
+        nbytes = _lib.lib.fold_bwd_workspace_bytes(B, H, H_KV, S, total, D, int(varlen), plan.subgroup, plan.record)
+        _lib.call("fold_bwd_workspace_layout", B, H, H_KV, S, total, D, int(varlen), plan.subgroup, plan.record, lay)
     workspace = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    lay = (ctypes.c_int64 * 11)()
-    _lib.call("fold_bwd_workspace_layout", B, H, H_KV, S, total, D, int(varlen), plan.subgroup, plan.record, lay)
     tensors = (q, k, v, o, do, dq, dk, dv)
     strides = _strides(tensors, varlen)
     cu = cu_seqlens
@@ -159,18 +182,28 @@ def prepare_backward(
         plan.subgroup, plan.record,
     )
 
+    if window:   # the same arguments without the mask and the plan
+        args = (*args[:17], *args[18:23], window, sinks)
+
     def run():
-        _lib.call("fold_bwd_run", *args, _lib.stream(dev))
+        if window:
+            run_phase(15)
+        else:
+            _lib.call("fold_bwd_run", *args, _lib.stream(dev))
         return dq, dk, dv
 
     def run_phase(phases):
         """One or more of the backward's phases (1 preprocess, 8 work list,
         2 main loop, 4 postprocess; in that order), for callers that time them
         apart or look at the work list between them."""
-        _lib.call("fold_bwd_run_phases", *args, int(phases), _lib.stream(dev))
+        if window:
+            with torch.cuda.device(dev):
+                _lib.call("fold_bwd_window", *args, int(phases), _lib.stream(dev))
+        else:
+            _lib.call("fold_bwd_run_phases", *args, int(phases), _lib.stream(dev))
 
     held = (q, k, v, o, do, lse, dq, dk, dv, workspace, cu, strides)
-    launch = BackwardLaunch(run, held, plan, workspace, tuple(lay))
+    launch = BackwardLaunch(run, held, plan, workspace, tuple(lay[:11]))
     launch.run_phase = run_phase
     launch.status = workspace[lay[5]: lay[5] + 4].view(torch.int32)
     # the work list as the device built it (n_items, 8): key block, KV head, request, first head,
@@ -187,14 +220,17 @@ def prepare_backward(
     return launch
 
 
-def attention_forward(q, k, v, *, causal, softmax_scale=None, cu_seqlens=None, max_seqlen=None, kernel="auto"):
+def attention_forward(q, k, v, *, causal, softmax_scale=None, cu_seqlens=None, max_seqlen=None, kernel="auto",
+                      window=None, sinks=0):
     """O and LSE (nats) of self-attention through the library's own forward.
 
     Dense: `(B, S, H, D)` tensors, lse `(B, H, S)`. Varlen: `(total, H, D)`,
     lse `(H, total)`. Stands in for the third-party forward the reference
     calls (src/fold_attention/interface.py:42-44,70-81). `kernel`: "mma" (warp-level,
     every head dim), "sm100" (tcgen05; head_dim 128) or
-    "auto"."""
+    "auto". `window` and `sinks` (causal calls): query i sees key j when
+    `i - j < window` or `j < sinks`."""
+    window, sinks = check_window(window, sinks, causal)
     if kernel not in ("auto", "mma", "sm100"):
         raise ValueError('kernel is one of ("auto", "mma", "sm100")')
     varlen = cu_seqlens is not None
@@ -235,22 +271,28 @@ def attention_forward(q, k, v, *, causal, softmax_scale=None, cu_seqlens=None, m
     can = bool(_lib.lib.fold_fwd_sm100_supported(D, int(q.dtype == torch.float16)))
     if kernel == "sm100" and not can:
         raise NotImplementedError("the tcgen05 forward takes head_dim 128")
+    args = [
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), ctypes.addressof(strides),
+        _lib.ptr(cu_seqlens), B, H, k.shape[-2], S, total, D, int(bool(causal)), int(q.dtype == torch.float16), sm,
+    ]
     if can and kernel != "mma":
         status = torch.zeros(1, device=q.device, dtype=torch.int32)
-        _lib.call(
-            "fold_fwd_run_sm100", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
-            ctypes.addressof(strides), _lib.ptr(cu_seqlens), B, H, k.shape[-2], S, total, D,
-            int(bool(causal)), int(q.dtype == torch.float16), sm, status.data_ptr(), _lib.stream(q.device),
-        )
+        if window:
+            del args[13]
+            with torch.cuda.device(q.device):
+                _lib.call("fold_fwd_window_sm100", *args, window, sinks, None, 0, status.data_ptr(), _lib.stream(q.device))
+        else:
+            _lib.call("fold_fwd_run_sm100", *args, status.data_ptr(), _lib.stream(q.device))
         attention_forward.last_status = status   # non-zero after a device-side wait ran out
         if attention_forward.check_status:
             check_status(status, "attention_forward")
         return o, lse
-    _lib.call(
-        "fold_fwd_run", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
-        ctypes.addressof(strides), _lib.ptr(cu_seqlens), B, H, k.shape[-2], S, total, D,
-        int(bool(causal)), int(q.dtype == torch.float16), sm, _lib.stream(q.device),
-    )
+    if window:
+        del args[13]
+        with torch.cuda.device(q.device):
+            _lib.call("fold_fwd_window", *args, window, sinks, None, 0, _lib.stream(q.device))
+    else:
+        _lib.call("fold_fwd_run", *args, _lib.stream(q.device))
     return o, lse
 
 

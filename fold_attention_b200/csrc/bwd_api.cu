@@ -16,7 +16,7 @@ struct PlanArgs {
     int subgroup, record, fold, dv_bits;
 };
 
-bool resolve_plan(int n_heads, int n_kv_heads, int max_seqlen, int subgroup, int record, PlanArgs* out) {
+bool resolve_plan(int n_heads, int n_kv_heads, int max_seqlen, int subgroup, int record, int window, PlanArgs* out) {
     const int G = n_heads / n_kv_heads;
     if (subgroup <= 0) subgroup = G;
     if (subgroup > G || G % subgroup || record < 0) return false;
@@ -25,8 +25,10 @@ bool resolve_plan(int n_heads, int n_kv_heads, int max_seqlen, int subgroup, int
     out->fold = (subgroup < G || record > 0) ? 1 : 0;
     // dV's bound carries only the column mass G * S: a 30-bit grid holds it up to 16384
     // (src/fold_attention/backward/launch.py:179-182)
-    out->dv_bits = static_cast<int64_t>(G) * max_seqlen <= 16384 ? 32 : 64;
-    return true;
+    // under a window the sinks' blocks always take the wide one: a sequence's bits then do not depend
+    // on the longest of the sequences it is packed with
+    out->dv_bits = window <= 0 && static_cast<int64_t>(G) * max_seqlen <= 16384 ? 32 : 64;
+    return window <= 0 || !out->fold;
 }
 
 struct WsLayout {
@@ -34,18 +36,26 @@ struct WsLayout {
     int64_t rows_p, n_items;
 };
 
-WsLayout ws_layout(int B, int H, int HKV, int S, int total, int D, bool varlen, const PlanArgs& plan) {
+// A window's sinks: their key blocks, rounded up to either main loop's block, which are all that folds.
+int sink_stride(int S, int window, int sinks) {
+    if (window <= 0 || sinks <= 0) return 0;
+    const int n = sinks < S ? sinks : S;
+    return (n + ROW_PAD - 1) / ROW_PAD * ROW_PAD;
+}
+
+WsLayout ws_layout(int B, int H, int HKV, int S, int total, int D, bool varlen, const PlanArgs& plan, int window, int sinks) {
     WsLayout w;
     w.rows_p = padded_rows(B, S, total, varlen);
-    w.n_items = D == 128 ? bwd_sm100_work_items(B, H, HKV, S, plan.subgroup, plan.record) : 0;
+    w.n_items = D == 128 ? bwd_sm100_work_items(B, H, HKV, S, plan.subgroup, plan.record, window, sinks) : 0;
+    const size_t acc = static_cast<size_t>(HKV) * D * (plan.fold ? static_cast<size_t>(w.rows_p) : static_cast<size_t>(B) * sink_stride(S, window, sinks));
     size_t off = 0;
     w.dq_acc = off; off = align256(off + sizeof(int) * static_cast<size_t>(H) * w.rows_p * D);
     w.dpsum = off;  off = align256(off + sizeof(float) * static_cast<size_t>(H) * w.rows_p);
     w.lse2 = off;   off = align256(off + sizeof(float) * static_cast<size_t>(H) * w.rows_p);
     // the maxima, then the status word, then the work list's two counters
     w.stats = off;  off = align256(off + sizeof(int) * (N_STATS * static_cast<size_t>(B) * HKV + 3));
-    w.dk_acc = off; off = align256(off + (plan.fold ? 8 * static_cast<size_t>(HKV) * w.rows_p * D : 0));
-    w.dv_acc = off; off = align256(off + (plan.fold ? (plan.dv_bits / 8) * static_cast<size_t>(HKV) * w.rows_p * D : 0));
+    w.dk_acc = off; off = align256(off + 8 * acc);
+    w.dv_acc = off; off = align256(off + (plan.dv_bits / 8) * acc);
     w.work = off;   off = align256(off + 32 * static_cast<size_t>(w.n_items));
     w.total = off;
     return w;
@@ -56,8 +66,8 @@ WsLayout ws_layout(int B, int H, int HKV, int S, int total, int D, bool varlen, 
 extern "C" size_t fold_bwd_workspace_bytes(int batch, int n_heads, int n_kv_heads, int max_seqlen,
                                            int total, int head_dim, int varlen, int subgroup, int record) {
     PlanArgs plan;
-    if (n_kv_heads <= 0 || n_heads % n_kv_heads || !resolve_plan(n_heads, n_kv_heads, max_seqlen, subgroup, record, &plan)) return 0;
-    return ws_layout(batch, n_heads, n_kv_heads, max_seqlen, total, head_dim, varlen != 0, plan).total;
+    if (n_kv_heads <= 0 || n_heads % n_kv_heads || !resolve_plan(n_heads, n_kv_heads, max_seqlen, subgroup, record, 0, &plan)) return 0;
+    return ws_layout(batch, n_heads, n_kv_heads, max_seqlen, total, head_dim, varlen != 0, plan, 0, 0).total;
 }
 
 static int bwd_run_phases(const void* q, const void* k, const void* v, const void* o,
@@ -65,7 +75,8 @@ static int bwd_run_phases(const void* q, const void* k, const void* v, const voi
                           const int64_t* strides, const int32_t* cu_seqlens, int batch,
                           int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim,
                           int causal, int is_f16, float softmax_scale, void* workspace,
-                          size_t workspace_bytes, int kernel, int subgroup, int record, int phases, void* stream) {
+                          size_t workspace_bytes, int kernel, int subgroup, int record, int window, int sinks, int phases,
+                          void* stream) {
     FOLD_CHECK_ARG(q && k && v && o && dout && lse && dq && dk && dv && strides && workspace,
                    "fold_bwd_run: null pointer");
     FOLD_CHECK_ARG(n_kv_heads > 0 && n_heads % n_kv_heads == 0,
@@ -77,10 +88,12 @@ static int bwd_run_phases(const void* q, const void* k, const void* v, const voi
     }
     const bool varlen = cu_seqlens != nullptr;
     PlanArgs plan;
-    FOLD_CHECK_ARG(resolve_plan(n_heads, n_kv_heads, max_seqlen, subgroup, record, &plan),
+    FOLD_CHECK_ARG(window >= 0 && window <= FOLD_MAX_WINDOW && sinks >= 0 && sinks <= FOLD_MAX_WINDOW && (window == 0 || causal),
+                   "fold_bwd_run: a window of %d keys and %d sinks (under a causal mask)", window, sinks);
+    FOLD_CHECK_ARG(resolve_plan(n_heads, n_kv_heads, max_seqlen, subgroup, record, window, &plan),
                    "fold_bwd_run: a plan of %d heads and %d query blocks per work item for groups of %d heads", subgroup, record,
                    n_heads / n_kv_heads);
-    const WsLayout w = ws_layout(batch, n_heads, n_kv_heads, max_seqlen, total, head_dim, varlen, plan);
+    const WsLayout w = ws_layout(batch, n_heads, n_kv_heads, max_seqlen, total, head_dim, varlen, plan, window, sinks);
     FOLD_CHECK_ARG(workspace_bytes >= w.total, "fold_bwd_run: workspace of %zu bytes, %zu needed",
                    workspace_bytes, w.total);
     FOLD_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "fold_bwd_run: workspace must be 256-byte aligned");
@@ -121,6 +134,9 @@ static int bwd_run_phases(const void* q, const void* k, const void* v, const voi
     p.work = reinterpret_cast<int*>(ws + w.work);
     p.n_items = static_cast<int>(w.n_items);
     p.rows_p = w.rows_p;
+    p.window = window; p.sinks = window > 0 ? sinks : 0;
+    p.sink_stride = sink_stride(max_seqlen, window, sinks);
+    p.sink_rows = p.sink_record = 0;
     p.S_r = (max_seqlen + ROW_PAD - 1) / ROW_PAD * ROW_PAD;
 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -140,6 +156,12 @@ static int bwd_run_phases(const void* q, const void* k, const void* v, const voi
         set_error("the mma.sync main loop keeps a key block's dK and dV in one CTA: it takes whole groups and whole query ranges "
                   "(subgroup 0, record 0)");
         return FOLD_ERR_UNSUPPORTED;
+    }
+    if (window > 0) {
+        const int tile = sm100 ? 128 : 64;   // the main loop's key block
+        const int n = p.sinks < max_seqlen ? p.sinks : max_seqlen;
+        p.sink_rows = (n + tile - 1) / tile * tile;
+        p.sink_record = sink_record_blocks(window, tile);
     }
     p.dq_bias = (sm100 && bwd_sm100_biased()) ? 1 : 0;
     int rc = FOLD_OK;
@@ -163,7 +185,7 @@ extern "C" int fold_bwd_run(const void* q, const void* k, const void* v, const v
                             size_t workspace_bytes, int kernel, int subgroup, int record, void* stream) {
     return bwd_run_phases(q, k, v, o, dout, lse, dq, dk, dv, strides, cu_seqlens, batch, n_heads,
                           n_kv_heads, max_seqlen, total, head_dim, causal, is_f16, softmax_scale,
-                          workspace, workspace_bytes, kernel, subgroup, record,
+                          workspace, workspace_bytes, kernel, subgroup, record, 0, 0,
                           FOLD_BWD_PHASE_PRE | FOLD_BWD_PHASE_LIST | FOLD_BWD_PHASE_MAIN | FOLD_BWD_PHASE_POST, stream);
 }
 
@@ -176,7 +198,34 @@ extern "C" int fold_bwd_run_phases(const void* q, const void* k, const void* v, 
                                    int record, int phases, void* stream) {
     return bwd_run_phases(q, k, v, o, dout, lse, dq, dk, dv, strides, cu_seqlens, batch, n_heads,
                           n_kv_heads, max_seqlen, total, head_dim, causal, is_f16, softmax_scale,
-                          workspace, workspace_bytes, kernel, subgroup, record, phases, stream);
+                          workspace, workspace_bytes, kernel, subgroup, record, 0, 0, phases, stream);
+}
+
+extern "C" int fold_bwd_window(const void* q, const void* k, const void* v, const void* o,
+                               const void* dout, const float* lse, void* dq, void* dk, void* dv,
+                               const int64_t* strides, const int32_t* cu_seqlens, int batch,
+                               int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim,
+                               int is_f16, float softmax_scale, void* workspace, size_t workspace_bytes,
+                               int kernel, int window, int sinks, int phases, void* stream) {
+    FOLD_CHECK_ARG(window > 0, "fold_bwd_window: a window of %d keys", window);
+    return bwd_run_phases(q, k, v, o, dout, lse, dq, dk, dv, strides, cu_seqlens, batch, n_heads,
+                          n_kv_heads, max_seqlen, total, head_dim, 1, is_f16, softmax_scale,
+                          workspace, workspace_bytes, kernel, 0, 0, window, sinks, phases, stream);
+}
+
+static int workspace_layout(int batch, int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim, int varlen,
+                            int subgroup, int record, int window, int sinks, int64_t* out, int64_t* bytes) {
+    FOLD_CHECK_ARG(out, "fold_bwd_workspace_layout: null pointer");
+    PlanArgs plan;
+    FOLD_CHECK_ARG(n_kv_heads > 0 && n_heads % n_kv_heads == 0 &&
+                       resolve_plan(n_heads, n_kv_heads, max_seqlen, subgroup, record, window, &plan),
+                   "fold_bwd_workspace_layout: bad head counts or plan");
+    const WsLayout w = ws_layout(batch, n_heads, n_kv_heads, max_seqlen, total, head_dim, varlen != 0, plan, window, sinks);
+    if (bytes) *bytes = static_cast<int64_t>(w.total);
+    out[0] = w.dq_acc; out[1] = w.dpsum; out[2] = w.lse2; out[3] = w.stats; out[4] = w.rows_p;
+    out[5] = w.stats + sizeof(int) * N_STATS * static_cast<size_t>(batch) * n_kv_heads;
+    out[6] = w.dk_acc; out[7] = w.dv_acc; out[8] = plan.fold ? plan.dv_bits : 0; out[9] = w.work; out[10] = w.n_items;
+    return FOLD_OK;
 }
 
 // The workspace's views, for tests that inspect the accumulators:
@@ -187,13 +236,13 @@ extern "C" int fold_bwd_run_phases(const void* q, const void* k, const void* v, 
 extern "C" int fold_bwd_workspace_layout(int batch, int n_heads, int n_kv_heads, int max_seqlen,
                                          int total, int head_dim, int varlen, int subgroup, int record,
                                          int64_t* out) {
-    FOLD_CHECK_ARG(out, "fold_bwd_workspace_layout: null pointer");
-    PlanArgs plan;
-    FOLD_CHECK_ARG(n_kv_heads > 0 && n_heads % n_kv_heads == 0 && resolve_plan(n_heads, n_kv_heads, max_seqlen, subgroup, record, &plan),
-                   "fold_bwd_workspace_layout: bad head counts or plan");
-    const WsLayout w = ws_layout(batch, n_heads, n_kv_heads, max_seqlen, total, head_dim, varlen != 0, plan);
-    out[0] = w.dq_acc; out[1] = w.dpsum; out[2] = w.lse2; out[3] = w.stats; out[4] = w.rows_p;
-    out[5] = w.stats + sizeof(int) * N_STATS * static_cast<size_t>(batch) * n_kv_heads;
-    out[6] = w.dk_acc; out[7] = w.dv_acc; out[8] = plan.fold ? plan.dv_bits : 0; out[9] = w.work; out[10] = w.n_items;
-    return FOLD_OK;
+    return workspace_layout(batch, n_heads, n_kv_heads, max_seqlen, total, head_dim, varlen, subgroup, record, 0, 0, out, nullptr);
+}
+
+// The same for a call under a window, and the workspace's size in out[11].
+extern "C" int fold_bwd_window_layout(int batch, int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim,
+                                      int varlen, int window, int sinks, int64_t* out) {
+    FOLD_CHECK_ARG(window > 0 && window <= FOLD_MAX_WINDOW && sinks >= 0 && sinks <= FOLD_MAX_WINDOW,
+                   "fold_bwd_window_layout: a window of %d keys and %d sinks", window, sinks);
+    return workspace_layout(batch, n_heads, n_kv_heads, max_seqlen, total, head_dim, varlen, 0, 0, window, sinks, out, out + 11);
 }

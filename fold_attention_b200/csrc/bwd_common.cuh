@@ -43,7 +43,26 @@ struct BwdParams {
     int n_items;
     int* sched;     // [2]: the list's claim counter and the count of finished CTAs, zero between launches
     int S_r;        // dense: S rounded up to ROW_PAD
+    // A causal call under a sliding window (window > 0): query i sees key j <= i when i - j < window or
+    // j < sinks. Key blocks past the sinks meet the few query blocks their window reaches and stay
+    // private to a CTA; a block that holds sinks meets every later query block, so its items are cut
+    // into records of `sink_record` query blocks and its dK, dV meet in the integer accumulators
+    // (dk_acc, dv_acc), which then hold [HKV][B][sink_stride][D] for the sinks' blocks alone.
+    int window, sinks, sink_record;
+    int sink_rows;      // rows of a sequence whose dK, dV the accumulators hold: the sinks' whole key blocks
+    int sink_stride;    // and how many are laid out
 };
+
+// The longest a window's key block is walked before an item is cut, in the main loop's query blocks:
+// about what a block past the sinks walks, so the launch's longest items stay its ordinary ones. It
+// depends on the window alone: a sequence's bits do not depend on its neighbours.
+inline int sink_record_blocks(int window, int tile) {
+    const int r = window / tile + 2;
+    return r < 8 ? 8 : r > (1 << 20) ? (1 << 20) : r;
+}
+// one past the last query block of `tile` rows that sees any key of [n0, n0 + tile) by the window
+__host__ __device__ inline int window_end(int n0, int tile, int window) { return (n0 + tile - 1 + window - 1) / tile + 1; }
+
 
 struct SeqInfo {
     int start;       // first row in the packed tensors (0 for dense)
@@ -65,6 +84,11 @@ __device__ __forceinline__ SeqInfo seq_info(const BwdParams& p, int b) {
     return s;
 }
 
+// first row of a (request, KV head) in dk_acc, dv_acc
+__device__ __forceinline__ int64_t dkv_acc_row(const BwdParams& p, const SeqInfo& sq, int b, int hkv) {
+    return p.window > 0 ? (static_cast<int64_t>(hkv) * p.B + b) * p.sink_stride : static_cast<int64_t>(hkv) * p.rows_p + sq.pstart;
+}
+
 template <typename T>
 __device__ __forceinline__ T* row_ptr(const TensorView& t, int b, int64_t row, int h) {
     return static_cast<T*>(t.ptr) + b * t.sb + row * t.sr + h * t.sh;
@@ -80,7 +104,7 @@ inline int64_t padded_rows(int B, int S, int total, bool varlen) {
 int launch_bwd_preprocess(const BwdParams& p, cudaStream_t st);
 int launch_bwd_postprocess(const BwdParams& p, int layout, cudaStream_t st);
 // how many work items the tcgen05 main loop's list holds for a call (0 for the other main loop)
-int64_t bwd_sm100_work_items(int B, int H, int HKV, int S, int subgroup, int record);
+int64_t bwd_sm100_work_items(int B, int H, int HKV, int S, int subgroup, int record, int window, int sinks);
 int launch_bwd_main_mma(const BwdParams& p, cudaStream_t st);
 int launch_bwd_main_sm100(const BwdParams& p, bool build_list, bool run_main, cudaStream_t st);
 bool bwd_sm100_supported(const BwdParams& p);

@@ -30,14 +30,26 @@ struct MmaSmem {
     static constexpr int BYTES = OFF_DL + 64 * 4;
 };
 
-template <int D, bool F16, bool CAUSAL>
+template <int D, bool F16, bool CAUSAL, bool WIN>
 __global__ void __launch_bounds__(NTHREADS, 2) bwd_main_mma_kernel(const BwdParams p) {
     using L = MmaSmem<D>;
     extern __shared__ __align__(128) uint8_t smem[];
-    const int nb = blockIdx.x, hkv = blockIdx.y, b = blockIdx.z;
+    int nb = blockIdx.x, rec = 0;
+    const int hkv = blockIdx.y, b = blockIdx.z;
+    if constexpr (WIN) {   // the sinks' key blocks come first, one CTA per record of query blocks
+        const int nsb = p.sink_rows / BN, nrec = ((p.S + BM - 1) / BM + p.sink_record - 1) / p.sink_record;
+        if (nb < nsb * nrec) {
+            rec = nb % nrec;
+            nb /= nrec;
+        } else {
+            nb -= nsb * (nrec - 1);
+        }
+    }
     const SeqInfo sq = seq_info(p, b);
     const int n0 = nb * BN;
     if (n0 >= sq.len) return;
+    const bool sink = WIN && n0 < p.sinks;
+    if (sink && rec * p.sink_record >= (sq.len + BM - 1) / BM) return;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int gid = lane >> 2, tq = lane & 3;
     const int wk = warp & 3, wd = warp >> 2;
@@ -73,8 +85,16 @@ __global__ void __launch_bounds__(NTHREADS, 2) bwd_main_mma_kernel(const BwdPara
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc_dk[i][e] = acc_dv[i][e] = 0.f;
 
-    const int nm = (sq.len + BM - 1) / BM;
-    const int m_min = CAUSAL ? nb : 0;   // BM == BN
+    int nm = (sq.len + BM - 1) / BM;
+    int m_min = CAUSAL ? nb : 0;   // BM == BN
+    if constexpr (WIN) {
+        if (sink) {
+            m_min = max(m_min, rec * p.sink_record);
+            nm = min(nm, (rec + 1) * p.sink_record);
+        } else {
+            nm = min(nm, window_end(n0, BN, p.window));
+        }
+    }
 
     for (int g = 0; g < p.G; ++g) {
         const int h = hkv * p.G + g;
@@ -118,7 +138,7 @@ __global__ void __launch_bounds__(NTHREADS, 2) bwd_main_mma_kernel(const BwdPara
                 }
             }
             // ---- P~ = exp2(S c - (L - s)), dS~ = P~ (dP - Delta) ----
-            const bool need_mask = (CAUSAL && mb == nb) || (n0 + BN > sq.len);
+            const bool need_mask = (CAUSAL && mb == nb) || (n0 + BN > sq.len) || (WIN && m0 + BM - 1 - n0 >= p.window);
 #pragma unroll
             for (int nt = 0; nt < 4; ++nt) {
                 const int ql = 32 * wd + 8 * nt + 2 * tq;
@@ -133,6 +153,7 @@ __global__ void __launch_bounds__(NTHREADS, 2) bwd_main_mma_kernel(const BwdPara
                     if (need_mask) {
                         const int kj = n0 + kl, qi = m0 + ql + (e & 1);
                         if (kj >= sq.len || (CAUSAL && kj > qi)) x = 0.f;
+                        if (WIN && qi - kj >= p.window && kj >= p.sinks) x = 0.f;
                     }
                     pv[e] = x;
                     ds[e] = x * (dp[nt][e] - de);
@@ -209,6 +230,28 @@ __global__ void __launch_bounds__(NTHREADS, 2) bwd_main_mma_kernel(const BwdPara
     // the whole loop, so both leave scaled by it and are put back exactly.
     const float un = F16 ? 1.f : pow2f(-s_exp);
     const float fk = p.scale * un;
+    if (sink) {
+        // a sinks' block: its records' sums meet on dK's and dV's integer grids (the postprocess converts them)
+        const int* st = p.stats + (static_cast<int64_t>(b) * p.HKV + hkv) * N_STATS;
+        const float rows = static_cast<float>(p.G) * static_cast<float>(sq.len);
+        const int carried = F16 ? 0 : s_exp;
+        const int ek = dk_scale_exp(st, rows, root_d(D)) - carried, ev = dv_scale_exp(st, rows, DKV_BITS) - carried;
+        unsigned long long* ak = reinterpret_cast<unsigned long long*>(p.dk_acc);
+        unsigned long long* av = static_cast<unsigned long long*>(p.dv_acc);
+        const int64_t row0 = dkv_acc_row(p, sq, b, hkv) + n0;
+#pragma unroll
+        for (int nt = 0; nt < NTD; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int kl = 16 * wk + gid + 8 * (e >> 1);
+                if (n0 + kl < sq.len) {
+                    const int64_t at = (row0 + kl) * D + wd * DH + 8 * nt + 2 * tq + (e & 1);
+                    atomicAdd(ak + at, static_cast<unsigned long long>(__float2ll_rn(scale_pow2(acc_dk[nt][e], ek))));
+                    atomicAdd(av + at, static_cast<unsigned long long>(__float2ll_rn(scale_pow2(acc_dv[nt][e], ev))));
+                }
+            }
+        return;
+    }
 #pragma unroll
     for (int nt = 0; nt < NTD; ++nt)
 #pragma unroll
@@ -224,24 +267,23 @@ __global__ void __launch_bounds__(NTHREADS, 2) bwd_main_mma_kernel(const BwdPara
         }
 }
 
-template <int D, bool F16, bool CAUSAL>
+template <int D, bool F16, bool CAUSAL, bool WIN>
 static int launch_one(const BwdParams& p, cudaStream_t st) {
     using L = MmaSmem<D>;
-    auto kern = bwd_main_mma_kernel<D, F16, CAUSAL>;
-    static bool configured = false;
-    if (!configured) {
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
-        configured = true;
-    }
-    dim3 grid((p.S + BN - 1) / BN, p.HKV, p.B);
+    auto kern = bwd_main_mma_kernel<D, F16, CAUSAL, WIN>;
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);   // per device: not kept in a static
+    int nblk = (p.S + BN - 1) / BN;
+    if (WIN) nblk += p.sink_rows / BN * ((nblk + p.sink_record - 1) / p.sink_record - 1);
+    dim3 grid(nblk, p.HKV, p.B);
     kern<<<grid, NTHREADS, L::BYTES, st>>>(p);
     return check_launch("bwd_main_mma");
 }
 
 template <int D>
 static int launch_d(const BwdParams& p, cudaStream_t st) {
-    if (p.f16) return p.causal ? launch_one<D, true, true>(p, st) : launch_one<D, true, false>(p, st);
-    return p.causal ? launch_one<D, false, true>(p, st) : launch_one<D, false, false>(p, st);
+    if (p.window > 0) return p.f16 ? launch_one<D, true, true, true>(p, st) : launch_one<D, false, true, true>(p, st);
+    if (p.f16) return p.causal ? launch_one<D, true, true, false>(p, st) : launch_one<D, true, false, false>(p, st);
+    return p.causal ? launch_one<D, false, true, false>(p, st) : launch_one<D, false, false, false>(p, st);
 }
 
 int launch_bwd_main_mma(const BwdParams& p, cudaStream_t st) {

@@ -36,6 +36,7 @@ __global__ void __launch_bounds__(PRE_THREADS) bwd_preprocess_kernel(const BwdPa
     const bool active = lane * 4 < D;
     const int hkv = h / p.G;
     const bool kv_owner = (h % p.G) == 0;
+    const bool acc_stats = p.fold || p.sink_rows > 0;   // dK's and dV's grids are used
     float mx_k = 0.f, mx_v = 0.f, mx_dn = 0.f, mx_dl = 0.f, mx_doc = 0.f, mx_q = 0.f;
     const int64_t wbase = static_cast<int64_t>(h) * p.rows_p + sq.pstart;
     // Four rows per pass: all of their loads are issued before the first row's reductions, so a
@@ -53,7 +54,7 @@ __global__ void __launch_bounds__(PRE_THREADS) bwd_preprocess_kernel(const BwdPa
                 if (active) {
                     ow[u] = ldg8(row_ptr<const uint16_t>(p.o, b, sq.start + i, h) + lane * 4);
                     gw[u] = ldg8(row_ptr<const uint16_t>(p.dout, b, sq.start + i, h) + lane * 4);
-                    if (p.fold) qw[u] = ldg8(row_ptr<const uint16_t>(p.q, b, sq.start + i, h) + lane * 4);
+                    if (acc_stats) qw[u] = ldg8(row_ptr<const uint16_t>(p.q, b, sq.start + i, h) + lane * 4);
                     if (kv_owner) {
                         kw[u] = ldg8(row_ptr<const uint16_t>(p.k, b, sq.start + i, hkv) + lane * 4);
                         vw[u] = ldg8(row_ptr<const uint16_t>(p.v, b, sq.start + i, hkv) + lane * 4);
@@ -77,7 +78,7 @@ __global__ void __launch_bounds__(PRE_THREADS) bwd_preprocess_kernel(const BwdPa
                 delta = d;
                 mx_dn = fmaxf(mx_dn, sqrtf(n2));
                 mx_dl = fmaxf(mx_dl, fabsf(d));
-                if (p.fold) {
+                if (acc_stats) {
                     float qq[4];
                     unpack4<F16>(qw[u], qq);
 #pragma unroll
@@ -108,7 +109,11 @@ __global__ void __launch_bounds__(PRE_THREADS) bwd_preprocess_kernel(const BwdPa
             int init = 0;
             if (p.dq_bias) {
                 const int tile = i / ROW_PAD, nkb = (sq.len + ROW_PAD - 1) / ROW_PAD;
-                const unsigned n_part = static_cast<unsigned>(p.causal ? min(tile + 1, nkb) : nkb);
+                unsigned n_part = static_cast<unsigned>(p.causal ? min(tile + 1, nkb) : nkb);
+                if (p.window > 0) {   // the blocks from the window's first on, and the sinks' before it
+                    const int lo = max(0, tile * ROW_PAD - p.window - (ROW_PAD - 2) + ROW_PAD - 1) / ROW_PAD;
+                    n_part -= static_cast<unsigned>(lo - min(lo, (p.sinks + ROW_PAD - 1) / ROW_PAD));
+                }
                 init = static_cast<int>(0u - n_part * 0x4B400000u);
             }
             int4* acc = reinterpret_cast<int4*>(p.dq_acc + (wbase + i) * D);
@@ -129,7 +134,7 @@ __global__ void __launch_bounds__(PRE_THREADS) bwd_preprocess_kernel(const BwdPa
         s_red[5][warp] = mx_q;
     }
     __syncthreads();
-    if (threadIdx.x < (p.fold ? 6 : 4)) {
+    if (threadIdx.x < (acc_stats ? 6 : 4)) {
         float r = s_red[threadIdx.x][0];
         for (int w = 1; w < PRE_THREADS / 32; ++w) r = fmaxf(r, s_red[threadIdx.x][w]);
         // the max of non-negative floats is the max of their bits, and a max
@@ -199,9 +204,10 @@ __global__ void __launch_bounds__(256) bwd_finalize_l_kernel(const BwdParams p) 
 int launch_bwd_preprocess(const BwdParams& p, cudaStream_t st) {
     // the maxima, the status word and the work list's two counters
     cudaMemsetAsync(p.stats, 0, sizeof(int) * (N_STATS * p.B * p.HKV + 3), st);
-    if (p.fold) {
-        cudaMemsetAsync(p.dk_acc, 0, 8 * static_cast<size_t>(p.HKV) * p.rows_p * p.D, st);
-        cudaMemsetAsync(p.dv_acc, 0, (p.dv_bits / 8) * static_cast<size_t>(p.HKV) * p.rows_p * p.D, st);
+    const size_t acc_rows = p.fold ? p.rows_p : static_cast<size_t>(p.B) * p.sink_stride;
+    if (p.fold || p.sink_rows > 0) {
+        cudaMemsetAsync(p.dk_acc, 0, 8 * static_cast<size_t>(p.HKV) * acc_rows * p.D, st);
+        cudaMemsetAsync(p.dv_acc, 0, (p.dv_bits / 8) * static_cast<size_t>(p.HKV) * acc_rows * p.D, st);
     }
     const int s_r = (p.S + ROW_PAD - 1) / ROW_PAD * ROW_PAD;
     dim3 grid(s_r / PRE_ROWS, p.H, p.B);
@@ -223,13 +229,14 @@ __global__ void __launch_bounds__(256) bwd_postprocess_dkv_kernel(const BwdParam
     const int D = p.D, cpr = D / 4;
     const int rows_per_block = 256 / cpr > 0 ? 256 / cpr : 1;
     const int r0 = blockIdx.x * 64;
-    if (r0 >= sq.len) return;
+    const int rows_end = p.window > 0 ? min(sq.len, p.sink_rows) : sq.len;   // a window folds the sinks' blocks alone
+    if (r0 >= rows_end) return;
     const int* st = p.stats + (static_cast<int64_t>(b) * p.HKV + hkv) * N_STATS;
     const float rows = static_cast<float>(p.G) * static_cast<float>(sq.len);
     const int s_k = dk_scale_exp(st, rows, root_d(D));
     const int s_v = dv_scale_exp(st, rows, p.dv_bits == 32 ? DQ_BITS : DKV_BITS);
     const float f_k = __fmul_rn(p.scale, pow2f(-s_k)), f_v = pow2f(-s_v);
-    const int64_t wbase = (static_cast<int64_t>(hkv) * p.rows_p + sq.pstart) * D;
+    const int64_t wbase = dkv_acc_row(p, sq, b, hkv) * D;
     auto pack4 = [](float x0, float x1, float x2, float x3) {
         uint2 w;
         w.x = F16 ? pack_f16x2(x0, x1) : pack_bf16x2(x0, x1);
@@ -239,7 +246,7 @@ __global__ void __launch_bounds__(256) bwd_postprocess_dkv_kernel(const BwdParam
     for (int rr = threadIdx.x / cpr; rr < 64; rr += rows_per_block) {
         const int i = r0 + rr;
         const int c = threadIdx.x % cpr;
-        if (i >= sq.len || threadIdx.x >= rows_per_block * cpr) continue;
+        if (i >= rows_end || threadIdx.x >= rows_per_block * cpr) continue;
         const int64_t at = wbase + static_cast<int64_t>(i) * D + c * 4;
         const longlong2 k0 = *reinterpret_cast<const longlong2*>(p.dk_acc + at), k1 = *reinterpret_cast<const longlong2*>(p.dk_acc + at + 2);
         *reinterpret_cast<uint2*>(row_ptr<uint16_t>(p.dk, b, sq.start + i, hkv) + c * 4) =
@@ -265,8 +272,9 @@ int launch_bwd_postprocess(const BwdParams& p, int layout, cudaStream_t st) {
         bwd_postprocess_dq_kernel<true><<<grid, 256, 0, st>>>(p, layout);
     else
         bwd_postprocess_dq_kernel<false><<<grid, 256, 0, st>>>(p, layout);
-    if (p.fold) {
-        dim3 gkv((p.S + 63) / 64, p.HKV, p.B);
+    if (p.fold || p.sink_rows > 0) {
+        const int rows = p.fold ? p.S : p.sink_rows;
+        dim3 gkv((rows + 63) / 64, p.HKV, p.B);
         if (p.f16)
             bwd_postprocess_dkv_kernel<true><<<gkv, 256, 0, st>>>(p);
         else

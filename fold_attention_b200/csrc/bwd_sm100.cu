@@ -360,19 +360,14 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t sr
                  ::"l"(map), "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
 }
 
-// x * 2^e for any e in [-250, 250] without leaving fp32's exponent range half way
-__device__ __forceinline__ float scale_pow2(float x, int e) {
-    const int e1 = max(-120, min(120, e));
-    return x * pow2f(e1) * pow2f(e - e1);
-}
-
 // A persistent CTA: every role loops over the work items its producer thread claims from the
 // list (an atomic counter), longest first, so the grid ends on short items and a CTA's fixed
 // costs (TMEM allocation, barrier set-up, the wait for the first loads) are paid once. The
 // roles run asynchronously across item boundaries: while the drain finishes an item's last
 // tile and the compute warps write its dK and dV out, K and V of the next item are already
 // on their way. Barrier phases count tiles (or items) since the CTA started.
-template <bool F16>
+// WIN: the build for a sliding window with sinks (its mask, and the fold exit of the sinks' key blocks).
+template <bool F16, bool WIN>
 __global__ void __launch_bounds__(NTHREADS, 1)
 bwd_main_sm100_kernel(const BwdParams p, const __grid_constant__ Maps maps) {
     extern __shared__ uint8_t smem_raw[];
@@ -627,7 +622,8 @@ bwd_main_sm100_kernel(const BwdParams p, const __grid_constant__ Maps maps) {
                 const int m0 = mb * BM + QPW * wg;   // the group's first query
                 const uint32_t sL_addr = base + SM_L + s * 512 + 4 * QPW * wg;
                 const uint32_t sDl_addr = base + SM_DL + s * 512 + 4 * QPW * wg;
-                const bool need_mask = (p.causal && m0 < it.n0 + BN) || (it.n0 + BN > it.sq.len);
+                const bool need_mask = (p.causal && m0 < it.n0 + BN) || (it.n0 + BN > it.sq.len) ||
+                                       (WIN && m0 + QPW - 1 - it.n0 >= p.window);
                 float x[QPW];
                 // ---- P~^T = exp2(S^T c - L), kept in registers for dS~ and written over S^T ----
                 // bf16 has fp32's range, so P~ and dS~ carry the grid's exponent (it comes in with the row
@@ -660,6 +656,7 @@ bwd_main_sm100_kernel(const BwdParams p, const __grid_constant__ Maps maps) {
                         for (int q = 0; q < 32; ++q) {
                             const int qi = m0 + 32 * c + q;
                             if (kj >= it.sq.len || (p.causal && kj > qi)) x[32 * c + q] = 0.f;
+                            if (WIN && qi - kj >= p.window && kj >= p.sinks) x[32 * c + q] = 0.f;
                         }
                     }
 #pragma unroll
@@ -729,7 +726,8 @@ bwd_main_sm100_kernel(const BwdParams p, const __grid_constant__ Maps maps) {
                 const uint32_t src = tmem + lane_addr + (is_dv ? T_DV : T_DK) + c0;
                 const bool ok = it.n0 + r < it.sq.len;
                 auto pk2 = [](float a, float b2) { return F16 ? pack_f16x2(a, b2) : pack_bf16x2(a, b2); };
-                if (NWG == 2 && !p.fold && it.n0 + BN <= it.sq.len) {
+                const bool folds = WIN ? it.n0 < p.sinks : p.fold != 0;
+                if (NWG == 2 && !folds && it.n0 + BN <= it.sq.len) {
                     // A whole key block: the 16-bit tile goes through shared memory in the swizzled layout of
                     // the loads, 64 channels (16 KB) at a time, and one thread per warpgroup stores each half
                     // with TMA: 32 KB in two instructions instead of 2048 scattered 16-byte stores. Each
@@ -772,7 +770,7 @@ bwd_main_sm100_kernel(const BwdParams p, const __grid_constant__ Maps maps) {
                         // the half has been read out: the group may stage the next one (or, after the second, its dS~)
                         if (is_dv) asm volatile("bar.sync 3, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");
                     }
-                } else if (!p.fold) {
+                } else if (!folds) {
                     const float un = F16 ? 1.f : pow2f(-s_exp);
                     const float f = is_dv ? un : p.scale * un;
                     uint16_t* dst = row_ptr<uint16_t>(is_dv ? p.dv : p.dk, it.b, it.sq.start + it.n0 + (ok ? r : 0), it.hkv) + c0;
@@ -803,7 +801,7 @@ bwd_main_sm100_kernel(const BwdParams p, const __grid_constant__ Maps maps) {
                     const float rows = static_cast<float>(p.G) * static_cast<float>(it.sq.len);
                     const int e = (is_dv ? dv_scale_exp(st, rows, p.dv_bits == 32 ? DQ_BITS : DKV_BITS) : dk_scale_exp(st, rows, root_d(HD))) -
                                   (F16 ? 0 : s_exp);
-                    const int64_t off = (static_cast<int64_t>(it.hkv) * p.rows_p + it.sq.pstart + it.n0 + r) * HD + c0;
+                    const int64_t off = (dkv_acc_row(p, it.sq, it.b, it.hkv) + it.n0 + r) * HD + c0;
                     const bool narrow = is_dv && p.dv_bits == 32;
 #pragma unroll
                     for (int c = 0; c < CW / 32; ++c) {
@@ -1042,27 +1040,33 @@ bwd_main_sm100_kernel(const BwdParams p, const __grid_constant__ Maps maps) {
 // last long items start while there is still a wave of work behind them. Built on the
 // device from cu_seqlens, in-stream: no host synchronisation, and a captured graph replays it.
 constexpr int WL_BINS = 1024;
-__global__ void __launch_bounds__(256) bwd_work_list_kernel(const BwdParams p, int n_trip, int nsub, int nb_max, int nrec, int sec,
-                                                            int tail_trip) {
+__global__ void __launch_bounds__(256) bwd_work_list_kernel(const BwdParams p, int n_trip, int nsub, int nb_max, int nsb, int nrec,
+                                                            int sec, int tail_trip) {
     __shared__ int hist[WL_BINS];
     __shared__ int offs[WL_BINS];
     // the last block sorts the merged tail (the last `tail_trip` triples as one section)
     const bool tail = blockIdx.x == gridDim.x - 1;
     const int body = n_trip - tail_trip;
     const int t0 = tail ? body : blockIdx.x * sec, t1 = tail ? n_trip : min(t0 + sec, body);
-    const int per = nb_max * nrec;
+    // key blocks [0, nsb) are cut into `nrec` records each, the others (under a window) are one item
+    const int per = nb_max + nsb * (nrec - 1);
     const int count = (t1 - t0) * per;
     int* out = const_cast<int*>(p.work) + static_cast<int64_t>(t0) * per * 8;
     for (int i = threadIdx.x; i < WL_BINS; i += blockDim.x) hist[i] = 0;
     __syncthreads();
     auto describe = [&](int li, int (&w)[8]) {
         const int trip = t0 + li / per, rem = li % per;
-        const int nb = rem / nrec, rec = rem % nrec;
+        const bool cut = rem < nsb * nrec;
+        const int nb = cut ? rem / nrec : rem - nsb * (nrec - 1), rec = cut ? rem % nrec : 0;
         const int b = trip / (p.HKV * nsub), hkv = (trip / nsub) % p.HKV, sub = trip % nsub;
         const SeqInfo sq = seq_info(p, b);
         const int nm = (sq.len + BM - 1) / BM;
-        const int m_lo = p.record > 0 ? rec * p.record : 0;
-        const int m_hi = p.record > 0 ? (rec + 1) * p.record : nm;
+        int m_lo = p.record > 0 ? rec * p.record : 0;
+        int m_hi = p.record > 0 ? (rec + 1) * p.record : nm;
+        if (p.window > 0) {
+            m_lo = cut ? rec * p.sink_record : 0;
+            m_hi = cut ? (rec + 1) * p.sink_record : window_end(nb * BN, BN, p.window);
+        }
         const int first = max(p.causal ? nb : 0, m_lo);
         const int blocks = (nb * BN < sq.len) ? max(min(nm, m_hi) - first, 0) : 0;
         w[0] = nb; w[1] = hkv; w[2] = b; w[3] = sub * p.subgroup; w[4] = p.subgroup;
@@ -1148,22 +1152,28 @@ bool bwd_sm100_biased() { return FOLD_BWD_BIAS != 0; }
 
 namespace {
 struct ListShape {
-    int nsub, nb_max, nrec;
+    int nsub, nb_max, nsb, nrec;
     int64_t n_trip, n_items;
 };
-ListShape list_shape(int B, int H, int HKV, int S, int subgroup, int record) {
+ListShape list_shape(int B, int H, int HKV, int S, int subgroup, int record, int window, int sinks) {
     ListShape l;
     l.nsub = (H / HKV) / subgroup;
     l.nb_max = (S + sm100::BN - 1) / sm100::BN;
     l.nrec = record > 0 ? (l.nb_max + record - 1) / record : 1;
+    l.nsb = l.nb_max;
+    if (window > 0) {
+        const int r = sink_record_blocks(window, sm100::BM);
+        l.nrec = (l.nb_max + r - 1) / r;
+        l.nsb = std::min(l.nb_max, (sinks + sm100::BN - 1) / sm100::BN);
+    }
     l.n_trip = static_cast<int64_t>(B) * HKV * l.nsub;
-    l.n_items = l.n_trip * l.nb_max * l.nrec;
+    l.n_items = l.n_trip * (l.nb_max + static_cast<int64_t>(l.nsb) * (l.nrec - 1));
     return l;
 }
 }  // namespace
 
-int64_t bwd_sm100_work_items(int B, int H, int HKV, int S, int subgroup, int record) {
-    return list_shape(B, H, HKV, S, subgroup, record).n_items;
+int64_t bwd_sm100_work_items(int B, int H, int HKV, int S, int subgroup, int record, int window, int sinks) {
+    return list_shape(B, H, HKV, S, subgroup, record, window, sinks).n_items;
 }
 
 bool bwd_sm100_supported(const BwdParams& p) {
@@ -1186,7 +1196,7 @@ int launch_bwd_main_sm100(const BwdParams& p, bool build_list, bool run_main, cu
     // The work list, then one persistent CTA per SM claiming from it. Sections: as many (request,
     // KV head, subgroup) triples as keep their Q, dO (16-bit) and dQ accumulator (int32) within a
     // share of L2 that leaves room for K, V and the other sections' tails.
-    const ListShape l = list_shape(p.B, p.H, p.HKV, p.S, p.subgroup, p.record);
+    const ListShape l = list_shape(p.B, p.H, p.HKV, p.S, p.subgroup, p.record, p.window, p.sinks);
     if (l.n_items != p.n_items || l.n_items > (1ll << 30)) {
         set_error("bwd_main_sm100: a work list of %lld items, %d laid out", static_cast<long long>(l.n_items), p.n_items);
         return FOLD_ERR_ARGUMENT;
@@ -1205,18 +1215,14 @@ int launch_bwd_main_sm100(const BwdParams& p, bool build_list, bool run_main, cu
     const int tail_trip = static_cast<int>(std::min<int64_t>(l.n_trip, std::max<int64_t>(sec, std::min<int64_t>(wave, 2 * kSectionBytes / std::max<int64_t>(trip_bytes, 1)))));
     const int n_sections = static_cast<int>((l.n_trip - tail_trip + sec - 1) / sec) + 1;
     if (build_list)
-        sm100::bwd_work_list_kernel<<<n_sections, 256, 0, st>>>(p, static_cast<int>(l.n_trip), l.nsub, l.nb_max, l.nrec, sec, tail_trip);
+        sm100::bwd_work_list_kernel<<<n_sections, 256, 0, st>>>(p, static_cast<int>(l.n_trip), l.nsub, l.nb_max, l.nsb, l.nrec, sec,
+                                                                tail_trip);
     if (!run_main) return check_launch("bwd_work_list");
     const int grid = static_cast<int>(std::min<int64_t>(std::max(sms[dev], 1), l.n_items));
-    if (f16) {
-        auto kern = sm100::bwd_main_sm100_kernel<true>;
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sm100::SMEM_BYTES);
-        kern<<<grid, sm100::NTHREADS, sm100::SMEM_BYTES, st>>>(p, maps);
-    } else {
-        auto kern = sm100::bwd_main_sm100_kernel<false>;
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sm100::SMEM_BYTES);
-        kern<<<grid, sm100::NTHREADS, sm100::SMEM_BYTES, st>>>(p, maps);
-    }
+    auto kern = p.window > 0 ? (f16 ? sm100::bwd_main_sm100_kernel<true, true> : sm100::bwd_main_sm100_kernel<false, true>)
+                             : (f16 ? sm100::bwd_main_sm100_kernel<true, false> : sm100::bwd_main_sm100_kernel<false, false>);
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sm100::SMEM_BYTES);
+    kern<<<grid, sm100::NTHREADS, sm100::SMEM_BYTES, st>>>(p, maps);
     return check_launch("bwd_main_sm100");
 }
 

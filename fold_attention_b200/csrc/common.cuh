@@ -139,6 +139,11 @@ __device__ __forceinline__ int dk_scale_exp(const int* stats, float rows, float 
     return pow2_scale_exp(__fmul_rn(rows, __fmul_rn(s, __int_as_float(stats[ST_Q]))), DKV_BITS);
 }
 __device__ __forceinline__ float pow2f(int e) { return __int_as_float((e + 127) << 23); }
+// x * 2^e for any e in [-250, 250] without leaving fp32's exponent range half way
+__device__ __forceinline__ float scale_pow2(float x, int e) {
+    const int e1 = max(-120, min(120, e));
+    return x * pow2f(e1) * pow2f(e - e1);
+}
 #endif
 
 }  // namespace fold

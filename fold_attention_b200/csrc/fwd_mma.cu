@@ -15,9 +15,15 @@ struct FwdParams {
     const int* cu;
     int B, H, HKV, G, S, D, causal, f16;
     float scale;
+    // a build with EXT = true only (it is causal): a row sees the `window` newest keys up to its own
+    // position and the first `sinks` keys; with `klens` the keys are request b's own rows
+    // [0, klens[b]) of a (batch, row, head) tensor of `krows` rows a request, and the queries are its last
+    int window, sinks;
+    const int* klens;
+    int krows;
 };
 
-template <int D, bool F16, bool CAUSAL>
+template <int D, bool F16, bool CAUSAL, bool EXT>
 __global__ void __launch_bounds__(128) fwd_mma_kernel(const FwdParams p) {
     constexpr int PITCH = D * 2 + 16, TILE = 64 * PITCH, NTO = D / 8;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -35,6 +41,15 @@ __global__ void __launch_bounds__(128) fwd_mma_kernel(const FwdParams p) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tq = lane & 3;
     const int hkv = h / p.G;
     const float c2 = p.scale * kLog2e;
+    int klen = len, qoff = 0, kstart = start;   // keys, and the first query's position among them
+    if constexpr (EXT) {
+        if (p.klens) {
+            const int n = p.klens[b];
+            qoff = n - len;
+            klen = min(n, p.krows);
+            kstart = 0;
+        }
+    }
 
     load_tile_async<D, PITCH, 128>(sQ, row_ptr<const uint16_t>(p.q, b, start + m0, h), p.q.sr, 64, min(64, len - m0), tid);
     cp_async_commit();
@@ -46,12 +61,18 @@ __global__ void __launch_bounds__(128) fwd_mma_kernel(const FwdParams p) {
         for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
     float mx[2] = {-INFINITY, -INFINITY}, ls[2] = {0.f, 0.f};
 
-    const int n_end = CAUSAL ? min(len, m0 + 64) : len;
+    const int n_end = EXT ? max(0, min(klen, qoff + min(len, m0 + 64))) : CAUSAL ? min(len, m0 + 64) : len;
+    // EXT: the first key tile of the block's window; between the sinks' tiles and it nothing is seen
+    const int n_low = EXT ? max(0, qoff + m0 - p.window + 1) / 64 * 64 : 0;
     for (int n0 = 0; n0 < n_end; n0 += 64) {
+        if (EXT && n0 >= p.sinks && n0 < n_low) {
+            n0 = n_low;
+            if (n0 >= n_end) break;
+        }
         __syncthreads();  // previous tile's reads are done
-        const int kvalid = min(64, len - n0);
-        load_tile_async<D, PITCH, 128>(sK, row_ptr<const uint16_t>(p.k, b, start + n0, hkv), p.k.sr, 64, kvalid, tid);
-        load_tile_async<D, PITCH, 128>(sV, row_ptr<const uint16_t>(p.v, b, start + n0, hkv), p.v.sr, 64, kvalid, tid);
+        const int kvalid = min(64, klen - n0);
+        load_tile_async<D, PITCH, 128>(sK, row_ptr<const uint16_t>(p.k, b, kstart + n0, hkv), p.k.sr, 64, kvalid, tid);
+        load_tile_async<D, PITCH, 128>(sV, row_ptr<const uint16_t>(p.v, b, kstart + n0, hkv), p.v.sr, 64, kvalid, tid);
         cp_async_commit();
         cp_async_wait<0>();
         __syncthreads();
@@ -75,7 +96,8 @@ __global__ void __launch_bounds__(128) fwd_mma_kernel(const FwdParams p) {
                 mma_16816<F16>(s[2 * np + 1], a, bk[2], bk[3]);
             }
         }
-        const bool need_mask = (CAUSAL && n0 + 64 > m0) || (n0 + 64 > len);
+        const bool need_mask = (CAUSAL && n0 + 64 > qoff + m0) || (n0 + 64 > klen) ||
+                               (EXT && n0 <= qoff + m0 + 63 - p.window && n0 + 64 > p.sinks);
         float rmax[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt)
@@ -84,8 +106,9 @@ __global__ void __launch_bounds__(128) fwd_mma_kernel(const FwdParams p) {
                 float x = s[nt][e] * c2;
                 if (need_mask) {
                     const int kj = n0 + 8 * nt + 2 * tq + (e & 1);
-                    const int qi = m0 + 16 * warp + gid + 8 * (e >> 1);
-                    if (kj >= len || (CAUSAL && kj > qi)) x = -INFINITY;
+                    const int qi = qoff + m0 + 16 * warp + gid + 8 * (e >> 1);
+                    if (kj >= klen || (CAUSAL && kj > qi)) x = -INFINITY;
+                    if (EXT && qi - kj >= p.window && kj >= p.sinks) x = -INFINITY;
                 }
                 s[nt][e] = x;
                 rmax[e >> 1] = fmaxf(rmax[e >> 1], x);
@@ -150,16 +173,16 @@ __global__ void __launch_bounds__(128) fwd_mma_kernel(const FwdParams p) {
 #pragma unroll
         for (int i = 0; i < NTO; ++i)
             *reinterpret_cast<uint32_t*>(orow + 8 * i + 2 * tq) = pack16x2<F16>(o[i][2 * r] * inv, o[i][2 * r + 1] * inv);
-        if (tq == 0)
+        if (tq == 0 && (!EXT || p.lse))
             p.lse[b * p.lse_sb + h * p.lse_sh + start + qi] =
                 ls[r] > 0.f ? (mx[r] + log2f(ls[r])) * 0.6931471805599453f : -INFINITY;
     }
 }
 
-template <int D, bool F16, bool CAUSAL>
+template <int D, bool F16, bool CAUSAL, bool EXT>
 static int fwd_launch_one(const FwdParams& p, cudaStream_t st) {
     constexpr int BYTES = 3 * 64 * (D * 2 + 16);
-    auto kern = fwd_mma_kernel<D, F16, CAUSAL>;
+    auto kern = fwd_mma_kernel<D, F16, CAUSAL, EXT>;
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES);
     dim3 grid((p.S + 63) / 64, p.H, p.B);
     kern<<<grid, 128, BYTES, st>>>(p);
@@ -168,21 +191,24 @@ static int fwd_launch_one(const FwdParams& p, cudaStream_t st) {
 
 template <int D>
 static int fwd_launch_d(const FwdParams& p, cudaStream_t st) {
-    if (p.f16) return p.causal ? fwd_launch_one<D, true, true>(p, st) : fwd_launch_one<D, true, false>(p, st);
-    return p.causal ? fwd_launch_one<D, false, true>(p, st) : fwd_launch_one<D, false, false>(p, st);
+    if (p.window > 0) return p.f16 ? fwd_launch_one<D, true, true, true>(p, st) : fwd_launch_one<D, false, true, true>(p, st);
+    if (p.f16) return p.causal ? fwd_launch_one<D, true, true, false>(p, st) : fwd_launch_one<D, true, false, false>(p, st);
+    return p.causal ? fwd_launch_one<D, false, true, false>(p, st) : fwd_launch_one<D, false, false, false>(p, st);
 }
 
 }  // namespace fold
 
 using namespace fold;
 
-extern "C" int fold_fwd_run(const void* q, const void* k, const void* v, void* o, float* lse,
-                            const int64_t* strides, const int32_t* cu_seqlens, int batch,
-                            int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim,
-                            int causal, int is_f16, float softmax_scale, void* stream) {
-    FOLD_CHECK_ARG(q && k && v && o && lse && strides, "fold_fwd_run: null pointer");
+// The causal and full forward (window 0, klens null), or the EXT build.
+static int fwd_run(const char* what, const void* q, const void* k, const void* v, void* o, float* lse,
+                   const int64_t* strides, const int32_t* cu_seqlens, int batch, int n_heads, int n_kv_heads,
+                   int max_seqlen, int total, int head_dim, int causal, int is_f16, float softmax_scale, int window,
+                   int sinks, const int32_t* klens, int krows, void* stream) {
+    FOLD_CHECK_ARG(q && k && v && o && (lse || klens) && strides, "%s: null pointer", what);
     FOLD_CHECK_ARG(n_kv_heads > 0 && n_heads % n_kv_heads == 0, "the query heads must be a multiple of the KV heads");
-    FOLD_CHECK_ARG(batch > 0 && max_seqlen > 0, "fold_fwd_run: empty call");
+    FOLD_CHECK_ARG(batch > 0 && max_seqlen > 0, "%s: empty call", what);
+    FOLD_CHECK_ARG(n_heads <= 65535 && batch <= 65535, "%s: %d heads, %d requests (65535 at most)", what, n_heads, batch);
     FwdParams p;
     const void* ptrs[4] = {q, k, v, o};
     TensorView* views[4] = {&p.q, &p.k, &p.v, &p.o};
@@ -193,7 +219,7 @@ extern "C" int fold_fwd_run(const void* q, const void* k, const void* v, void* o
         views[i]->sh = strides[3 * i + 2];
         FOLD_CHECK_ARG(views[i]->sr % 8 == 0 && views[i]->sh % 8 == 0 && views[i]->sb % 8 == 0 &&
                            reinterpret_cast<uintptr_t>(ptrs[i]) % 16 == 0,
-                       "fold_fwd_run: rows must be 16-byte aligned");
+                       "%s: rows must be 16-byte aligned", what);
     }
     p.lse = lse;
     p.cu = cu_seqlens;
@@ -206,6 +232,7 @@ extern "C" int fold_fwd_run(const void* q, const void* k, const void* v, void* o
     }
     p.B = batch; p.H = n_heads; p.HKV = n_kv_heads; p.G = n_heads / n_kv_heads;
     p.S = max_seqlen; p.D = head_dim; p.causal = causal; p.f16 = is_f16; p.scale = softmax_scale;
+    p.window = window; p.sinks = sinks; p.klens = klens; p.krows = krows;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (head_dim) {
         case 64: return fwd_launch_d<64>(p, st);
@@ -214,4 +241,25 @@ extern "C" int fold_fwd_run(const void* q, const void* k, const void* v, void* o
     }
     set_error("head_dim %d: 64, 96 and 128 are supported", head_dim);
     return FOLD_ERR_UNSUPPORTED;
+}
+
+extern "C" int fold_fwd_run(const void* q, const void* k, const void* v, void* o, float* lse,
+                            const int64_t* strides, const int32_t* cu_seqlens, int batch,
+                            int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim,
+                            int causal, int is_f16, float softmax_scale, void* stream) {
+    FOLD_CHECK_ARG(lse, "fold_fwd_run: null pointer");
+    return fwd_run("fold_fwd_run", q, k, v, o, lse, strides, cu_seqlens, batch, n_heads, n_kv_heads, max_seqlen, total,
+                   head_dim, causal, is_f16, softmax_scale, 0, 0, nullptr, 0, stream);
+}
+
+extern "C" int fold_fwd_window(const void* q, const void* k, const void* v, void* o, float* lse,
+                               const int64_t* strides, const int32_t* cu_seqlens, int batch, int n_heads,
+                               int n_kv_heads, int max_seqlen, int total, int head_dim, int is_f16,
+                               float softmax_scale, int window, int sinks, const int32_t* key_lens, int key_rows,
+                               void* stream) {
+    FOLD_CHECK_ARG(window > 0 && window <= FOLD_MAX_WINDOW && sinks >= 0 && sinks <= FOLD_MAX_WINDOW,
+                   "fold_fwd_window: a window of %d keys and %d sinks (1 .. 2^30 and 0 .. 2^30)", window, sinks);
+    FOLD_CHECK_ARG(!key_lens || key_rows > 0, "fold_fwd_window: %d key rows", key_rows);
+    return fwd_run("fold_fwd_window", q, k, v, o, lse, strides, cu_seqlens, batch, n_heads, n_kv_heads, max_seqlen, total,
+                   head_dim, 1, is_f16, softmax_scale, window, sinks, key_lens, key_rows, stream);
 }

@@ -176,12 +176,33 @@ struct Params {
     int B, H, HKV, G, S, causal;
     float scale;
     int* status;
+    // a build with EXT = true only (it is causal): a row sees the `window` newest keys up to its own
+    // position and the first `sinks` keys; with `klens` the keys are request b's own rows
+    // [0, klens[b]) of a (batch, row, head) tensor of `krows` rows a request, and the queries are its last
+    int window, sinks;
+    const int* klens;
+    int krows;
 };
 struct Maps {
     CUtensorMap q, k, v;   // (channel, row, head, batch), boxes (64, 128, 1, 1)
 };
 
-template <bool F16>
+// The key tiles one CTA walks, in order: the tiles that hold sinks, then the window's, for both of
+// its query tiles; each query tile takes the ones it sees (`active`).
+struct TileList {
+    int ns, lo, n;          // tiles [0, ns), then [lo, lo + n - ns)
+    int end[2], low[2];     // query tile x sees tiles [low[x], end[x]) and the sinks'
+    int sinks;
+    __device__ __forceinline__ int tile(int j) const { return j < ns ? j : lo + j - ns; }
+    __device__ __forceinline__ bool active(int x, int j) const {
+        const int t = tile(j);
+        return j < n && t < end[x] && (t >= low[x] || t * BN < sinks);
+    }
+};
+
+// EXT: the build with a window, sinks and keys of another length than the queries. The causal and
+// full builds keep their own tile arithmetic (and their bits).
+template <bool F16, bool EXT>
 __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, const __grid_constant__ Maps maps) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = static_cast<uint32_t>(__cvta_generic_to_shared(smem_raw));
@@ -203,15 +224,44 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
     if (m0 >= len) return;
     const int hkv = h / p.G;
     const int bb = p.cu ? 0 : b;
+    int klen = len, qoff = 0, kstart = start, kb = bb;   // keys, and the first query's position among them
+    if constexpr (EXT) {
+        if (p.klens) {
+            const int n = p.klens[b];
+            qoff = n - len;
+            klen = min(n, p.krows);
+            kstart = 0;
+            kb = b;
+        }
+    }
     // key tiles each of the two query tiles meets (the second tile may lie past the sequence)
     int nt[2];
+    TileList tl{};
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int mx = m0 + x * BM;
-        const int kv_end = mx >= len ? 0 : (p.causal ? min(len, mx + BM) : len);
-        nt[x] = (kv_end + BN - 1) / BN;
+        if constexpr (EXT) {
+            const int kv_end = mx >= len ? 0 : max(0, min(klen, qoff + min(mx + BM, len)));
+            tl.end[x] = (kv_end + BN - 1) / BN;
+            tl.low[x] = max(0, qoff + mx - p.window + 1) / BN;
+        } else {
+            const int kv_end = mx >= len ? 0 : (p.causal ? min(len, mx + BM) : len);
+            nt[x] = (kv_end + BN - 1) / BN;
+        }
     }
-    const int n_tiles = max(nt[0], nt[1]);
+    if constexpr (EXT) {
+        tl.sinks = p.sinks;
+        tl.ns = (p.sinks + BN - 1) / BN;
+        tl.lo = tl.low[0];
+        if (tl.ns >= tl.lo) tl.ns = tl.lo = 0;   // the sinks' tiles run into the window's
+        tl.n = max(0, tl.ns + max(tl.end[0], tl.end[1]) - tl.lo);
+        const int st = (p.sinks + BN - 1) / BN;
+        for (int x = 0; x < 2; ++x)              // tiles each query tile takes
+            nt[x] = min(tl.end[x], st) + max(0, tl.end[x] - max(tl.low[x], st));
+    }
+    const int n_tiles = EXT ? tl.n : max(nt[0], nt[1]);
+    auto tile_of = [&](int j) { return EXT ? tl.tile(j) : j; };
+    auto takes = [&](int x, int j) { return EXT ? tl.active(x, j) : j < nt[x]; };
 
     if (tid == 0) {
         *abort_flag = 0;
@@ -238,7 +288,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
     if (warp == 0) {
         // ================= TMA producer =================
         if (lane == 0) {
-            mbar_expect_tx(bar(B_Q), nt[1] > 0 ? 65536 : 32768);
+            if (nt[0] > 0 || nt[1] > 0) mbar_expect_tx(bar(B_Q), nt[0] > 0 && nt[1] > 0 ? 65536 : 32768);
             for (int x = 0; x < 2; ++x) {
                 if (nt[x] == 0) continue;
                 for (int c = 0; c < 2; ++c)
@@ -250,8 +300,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
                 const uint32_t st = base + SM_KV + s * STAGE;
                 mbar_expect_tx(bar(B_KVFULL + s), 65536);
                 for (int c = 0; c < 2; ++c) {
-                    tma_load_4d(st + c * 16384, &maps.k, 64 * c, start + j * BN, hkv, bb, bar(B_KVFULL + s));
-                    tma_load_4d(st + 32768 + c * 16384, &maps.v, 64 * c, start + j * BN, hkv, bb, bar(B_KVFULL + s));
+                    tma_load_4d(st + c * 16384, &maps.k, 64 * c, kstart + tile_of(j) * BN, hkv, kb, bar(B_KVFULL + s));
+                    tma_load_4d(st + 32768 + c * 16384, &maps.v, 64 * c, kstart + tile_of(j) * BN, hkv, kb, bar(B_KVFULL + s));
                 }
             }
         }
@@ -260,7 +310,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
         if (lane == 0) {
             constexpr uint32_t ID_S = instr_desc(F16 ? 0 : 1, 128, 128, 0, 0);    // Q (K-major) x K (K-major)
             constexpr uint32_t ID_PV = instr_desc(F16 ? 0 : 1, 128, 128, 0, 1);   // P (TMEM) x V (MN-major)
-            mbar_wait(bar(B_Q), 0, abort_flag, p.status);
+            if (nt[0] > 0 || nt[1] > 0) mbar_wait(bar(B_Q), 0, abort_flag, p.status);
             auto issue_s = [&](int x, int j) {
                 const int s = j & 1;
                 mbar_wait(bar(B_KVFULL + s), (j >> 1) & 1, abort_flag, p.status);
@@ -274,23 +324,30 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
                 tc_commit(bar(B_SFULL + x));
             };
             for (int x = 0; x < 2; ++x)
-                if (nt[x] > 0) issue_s(x, 0);
+                if (takes(x, 0)) issue_s(x, 0);
+            int done[2] = {0, 0};   // EXT: products issued so far (a query tile may sit a key tile out)
             for (int j = 0; j < n_tiles; ++j) {
                 const int s = j & 1;
                 const uint32_t vt = base + SM_KV + s * STAGE + 32768;
                 for (int x = 0; x < 2; ++x) {
-                    if (j >= nt[x]) continue;
-                    mbar_wait(bar(B_PREADY + x), j & 1, abort_flag, p.status);
-                    tc_fence_after();
+                    if (takes(x, j)) {
+                        const int it = EXT ? done[x] : j;
+                        mbar_wait(bar(B_PREADY + x), it & 1, abort_flag, p.status);
+                        tc_fence_after();
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks)   // 16 keys per step: 8 TMEM columns of P, 2048 bytes of V per box
-                        mma_ts(tmem + T_O + 128 * x, tmem + T_S + 128 * x + 8 * ks, smem_desc(vt + ks * 2048, 16384, 1024), ID_PV,
-                               (j > 0) || (ks > 0));
-                    tc_commit(bar(B_ODONE + x));
+                        for (int ks = 0; ks < 8; ++ks)   // 16 keys per step: 8 TMEM columns of P, 2048 bytes of V per box
+                            mma_ts(tmem + T_O + 128 * x, tmem + T_S + 128 * x + 8 * ks, smem_desc(vt + ks * 2048, 16384, 1024), ID_PV,
+                                   (it > 0) || (ks > 0));
+                        tc_commit(bar(B_ODONE + x));
+                        if constexpr (EXT) ++done[x];
+                    }
                     // the next scores overwrite S (and the P just consumed): the tensor pipe runs a
-                    // thread's MMAs in the order it issued them
-                    if (j + 1 < nt[x]) issue_s(x, j + 1);
+                    // thread's MMAs in the order it issued them. (Only ever the next key tile's: a later
+                    // one's stage is not free before this tile is done with it.)
+                    if (takes(x, j + 1)) issue_s(x, j + 1);
                 }
+                // EXT: a tile that no product of this thread reads has still to land before its stage is filled again
+                if (EXT && !takes(0, j) && !takes(1, j)) mbar_wait(bar(B_KVFULL + s), (j >> 1) & 1, abort_flag, p.status);
                 tc_commit(bar(B_KVEMPTY + s));
             }
         }
@@ -302,15 +359,30 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
         const float c2 = p.scale * kLog2e;
         const uint64_t c2x2 = pack2(c2, c2);
         const int mx = m0 + x * BM;
-        const int qi = mx + r;                 // the row's position in its sequence
+        const int qr = mx + r;                 // the query's row in its sequence
+        const int qi = qr + qoff;              // its position among the keys
         const int my_tiles = nt[x];
         float m_run = -INFINITY, l_run = 0.f;  // running maximum (log2 domain) and sum
         const uint32_t ts = tmem + lane_addr + T_S + 128 * x;
         const uint32_t to = tmem + lane_addr + T_O + 128 * x;
-        for (int j = 0; j < my_tiles; ++j) {
-            const int n0 = j * BN;
-            const bool need_mask = (p.causal && n0 + BN > mx) || (n0 + BN > len);
-            const int kmax = min(len - 1, p.causal ? qi : len - 1) - n0;   // last key column this row may see
+        int it = 0;
+        for (int jj = 0; jj < (EXT ? n_tiles : my_tiles); ++jj) {
+            if (EXT && !takes(x, jj)) continue;
+            const int j = EXT ? it++ : jj;     // the query tile's own count of key tiles
+            const int n0 = tile_of(jj) * BN;
+            bool need_mask;
+            int kmax, kmin = 0, ksink = 0;     // the key columns this row sees: kmin .. kmax, and those under ksink
+            if constexpr (EXT) {
+                const bool cuts = n0 <= qoff + mx + BM - 1 - p.window && n0 + BN > p.sinks;   // the tile's last row has moved past its first key
+                need_mask = n0 + BN > qoff + mx || n0 + BN > klen || cuts;
+                kmax = min(klen - 1, qi) - n0;
+                kmin = qi - p.window + 1 - n0;
+                ksink = p.sinks - n0;
+            } else {
+                need_mask = (p.causal && n0 + BN > mx) || (n0 + BN > len);
+                kmax = min(len - 1, p.causal ? qi : len - 1) - n0;   // last key column this row may see
+            }
+            auto hidden = [&](int e) { return e > kmax || (EXT && e < kmin && e >= ksink); };
             mbar_wait(bar(B_SFULL + x), j & 1, abort_flag, p.status);
             tc_fence_after();
             // pass 1: the row's maximum over the tile
@@ -323,7 +395,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
                 if (need_mask) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
-                        if (32 * c + e > kmax) sv[e] = 0xff800000u;   // -inf
+                        if (hidden(32 * c + e)) sv[e] = 0xff800000u;   // -inf
                 }
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) mxv = max3f(mxv, __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
@@ -355,8 +427,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
                     x0 = ex2f(x0);
                     x1 = ex2f(x1);
                     if (need_mask) {
-                        if (32 * c + e > kmax) x0 = 0.f;
-                        if (32 * c + e + 1 > kmax) x1 = 0.f;
+                        if (hidden(32 * c + e)) x0 = 0.f;
+                        if (hidden(32 * c + e + 1)) x1 = 0.f;
                     }
                     asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum2) : "l"(pack2(x0, x1)));   // even and odd columns apart
                     pp[e >> 1] = F16 ? pack_f16x2(x0, x1) : pack_bf16x2(x0, x1);
@@ -392,10 +464,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
             mbar_wait(bar(B_ODONE + x), (my_tiles - 1) & 1, abort_flag, p.status);
             tc_fence_after();
             // the warp's tcgen05.ld is collective: every lane reads, rows past the sequence store nothing
-            const bool row_ok = qi < len;
+            const bool row_ok = qr < len;
             auto pk2 = [](float a, float b2) { return F16 ? pack_f16x2(a, b2) : pack_bf16x2(a, b2); };
             const float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
-            uint16_t* orow = row_ptr<uint16_t>(p.o, b, start + (row_ok ? qi : 0), h);
+            uint16_t* orow = row_ptr<uint16_t>(p.o, b, start + (row_ok ? qr : 0), h);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 uint32_t ov[32];
@@ -413,11 +485,15 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
                     }
                 }
             }
-            if (row_ok) {
+            if (row_ok && (!EXT || p.lse)) {
                 const float lse = l_run > 0.f ? (m_run + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
-                p.lse[static_cast<int64_t>(b) * p.lse_sb + static_cast<int64_t>(h) * p.lse_sh + start + qi] = lse;
+                p.lse[static_cast<int64_t>(b) * p.lse_sb + static_cast<int64_t>(h) * p.lse_sh + start + qr] = lse;
             }
             tc_fence_before();
+        } else if (EXT && qr < len) {   // rows that see no key at all
+            uint16_t* orow = row_ptr<uint16_t>(p.o, b, start + qr, h);
+            for (int u = 0; u < 16; ++u) *reinterpret_cast<uint4*>(orow + 8 * u) = make_uint4(0u, 0u, 0u, 0u);
+            if (p.lse) p.lse[static_cast<int64_t>(b) * p.lse_sb + static_cast<int64_t>(h) * p.lse_sh + start + qr] = -INFINITY;
         }
     }
     __syncthreads();
@@ -472,13 +548,18 @@ extern "C" int fold_fwd_sm100_supported(int head_dim, int is_f16) {
     return head_dim == 128 && encode_fn() != nullptr;
 }
 
-extern "C" int fold_fwd_run_sm100(const void* q, const void* k, const void* v, void* o, float* lse,
-                                  const int64_t* strides, const int32_t* cu_seqlens, int batch, int n_heads,
-                                  int n_kv_heads, int max_seqlen, int total, int head_dim, int causal, int is_f16,
-                                  float softmax_scale, int32_t* status, void* stream) {
-    FOLD_CHECK_ARG(q && k && v && o && lse && strides && status, "fold_fwd_run_sm100: null pointer");
+namespace {
+
+// The causal and full forward (window 0, klens null), or the EXT build. `k_strides`-like entries of
+// `strides` are in elements: (batch, row, head) of q, k, v, o.
+int run_sm100(const char* what, const void* q, const void* k, const void* v, void* o, float* lse, const int64_t* strides,
+              const int32_t* cu_seqlens, int batch, int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim,
+              int causal, int is_f16, float softmax_scale, int ext, int window, int sinks, const int32_t* klens, int krows,
+              int32_t* status, void* stream) {
+    FOLD_CHECK_ARG(q && k && v && o && (lse || klens) && strides && status, "%s: null pointer", what);
     FOLD_CHECK_ARG(n_kv_heads > 0 && n_heads % n_kv_heads == 0, "the query heads must be a multiple of the KV heads");
-    FOLD_CHECK_ARG(batch > 0 && max_seqlen > 0, "fold_fwd_run_sm100: empty call");
+    FOLD_CHECK_ARG(batch > 0 && max_seqlen > 0, "%s: empty call", what);
+    FOLD_CHECK_ARG(n_heads <= 65535 && batch <= 65535, "%s: %d heads, %d requests (65535 at most)", what, n_heads, batch);
     if (!fold_fwd_sm100_supported(head_dim, 0)) {
         set_error("the tcgen05 forward takes head_dim 128");
         return FOLD_ERR_UNSUPPORTED;
@@ -487,7 +568,7 @@ extern "C" int fold_fwd_run_sm100(const void* q, const void* k, const void* v, v
     for (int i = 0; i < 4; ++i)
         FOLD_CHECK_ARG(strides[3 * i] % 8 == 0 && strides[3 * i + 1] % 8 == 0 && strides[3 * i + 2] % 8 == 0 &&
                            reinterpret_cast<uintptr_t>(ptrs[i]) % 16 == 0,
-                       "fold_fwd_run_sm100: rows must be 16-byte aligned");
+                       "%s: rows must be 16-byte aligned", what);
     fsm100::Params p;
     p.o.ptr = o; p.o.sb = strides[9]; p.o.sr = strides[10]; p.o.sh = strides[11];
     p.lse = lse;
@@ -501,25 +582,46 @@ extern "C" int fold_fwd_run_sm100(const void* q, const void* k, const void* v, v
     }
     p.B = batch; p.H = n_heads; p.HKV = n_kv_heads; p.G = n_heads / n_kv_heads;
     p.S = max_seqlen; p.causal = causal; p.scale = softmax_scale; p.status = status;
+    p.window = window; p.sinks = sinks; p.klens = klens; p.krows = krows;
     const int64_t rows = cu_seqlens ? total : max_seqlen;
     const int mbatch = cu_seqlens ? 1 : batch;
+    const int64_t kvrows = klens ? krows : rows;
+    const int kvbatch = klens ? batch : mbatch;
     fsm100::Maps maps;
     const bool f16 = is_f16 != 0;
     if (!make_map(&maps.q, q, strides[0], strides[1], strides[2], rows, n_heads, mbatch, f16) ||
-        !make_map(&maps.k, k, strides[3], strides[4], strides[5], rows, n_kv_heads, mbatch, f16) ||
-        !make_map(&maps.v, v, strides[6], strides[7], strides[8], rows, n_kv_heads, mbatch, f16)) {
-        set_error("fold_fwd_run_sm100: cuTensorMapEncodeTiled failed");
+        !make_map(&maps.k, k, strides[3], strides[4], strides[5], kvrows, n_kv_heads, kvbatch, f16) ||
+        !make_map(&maps.v, v, strides[6], strides[7], strides[8], kvrows, n_kv_heads, kvbatch, f16)) {
+        set_error("%s: cuTensorMapEncodeTiled failed", what);
         return FOLD_ERR_LAUNCH;
     }
     dim3 grid((max_seqlen + fsm100::CTA_M - 1) / fsm100::CTA_M, n_heads, batch);
-    if (f16) {
-        auto kern = fsm100::fwd_sm100_kernel<true>;
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fsm100::SMEM_BYTES);
-        kern<<<grid, fsm100::NTHREADS, fsm100::SMEM_BYTES, static_cast<cudaStream_t>(stream)>>>(p, maps);
-    } else {
-        auto kern = fsm100::fwd_sm100_kernel<false>;
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fsm100::SMEM_BYTES);
-        kern<<<grid, fsm100::NTHREADS, fsm100::SMEM_BYTES, static_cast<cudaStream_t>(stream)>>>(p, maps);
-    }
-    return check_launch("fold_fwd_run_sm100");
+    auto kern = f16 ? (ext ? fsm100::fwd_sm100_kernel<true, true> : fsm100::fwd_sm100_kernel<true, false>)
+                    : (ext ? fsm100::fwd_sm100_kernel<false, true> : fsm100::fwd_sm100_kernel<false, false>);
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fsm100::SMEM_BYTES);
+    kern<<<grid, fsm100::NTHREADS, fsm100::SMEM_BYTES, static_cast<cudaStream_t>(stream)>>>(p, maps);
+    return check_launch(what);
+}
+
+}  // namespace
+
+extern "C" int fold_fwd_run_sm100(const void* q, const void* k, const void* v, void* o, float* lse,
+                                  const int64_t* strides, const int32_t* cu_seqlens, int batch, int n_heads,
+                                  int n_kv_heads, int max_seqlen, int total, int head_dim, int causal, int is_f16,
+                                  float softmax_scale, int32_t* status, void* stream) {
+    FOLD_CHECK_ARG(lse, "fold_fwd_run_sm100: null pointer");
+    return run_sm100("fold_fwd_run_sm100", q, k, v, o, lse, strides, cu_seqlens, batch, n_heads, n_kv_heads, max_seqlen, total,
+                     head_dim, causal, is_f16, softmax_scale, 0, 0, 0, nullptr, 0, status, stream);
+}
+
+extern "C" int fold_fwd_window_sm100(const void* q, const void* k, const void* v, void* o, float* lse,
+                                     const int64_t* strides, const int32_t* cu_seqlens, int batch, int n_heads,
+                                     int n_kv_heads, int max_seqlen, int total, int head_dim, int is_f16,
+                                     float softmax_scale, int window, int sinks, const int32_t* key_lens, int key_rows,
+                                     int32_t* status, void* stream) {
+    FOLD_CHECK_ARG(window > 0 && window <= FOLD_MAX_WINDOW && sinks >= 0 && sinks <= FOLD_MAX_WINDOW,
+                   "fold_fwd_window_sm100: a window of %d keys and %d sinks (1 .. 2^30 and 0 .. 2^30)", window, sinks);
+    FOLD_CHECK_ARG(!key_lens || key_rows > 0, "fold_fwd_window_sm100: %d key rows", key_rows);
+    return run_sm100("fold_fwd_window_sm100", q, k, v, o, lse, strides, cu_seqlens, batch, n_heads, n_kv_heads, max_seqlen, total,
+                     head_dim, 1, is_f16, softmax_scale, 1, window, sinks, key_lens, key_rows, status, stream);
 }

@@ -16,7 +16,7 @@ import math
 import torch
 
 from .backward.launch import attention_forward, prepare_backward
-from .utils import require_sm100
+from .utils import check_window, require_sm100
 
 # Set to True to read the backward's device status word after every backward (one host
 # synchronisation each) and raise FoldLibraryError if a kernel gave up a bounded wait; by
@@ -42,11 +42,11 @@ def _check_qkv(q, k, v, ndim):
 
 class _FoldAttnFunc(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, softmax_scale, causal):
+    def forward(ctx, q, k, v, softmax_scale, causal, window, sinks):
         q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, v))
-        out, lse = attention_forward(q, k, v, causal=causal, softmax_scale=softmax_scale)
+        out, lse = attention_forward(q, k, v, causal=causal, softmax_scale=softmax_scale, window=window, sinks=sinks)
         ctx.save_for_backward(q, k, v, out, lse)
-        ctx.softmax_scale, ctx.causal = softmax_scale, causal
+        ctx.softmax_scale, ctx.causal, ctx.window, ctx.sinks = softmax_scale, causal, window, sinks
         return out
 
     @staticmethod
@@ -62,23 +62,26 @@ class _FoldAttnFunc(torch.autograd.Function):
             lse,
             causal=ctx.causal,
             softmax_scale=ctx.softmax_scale,
+            window=ctx.window,
+            sinks=ctx.sinks,
         )
         dq, dk, dv = run()
         if check_status:
             run.check()
-        return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), None, None
+        return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), None, None, None, None
 
 
 class _FoldAttnVarlenFunc(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, cu_seqlens, max_seqlen, softmax_scale, causal):
+    def forward(ctx, q, k, v, cu_seqlens, max_seqlen, softmax_scale, causal, window, sinks):
         q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, v))
         out, lse = attention_forward(
             q, k, v, causal=causal, softmax_scale=softmax_scale,
-            cu_seqlens=cu_seqlens, max_seqlen=max_seqlen,
+            cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, window=window, sinks=sinks,
         )
         ctx.save_for_backward(q, k, v, out, lse, cu_seqlens)
         ctx.max_seqlen, ctx.softmax_scale, ctx.causal = max_seqlen, softmax_scale, causal
+        ctx.window, ctx.sinks = window, sinks
         return out
 
     @staticmethod
@@ -96,26 +99,34 @@ class _FoldAttnVarlenFunc(torch.autograd.Function):
             softmax_scale=ctx.softmax_scale,
             cu_seqlens=cu_seqlens,
             max_seqlen=ctx.max_seqlen,
+            window=ctx.window,
+            sinks=ctx.sinks,
         )
         dq, dk, dv = run()
         if check_status:
             run.check()
-        return dq, dk, dv, None, None, None, None
+        return dq, dk, dv, None, None, None, None, None, None
 
 
-def fold_attn_func(q, k, v, softmax_scale=None, causal=False):
+def fold_attn_func(q, k, v, softmax_scale=None, causal=False, window=None, sinks=0):
     """Self-attention over `(batch, seqlen, nheads, headdim)` tensors.
 
     `k` and `v` may have fewer heads than `q` (GQA/MQA). Returns the output,
     shaped and typed as `q`. The backward reduces across CTAs in integers, so
     the gradients do not depend on the order work runs in. Head dims 64, 96
     and 128, bf16 or fp16, SM100.
+
+    `window` (with `causal=True`) is a sliding window: the query at position i
+    sees the `window` newest keys up to its own, `i - window < j <= i`, and the
+    sequence's first `sinks` keys. The work is the window's, not the
+    sequence's, and the gradients keep their order-free bits.
     """
+    window, sinks = check_window(window, sinks, causal)
     _check_qkv(q, k, v, 4)
     if q.shape[1] != k.shape[1]:
         raise ValueError("self-attention needs equal query and key lengths")
     scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else float(softmax_scale)
-    return _FoldAttnFunc.apply(q, k, v, scale, bool(causal))
+    return _FoldAttnFunc.apply(q, k, v, scale, bool(causal), window or None, sinks)
 
 
 def fold_attn_varlen_func(
@@ -128,6 +139,8 @@ def fold_attn_varlen_func(
     max_seqlen_k=None,
     softmax_scale=None,
     causal=False,
+    window=None,
+    sinks=0,
 ):
     """Self-attention over sequences packed along the first axis.
 
@@ -135,8 +148,10 @@ def fold_attn_varlen_func(
     headdim)`, split by `cu_seqlens_q`, a CUDA int32 `(batch + 1,)` tensor.
     The keys are the queries' own sequences, so `cu_seqlens_k` and
     `max_seqlen_k` may be left out; if given they must match. A request's
-    gradients are the same bits alone and packed with others.
+    gradients are the same bits alone and packed with others. `window` and
+    `sinks` as for `fold_attn_func`, counted within each sequence.
     """
+    window, sinks = check_window(window, sinks, causal)
     _check_qkv(q, k, v, 3)
     cu = cu_seqlens_q
     if cu.ndim != 1 or cu.dtype != torch.int32 or cu.device != q.device:
@@ -148,7 +163,7 @@ def fold_attn_varlen_func(
     if max_seqlen_k is not None and int(max_seqlen_k) != int(max_seqlen_q):
         raise ValueError("self-attention needs max_seqlen_k == max_seqlen_q")
     scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else float(softmax_scale)
-    return _FoldAttnVarlenFunc.apply(q, k, v, cu, int(max_seqlen_q), scale, bool(causal))
+    return _FoldAttnVarlenFunc.apply(q, k, v, cu, int(max_seqlen_q), scale, bool(causal), window or None, sinks)
 
 
 def fold_attn_with_kvcache(q, cache, k=None, v=None):

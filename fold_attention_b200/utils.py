@@ -12,6 +12,28 @@ import torch
 LOG2E = 1.4426950408889634
 
 
+# the most keys a sliding window, or its sinks, may name (FOLD_MAX_WINDOW of the header)
+MAX_WINDOW = 1 << 30
+
+
+def check_window(window, sinks, causal=True):
+    """`(window, sinks)` as ints, 0 keys for no window. Under a window the query at
+    position i sees key j <= i when `i - j < window` or `j < sinks`."""
+    if isinstance(window, bool) or isinstance(sinks, bool) or (window is not None and int(window) != window) or int(sinks) != sinks:
+        raise ValueError(f"window and sinks are whole numbers of keys (got {window}, {sinks})")
+    sinks = int(sinks)
+    if window is None:
+        if sinks:
+            raise ValueError("sinks are the first keys that stay visible beside a window: give a window")
+        return 0, 0
+    window = int(window)
+    if not 1 <= window <= MAX_WINDOW or not 0 <= sinks <= MAX_WINDOW:
+        raise ValueError(f"a window of {window} keys and {sinks} sinks: 1..2^30 and 0..2^30")
+    if not causal:
+        raise ValueError("a sliding window needs causal=True")
+    return window, sinks
+
+
 @dataclass(eq=False)
 class Launch:
     """A prepared launch: calling it calls `run`. Kernels take the bound

@@ -27,6 +27,9 @@ extern "C" {
 #define FOLD_ERR_TIMEOUT 3
 #define FOLD_ERR_UNSUPPORTED 4
 
+/* the most keys a sliding window, or its sinks, may name */
+#define FOLD_MAX_WINDOW (1 << 30)
+
 /* Message of the calling thread's last failed call ("" if none). */
 const char* fold_last_error(void);
 int fold_abi_version(void);
@@ -334,6 +337,22 @@ int fold_bwd_run_phases(const void* q, const void* k, const void* v, const void*
                         size_t workspace_bytes, int kernel, int subgroup, int record, int phases,
                         void* stream);
 
+/* The deterministic backward of causal self-attention under a sliding window with sinks: query i
+ * sees key j <= i when i - j < window or j < sinks. `lse` is fold_fwd_window's. Arguments as
+ * fold_bwd_run_phases, without a plan: key blocks past the sinks are private to a CTA, the sinks'
+ * blocks are cut into records of query blocks and folded on the integer grids; a packed sequence's
+ * gradients are the same bits whatever it is packed with. fold_bwd_window_layout describes the
+ * workspace as fold_bwd_workspace_layout does ([6], [7]: the sinks' accumulators
+ * [n_kv_heads][batch][sinks rounded up to 128][head_dim]) with its size in bytes in out12[11].
+ * No counterpart in the reference. */
+int fold_bwd_window_layout(int batch, int n_heads, int n_kv_heads, int max_seqlen, int total,
+                           int head_dim, int varlen, int window, int sinks, int64_t* out12);
+int fold_bwd_window(const void* q, const void* k, const void* v, const void* o, const void* dout,
+                    const float* lse, void* dq, void* dk, void* dv, const int64_t* strides /* host */,
+                    const int32_t* cu_seqlens, int batch, int n_heads, int n_kv_heads, int max_seqlen,
+                    int total, int head_dim, int is_f16, float softmax_scale, void* workspace,
+                    size_t workspace_bytes, int kernel, int window, int sinks, int phases, void* stream);
+
 /* Cycle counters of the tcgen05 backward's main loop, summed over the launches since the
  * last reset: out24 (host, 24 entries) receives CTAs, tiles, CTA lifetime, prologue, epilogue,
  * the compute warps' wait for S^T / exponential phase / wait for dP^T / dS~ phase, the MMA
@@ -368,6 +387,24 @@ int fold_fwd_run_sm100(const void* q, const void* k, const void* v, void* o, flo
                        const int64_t* strides /* host */, const int32_t* cu_seqlens, int batch,
                        int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim,
                        int causal, int is_f16, float softmax_scale, int32_t* status, void* stream);
+
+/* The causal forward under a sliding window with sinks, on the warp-level and on the tcgen05
+ * kernel: the query at position i sees key j when j <= i and (i - j < window or j < sinks).
+ * Arguments as fold_fwd_run / fold_fwd_run_sm100. With key_lens (int32[batch] on the device) the
+ * keys and values are request b's own key_lens[b] rows of (batch, row, head) tensors of key_rows
+ * rows a request, the queries are the request's last positions (cu_seqlens cuts q and o alone),
+ * and lse may be NULL. A row that sees no key gets zeros and an lse of -infinity. A window that no
+ * sequence fills is plain causal attention. No counterpart in the reference. */
+int fold_fwd_window(const void* q, const void* k, const void* v, void* o, float* lse,
+                    const int64_t* strides /* host */, const int32_t* cu_seqlens, int batch,
+                    int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim, int is_f16,
+                    float softmax_scale, int window, int sinks, const int32_t* key_lens, int key_rows,
+                    void* stream);
+int fold_fwd_window_sm100(const void* q, const void* k, const void* v, void* o, float* lse,
+                          const int64_t* strides /* host */, const int32_t* cu_seqlens, int batch,
+                          int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim,
+                          int is_f16, float softmax_scale, int window, int sinks,
+                          const int32_t* key_lens, int key_rows, int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

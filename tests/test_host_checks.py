@@ -104,3 +104,26 @@ def test_a_decode_launch_binds_on_the_host_for_every_layout():
         prepare_fold_decode(*planes(4, 16), draft_len=2, causal=True, **kw)
     with pytest.raises(ValueError, match="names the 16 groups of 8"):
         prepare_fold_decode(*planes(4, 32), order=torch.arange(4, dtype=torch.int32), **kw)
+
+
+@pytest.mark.parametrize("window,sinks,causal", [
+    (0, 0, True), (-1, 0, True), (2.5, 0, True), (True, 0, True), (4, -1, True), (4, 1.5, True), (4, 0, False),
+    (None, 3, True), ((1 << 30) + 1, 0, True), (4, (1 << 30) + 1, True),
+])
+def test_a_window_that_means_nothing_is_refused(window, sinks, causal):
+    import fold_attention_b200 as fa
+
+    x = torch.zeros(1, 8, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="window"):
+        fa.fold_attn_func(x, x, x, causal=causal, window=window, sinks=sinks)
+    cu = torch.tensor([0, 8], dtype=torch.int32)
+    with pytest.raises(ValueError, match="window"):
+        fa.fold_attn_varlen_func(x[0], x[0], x[0], cu, causal=causal, window=window, sinks=sinks)
+
+
+def test_a_windowed_backward_takes_no_plan():
+    from fold_attention_b200.backward import Plan, prepare_backward
+
+    x = torch.zeros(1, 2, 8, 64, dtype=torch.bfloat16)
+    with pytest.raises(NotImplementedError, match="plan"):
+        prepare_backward(x, x, x, x, x, torch.zeros(1, 2, 8), causal=True, window=4, plan=Plan(1, 0))
