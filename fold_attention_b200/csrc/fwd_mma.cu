@@ -16,11 +16,11 @@ struct FwdParams {
     int B, H, HKV, G, S, D, causal, f16;
     float scale;
     // a build with EXT = true only (it is causal): a row sees the `window` newest keys up to its own
-    // position and the first `sinks` keys; with `klens` the keys are request b's own rows
-    // [0, klens[b]) of a (batch, row, head) tensor of `krows` rows a request, and the queries are its last
+    // position and the first `sinks` keys; with `plan` the queries are request b's last positions and its
+    // keys plan[b].x rows of (row, head) tensors from row plan[b].y on, without the plan[b].z tiles of 128
+    // keys between the sinks' tiles and the window's that no query of the chunk sees
     int window, sinks;
-    const int* klens;
-    int krows;
+    const int4* plan;
 };
 
 template <int D, bool F16, bool CAUSAL, bool EXT>
@@ -41,13 +41,14 @@ __global__ void __launch_bounds__(128) fwd_mma_kernel(const FwdParams p) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tq = lane & 3;
     const int hkv = h / p.G;
     const float c2 = p.scale * kLog2e;
-    int klen = len, qoff = 0, kstart = start;   // keys, and the first query's position among them
+    int klen = len, qoff = 0, kstart = start, kshift = 0;   // keys, and the first query's position among them
     if constexpr (EXT) {
-        if (p.klens) {
-            const int n = p.klens[b];
-            qoff = n - len;
-            klen = min(n, p.krows);
-            kstart = 0;
+        if (p.plan) {
+            const int4 pl = p.plan[b];
+            klen = pl.x;
+            qoff = klen - len;
+            kstart = pl.y;
+            kshift = 128 * pl.z;
         }
     }
 
@@ -71,8 +72,9 @@ __global__ void __launch_bounds__(128) fwd_mma_kernel(const FwdParams p) {
         }
         __syncthreads();  // previous tile's reads are done
         const int kvalid = min(64, klen - n0);
-        load_tile_async<D, PITCH, 128>(sK, row_ptr<const uint16_t>(p.k, b, kstart + n0, hkv), p.k.sr, 64, kvalid, tid);
-        load_tile_async<D, PITCH, 128>(sV, row_ptr<const uint16_t>(p.v, b, kstart + n0, hkv), p.v.sr, 64, kvalid, tid);
+        const int krow = kstart + (EXT && n0 >= (p.sinks + 127) / 128 * 128 ? n0 - kshift : n0);   // whole tiles of 128 keys are left out
+        load_tile_async<D, PITCH, 128>(sK, row_ptr<const uint16_t>(p.k, b, krow, hkv), p.k.sr, 64, kvalid, tid);
+        load_tile_async<D, PITCH, 128>(sV, row_ptr<const uint16_t>(p.v, b, krow, hkv), p.v.sr, 64, kvalid, tid);
         cp_async_commit();
         cp_async_wait<0>();
         __syncthreads();
@@ -149,11 +151,11 @@ __global__ void __launch_bounds__(128) fwd_mma_kernel(const FwdParams p) {
             a[1] = pack16x2<F16>(s[2 * kk][2], s[2 * kk][3]);
             a[2] = pack16x2<F16>(s[2 * kk + 1][0], s[2 * kk + 1][1]);
             a[3] = pack16x2<F16>(s[2 * kk + 1][2], s[2 * kk + 1][3]);
-            const int krow = 16 * kk + (lane & 7) + 8 * ((lane >> 3) & 1);
+            const int vrow = 16 * kk + (lane & 7) + 8 * ((lane >> 3) & 1);
 #pragma unroll
             for (int np = 0; np < NTO / 2; ++np) {
                 uint32_t bv[4];
-                ldmatrix_x4_trans(bv, smem_u32(sV + krow * PITCH + (2 * np + (lane >> 4)) * 16));
+                ldmatrix_x4_trans(bv, smem_u32(sV + vrow * PITCH + (2 * np + (lane >> 4)) * 16));
                 mma_16816<F16>(o[2 * np], a, bv[0], bv[1]);
                 mma_16816<F16>(o[2 * np + 1], a, bv[2], bv[3]);
             }
@@ -200,12 +202,12 @@ static int fwd_launch_d(const FwdParams& p, cudaStream_t st) {
 
 using namespace fold;
 
-// The causal and full forward (window 0, klens null), or the EXT build.
+// The causal and full forward (window 0, plan null), or the EXT build.
 static int fwd_run(const char* what, const void* q, const void* k, const void* v, void* o, float* lse,
                    const int64_t* strides, const int32_t* cu_seqlens, int batch, int n_heads, int n_kv_heads,
                    int max_seqlen, int total, int head_dim, int causal, int is_f16, float softmax_scale, int window,
-                   int sinks, const int32_t* klens, int krows, void* stream) {
-    FOLD_CHECK_ARG(q && k && v && o && (lse || klens) && strides, "%s: null pointer", what);
+                   int sinks, const int32_t* plan, int krows, void* stream) {
+    FOLD_CHECK_ARG(q && k && v && o && (lse || plan) && strides, "%s: null pointer", what);
     FOLD_CHECK_ARG(n_kv_heads > 0 && n_heads % n_kv_heads == 0, "the query heads must be a multiple of the KV heads");
     FOLD_CHECK_ARG(batch > 0 && max_seqlen > 0, "%s: empty call", what);
     FOLD_CHECK_ARG(n_heads <= 65535 && batch <= 65535, "%s: %d heads, %d requests (65535 at most)", what, n_heads, batch);
@@ -232,7 +234,7 @@ static int fwd_run(const char* what, const void* q, const void* k, const void* v
     }
     p.B = batch; p.H = n_heads; p.HKV = n_kv_heads; p.G = n_heads / n_kv_heads;
     p.S = max_seqlen; p.D = head_dim; p.causal = causal; p.f16 = is_f16; p.scale = softmax_scale;
-    p.window = window; p.sinks = sinks; p.klens = klens; p.krows = krows;
+    p.window = window; p.sinks = sinks; p.plan = reinterpret_cast<const int4*>(plan);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (head_dim) {
         case 64: return fwd_launch_d<64>(p, st);
@@ -255,11 +257,11 @@ extern "C" int fold_fwd_run(const void* q, const void* k, const void* v, void* o
 extern "C" int fold_fwd_window(const void* q, const void* k, const void* v, void* o, float* lse,
                                const int64_t* strides, const int32_t* cu_seqlens, int batch, int n_heads,
                                int n_kv_heads, int max_seqlen, int total, int head_dim, int is_f16,
-                               float softmax_scale, int window, int sinks, const int32_t* key_lens, int key_rows,
+                               float softmax_scale, int window, int sinks, const int32_t* plan, int key_rows,
                                void* stream) {
     FOLD_CHECK_ARG(window > 0 && window <= FOLD_MAX_WINDOW && sinks >= 0 && sinks <= FOLD_MAX_WINDOW,
                    "fold_fwd_window: a window of %d keys and %d sinks (1 .. 2^30 and 0 .. 2^30)", window, sinks);
-    FOLD_CHECK_ARG(!key_lens || key_rows > 0, "fold_fwd_window: %d key rows", key_rows);
+    FOLD_CHECK_ARG(!plan || key_rows > 0, "fold_fwd_window: %d key rows", key_rows);
     return fwd_run("fold_fwd_window", q, k, v, o, lse, strides, cu_seqlens, batch, n_heads, n_kv_heads, max_seqlen, total,
-                   head_dim, 1, is_f16, softmax_scale, window, sinks, key_lens, key_rows, stream);
+                   head_dim, 1, is_f16, softmax_scale, window, sinks, plan, key_rows, stream);
 }

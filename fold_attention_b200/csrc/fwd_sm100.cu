@@ -177,11 +177,11 @@ struct Params {
     float scale;
     int* status;
     // a build with EXT = true only (it is causal): a row sees the `window` newest keys up to its own
-    // position and the first `sinks` keys; with `klens` the keys are request b's own rows
-    // [0, klens[b]) of a (batch, row, head) tensor of `krows` rows a request, and the queries are its last
+    // position and the first `sinks` keys; with `plan` the queries are request b's last positions and its
+    // keys plan[b].x rows of (row, head) tensors from row plan[b].y on, without the plan[b].z tiles of 128
+    // keys between the sinks' tiles and the window's that no query of the chunk sees
     int window, sinks;
-    const int* klens;
-    int krows;
+    const int4* plan;
 };
 struct Maps {
     CUtensorMap q, k, v;   // (channel, row, head, batch), boxes (64, 128, 1, 1)
@@ -224,14 +224,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
     if (m0 >= len) return;
     const int hkv = h / p.G;
     const int bb = p.cu ? 0 : b;
-    int klen = len, qoff = 0, kstart = start, kb = bb;   // keys, and the first query's position among them
+    int klen = len, qoff = 0, kstart = start, kshift = 0;   // keys, and the first query's position among them
     if constexpr (EXT) {
-        if (p.klens) {
-            const int n = p.klens[b];
-            qoff = n - len;
-            klen = min(n, p.krows);
-            kstart = 0;
-            kb = b;
+        if (p.plan) {
+            const int4 pl = p.plan[b];
+            klen = pl.x;
+            qoff = klen - len;
+            kstart = pl.y;
+            kshift = pl.z;
         }
     }
     // key tiles each of the two query tiles meets (the second tile may lie past the sequence)
@@ -261,6 +261,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
     }
     const int n_tiles = EXT ? tl.n : max(nt[0], nt[1]);
     auto tile_of = [&](int j) { return EXT ? tl.tile(j) : j; };
+    // the tile's first row: tiles that the chunk leaves out have none
+    auto row_of = [&](int j) {
+        const int t = tile_of(j);
+        return kstart + (EXT && t * BN >= p.sinks ? t - kshift : t) * BN;
+    };
     auto takes = [&](int x, int j) { return EXT ? tl.active(x, j) : j < nt[x]; };
 
     if (tid == 0) {
@@ -300,8 +305,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
                 const uint32_t st = base + SM_KV + s * STAGE;
                 mbar_expect_tx(bar(B_KVFULL + s), 65536);
                 for (int c = 0; c < 2; ++c) {
-                    tma_load_4d(st + c * 16384, &maps.k, 64 * c, kstart + tile_of(j) * BN, hkv, kb, bar(B_KVFULL + s));
-                    tma_load_4d(st + 32768 + c * 16384, &maps.v, 64 * c, kstart + tile_of(j) * BN, hkv, kb, bar(B_KVFULL + s));
+                    tma_load_4d(st + c * 16384, &maps.k, 64 * c, row_of(j), hkv, bb, bar(B_KVFULL + s));
+                    tma_load_4d(st + 32768 + c * 16384, &maps.v, 64 * c, row_of(j), hkv, bb, bar(B_KVFULL + s));
                 }
             }
         }
@@ -550,13 +555,13 @@ extern "C" int fold_fwd_sm100_supported(int head_dim, int is_f16) {
 
 namespace {
 
-// The causal and full forward (window 0, klens null), or the EXT build. `k_strides`-like entries of
+// The causal and full forward (window 0, plan null), or the EXT build. `k_strides`-like entries of
 // `strides` are in elements: (batch, row, head) of q, k, v, o.
 int run_sm100(const char* what, const void* q, const void* k, const void* v, void* o, float* lse, const int64_t* strides,
               const int32_t* cu_seqlens, int batch, int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim,
-              int causal, int is_f16, float softmax_scale, int ext, int window, int sinks, const int32_t* klens, int krows,
+              int causal, int is_f16, float softmax_scale, int ext, int window, int sinks, const int32_t* plan, int krows,
               int32_t* status, void* stream) {
-    FOLD_CHECK_ARG(q && k && v && o && (lse || klens) && strides && status, "%s: null pointer", what);
+    FOLD_CHECK_ARG(q && k && v && o && (lse || plan) && strides && status, "%s: null pointer", what);
     FOLD_CHECK_ARG(n_kv_heads > 0 && n_heads % n_kv_heads == 0, "the query heads must be a multiple of the KV heads");
     FOLD_CHECK_ARG(batch > 0 && max_seqlen > 0, "%s: empty call", what);
     FOLD_CHECK_ARG(n_heads <= 65535 && batch <= 65535, "%s: %d heads, %d requests (65535 at most)", what, n_heads, batch);
@@ -582,16 +587,15 @@ int run_sm100(const char* what, const void* q, const void* k, const void* v, voi
     }
     p.B = batch; p.H = n_heads; p.HKV = n_kv_heads; p.G = n_heads / n_kv_heads;
     p.S = max_seqlen; p.causal = causal; p.scale = softmax_scale; p.status = status;
-    p.window = window; p.sinks = sinks; p.klens = klens; p.krows = krows;
+    p.window = window; p.sinks = sinks; p.plan = reinterpret_cast<const int4*>(plan);
     const int64_t rows = cu_seqlens ? total : max_seqlen;
     const int mbatch = cu_seqlens ? 1 : batch;
-    const int64_t kvrows = klens ? krows : rows;
-    const int kvbatch = klens ? batch : mbatch;
+    const int64_t kvrows = plan ? krows : rows;
     fsm100::Maps maps;
     const bool f16 = is_f16 != 0;
     if (!make_map(&maps.q, q, strides[0], strides[1], strides[2], rows, n_heads, mbatch, f16) ||
-        !make_map(&maps.k, k, strides[3], strides[4], strides[5], kvrows, n_kv_heads, kvbatch, f16) ||
-        !make_map(&maps.v, v, strides[6], strides[7], strides[8], kvrows, n_kv_heads, kvbatch, f16)) {
+        !make_map(&maps.k, k, strides[3], strides[4], strides[5], kvrows, n_kv_heads, mbatch, f16) ||
+        !make_map(&maps.v, v, strides[6], strides[7], strides[8], kvrows, n_kv_heads, mbatch, f16)) {
         set_error("%s: cuTensorMapEncodeTiled failed", what);
         return FOLD_ERR_LAUNCH;
     }
@@ -617,11 +621,11 @@ extern "C" int fold_fwd_run_sm100(const void* q, const void* k, const void* v, v
 extern "C" int fold_fwd_window_sm100(const void* q, const void* k, const void* v, void* o, float* lse,
                                      const int64_t* strides, const int32_t* cu_seqlens, int batch, int n_heads,
                                      int n_kv_heads, int max_seqlen, int total, int head_dim, int is_f16,
-                                     float softmax_scale, int window, int sinks, const int32_t* key_lens, int key_rows,
+                                     float softmax_scale, int window, int sinks, const int32_t* plan, int key_rows,
                                      int32_t* status, void* stream) {
     FOLD_CHECK_ARG(window > 0 && window <= FOLD_MAX_WINDOW && sinks >= 0 && sinks <= FOLD_MAX_WINDOW,
                    "fold_fwd_window_sm100: a window of %d keys and %d sinks (1 .. 2^30 and 0 .. 2^30)", window, sinks);
-    FOLD_CHECK_ARG(!key_lens || key_rows > 0, "fold_fwd_window_sm100: %d key rows", key_rows);
+    FOLD_CHECK_ARG(!plan || key_rows > 0, "fold_fwd_window_sm100: %d key rows", key_rows);
     return run_sm100("fold_fwd_window_sm100", q, k, v, o, lse, strides, cu_seqlens, batch, n_heads, n_kv_heads, max_seqlen, total,
-                     head_dim, 1, is_f16, softmax_scale, 1, window, sinks, key_lens, key_rows, status, stream);
+                     head_dim, 1, is_f16, softmax_scale, 1, window, sinks, plan, key_rows, status, stream);
 }

@@ -1,0 +1,188 @@
+"""The paged cache a piece at a time (host side): block tables and slots from
+request lengths, new tokens into the pool and back, and the attention of a
+chunk of new tokens over the cache that holds them.
+
+A token's slot is `page * page_size + offset`: the same for every KV head, and
+for every layer whose cache shares the table, so one `build_tables` serves a
+whole model's step. Its pool row for KV head h is
+`(page * n_kv_heads + h) * page_size + offset`. A slot of -1 stands for no place:
+`write_tokens` skips it and `read_tokens` returns zeros.
+
+No counterpart in the reference, whose tables are the host's and whose cache
+takes prompts whole and then one token a request.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .. import _lib
+
+P, I, F, L = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_int64
+_lib.register("fold_build_tables", [P, P, I, P, I, I, I, P, I, P, P, P, P, P])
+_lib.register("fold_write_tokens", [P, P, I, L, L, L, L, P, L, I, I, I, P, P, P, P, P, F, P])
+_lib.register("fold_read_tokens", [P, L, I, I, I, P, P, P, P, P, F, P, P, I, P])
+_lib.register("fold_chunk_sums", [P, I, L, L, I, I, I, P, I, P, P, F, P, P, P])
+_lib.register("fold_chunk_gather", [P, P, I, P, I, I, I, I, I, I, P, P, P, P, P, F, I, I, P, P, P, P, P, P])
+
+_HALF = (torch.bfloat16, torch.float16)
+_OUT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _int32(name, t, shape, device):
+    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} is a contiguous int32 {tuple(shape)} on {device} (got {t.dtype} {tuple(t.shape)} on {t.device})")
+
+
+def build_tables(cu_seqlens, seq_lens, page_table, page_size, total, *, free_pages=None, taken=None):
+    """Block tables and the new tokens' slots, on the device, from lengths.
+
+    Request b holds `seq_lens[b]` tokens and brings rows `cu_seqlens[b] ..
+    cu_seqlens[b + 1]` of `total` packed ones (none is allowed). With
+    `free_pages`, an int32 list of page numbers whose first `taken[0]` are in
+    use, the pages a request grows by are taken from it in request order and
+    written into `page_table` `(batch, pages)`, in place; without, the table
+    stands as it is. Returns `(slots, lens, taken)`: each new token's slot
+    (int32 `(total,)`), the lengths with the new tokens, and the pages then in
+    use (None without `free_pages`). A token that its request's table row or
+    the pool has no page for, and a row that no request covers, gets slot -1;
+    `taken` past the list's end says that the pool ran out. The arguments other
+    than the table are left as they are, so the same call gives the same
+    answer. All tensors are int32 on one device; nothing waits on it.
+    """
+    dev = seq_lens.device
+    if seq_lens.ndim != 1 or page_table.ndim != 2 or seq_lens.shape[0] < 1 or page_table.shape[1] < 1:
+        raise ValueError(f"seq_lens is (batch,) and page_table (batch, pages), got {tuple(seq_lens.shape)}, {tuple(page_table.shape)}")
+    B = seq_lens.shape[0]
+    _int32("seq_lens", seq_lens, (B,), dev)
+    _int32("cu_seqlens", cu_seqlens, (B + 1,), dev)
+    _int32("page_table", page_table, (B, page_table.shape[1]), dev)
+    total, page_size = int(total), int(page_size)
+    if total < 0 or page_size < 1:
+        raise ValueError(f"{total} tokens, pages of {page_size} keys")
+    if (free_pages is None) != (taken is None):
+        raise ValueError("free_pages and taken are both given or both left out")
+    n_free = 0
+    if free_pages is not None:
+        n_free = free_pages.numel()
+        _int32("free_pages", free_pages, (n_free,), dev)
+        _int32("taken", taken, (1,), dev)
+    out = torch.empty(total + B + 1, device=dev, dtype=torch.int32)
+    slots, lens, used = out[:total], out[total:total + B], out[total + B:]
+    with torch.cuda.device(dev):
+        _lib.call(
+            "fold_build_tables", cu_seqlens.data_ptr(), seq_lens.data_ptr(), B, page_table.data_ptr(), page_table.shape[1], page_size,
+            total, _lib.ptr(free_pages) or None, n_free, _lib.ptr(taken), slots.data_ptr(), lens.data_ptr(),
+            used.data_ptr() if free_pages is not None else None, _lib.stream(dev),
+        )
+    return slots, lens, used if free_pages is not None else None
+
+
+def _planes(D, ka, kb, va, vb, ek, dev):
+    """The pool's planes, checked against each other: the kernels index all of them by one row."""
+    rows = ka.shape[0]
+    vdt = torch.bfloat16 if vb is None else torch.float8_e4m3fn
+    for name, t, dt in (("ka", ka, torch.int8), ("kb", kb, torch.int8), ("va", va, vdt), ("vb", vb, vdt)):
+        if t is not None and (t.dtype != dt or tuple(t.shape) != (rows, D) or t.device != dev or not t.is_contiguous()):
+            raise ValueError(f"{name} is a contiguous {dt} ({rows}, {D}) on {dev} (got {t.dtype} {tuple(t.shape)} on {t.device})")
+    if ek.dtype != torch.bfloat16 or tuple(ek.shape) != (rows,) or ek.device != dev or not ek.is_contiguous():
+        raise ValueError(f"ek is a contiguous bf16 ({rows},) on {dev} (got {ek.dtype} {tuple(ek.shape)} on {ek.device})")
+
+
+def _rows(t):
+    """`t` with 16-byte rows the kernels can read in place, or a copy."""
+    ok = t.stride(-1) == 1 and all(s % 8 == 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0
+    return t if ok else t.contiguous()
+
+
+def write_tokens(k, v, slots, page_size, ka, kb, va, vb, ek, *, v_scale=1.0):
+    """Quantise `k`, `v` `(total, H_KV, D)` (bf16 or fp16) into the pool at
+    `slots`: the planes a prompt's write or a step's append puts there. `vb`
+    None is a bf16 V; `v_scale` is an 8-bit V's power of two. The slots are
+    distinct, each within the pool (or negative: skipped); two tokens of one
+    call in one slot would leave a mixture."""
+    if k.ndim != 3 or v.shape != k.shape or k.dtype not in _HALF or v.dtype != k.dtype:
+        raise ValueError(f"k and v are (total, H_KV, D) of one 16-bit type (got {k.dtype} {tuple(k.shape)}, {v.dtype} {tuple(v.shape)})")
+    n, HKV, D = k.shape
+    dev = k.device
+    if D not in (64, 128):
+        raise NotImplementedError(f"head_dim {D}: the cache takes 64 or 128")
+    if v.device != dev:
+        raise ValueError(f"k is on {dev}, v on {v.device}")
+    _int32("slots", slots, (n,), dev)
+    _planes(D, ka, kb, va, vb, ek, dev)
+    k, v = _rows(k), _rows(v)
+    with torch.cuda.device(dev):
+        _lib.call(
+            "fold_write_tokens", k.data_ptr(), v.data_ptr(), int(k.dtype == torch.float16), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+            slots.data_ptr(), n, HKV, D, int(page_size), ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb), ek.data_ptr(),
+            float(v_scale), _lib.stream(dev),
+        )
+
+
+def read_tokens(slots, page_size, n_kv_heads, ka, kb, va, vb, ek, *, v_scale=1.0, dtype=torch.bfloat16):
+    """The tokens at `slots` as the values their codes stand for: `(k, v)`, each
+    `(total, H_KV, D)` in `dtype` (float32, bfloat16 or float16, which
+    saturates), keys in their own basis. Slots may repeat; zeros at -1."""
+    if dtype not in _OUT:
+        raise ValueError(f"dtype is float32, bfloat16 or float16 (got {dtype})")
+    dev, D = ka.device, ka.shape[-1]
+    if D not in (64, 128):
+        raise NotImplementedError(f"head_dim {D}: the cache takes 64 or 128")
+    n, HKV = slots.shape[0], int(n_kv_heads)
+    _int32("slots", slots, (n,), dev)
+    _planes(D, ka, kb, va, vb, ek, dev)
+    k = torch.empty((n, HKV, D), device=dev, dtype=dtype)
+    v = torch.empty_like(k)
+    with torch.cuda.device(dev):
+        _lib.call(
+            "fold_read_tokens", slots.data_ptr(), n, HKV, D, int(page_size), ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb),
+            ek.data_ptr(), float(v_scale), k.data_ptr(), v.data_ptr(), _OUT[dtype], _lib.stream(dev),
+        )
+    return k, v
+
+
+def chunk_sums(v, cu_seqlens, lens_new, seq_lens, v_scale, vsum, vmean):
+    """The running V sums and means with a chunk's `v` added, and `seq_lens` set to `lens_new`."""
+    n, HKV, D = v.shape
+    v = _rows(v)
+    with torch.cuda.device(v.device):
+        _lib.call(
+            "fold_chunk_sums", v.data_ptr(), int(v.dtype == torch.float16), v.stride(0), v.stride(1), seq_lens.shape[0], HKV, D,
+            cu_seqlens.data_ptr(), n, lens_new.data_ptr(), seq_lens.data_ptr(), float(v_scale), vsum.data_ptr(), vmean.data_ptr(),
+            _lib.stream(v.device),
+        )
+
+
+def chunk_attention(q, cu_seqlens, max_new, cap_tiles, seq_lens, page_table, page_size, ka, kb, va, vb, ek, v_scale, n_kv_heads,
+                    window, sinks, softmax_scale):
+    """Attention of each request's last tokens over the pool: `q` `(total, H,
+    D)`, cut by `cu_seqlens`, at most `max_new` a request. `cap_tiles` is how many
+    128-key tiles the requests' visible keys fill, at most. Returns `(out, status)`."""
+    total, H, D = q.shape
+    dev, dt = q.device, q.dtype
+    B = seq_lens.shape[0]
+    out = torch.empty((total, H, D), device=dev, dtype=dt)
+    work = torch.zeros(1 + 4 * B + 2 * cap_tiles + 3, device=dev, dtype=torch.int32)
+    status, plan, tiles = work[:1], work[4:4 + 4 * B], work[4 + 4 * B:4 + 4 * B + 2 * cap_tiles]
+    rows = cap_tiles * 128
+    kw = torch.empty((2, n_kv_heads, rows, D), device=dev, dtype=dt)
+    vw = kw[1]
+    win = window or 1 << 30
+    f16 = int(dt == torch.float16)
+    strides = (ctypes.c_int64 * 12)(0, q.stride(0), q.stride(1), 0, D, rows * D, 0, D, rows * D, 0, out.stride(0), out.stride(1))
+    args = (q.data_ptr(), kw.data_ptr(), vw.data_ptr(), out.data_ptr(), None, ctypes.addressof(strides), cu_seqlens.data_ptr(), B, H,
+            n_kv_heads, max_new, total, D, f16, softmax_scale, win, sinks, plan.data_ptr(), rows)
+    with torch.cuda.device(dev):
+        _lib.call(
+            "fold_chunk_gather", cu_seqlens.data_ptr(), seq_lens.data_ptr(), B, page_table.data_ptr(), page_table.shape[1], int(page_size),
+            n_kv_heads, D, win, sinks, ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb), ek.data_ptr(), float(v_scale),
+            f16, cap_tiles, plan.data_ptr(), tiles.data_ptr(), kw.data_ptr(), vw.data_ptr(), status.data_ptr(), _lib.stream(dev),
+        )
+        if _lib.lib.fold_fwd_sm100_supported(D, f16):
+            _lib.call("fold_fwd_window_sm100", *args, status.data_ptr(), _lib.stream(dev))
+        else:
+            _lib.call("fold_fwd_window", *args, _lib.stream(dev))
+    return out, status

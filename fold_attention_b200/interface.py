@@ -166,23 +166,34 @@ def fold_attn_varlen_func(
     return _FoldAttnVarlenFunc.apply(q, k, v, cu, int(max_seqlen_q), scale, bool(causal), window or None, sinks)
 
 
-def fold_attn_with_kvcache(q, cache, k=None, v=None):
-    """Attention of one query token per request over `cache`.
+def fold_attn_with_kvcache(q, cache, k=None, v=None, cu_seqlens=None, lens=None):
+    """Attention of one query token per request over `cache`, or of a chunk of
+    new tokens per request.
 
     `q` is `(batch, nheads, headdim)` or `(batch, 1, nheads, headdim)`. With
     `k` and `v` (`(batch, nheads_k, headdim)`, or with the extra axis of 1)
     the token is appended first, so the query sees it. Returns the output in
     `q`'s shape and dtype.
+
+    With `cu_seqlens` (int32 `(batch + 1,)` on the device; `lens` the host's copy
+    of the counts, without which the call waits for the device) `q` is `(total,
+    nheads, headdim)`, each request's new tokens packed, and `k` and `v` `(total,
+    nheads_k, headdim)`: they are appended, and each query sees the keys up to its
+    own (`FoldKVCache.extend`). Without `k` and `v` the cache already holds them.
     """
+    if (k is None) != (v is None):
+        raise ValueError("k and v are both given or both left out")
+    if cu_seqlens is not None:
+        return cache.attend_chunk(q, cu_seqlens, lens) if k is None else cache.extend(q, k, v, cu_seqlens, lens)
+    if lens is not None:
+        raise ValueError("lens are the counts that cu_seqlens describes: give both")
     squeeze = q.ndim == 4
     if squeeze and q.shape[1] != 1:
         raise ValueError("fold_attn_with_kvcache takes one query token per request")
     if squeeze:
         q = q[:, 0]
-    if k is None and v is None:
+    if k is None:
         out = cache.attend(q)
-    elif k is not None and v is not None:
-        out = cache.decode(q, k[:, 0] if squeeze else k, v[:, 0] if squeeze else v)
     else:
-        raise ValueError("k and v are both given or both left out")
+        out = cache.decode(q, k[:, 0] if squeeze else k, v[:, 0] if squeeze else v)
     return out[:, None] if squeeze else out

@@ -16,7 +16,7 @@ import torch
 
 from .backward.launch import attention_forward
 from .decode import tail as tail_fit
-from .decode import write
+from .decode import tokens, write
 from .decode.heuristics import (
     pick_split,
     refine_bands_for,
@@ -25,7 +25,7 @@ from .decode.heuristics import (
     weight_terms_for,
 )
 from .decode.launch import mass_z, prepare_fold_decode
-from .utils import Launch
+from .utils import Launch, check_status, check_window
 
 
 class ReplayStep(Launch):
@@ -40,7 +40,11 @@ class FoldKVCache:
 
     `prefill` takes the prompts, packed, and returns their causal attention;
     `decode` appends one token per request and returns its attention over
-    everything so far (`append` and `attend` do the two halves).
+    everything so far (`append` and `attend` do the two halves). `extend`
+    appends any number of tokens per request and returns their causal attention
+    over everything so far (`append_chunk` and `attend_chunk` are its halves): a
+    prompt prefilled piece by piece, drafted tokens to verify, a batch in which
+    some requests prefill while others decode.
 
     `depth` is the truncation depth: a key whose weight is under `2^-depth`
     of its row's mass is dropped (its mass re-enters at V's mean), and None
@@ -76,6 +80,13 @@ class FoldKVCache:
     `check_range` reads each
     step's denominators on the host and reruns the rows whose reference sat
     outside `[0.5, 2^60]` (`2^100` on a bf16 V) of their mass.
+
+    `window` and `sinks` (not reference arguments) make it a sliding-window
+    layer's cache: a token at position i attends keys j with `i - window < j <= i`
+    or `j < sinks`, in `prefill`, `extend` and `decode` alike. Every key it sees
+    counts (`depth=None`), and its step runs the chunk's kernels. `pages` is
+    the size of a pool that the requests share: pages are handed out on the
+    device as requests grow, instead of `max_len` keys' worth to each.
     """
 
     SM100_MIN_KEYS = 2048    # requests shorter than this stay on the warp-level kernel under kernel="auto"
@@ -102,6 +113,9 @@ class FoldKVCache:
         chunk=None,
         device="cuda",
         kernel="auto",
+        window=None,
+        sinks=0,
+        pages=None,
     ):
         if n_heads % n_kv_heads:
             raise ValueError(f"{n_heads} query heads do not group over {n_kv_heads} KV heads")
@@ -115,6 +129,10 @@ class FoldKVCache:
         self.v_headroom = float(v_headroom)
         self.split = split
         self.device = torch.device(device)
+        window, self.sinks = check_window(window, sinks)
+        self.window = window or None
+        if window and depth is not None:
+            raise NotImplementedError("a windowed cache attends every key its window holds: depth=None")
         # the split-KV kernel (not a reference argument): "mma", "sm100" or "auto"
         self.kernel = kernel
         self.mix_kernels = False
@@ -132,9 +150,20 @@ class FoldKVCache:
             raise ValueError(f"page_size={page_size}: a multiple of 64, or 16 or 32")
 
         dev, D, HKV, PS = self.device, head_dim, n_kv_heads, page_size
-        pages = -(-max_len // PS)
-        rows = batch * pages * HKV * PS
-        self.page_table = torch.arange(batch * pages, device=dev, dtype=torch.int32).view(batch, pages)
+        per = -(-max_len // PS)
+        if pages is None:
+            pool = batch * per
+            self.page_table = torch.arange(pool, device=dev, dtype=torch.int32).view(batch, per)
+            self.free_pages = self.taken = None
+        else:
+            pool = int(pages)
+            if pool < 1:
+                raise ValueError(f"a pool of {pages} pages")
+            self.page_table = torch.zeros((batch, per), device=dev, dtype=torch.int32)
+            self.free_pages = torch.arange(pool, device=dev, dtype=torch.int32)
+            self.taken = torch.zeros(1, device=dev, dtype=torch.int32)
+        self.n_pages = pool
+        rows = pool * HKV * PS
         self.ka = torch.zeros((rows, D), device=dev, dtype=torch.int8)
         self.kb = torch.zeros_like(self.ka)
         if self.v8:
@@ -196,6 +225,7 @@ class FoldKVCache:
         # under `check_range` synchronise anyway and always check.
         self.check_status = False
         self._z_given = None
+        self._chunk_status = None      # the last chunk attention's device status word
         if chunk is not None and (split is not None or chunk % BN):
             raise ValueError(f"chunk={chunk} is a multiple of {BN} and replaces split")
         self.chunk = chunk
@@ -227,9 +257,10 @@ class FoldKVCache:
             raise ValueError(f"prompt lengths {min(lens)}..{max(lens)} are not in 1..{self.max_len}")
         if max_seqlen is None:
             max_seqlen = max(lens)
+        self._check_pool(lens)
         out, _ = attention_forward(
             q, k, v, causal=True, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen,
-            softmax_scale=1.0 / math.sqrt(self.head_dim),
+            softmax_scale=1.0 / math.sqrt(self.head_dim), window=self.window, sinks=self.sinks,
         )
         self.write_prompt(k, v, cu_seqlens, lens)
         return out
@@ -244,6 +275,10 @@ class FoldKVCache:
             raise ValueError(f"{len(lens)} prompts for a batch of {self.batch}")
         if min(lens) < 1 or max(lens) > self.max_len:
             raise ValueError(f"prompt lengths {min(lens)}..{max(lens)} are not in 1..{self.max_len}")
+        self._check_pool(lens)
+        if self.free_pages is not None:      # every page is free again: the prompts replace what there was
+            fresh = torch.zeros_like(self.seq_lens)
+            self._take_pages(self._cu(lens), fresh, 0, torch.zeros_like(self.taken))
         self._v_scale = write.write_prompt(
             k, v, lens, self.page_table, self.page_size, self.ka, self.kb, self.va, self.vb,
             self.ek, self.vsum, self.vmean, v_headroom=self.v_headroom,
@@ -298,24 +333,166 @@ class FoldKVCache:
 
     def append(self, k, v):
         """Write one token per request, `(batch, H_KV, D)` each, at its length."""
-        if max(self.lens) >= self.max_len:
-            raise ValueError(f"a request is at max_len={self.max_len}")
+        self._room_for_one()
         self._step(None, k, v)
         self.lens = [x + 1 for x in self.lens]
 
     def attend(self, q, split=None):
         """Attention of `q` `(batch, H, D)` over the cache as it stands."""
+        if self.window:
+            return self._attend_last(q)
         self._step(q, None, None)
         return self._run(q, split)
 
     def decode(self, q, k, v, split=None):
         """One decode step: append `k`, `v` `(batch, H_KV, D)` and attend with
         `q` `(batch, H, D)`."""
-        if max(self.lens) >= self.max_len:
-            raise ValueError(f"a request is at max_len={self.max_len}")
+        self._room_for_one()
+        if self.window:
+            if q.shape != (self.batch, self.n_heads, self.head_dim):
+                raise ValueError(f"q is ({self.batch}, {self.n_heads}, {self.head_dim})")
+            self._step(None, k, v)
+            self.lens = [x + 1 for x in self.lens]
+            return self._attend_last(q)
         self._step(q, k, v)
         self.lens = [x + 1 for x in self.lens]
         return self._run(q, split)
+
+    # ---- any number of tokens per request ----
+
+    def extend(self, q, k, v, cu_seqlens, lens=None):
+        """Append each request's new tokens and attend with them.
+
+        `q` is `(total, H, D)`, `k` and `v` `(total, H_KV, D)`, packed by
+        `cu_seqlens` `(batch + 1,)` int32 on the device; a request may bring none.
+        Token i of a request sees the cache's keys up to and with its own (and of
+        those its window). `lens` are the host's copy of the counts that
+        `cu_seqlens` describes: without them the call reads `cu_seqlens` back,
+        which waits for the device. Returns `(total, H, D)` in q's dtype.
+
+        Captured in a CUDA graph (with `lens`), each replay appends and attends at the
+        lengths the device then holds, up to `max_len`: call `sync_lens` before
+        the next eager call. A shared pool's pages are taken by the replays too.
+        """
+        lens = self._chunk_lens(cu_seqlens, lens)
+        self._check_chunk_q(q, lens)     # before anything is written
+        self.append_chunk(k, v, cu_seqlens, lens)
+        return self.attend_chunk(q, cu_seqlens, lens)
+
+    def append_chunk(self, k, v, cu_seqlens, lens=None):
+        """`extend`'s first half: the new tokens quantised into the cache, in the
+        format of a prompt's, and the lengths moved. An 8-bit V keeps the scale
+        of the prompt, or the one the cache was given."""
+        lens = self._chunk_lens(cu_seqlens, lens)
+        total = sum(lens)
+        shape = (total, self.n_kv_heads, self.head_dim)
+        if k.shape != shape or v.shape != shape or k.dtype not in (torch.bfloat16, torch.float16) or v.dtype != k.dtype:
+            raise ValueError(f"k and v are {shape} of one 16-bit type (got {k.dtype} {tuple(k.shape)}, {v.dtype} {tuple(v.shape)})")
+        if k.device != self.seq_lens.device or v.device != self.seq_lens.device:
+            raise ValueError(f"k and v are on {k.device} and {v.device}, the cache on {self.seq_lens.device}")
+        if self.tail is not None:
+            raise NotImplementedError("the decode tail's block rows are kept one token at a time: a cache that takes chunks has tail=None")
+        after = [a + n for a, n in zip(self.lens, lens)]
+        if max(after) > self.max_len:
+            raise ValueError(f"a request would hold {max(after)} tokens, max_len={self.max_len}")
+        self._check_pool(after)
+        if total == 0:
+            return
+        slots, lens_new = self._take_pages(cu_seqlens, self.seq_lens, total)
+        tokens.write_tokens(k, v, slots, self.page_size, self.ka, self.kb, self.va, self.vb, self.ek, v_scale=self.v_scale)
+        tokens.chunk_sums(v, cu_seqlens, lens_new, self.seq_lens, self.v_scale, self.vsum, self.vmean)
+        self.lens = after
+
+    def attend_chunk(self, q, cu_seqlens, lens=None):
+        """`extend`'s second half: attention of the last tokens of each request,
+        which the cache already holds, over the cache. `q` `(total, H, D)` packed by
+        `cu_seqlens`, as many rows of a request as it has tokens at most. Every
+        key counts in full, whatever the cache's `depth`: both planes of K and of
+        an 8-bit V. fp16 queries see K and V saturated to fp16's range."""
+        lens = self._chunk_lens(cu_seqlens, lens)
+        self._check_chunk_q(q, lens)
+        if any(n > a for n, a in zip(lens, self.lens)):
+            raise ValueError("a request has more query rows than tokens in the cache")
+        if sum(lens) == 0:
+            return torch.empty_like(q)
+        q = tokens._rows(q)
+        # a captured call is replayed on longer requests: it is laid out for the longest there can be
+        capturing = torch.cuda.is_current_stream_capturing()
+        cap = 0
+        for n, a in zip(lens, self.lens):
+            if capturing:
+                cap += -(-self.max_len // 128)
+            elif n:
+                first = max(0, a - n - (self.window or a) + 1) // 128
+                cap += -(-a // 128) - max(0, first - -(-self.sinks // 128))
+        out, self._chunk_status = tokens.chunk_attention(
+            q, cu_seqlens, q.shape[0] if capturing else max(lens), cap, self.seq_lens, self.page_table, self.page_size, self.ka, self.kb, self.va,
+            self.vb, self.ek, self.v_scale, self.n_kv_heads, self.window, self.sinks, 1.0 / math.sqrt(self.head_dim),
+        )
+        if self.check_range or self.check_status:
+            check_status(self._chunk_status, "attend_chunk")
+        return out
+
+    def sync_lens(self):
+        """Read the lengths back from the device. A captured step moves them there
+        on every replay; the host's copy, which the next eager call plans by, does
+        not follow by itself."""
+        self.lens = self.seq_lens.tolist()
+
+    def _attend_last(self, q):
+        """A windowed layer's step: each request's newest token."""
+        if q.shape != (self.batch, self.n_heads, self.head_dim):
+            raise ValueError(f"q is ({self.batch}, {self.n_heads}, {self.head_dim})")
+        cu = torch.arange(self.batch + 1, device=self.seq_lens.device, dtype=torch.int32)
+        return self.attend_chunk(q, cu, [1] * self.batch)
+
+    def _cu(self, lens):
+        out = [0]
+        for n in lens:
+            out.append(out[-1] + n)
+        return torch.tensor(out, dtype=torch.int32).to(self.seq_lens.device, non_blocking=True)
+
+    def _chunk_lens(self, cu_seqlens, lens):
+        if cu_seqlens.dtype != torch.int32 or cu_seqlens.shape != (self.batch + 1,) or cu_seqlens.device != self.seq_lens.device:
+            raise ValueError(f"cu_seqlens is int32 ({self.batch + 1},) on {self.seq_lens.device}")
+        if lens is None:
+            lens = torch.diff(cu_seqlens).tolist()
+        lens = [int(n) for n in lens]
+        if len(lens) != self.batch or min(lens) < 0:
+            raise ValueError(f"{len(lens)} counts, the least {min(lens, default=0)}, for a batch of {self.batch}")
+        return lens
+
+    def _check_chunk_q(self, q, lens):
+        if q.shape != (sum(lens), self.n_heads, self.head_dim) or q.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"q is ({sum(lens)}, {self.n_heads}, {self.head_dim}) bf16 or fp16 (got {q.dtype} {tuple(q.shape)})")
+        if q.device != self.seq_lens.device:
+            raise ValueError(f"q is on {q.device}, the cache on {self.seq_lens.device}")
+
+    def _check_pool(self, lens):
+        """Whether a shared pool holds requests of these lengths."""
+        if self.free_pages is not None:
+            need = sum(-(-n // self.page_size) for n in lens)
+            if need > self.n_pages:
+                raise ValueError(f"the requests would need {need} pages, the pool has {self.n_pages}")
+
+    def _take_pages(self, cu_seqlens, seq_lens, total, taken=None):
+        """The new tokens' slots and the lengths with them; a shared pool's pages are handed out first."""
+        slots, lens, used = tokens.build_tables(
+            cu_seqlens, seq_lens, self.page_table, self.page_size, total, free_pages=self.free_pages,
+            taken=(self.taken if taken is None else taken) if self.free_pages is not None else None)
+        if used is not None:
+            self.taken.copy_(used)
+        return slots, lens
+
+    def _room_for_one(self):
+        """A page for every request's next token."""
+        if max(self.lens) >= self.max_len:
+            raise ValueError(f"a request is at max_len={self.max_len}")
+        if self.free_pages is not None:
+            self._check_pool([n + 1 for n in self.lens])
+            if any(n % self.page_size == 0 for n in self.lens) or torch.cuda.is_current_stream_capturing():
+                cu = torch.arange(self.batch + 1, device=self.seq_lens.device, dtype=torch.int32)
+                self._take_pages(cu, self.seq_lens, 0)
 
     # ---- replay and tuning helpers (src/fold_attention/kv_cache.py:441-570) ----
 
@@ -325,6 +502,7 @@ class FoldKVCache:
         and partial buffers are its own, so replaying it leaves the layer's
         state untouched. `out_dtype` is the output it writes, so a benchmark
         times the launch it scores. Returns the launch (`(out, den, counts)`)."""
+        self._no_window("prepare_replay_decode")
         split = self._resolve_split(split)
         refine = self._refine()
         truncate = self.depth is not None
@@ -351,6 +529,9 @@ class FoldKVCache:
         and the Q planes are rewritten, with the same values every time."""
         if (k is None) != (v is None):
             raise ValueError("k and v are both given or both left out")
+        self._no_window("prepare_replay_step")
+        if self.free_pages is not None and k is not None:
+            raise NotImplementedError("a replayed step that appends has no page of a shared pool to append to: pages=None")
         qf = q.reshape(-1, self.head_dim)
         at = (self.seq_lens if at is None else at).clone()
         appends = k is not None
@@ -420,6 +601,7 @@ class FoldKVCache:
         not what is timed), in rotating order across `rounds` so a drifting
         clock cancels; the replays write only buffers of their own. Returns
         `{split: us}`."""
+        self._no_window("tune_split")
         if self.chunk is not None:
             raise ValueError("a fixed chunk sets the split: there is nothing to tune")
         tiles = -(-(sum(self.lens) // self.batch) // BN)
@@ -457,6 +639,10 @@ class FoldKVCache:
         return med
 
     # ---- internals -------------------------------------------------------
+
+    def _no_window(self, what):
+        if self.window:
+            raise NotImplementedError(f"{what} runs the decode over whole requests: a windowed cache's step is attend_chunk's")
 
     def _set_order(self):
         """Which row group each grid slot takes; it changes no bit. Without a

@@ -34,6 +34,52 @@ extern "C" {
 const char* fold_last_error(void);
 int fold_abi_version(void);
 
+/* ---- the paged cache a piece at a time --------------------------------------
+ * No counterpart in the reference, which appends one token a request and whose tables are the
+ * host's. A token's slot is page * page_size + offset, the same for every KV head and every layer
+ * that shares the table; -1 stands for no place: writers skip it, readers return zeros. */
+
+/* Block tables and the new tokens' slots from request lengths. Request b holds seq_lens[b] tokens
+ * and brings cu_seqlens[b + 1] - cu_seqlens[b] more. With free_pages (n_free page numbers, of which
+ * the first *taken are in use) the pages it grows by are taken in request order and written to its
+ * row of page_table; without, the table stands. slots[total] gets each new token's slot (-1 past the
+ * table's end, where the pool ran out, and for rows no request covers), lens_out[b] the lengths
+ * moved, *taken_out the pages then in use (beyond n_free: the pool ran out). The outputs are other
+ * tensors than the inputs. */
+int fold_build_tables(const int32_t* cu_seqlens, const int32_t* seq_lens, int batch, int32_t* page_table,
+                      int pages_per_request, int page_size, int total, const int32_t* free_pages, int n_free,
+                      const int32_t* taken, int32_t* slots, int32_t* lens_out, int32_t* taken_out, void* stream);
+
+/* `total` tokens quantised into the pool at their slots (distinct ones): the planes fold_step_append
+ * would write. k, v (total, n_kv_heads, head_dim) 16-bit with element strides; vb NULL for a bf16 V. */
+int fold_write_tokens(const void* k, const void* v, int is_f16, int64_t k_token_stride, int64_t k_head_stride,
+                      int64_t v_token_stride, int64_t v_head_stride, const int32_t* slots, int64_t total,
+                      int n_kv_heads, int head_dim, int page_size, int8_t* ka, int8_t* kb, void* va, void* vb,
+                      void* ek, float v_scale, void* stream);
+
+/* The tokens at `slots` as the values their codes stand for, keys in their own basis: k, v
+ * (total, n_kv_heads, head_dim) fp32 (out_dtype 0), bf16 (1) or fp16 (2, saturating). */
+int fold_read_tokens(const int32_t* slots, int64_t total, int n_kv_heads, int head_dim, int page_size,
+                     const int8_t* ka, const int8_t* kb, const void* va, const void* vb, const void* ek,
+                     float v_scale, void* k, void* v, int out_dtype, void* stream);
+
+/* A chunk's share of the running V sums and means (fp32 (batch * n_kv_heads, head_dim)), and the
+ * lengths moved: lens[b] = lens_new[b]. Every element of v counts once, in an order of the chunk's own. */
+int fold_chunk_sums(const void* v, int is_f16, int64_t v_token_stride, int64_t v_head_stride, int batch,
+                    int n_kv_heads, int head_dim, const int32_t* cu_seqlens, int total, const int32_t* lens_new,
+                    int32_t* lens, float v_scale, float* vsum, float* vmean, void* stream);
+
+/* The keys and values that the last cu_seqlens[b + 1] - cu_seqlens[b] tokens of each request can see,
+ * as 16-bit rows for fold_fwd_window: whole tiles of 128 keys, requests one after another, zeros past
+ * a request's end. kw, vw [n_kv_heads][cap_tiles * 128][head_dim] in bf16, or fp16 (is_f16,
+ * saturating); plan int32[4 * batch]; tiles int32[2 * cap_tiles]. Requests that do not fit cap_tiles
+ * see no key and raise *status (FOLD_ERR_ARGUMENT). */
+int fold_chunk_gather(const int32_t* cu_seqlens, const int32_t* seq_lens, int batch, const int32_t* page_table,
+                      int pages_per_request, int page_size, int n_kv_heads, int head_dim, int window, int sinks,
+                      const int8_t* ka, const int8_t* kb, const void* va, const void* vb, const void* ek,
+                      float v_scale, int is_f16, int cap_tiles, int32_t* plan, int32_t* tiles, void* kw, void* vw,
+                      int32_t* status, void* stream);
+
 /* ---- Path B: cache writes ------------------------------------------------ */
 
 /* Quantise packed prompts into the paged cache.
@@ -390,21 +436,21 @@ int fold_fwd_run_sm100(const void* q, const void* k, const void* v, void* o, flo
 
 /* The causal forward under a sliding window with sinks, on the warp-level and on the tcgen05
  * kernel: the query at position i sees key j when j <= i and (i - j < window or j < sinks).
- * Arguments as fold_fwd_run / fold_fwd_run_sm100. With key_lens (int32[batch] on the device) the
- * keys and values are request b's own key_lens[b] rows of (batch, row, head) tensors of key_rows
- * rows a request, the queries are the request's last positions (cu_seqlens cuts q and o alone),
+ * Arguments as fold_fwd_run / fold_fwd_run_sm100. With `plan` (fold_chunk_gather's) the keys and
+ * values are the rows it laid out, (key_rows, head) tensors whose batch strides are not used, the
+ * queries are each request's last positions (cu_seqlens, which must be given, cuts q and o alone)
  * and lse may be NULL. A row that sees no key gets zeros and an lse of -infinity. A window that no
  * sequence fills is plain causal attention. No counterpart in the reference. */
 int fold_fwd_window(const void* q, const void* k, const void* v, void* o, float* lse,
                     const int64_t* strides /* host */, const int32_t* cu_seqlens, int batch,
                     int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim, int is_f16,
-                    float softmax_scale, int window, int sinks, const int32_t* key_lens, int key_rows,
+                    float softmax_scale, int window, int sinks, const int32_t* plan, int key_rows,
                     void* stream);
 int fold_fwd_window_sm100(const void* q, const void* k, const void* v, void* o, float* lse,
                           const int64_t* strides /* host */, const int32_t* cu_seqlens, int batch,
                           int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim,
                           int is_f16, float softmax_scale, int window, int sinks,
-                          const int32_t* key_lens, int key_rows, int32_t* status, void* stream);
+                          const int32_t* plan, int key_rows, int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

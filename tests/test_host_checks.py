@@ -127,3 +127,85 @@ def test_a_windowed_backward_takes_no_plan():
     x = torch.zeros(1, 2, 8, 64, dtype=torch.bfloat16)
     with pytest.raises(NotImplementedError, match="plan"):
         prepare_backward(x, x, x, x, x, torch.zeros(1, 2, 8), causal=True, window=4, plan=Plan(1, 0))
+
+
+def _cpu_cache(**kw):
+    import fold_attention_b200 as fa
+
+    return fa.FoldKVCache(2, 4, 2, 64, 96, page_size=16, device="cpu", **kw)
+
+
+@pytest.mark.parametrize("kw,error,match", [
+    (dict(window=0), ValueError, "window"), (dict(sinks=2), ValueError, "window"), (dict(window=8, sinks=-1), ValueError, "window"),
+    (dict(window=8, depth=12.0), NotImplementedError, "depth=None"), (dict(pages=0), ValueError, "pool"),
+])
+def test_a_cache_refuses_windows_and_pools_that_mean_nothing(kw, error, match):
+    with pytest.raises(error, match=match):
+        _cpu_cache(**kw)
+
+
+def test_chunks_are_checked_before_anything_is_written():
+    bf = torch.bfloat16
+    c = _cpu_cache(pages=7)
+    cu = torch.tensor([0, 3, 5], dtype=torch.int32)
+    q, k = torch.zeros(5, 4, 64, dtype=bf), torch.zeros(5, 2, 64, dtype=bf)
+    for bad in (cu.long(), cu[:2]):
+        with pytest.raises(ValueError, match="cu_seqlens"):
+            c.extend(q, k, k, bad, [3, 2])
+    for lens in ([3], [6, -1]):
+        with pytest.raises(ValueError, match="counts"):
+            c.extend(q, k, k, cu, lens)
+    for bad in (q[:4], q.float(), q[:, :2], q[..., :32]):
+        with pytest.raises(ValueError, match="q is"):
+            c.extend(bad, k, k, cu, [3, 2])
+    for bk, bv in ((k[:4], k), (k, k[:, :1]), (k, k.half()), (k.float(), k.float())):
+        with pytest.raises(ValueError, match="k and v"):
+            c.extend(q, bk, bv, cu, [3, 2])
+    with pytest.raises(ValueError, match="more query rows"):
+        c.attend_chunk(q, cu, [3, 2])
+    long = torch.zeros(97, 2, 64, dtype=bf)
+    with pytest.raises(ValueError, match="max_len"):
+        c.append_chunk(long, long, torch.tensor([0, 97, 97], dtype=torch.int32), [97, 0])
+    with pytest.raises(ValueError, match="pool has 7"):
+        c.append_chunk(torch.cat((long, long))[:120], torch.cat((long, long))[:120], torch.tensor([0, 60, 120], dtype=torch.int32), [60, 60])
+    assert c.lens == [0, 0]
+    t = _cpu_cache(depth=8.0, tail=None)
+    assert t.tail is None
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        import fold_attention_b200 as fa
+
+        fa.fold_attn_with_kvcache(q, c, lens=[3, 2])
+    for call in (lambda c: c.prepare_replay_decode(), lambda c: c.tune_split(), lambda c: c.prepare_replay_step(q)):
+        with pytest.raises(NotImplementedError, match="windowed"):
+            call(_cpu_cache(window=8))
+
+
+def test_tables_and_tokens_are_checked():
+    from fold_attention_b200 import decode
+
+    i32 = torch.int32
+    cu, lens, table = torch.zeros(3, dtype=i32), torch.zeros(2, dtype=i32), torch.zeros(2, 4, dtype=i32)
+    one = torch.zeros(1, dtype=i32)
+    for args, kw in (
+        ((cu.long(), lens, table, 16, 0), {}), ((cu[:2], lens, table, 16, 0), {}), ((cu, lens, table.t(), 16, 0), {}),
+        ((cu, lens, table, 0, 0), {}), ((cu, lens, table, 16, -1), {}), ((cu, lens, table, 16, 0), dict(free_pages=one)),
+        ((cu, lens, table, 16, 0), dict(free_pages=one, taken=torch.zeros(2, dtype=i32))), ((cu, lens[:0], table[:0], 16, 0), {}),
+    ):
+        with pytest.raises(ValueError):
+            decode.build_tables(*args, **kw)
+    ka = torch.zeros(32, 64, dtype=torch.int8)
+    va, ek = torch.zeros(32, 64, dtype=torch.bfloat16), torch.zeros(32, dtype=torch.bfloat16)
+    k, slots = torch.zeros(5, 2, 64, dtype=torch.bfloat16), torch.zeros(5, dtype=i32)
+    for bad in (dict(k=k.float()), dict(k=k[:4]), dict(slots=slots.long()), dict(slots=slots[:4]), dict(ka=ka[:16]), dict(va=va.half()),
+                dict(ek=ek.float()), dict(vb=va)):
+        a = dict(k=k, v=k, slots=slots, page_size=16, ka=ka, kb=ka, va=va, vb=None, ek=ek)
+        a.update(bad)
+        with pytest.raises(ValueError):
+            decode.write_tokens(**a)
+    with pytest.raises(NotImplementedError, match="head_dim"):
+        decode.write_tokens(k[..., :32], k[..., :32], slots, 16, ka, ka, va, None, ek)
+    for bad in (dict(dtype=torch.int8), dict(slots=slots.long()), dict(ka=ka.float()), dict(ek=ek[:8])):
+        a = dict(slots=slots, page_size=16, n_kv_heads=2, ka=ka, kb=ka, va=va, vb=None, ek=ek)
+        a.update(bad)
+        with pytest.raises(ValueError):
+            decode.read_tokens(**a)
