@@ -246,22 +246,26 @@ __global__ void __launch_bounds__(16 * D / 4) chunk_sums_kernel(const uint16_t* 
 // are laid out in whole tiles of 128 keys, requests one after another: [KV head][row][channel].
 //
 // chunk_plan_kernel (one CTA) lays them out: plan[b] = (keys, first row, tiles left out between the
-// sinks' tiles and the window's, 0), and for each 128-row tile (request, tile in the request).
+// sinks' tiles and the window's, last position before the first query's window); keys -1: the request is
+// another kernel's; and for each 128-row tile (request, tile in the request).
 constexpr int CP_THREADS = 256;
 __global__ void __launch_bounds__(CP_THREADS) chunk_plan_kernel(const int* __restrict__ cu, const int* __restrict__ lens, int batch, int max_keys,
-                                                                int window, int sinks, int cap_tiles, int4* plan, int2* tiles, int* status) {
+                                                                int window, int sinks, int rows_over, int group, int cap_tiles, int4* plan, int2* tiles, int* status) {
     __shared__ int s_warp[CP_THREADS / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ns = (sinks + 127) / 128;
     int base = 0;
     for (int b0 = 0; b0 < batch; b0 += CP_THREADS) {
         const int b = b0 + tid;
-        int klen = 0, shift = 0, nt = 0;
+        int klen = 0, shift = 0, nt = 0, before = -1;
         if (b < batch) {
             const int n = cu[b + 1] - cu[b], len = lens[b];
-            if (n > 0 && len > 0) {
+            if (static_cast<int64_t>(n) * group <= rows_over) {
+                klen = -1;                     // another kernel's
+            } else if (n > 0 && len > 0) {
                 klen = min(len, max_keys);
-                const int low = max(0, len - n - window + 1) / 128;
+                before = len - n - window;
+                const int low = max(0, before + 1) / 128;
                 shift = max(0, low - ns);
                 nt = max(0, (klen + 127) / 128 - shift);
             }
@@ -283,7 +287,7 @@ __global__ void __launch_bounds__(CP_THREADS) chunk_plan_kernel(const int* __res
             const int first = add + x - nt;
             const bool fits = first + nt <= cap_tiles;
             if (!fits) atomicExch(status, FOLD_ERR_ARGUMENT);   // lengths the host did not plan for: the request sees nothing
-            plan[b] = make_int4(fits ? klen : 0, first * 128, shift, 0);
+            plan[b] = make_int4(fits || klen < 0 ? klen : 0, first * 128, shift, before);
         }
         base += sum;
         __syncthreads();
@@ -303,7 +307,7 @@ __global__ void __launch_bounds__(CP_THREADS) chunk_plan_kernel(const int* __res
 
 template <int D, bool V8, int OUT>
 __global__ void __launch_bounds__(NT) chunk_gather_kernel(const int4* __restrict__ plan, const int2* __restrict__ tiles,
-                                                          const int* __restrict__ table, int ppr, int page_size, int hkv, const Planes p,
+                                                          const int* __restrict__ table, int ppr, int page_size, int hkv, int sinks, const Planes p,
                                                           int64_t rows, uint16_t* kw, uint16_t* vw) {
     constexpr int TPR = D / 16, RPB = NT / TPR, PER = 128 / RPB;
     const int g = blockIdx.x / PER, h = blockIdx.y;
@@ -312,7 +316,10 @@ __global__ void __launch_bounds__(NT) chunk_gather_kernel(const int4* __restrict
     const int lane = threadIdx.x % TPR;
     const int r = blockIdx.x % PER * RPB + threadIdx.x / TPR;
     const int pos = tl.y * 128 + r;
-    const bool ok = pos < plan[tl.x].x;     // rows past the request's end are zeros: whatever the pool holds there
+    // rows that no query sees (past the request's end, before its first query's window) are zeros, whatever
+    // the pool holds there: their weights are 0, but 0 times a NaN is not
+    const int4 pl = plan[tl.x];
+    const bool ok = pos < pl.x && (pos > pl.w || pos < sinks);
     int64_t prow = 0;
     int off = 0;
     if (ok) {
@@ -421,16 +428,17 @@ extern "C" int fold_chunk_sums(const void* v, int is_f16, int64_t v_token_stride
 
 extern "C" int fold_chunk_gather(const int32_t* cu_seqlens, const int32_t* seq_lens, int batch, const int32_t* page_table, int pages_per_request,
                                  int page_size, int n_kv_heads, int head_dim, int window, int sinks, const int8_t* ka, const int8_t* kb, const void* va,
-                                 const void* vb, const void* ek, float v_scale, int is_f16, int cap_tiles, int32_t* plan, int32_t* tiles, void* kw,
+                                 const void* vb, const void* ek, float v_scale, int is_f16, int rows_over, int group, int cap_tiles, int32_t* plan, int32_t* tiles, void* kw,
                                  void* vw, int32_t* status, void* stream) {
     FOLD_CHECK_ARG(head_dim == 64 || head_dim == 128, "head_dim %d: the cache holds 64 or 128", head_dim);
     FOLD_CHECK_ARG(cu_seqlens && seq_lens && page_table && ka && kb && va && ek && plan && tiles && kw && vw && status, "fold_chunk_gather: null pointer");
-    FOLD_CHECK_ARG(batch > 0 && n_kv_heads > 0 && n_kv_heads <= 65535 && pages_per_request > 0 && page_size > 0 && cap_tiles > 0 && cap_tiles <= (1 << 24),
+    FOLD_CHECK_ARG(batch > 0 && n_kv_heads > 0 && n_kv_heads <= 65535 && pages_per_request > 0 && page_size > 0 && cap_tiles > 0 && cap_tiles <= (1 << 24) &&
+                       rows_over >= 0 && group > 0,
                    "fold_chunk_gather: %d requests, %d heads, %d pages of %d keys, %d tiles", batch, n_kv_heads, pages_per_request, page_size, cap_tiles);
     FOLD_CHECK_ARG(window > 0 && window <= FOLD_MAX_WINDOW && sinks >= 0 && sinks <= FOLD_MAX_WINDOW, "fold_chunk_gather: a window of %d keys and %d sinks", window, sinks);
     const int64_t cap = static_cast<int64_t>(pages_per_request) * page_size;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    chunk_plan_kernel<<<1, CP_THREADS, 0, st>>>(cu_seqlens, seq_lens, batch, static_cast<int>(cap < (1 << 30) ? cap : (1 << 30)), window, sinks, cap_tiles,
+    chunk_plan_kernel<<<1, CP_THREADS, 0, st>>>(cu_seqlens, seq_lens, batch, static_cast<int>(cap < (1 << 30) ? cap : (1 << 30)), window, sinks, rows_over, group, cap_tiles,
                                                 reinterpret_cast<int4*>(plan), reinterpret_cast<int2*>(tiles), status);
     const Planes p = {ka, kb, static_cast<const uint16_t*>(ek), static_cast<const uint8_t*>(va), static_cast<const uint8_t*>(vb), v_scale};
     const int rpb = NT / (head_dim / 16);
@@ -438,7 +446,7 @@ extern "C" int fold_chunk_gather(const int32_t* cu_seqlens, const int32_t* seq_l
     const int64_t rows = static_cast<int64_t>(cap_tiles) * 128;
 #define FOLD_CG(DD, VV, OO)                                                                                                                  \
     chunk_gather_kernel<DD, VV, OO><<<grid, NT, 0, st>>>(reinterpret_cast<const int4*>(plan), reinterpret_cast<const int2*>(tiles), page_table, \
-        pages_per_request, page_size, n_kv_heads, p, rows, static_cast<uint16_t*>(kw), static_cast<uint16_t*>(vw))
+        pages_per_request, page_size, n_kv_heads, sinks, p, rows, static_cast<uint16_t*>(kw), static_cast<uint16_t*>(vw))
     if (head_dim == 64) {
         if (vb) { if (is_f16) FOLD_CG(64, true, OUT_F16); else FOLD_CG(64, true, OUT_BF16); }
         else    { if (is_f16) FOLD_CG(64, false, OUT_F16); else FOLD_CG(64, false, OUT_BF16); }

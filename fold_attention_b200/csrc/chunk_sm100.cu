@@ -1,0 +1,895 @@
+// Attention of a few new tokens per request over the paged, quantised cache: each KV head's query
+// rows (new tokens x query heads of the group, 128 at most) meet every key the request's window
+// holds, straight from the pool's codes. Bytes bound it (a key is 4 D + 2 of them, and a row group
+// does at most 128 rows' work with it), so the codes are what travels and nothing is written back but O.
+//
+//   S1 = Qa Ka^T, S2 = Qa Kb^T + Qb Ka^T    tcgen05.mma kind::i8, M=128 rows, N=128 keys, on the planes as
+//                stored (their XOR swizzle is the tensor core's), exact int32 in TMEM
+//   logit = (256 S1 + S2) ek (eq / 256)     the query's planes as a decode step's (16 bits of its largest); the
+//                product of the two second planes, under 2^-16 of the largest logit, is left out
+//   P  = exp2(logit - m)                    per row, written as 16-bit to TMEM (fp16 queries on a bf16 V: as two
+//                bf16 terms, or P would be 8 bits where the output has 11); a row's reference m moves only when
+//                the row's maximum passes it by more than 2^8
+//   O += P V     kind::f16, A = P from TMEM, B = V (MN-major): a bf16 V as TMA lays it down; an 8-bit V's two
+//                planes converted to fp16 in shared memory, where a + b / 8 fits but for its last bits
+//
+// Few rows would leave most of the 128 TMEM lanes, and three of the four softmax warps, without work:
+// a group of up to 32 (64) rows is stacked four (two) times, each copy's warp takes a quarter (half)
+// of a tile's keys, with zeros in P for the others, and the copies' sums meet in the epilogue.
+//
+// Work is one list of 128-key tiles, request by request and head by head, cut evenly over one
+// persistent CTA per SM: a (request, head) spans neighbouring CTAs at most where their ranges meet.
+// Each leaves its piece (m, l, O) in the workspace and the last to arrive adds the pieces in list
+// order, so the bits do not depend on who that is.
+//
+// Warps: 0 K producer (both planes, scales), 3 V producer, 1 MMA issuer, 2 V's dead rows (bf16 V),
+// 4-7 Q, softmax and epilogue, 8-11 V's conversion (8-bit V). Every wait is bounded.
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "cache_common.cuh"
+#include "fold_b200.h"
+
+namespace fold {
+namespace csm100 {
+
+constexpr int BN = 128;
+constexpr long long WAIT_CYCLES = 1ll << 31;
+constexpr float LAZY = 8.0f;
+constexpr int MIN_TILES = 4;     // tiles a CTA takes at least: its fixed costs are two or three tiles' time
+
+template <int D, bool V8>
+struct Lay {
+    static constexpr int PLANE = 128 * D;                  // a tile of one 8-bit plane
+    static constexpr int NK = D == 128 ? 3 : 6, NV = D == 128 ? (V8 ? 2 : 3) : 5;
+    static constexpr int KSLOT = 2 * PLANE, VSLOT = 2 * PLANE;
+    static constexpr int SM_Q = 0;                         // plane A, plane B; between items the copies' sums
+    static constexpr int SM_V16 = 2 * PLANE;               // the converted tile (8-bit V)
+    static constexpr int SM_K = SM_V16 + (V8 ? 2 * PLANE : 0);
+    static constexpr int SM_V = SM_K + NK * KSLOT;
+    static constexpr int SM_EK = SM_V + NV * VSLOT;        // [NK][128] bf16
+    static constexpr int SM_ROW = SM_EK + NK * 256;        // eq, m, l [128] f32
+    static constexpr int SM_BAR = SM_ROW + 3 * 512;
+    static constexpr int SM_MISC = SM_BAR + 256;           // scan [12], walk [4], flags [2], TMEM address
+    static constexpr int USED = SM_MISC + 128;
+    static constexpr int SLACK = 232448 - USED < 1024 ? 232448 - USED : 1024;   // room to align the base
+    static constexpr int BYTES = USED + SLACK;
+    static constexpr int NTHREADS = V8 ? 384 : 256;
+    static_assert(SLACK >= 0, "shared memory");
+};
+
+// barriers: [6] K slots, [5] V slots, then one each
+enum { B_KFULL = 0, B_KEMPTY = 6, B_VFULL = 12, B_VEMPTY = 17, B_VREADY = 22, B_SFULL = 27, B_SEMPTY = 28, B_PREADY = 29, B_ODONE = 30, B_QREADY = 31 };
+
+constexpr uint32_t T_S1 = 0, T_S2 = 128, T_P = 256, T_P2 = 320, T_O = 384;   // TMEM columns: 128, 128, 64, 64, D
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// Bounded wait: `abort` (shared) is raised by whoever runs out first, and then nobody waits any more.
+__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status) {
+    if (mbar_try(bar, parity)) return;
+    if (*abort_flag) return;
+    const long long t0 = clock64();
+    for (int i = 0;; ++i) {
+        if (mbar_try(bar, parity)) return;
+        if ((i & 63) == 63) {
+            if (*abort_flag) return;
+            if (clock64() - t0 > WAIT_CYCLES) break;
+        }
+    }
+    *abort_flag = 1;
+    atomicExch(status, FOLD_ERR_TIMEOUT);
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p; }"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+                   "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+                   "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2f(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ float4 as_float4(uint4 v) {
+    return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
+__device__ __forceinline__ uint4 as_uint4(float4 v) {
+    return make_uint4(__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w));
+}
+// shared-memory matrix descriptor; layout 2 = 128-byte swizzle, 4 = 64-byte
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo, uint32_t layout) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((addr & 0x3FFFF) >> 4);
+    d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFF) << 16;
+    d |= static_cast<uint64_t>((sbo >> 4) & 0x3FFF) << 32;
+    d |= 1ull << 46;
+    d |= static_cast<uint64_t>(layout) << 61;
+    return d;
+}
+// instruction descriptor: c_fmt (1 f32, 2 s32), a/b formats, majors (0 K, 1 MN), N, M
+__host__ __device__ constexpr uint32_t instr_desc(int c_fmt, int a_fmt, int b_fmt, int a_mn, int b_mn, int N, int M) {
+    return (static_cast<uint32_t>(c_fmt) << 4) | (static_cast<uint32_t>(a_fmt) << 7) |
+           (static_cast<uint32_t>(b_fmt) << 10) | (static_cast<uint32_t>(a_mn) << 15) |
+           (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(N >> 3) << 17) |
+           (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+struct Params {
+    const uint16_t* q;
+    int64_t q_st, q_sh;     // token, head
+    uint16_t* o;
+    int64_t o_st, o_sh;
+    const int* cu;
+    const int* lens;
+    const int* table;
+    int batch, hkv, G, ppr, page_size, piece;   // piece: keys that one load may take (a page's power of two, 128 at most)
+    int max_keys, total, window, sinks;
+    const int8_t* ka;
+    const int8_t* kb;
+    const uint16_t* ek;
+    const uint8_t* va;
+    const uint8_t* vb;
+    float evs;
+    int* counters;          // [batch * hkv], zero
+    float* parts;           // [2 * CTAs][128 * D + 256]: O, then m and l
+    int* status;
+    int others;             // whether another kernel takes the requests with more rows
+};
+
+// One request as this kernel sees it; nt = 0: not its (no new tokens, or more rows than 128).
+struct Geo {
+    int n, L, first, shift, nt;
+    bool wide;      // more rows than the kernel takes
+};
+__device__ __forceinline__ Geo geo_of(const Params& p, int b) {
+    Geo g;
+    const int t0 = __ldg(p.cu + b), t1 = __ldg(p.cu + b + 1);
+    g.n = t0 < 0 || t1 > p.total ? 0 : t1 - t0;
+    g.L = max(0, min(__ldg(p.lens + b), p.max_keys));
+    g.first = g.L - g.n;                       // position of the first new token
+    const int ns = (p.sinks + BN - 1) / BN;
+    g.shift = max(0, max(0, g.first - p.window + 1) / BN - ns);   // tiles between the sinks' and the window's first
+    g.wide = static_cast<int64_t>(g.n) * p.G > 128;
+    g.nt = g.n <= 0 || g.wide ? 0 : max(1, (g.L + BN - 1) / BN - g.shift);
+    return g;
+}
+// A CTA's walk over its share of the list, a segment (tiles [t0, t1) of one (request, head)) at a time.
+struct Walk {
+    int b, h, t;
+    int left;
+    Geo g;
+    int t0, t1, segment;
+    __device__ __forceinline__ bool next(const Params& p) {
+        if (left <= 0) return false;
+        if (t < 0) {                           // the next item
+            t = 0;
+            if (++h == p.hkv) {
+                h = 0;
+                do {
+                    if (++b >= p.batch) { left = 0; return false; }
+                    g = geo_of(p, b);
+                } while (g.nt == 0);
+            }
+        }
+        t0 = t;
+        t1 = min(g.nt, t + left);
+        left -= t1 - t0;
+        t = t1 == g.nt ? -1 : t1;
+        ++segment;
+        return true;
+    }
+    __device__ __forceinline__ int pos(const Params& p, int j) const {     // first position of the item's j-th tile
+        return (j * BN < p.sinks ? j : j + g.shift) * BN;
+    }
+};
+
+// first CTA-independent tile of CTA c's share, and whose share tile x is
+__device__ __forceinline__ int share_start(int64_t total, int n, int c) { return static_cast<int>(total * c / n); }
+__device__ __forceinline__ int share_of(int64_t total, int n, int64_t x) { return static_cast<int>(((x + 1) * n - 1) / total); }
+
+template <int D, bool V8, bool F16>
+__global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(const Params p, const __grid_constant__ CUtensorMap vmap) {
+    using L = Lay<D, V8>;
+    constexpr int TERMS = F16 && !V8 ? 2 : 1;      // of P
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = static_cast<uint32_t>(__cvta_generic_to_shared(smem_raw));
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    if (base - raw > static_cast<uint32_t>(L::SLACK)) {   // the map would not fit: refuse, loudly
+        if (threadIdx.x == 0) atomicExch(p.status, FOLD_ERR_LAUNCH);
+        return;
+    }
+    uint8_t* smem = smem_raw + (base - raw);
+    int* s_scan = reinterpret_cast<int*>(smem + L::SM_MISC);
+    int* s_walk = s_scan + 12;
+    int* s_flag = s_scan + 16;
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_scan + 18);
+    auto bar = [&](int i) { return base + L::SM_BAR + 8 * i; };
+    volatile int* abort_flag = s_flag;
+    volatile int* last_flag = s_flag + 1;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        s_flag[0] = s_flag[1] = 0;
+        s_walk[0] = -1;
+        for (int i = 0; i < L::NK; ++i) {
+            mbar_init(bar(B_KFULL + i), 1);
+            mbar_init(bar(B_KEMPTY + i), 1 + 4);      // the tile's logits are out, and the softmax warps have its scales
+        }
+        for (int i = 0; i < L::NV; ++i) {
+            mbar_init(bar(B_VFULL + i), 1);
+            mbar_init(bar(B_VEMPTY + i), V8 ? 4 : 1);
+            mbar_init(bar(B_VREADY + i), V8 ? 4 : 1);
+        }
+        mbar_init(bar(B_SFULL), 1);
+        mbar_init(bar(B_SEMPTY), 128);
+        mbar_init(bar(B_PREADY), 128);
+        mbar_init(bar(B_ODONE), 1);
+        mbar_init(bar(B_QREADY), 128);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;"
+                     ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(s_tmem))) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // ---- this CTA's share of the list: a block scan over the requests, twice (the total, then the place) ----
+    int64_t total = 0;
+    int n_cta = 1, g0 = 0, g1 = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        int64_t run = 0;
+        for (int b0 = 0; b0 < p.batch; b0 += L::NTHREADS) {
+            const int b = b0 + tid;
+            int mine = 0;
+            if (b < p.batch) {
+                const Geo g = geo_of(p, b);
+                mine = g.nt * p.hkv;
+                if (g.wide && !p.others) atomicExch(p.status, FOLD_ERR_ARGUMENT);   // counts the host did not plan for
+            }
+            int x = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            __syncthreads();
+            if (lane == 31) s_scan[warp] = x;
+            __syncthreads();
+            int before = 0, sum = 0;
+            for (int w = 0; w < L::NTHREADS / 32; ++w) {
+                if (w < warp) before += s_scan[w];
+                sum += s_scan[w];
+            }
+            const int64_t at = run + before + x - mine;
+            if (pass == 1 && mine > 0 && g0 >= at && g0 < at + mine && g0 < g1) {
+                const int nt = mine / p.hkv, off = static_cast<int>(g0 - at);
+                s_walk[0] = b;
+                s_walk[1] = off / nt;
+                s_walk[2] = off % nt;
+            }
+            run += sum;
+        }
+        total = run;
+        if (pass == 0) {
+            n_cta = static_cast<int>(max(static_cast<int64_t>(1), min(static_cast<int64_t>(gridDim.x), (total + MIN_TILES - 1) / MIN_TILES)));
+            if (static_cast<int>(blockIdx.x) < n_cta) {
+                g0 = share_start(total, n_cta, blockIdx.x);
+                g1 = share_start(total, n_cta, blockIdx.x + 1);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *s_tmem;
+    Walk w;
+    w.b = s_walk[0];
+    w.h = s_walk[1];
+    w.t = s_walk[2];
+    w.left = w.b < 0 ? 0 : g1 - g0;
+    w.segment = -1;
+    if (w.left > 0) w.g = geo_of(p, w.b);
+
+    const int np = BN / p.piece;
+    // Whether any new token sees a key of [a, a + len): what is loaded; the rest of a tile's rows are masked in
+    // the logits and zeroed in V, whatever the pool (or the ring) holds there
+    auto wanted = [&](const Geo& g, int a, int len) { return a < g.L && (a + len - 1 > g.first - p.window || a < p.sinks); };
+    auto pool_row = [&](const Walk& x, int pos) -> int64_t {
+        const int pg = __ldg(p.table + static_cast<int64_t>(x.b) * p.ppr + pos / p.page_size);
+        return (static_cast<int64_t>(pg) * p.hkv + x.h) * p.page_size + pos % p.page_size;
+    };
+
+    if (warp == 0 || warp == 3) {
+        // ================= producers: a lane per piece of the tile =================
+        const bool is_k = warp == 0;
+        int j = 0;
+        while (w.next(p)) {
+            for (int t = w.t0; t < w.t1; ++t, ++j) {
+                const int s = j % (is_k ? L::NK : L::NV), round = j / (is_k ? L::NK : L::NV);
+                const int pos = w.pos(p, t) + lane * p.piece;
+                const bool mine = lane < np && wanted(w.g, pos, p.piece);
+                const int64_t row = mine ? pool_row(w, pos) : 0;
+                const int count = __popc(__ballot_sync(0xffffffffu, mine));
+                const uint32_t full = bar((is_k ? B_KFULL : B_VFULL) + s);
+                if (lane == 0) {
+                    if (round > 0) mbar_wait(bar((is_k ? B_KEMPTY : B_VEMPTY) + s), (round - 1) & 1, abort_flag, p.status);
+                    mbar_expect_tx(full, static_cast<uint32_t>(count) * p.piece * (2 * D + (is_k ? 2 : 0)));
+                }
+                __syncwarp();
+                if (mine) {
+                    const uint32_t r0 = lane * p.piece;
+                    if (is_k) {
+                        const uint32_t dst = base + L::SM_K + s * L::KSLOT + r0 * D;
+                        bulk_load(dst, p.ka + row * D, p.piece * D, full);
+                        bulk_load(dst + L::PLANE, p.kb + row * D, p.piece * D, full);
+                        bulk_load(base + L::SM_EK + s * 256 + r0 * 2, p.ek + row, p.piece * 2, full);
+                    } else if (V8) {
+                        const uint32_t dst = base + L::SM_V + s * L::VSLOT + r0 * D;
+                        bulk_load(dst, p.va + row * D, p.piece * D, full);
+                        bulk_load(dst + L::PLANE, p.vb + row * D, p.piece * D, full);
+                    } else {
+                        for (int c = 0; c < D / 64; ++c)
+                            tma_load_2d(base + L::SM_V + s * L::VSLOT + c * 16384 + r0 * 128, &vmap, 64 * c, static_cast<int>(row), full);
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ================= MMA issuer =================
+        if (lane == 0) {
+            constexpr uint32_t ID_S = instr_desc(2, 1, 1, 0, 0, 128, 128);                             // s8 x s8 -> s32
+            constexpr uint32_t ID_PV = instr_desc(1, V8 ? 0 : 1, V8 ? 0 : 1, 0, 1, D, 128);            // P x V, V MN-major
+            constexpr uint32_t SW = D == 128 ? 2 : 4, SBO = 8 * D;
+            const uint64_t qa = smem_desc(base + L::SM_Q, 16, SBO, SW), qb = smem_desc(base + L::SM_Q + L::PLANE, 16, SBO, SW);
+            int j = 0;
+            while (w.next(p)) {
+                mbar_wait(bar(B_QREADY), w.segment & 1, abort_flag, p.status);
+                auto issue_pv = [&](int jj, bool acc) {
+                    const int vs = jj % L::NV;
+                    mbar_wait(bar(B_PREADY), jj & 1, abort_flag, p.status);
+                    if (V8) mbar_wait(bar(B_VREADY), jj & 1, abort_flag, p.status);
+                    else mbar_wait(bar(B_VREADY + vs), (jj / L::NV) & 1, abort_flag, p.status);
+                    tc_fence_after();
+                    const uint32_t vt = base + (V8 ? L::SM_V16 : L::SM_V + vs * L::VSLOT);
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks)     // 16 keys per step
+                        mma_ts(tmem + T_O, tmem + T_P + 8 * ks, smem_desc(vt + ks * 2048, 16384, 1024, 2), ID_PV, acc || ks > 0);
+                    if (TERMS == 2) {
+#pragma unroll
+                        for (int ks = 0; ks < 8; ++ks)
+                            mma_ts(tmem + T_O, tmem + T_P2 + 8 * ks, smem_desc(vt + ks * 2048, 16384, 1024, 2), ID_PV, 1u);
+                    }
+                    if (!V8) tc_commit(bar(B_VEMPTY + vs));
+                    tc_commit(bar(B_ODONE));
+                };
+                for (int t = w.t0; t < w.t1; ++t, ++j) {
+                    const int s = j % L::NK;
+                    mbar_wait(bar(B_KFULL + s), (j / L::NK) & 1, abort_flag, p.status);
+                    if (j > 0) mbar_wait(bar(B_SEMPTY), (j - 1) & 1, abort_flag, p.status);
+                    tc_fence_after();
+                    const uint64_t ka = smem_desc(base + L::SM_K + s * L::KSLOT, 16, SBO, SW);
+                    const uint64_t kb = smem_desc(base + L::SM_K + s * L::KSLOT + L::PLANE, 16, SBO, SW);
+#pragma unroll
+                    for (int ks = 0; ks < D / 32; ++ks) mma_i8(tmem + T_S1, qa + 2 * ks, ka + 2 * ks, ID_S, ks > 0);
+#pragma unroll
+                    for (int ks = 0; ks < D / 32; ++ks) mma_i8(tmem + T_S2, qa + 2 * ks, kb + 2 * ks, ID_S, ks > 0);
+#pragma unroll
+                    for (int ks = 0; ks < D / 32; ++ks) mma_i8(tmem + T_S2, qb + 2 * ks, ka + 2 * ks, ID_S, 1u);
+                    tc_commit(bar(B_SFULL));
+                    tc_commit(bar(B_KEMPTY + s));
+                    if (t > w.t0) issue_pv(j - 1, t - 1 > w.t0);
+                }
+                // the item's last product before the next item's Q may be laid down
+                issue_pv(j - 1, w.t1 - w.t0 > 1);
+            }
+        }
+    } else if (warp == 2) {
+        // ================= bf16 V: rows that no new token sees are zeroed in shared memory =================
+        if (!V8) {
+            int j = 0;
+            while (w.next(p)) {
+                for (int t = w.t0; t < w.t1; ++t, ++j) {
+                    const int s = j % L::NV, pos = w.pos(p, t);
+                    mbar_wait(bar(B_VFULL + s), (j / L::NV) & 1, abort_flag, p.status);
+                    if (pos + BN > w.g.L || (pos <= w.g.first - p.window && pos + BN > p.sinks)) {
+                        for (int r = 0; r < BN; ++r) {
+                            if (wanted(w.g, pos + r, 1)) continue;
+                            if (lane < D / 8)
+                                sts128(base + L::SM_V + s * L::VSLOT + (lane >> 3) * 16384 + r * 128 + (lane & 7) * 16, make_uint4(0u, 0u, 0u, 0u));
+                        }
+                        fence_async_smem();
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(B_VREADY + s));
+                }
+            }
+        }
+    } else if (warp < 8) {
+        // ================= Q, softmax, epilogue: thread = TMEM lane =================
+        const int wq = warp - 4, m_row = 32 * wq + lane, t128 = tid - 128;
+        const uint32_t lane_addr = static_cast<uint32_t>(32 * wq) << 16;
+        float* s_eq = reinterpret_cast<float*>(smem + L::SM_ROW);
+        float* s_m = s_eq + 128;
+        float* s_l = s_eq + 256;
+        int j = 0;
+        while (w.next(p)) {
+            const Geo& g = w.g;
+            const int R = g.n * p.G;
+            const int copies = R <= 32 ? 4 : R <= 64 ? 2 : 1;
+            const int rows = 128 / copies;                // a copy's lanes
+            const int r = m_row & (rows - 1);             // the thread's query row: token r / G, head r % G of the group
+            const int copy = m_row / rows;
+            // ---- Q's planes, for every copy ----
+            {
+                constexpr int TPR = D / 16, RPP = 128 / TPR;
+                const int ql = t128 % TPR;
+                for (int q0 = 0; q0 < rows; q0 += RPP) {
+                    const int qr = q0 + t128 / TPR;
+                    const bool ok = qr < R;
+                    const int tok = __ldg(p.cu + w.b) + (ok ? qr / p.G : 0), hd = w.h * p.G + (ok ? qr % p.G : 0);
+                    float x[16];
+                    uint4 raw16[2];
+                    load16<F16>(p.q + static_cast<int64_t>(tok) * p.q_st + static_cast<int64_t>(hd) * p.q_sh + ql * 16, x, raw16);
+                    const float qscale = D == 64 ? 0.18033688011112042f : 0.12751743082459868f;   // log2(e) / sqrt(D)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = ok ? __fmul_rn(x[i], qscale) : 0.f;
+                    rotate16<TPR>(x, ql, D == 64 ? 0.125f : 0.08838834764831845f);
+                    const float e = __fmul_rn(fmaxf(row_amax16<TPR>(x), 1e-30f), INV127);
+                    uint4 wa, wb;
+                    int8_planes16(x, e, wa, wb);
+                    if (qr < rows)
+                        for (int c = 0; c < copies; ++c) {
+                            const int mr = c * rows + qr;
+                            const uint32_t at = base + L::SM_Q + mr * D + ((ql ^ (D == 128 ? mr & 7 : (mr >> 1) & 3)) << 4);
+                            sts128(at, wa);
+                            sts128(at + L::PLANE, wb);
+                            if (ql == 0) s_eq[mr] = e * 0.00390625f;
+                        }
+                }
+                if (copies > 1) {       // P's columns of the other copies' keys stay zero
+                    uint32_t z[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) z[i] = 0u;
+                    tmem_st32(tmem + lane_addr + T_P, z);
+                    tmem_st32(tmem + lane_addr + T_P + 32, z);
+                    if (TERMS == 2) {
+                        tmem_st32(tmem + lane_addr + T_P2, z);
+                        tmem_st32(tmem + lane_addr + T_P2 + 32, z);
+                    }
+                    tmem_wait_st();
+                }
+                fence_async_smem();
+                tc_fence_before();
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                mbar_arrive(bar(B_QREADY));
+            }
+            const float eq = s_eq[m_row];
+            const int rpos = g.first + r / p.G;           // the row's position (rows past R: never written)
+            float m_run = -INFINITY, l_run = 0.f;
+            const int seg0 = j;
+            // one tile: NCH chunks of 32 keys from the copy's first
+            auto tile = [&](auto nch, int t) {
+                constexpr int NCH = decltype(nch)::value;
+                const int s = j % L::NK, pos = w.pos(p, t), k0 = copy * 32 * NCH;
+                const bool need_mask = pos + BN - 1 > g.first || (pos <= g.L - 1 - p.window && pos + BN > p.sinks);
+                const int kmax = rpos - pos, kmin = rpos - p.window + 1 - pos, ksink = p.sinks - pos;
+                mbar_wait(bar(B_SFULL), j & 1, abort_flag, p.status);
+                tc_fence_after();
+                float x[32 * NCH];
+                float mx = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < NCH; ++c) {
+                    uint32_t a[32], b2[32];
+                    tmem_ld32(tmem + lane_addr + T_S1 + k0 + 32 * c, a);
+                    tmem_ld32(tmem + lane_addr + T_S2 + k0 + 32 * c, b2);
+                    uint4 ew[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) ew[u] = lds128(base + L::SM_EK + s * 256 + 2 * (k0 + 32 * c) + 16 * u);
+                    tmem_wait_ld();
+                    const uint32_t* ep = reinterpret_cast<const uint32_t*>(ew);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const float ekf = __uint_as_float((e & 1) ? (ep[e >> 1] & 0xFFFF0000u) : (ep[e >> 1] << 16));
+                        x[32 * c + e] = static_cast<float>(static_cast<int>(a[e]) * 256 + static_cast<int>(b2[e])) * ekf;
+                    }
+                    if (need_mask) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const int k = k0 + 32 * c + e;
+                            if (k > kmax || (k < kmin && k >= ksink)) x[32 * c + e] = -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) mx = fmaxf(mx, x[32 * c + e]);
+                }
+                tc_fence_before();
+                mbar_arrive(bar(B_SEMPTY));            // the logits are in registers: the next tile's may come
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(B_KEMPTY + s));
+                const float m_cand = fmaxf(m_run, mx * eq);
+                const float m_new = m_cand > m_run + LAZY ? m_cand : m_run;
+                const float m_use = m_new == -INFINITY ? 0.f : m_new;
+                const float alpha = ex2f(m_run - m_use);
+                float sum = 0.f, sum2 = 0.f;
+                uint32_t pk[16 * NCH], pk2nd[TERMS == 2 ? 16 * NCH : 1];
+#pragma unroll
+                for (int e = 0; e < 32 * NCH; e += 2) {
+                    const float p0 = ex2f(fmaf(x[e], eq, -m_use)), p1 = ex2f(fmaf(x[e + 1], eq, -m_use));
+                    sum += p0;
+                    sum2 += p1;
+                    pk[e >> 1] = V8 ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1);
+                    if (TERMS == 2)
+                        pk2nd[e >> 1] = pack_bf16x2(p0 - __uint_as_float(pk[e >> 1] << 16), p1 - __uint_as_float(pk[e >> 1] & 0xFFFF0000u));
+                }
+                l_run = l_run * alpha + (sum + sum2);
+                m_run = m_new;
+                if (j > seg0) {                        // P's columns and O: the product before has read and written them
+                    mbar_wait(bar(B_ODONE), (j - 1) & 1, abort_flag, p.status);
+                    tc_fence_after();
+                    if (__any_sync(0xffffffffu, alpha != 1.0f)) {
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t ov[32];
+                            tmem_ld32(tmem + lane_addr + T_O + 32 * c, ov);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+                            tmem_st32(tmem + lane_addr + T_O + 32 * c, ov);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < NCH; ++c) {
+                    uint32_t pc[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) pc[e] = pk[16 * c + e];
+                    tmem_st16(tmem + lane_addr + T_P + (k0 + 32 * c) / 2, pc);
+                    if (TERMS == 2) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) pc[e] = pk2nd[16 * c + e];
+                        tmem_st16(tmem + lane_addr + T_P2 + (k0 + 32 * c) / 2, pc);
+                    }
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(bar(B_PREADY));
+            };
+            for (int t = w.t0; t < w.t1; ++t, ++j) {
+                if (copies == 4) tile(std::integral_constant<int, 1>{}, t);
+                else if (copies == 2) tile(std::integral_constant<int, 2>{}, t);
+                else tile(std::integral_constant<int, 4>{}, t);
+            }
+            // ---- epilogue: the copies' sums together, then the output or this CTA's piece of it ----
+            mbar_wait(bar(B_ODONE), (j - 1) & 1, abort_flag, p.status);
+            tc_fence_after();
+            s_m[m_row] = m_run;
+            s_l[m_row] = l_run;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            float mt = -INFINITY;
+            for (int c = 0; c < copies; ++c) mt = fmaxf(mt, s_m[c * rows + r]);
+            const float mu = mt == -INFINITY ? 0.f : mt;
+            float lt = 0.f;
+            for (int c = 0; c < copies; ++c) lt += s_l[c * rows + r] * ex2f(s_m[c * rows + r] - mu);
+            const float f = ex2f(m_run - mu);           // 0 for a copy that saw no key
+            // the item's place in the list: which CTAs share it
+            const int64_t gs = static_cast<int64_t>(g0) + (j - (w.t1 - w.t0)) - w.t0;   // its first tile (j counts this CTA's tiles)
+            const int c_first = share_of(total, n_cta, gs), c_last = share_of(total, n_cta, gs + g.nt - 1);
+            const bool whole = c_first == c_last;
+            float* part = p.parts + static_cast<int64_t>(2 * blockIdx.x + (w.t0 > 0 ? 0 : 1)) * (128 * D + 256);
+            // a row's 16-byte unit u of the sums in shared memory, swizzled so that a quarter warp's rows fall in other banks
+            auto sum_at = [&](int row, int u) { return base + L::SM_Q + row * (4 * D) + ((u ^ (row & 7)) << 4); };
+            const int tok0 = __ldg(p.cu + w.b);
+            auto out_at = [&](int row) { return p.o + static_cast<int64_t>(tok0 + row / p.G) * p.o_st + static_cast<int64_t>(w.h * p.G + row % p.G) * p.o_sh; };
+            auto pk2 = [](float a, float b2) { return F16 ? pack_f16x2(a, b2) : pack_bf16x2(a, b2); };
+            if (copies > 1) {
+                // each copy adds a column block of its own at a time, so nobody meets anybody
+                const int blocks = D / 32 / copies > 0 ? D / 32 / copies : 1;     // 32-column blocks per turn
+                for (int turn = 0; turn < copies; ++turn) {
+                    for (int k = 0; k < blocks; ++k) {
+                        const int blk = ((copy + turn) % copies) * blocks + k;
+                        if (blk < D / 32) {
+                            uint32_t ov[32];
+                            tmem_ld32(tmem + lane_addr + T_O + 32 * blk, ov);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int u = 0; u < 8; ++u) {
+                                float4 v = make_float4(__uint_as_float(ov[4 * u]) * f, __uint_as_float(ov[4 * u + 1]) * f,
+                                                       __uint_as_float(ov[4 * u + 2]) * f, __uint_as_float(ov[4 * u + 3]) * f);
+                                const uint32_t at = sum_at(r, 8 * blk + u);
+                                if (turn > 0) {
+                                    const float4 y = as_float4(lds128(at));
+                                    v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+                                }
+                                sts128(at, as_uint4(v));
+                            }
+                        }
+                    }
+                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                }
+                if (copy == 0) {
+                    s_m[r] = mt;
+                    s_l[r] = lt;
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                for (int i = t128; i < R * (D / 8); i += 128) {
+                    const int row = i / (D / 8), u = i % (D / 8);
+                    const float4 x = as_float4(lds128(sum_at(row, 2 * u))), y = as_float4(lds128(sum_at(row, 2 * u + 1)));
+                    if (whole) {
+                        const float l = s_l[row], inv = l > 0.f ? (V8 ? p.evs : 1.f) / l : 0.f;
+                        *reinterpret_cast<uint4*>(out_at(row) + 8 * u) =
+                            make_uint4(pk2(x.x * inv, x.y * inv), pk2(x.z * inv, x.w * inv), pk2(y.x * inv, y.y * inv), pk2(y.z * inv, y.w * inv));
+                    } else {
+                        float4* d = reinterpret_cast<float4*>(part + row * D + 8 * u);
+                        d[0] = x;
+                        d[1] = y;
+                    }
+                }
+                if (!whole && t128 < R) {
+                    part[128 * D + t128] = s_m[t128];
+                    part[128 * D + 128 + t128] = s_l[t128];
+                }
+            } else {
+                const float inv = l_run > 0.f ? (V8 ? p.evs : 1.f) / l_run : 0.f;
+                uint16_t* orow = out_at(r < R ? r : 0);
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t ov[32];
+                    tmem_ld32(tmem + lane_addr + T_O + 32 * c, ov);
+                    tmem_wait_ld();
+                    if (r < R) {
+                        if (whole) {
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) {
+                                uint4 v;
+                                v.x = pk2(__uint_as_float(ov[8 * u]) * inv, __uint_as_float(ov[8 * u + 1]) * inv);
+                                v.y = pk2(__uint_as_float(ov[8 * u + 2]) * inv, __uint_as_float(ov[8 * u + 3]) * inv);
+                                v.z = pk2(__uint_as_float(ov[8 * u + 4]) * inv, __uint_as_float(ov[8 * u + 5]) * inv);
+                                v.w = pk2(__uint_as_float(ov[8 * u + 6]) * inv, __uint_as_float(ov[8 * u + 7]) * inv);
+                                *reinterpret_cast<uint4*>(orow + 32 * c + 8 * u) = v;
+                            }
+                        } else {
+                            uint4* d = reinterpret_cast<uint4*>(part + r * D + 32 * c);
+#pragma unroll
+                            for (int u = 0; u < 8; ++u) d[u] = make_uint4(ov[4 * u], ov[4 * u + 1], ov[4 * u + 2], ov[4 * u + 3]);
+                        }
+                    }
+                }
+                if (!whole && r < R) {
+                    part[128 * D + r] = m_run;
+                    part[128 * D + 128 + r] = l_run;
+                }
+            }
+            tc_fence_before();
+            if (!whole) {
+                __threadfence();
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (t128 == 0) *last_flag = atomicAdd(p.counters + static_cast<int64_t>(w.b) * p.hkv + w.h, 1) == c_last - c_first;
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (*last_flag) {       // every piece is there: add them in list order
+                    __threadfence();
+                    auto piece = [&](int c) { return p.parts + static_cast<int64_t>(2 * c + (c == c_first ? 1 : 0)) * (128 * D + 256); };
+                    if (t128 < R) {
+                        float mm = -INFINITY, ll = 0.f;
+                        for (int c = c_first; c <= c_last; ++c) mm = fmaxf(mm, __ldcg(piece(c) + 128 * D + t128));
+                        if (mm == -INFINITY) mm = 0.f;
+                        for (int c = c_first; c <= c_last; ++c)
+                            ll += __ldcg(piece(c) + 128 * D + 128 + t128) * ex2f(__ldcg(piece(c) + 128 * D + t128) - mm);
+                        s_m[t128] = mm;
+                        s_l[t128] = ll > 0.f ? (V8 ? p.evs : 1.f) / ll : 0.f;
+                    }
+                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    for (int i = t128; i < R * (D / 8); i += 128) {
+                        const int row = i / (D / 8), u = i % (D / 8);
+                        const float mm = s_m[row], inv = s_l[row];
+                        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+                        for (int c = c_first; c <= c_last; ++c) {
+                            const float fc = ex2f(__ldcg(piece(c) + 128 * D + row) - mm);
+                            const float4* src = reinterpret_cast<const float4*>(piece(c) + row * D + 8 * u);
+                            const float4 a = __ldcg(src), b2 = __ldcg(src + 1);
+                            x.x = fmaf(a.x, fc, x.x); x.y = fmaf(a.y, fc, x.y); x.z = fmaf(a.z, fc, x.z); x.w = fmaf(a.w, fc, x.w);
+                            y.x = fmaf(b2.x, fc, y.x); y.y = fmaf(b2.y, fc, y.y); y.z = fmaf(b2.z, fc, y.z); y.w = fmaf(b2.w, fc, y.w);
+                        }
+                        *reinterpret_cast<uint4*>(out_at(row) + 8 * u) =
+                            make_uint4(pk2(x.x * inv, x.y * inv), pk2(x.z * inv, x.w * inv), pk2(y.x * inv, y.y * inv), pk2(y.z * inv, y.w * inv));
+                    }
+                }
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");   // the sums' memory is Q's again
+        }
+    } else {
+        // ================= 8-bit V: two planes -> fp16 rows, MN-major, swizzled; dead rows are zeros =================
+        int j = 0;
+        const int c0 = tid - 256;
+        constexpr int UPR = D / 16;             // 16-channel units a row
+        while (w.next(p)) {
+            for (int t = w.t0; t < w.t1; ++t, ++j) {
+                const int s = j % L::NV, pos = w.pos(p, t);
+                const bool cut = pos + BN > w.g.L || (pos <= w.g.first - p.window && pos + BN > p.sinks);
+                mbar_wait(bar(B_VFULL + s), (j / L::NV) & 1, abort_flag, p.status);
+                if (j > 0) mbar_wait(bar(B_ODONE), (j - 1) & 1, abort_flag, p.status);   // the product before has read its rows
+                const uint32_t src = base + L::SM_V + s * L::VSLOT;
+#pragma unroll 4
+                for (int i = c0; i < BN * UPR; i += 128) {
+                    const int r = i / UPR, u = i % UPR;
+                    const uint4 a = lds128(src + r * D + u * 16), b2 = lds128(src + L::PLANE + r * D + u * 16);
+                    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b2.x, b2.y, b2.z, b2.w};
+                    uint32_t o[8];
+                    const bool live = !cut || wanted(w.g, pos + r, 1);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        uint32_t ha, hb;
+                        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(ha) : "h"(static_cast<uint16_t>(aw[k >> 1] >> (16 * (k & 1)))));
+                        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hb) : "h"(static_cast<uint16_t>(bw[k >> 1] >> (16 * (k & 1)))));
+                        uint32_t x;
+                        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(x) : "r"(hb), "r"(0x30003000u), "r"(ha));   // a + b / 8
+                        o[k] = live ? x : 0u;
+                    }
+                    const uint32_t dst = base + L::SM_V16 + (u >> 2) * 16384 + r * 128;
+                    const int ch = 2 * (u & 3);
+                    sts128(dst + ((ch ^ (r & 7)) << 4), make_uint4(o[0], o[1], o[2], o[3]));
+                    sts128(dst + (((ch + 1) ^ (r & 7)) << 4), make_uint4(o[4], o[5], o[6], o[7]));
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(bar(B_VREADY));
+                    mbar_arrive(bar(B_VEMPTY + s));
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+}  // namespace csm100
+}  // namespace fold
+
+using namespace fold;
+
+namespace {
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                              CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                              CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+    static EncodeFn fn = nullptr;
+    if (!fn) {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeFn>(ptr);
+    }
+    return fn;
+}
+
+template <int D, bool V8, bool F16>
+int launch(const csm100::Params& p, const CUtensorMap& vmap, int ctas, cudaStream_t st) {
+    using L = csm100::Lay<D, V8>;
+    auto kern = csm100::chunk_sm100_kernel<D, V8, F16>;
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
+    kern<<<ctas, L::NTHREADS, L::BYTES, st>>>(p, vmap);
+    return check_launch("fold_chunk_sm100");
+}
+
+}  // namespace
+
+extern "C" int fold_chunk_sm100(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* o, int64_t o_token_stride, int64_t o_head_stride,
+                                int is_f16, const int32_t* cu_seqlens, const int32_t* seq_lens, int batch, int total, int n_heads, int n_kv_heads,
+                                int head_dim, const int32_t* page_table, int pages_per_request, int page_size, int64_t pool_rows, const int8_t* ka,
+                                const int8_t* kb, const void* va, const void* vb, const void* ek, float v_scale, int window, int sinks, int others, int ctas,
+                                int32_t* counters, float* parts, int32_t* status, void* stream) {
+    FOLD_CHECK_ARG(head_dim == 64 || head_dim == 128, "head_dim %d: the cache holds 64 or 128", head_dim);
+    FOLD_CHECK_ARG(q && o && cu_seqlens && seq_lens && page_table && ka && kb && va && ek && counters && parts && status, "fold_chunk_sm100: null pointer");
+    FOLD_CHECK_ARG(n_kv_heads > 0 && n_heads % n_kv_heads == 0 && n_heads / n_kv_heads <= 128, "fold_chunk_sm100: %d query heads over %d KV heads (128 a group at most)", n_heads, n_kv_heads);
+    FOLD_CHECK_ARG(batch > 0 && total > 0 && pages_per_request > 0 && ctas > 0 && pool_rows > 0 && pool_rows < (1ll << 31),
+                   "fold_chunk_sm100: %d requests, %d tokens, %d pages a request, %d CTAs, %lld pool rows", batch, total, pages_per_request, ctas, static_cast<long long>(pool_rows));
+    FOLD_CHECK_ARG(page_size > 0 && page_size % 16 == 0, "fold_chunk_sm100: pages of %d keys (a multiple of 16)", page_size);
+    FOLD_CHECK_ARG(window > 0 && window <= FOLD_MAX_WINDOW && sinks >= 0 && sinks <= FOLD_MAX_WINDOW, "fold_chunk_sm100: a window of %d keys and %d sinks", window, sinks);
+    FOLD_CHECK_ARG(q_token_stride % 8 == 0 && q_head_stride % 8 == 0 && o_token_stride % 8 == 0 && o_head_stride % 8 == 0 &&
+                       reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(o) % 16 == 0 &&
+                       reinterpret_cast<uintptr_t>(parts) % 16 == 0 && reinterpret_cast<uintptr_t>(va) % 16 == 0,
+                   "fold_chunk_sm100: rows must be 16-byte aligned");
+    csm100::Params p;
+    p.q = static_cast<const uint16_t*>(q); p.q_st = q_token_stride; p.q_sh = q_head_stride;
+    p.o = static_cast<uint16_t*>(o); p.o_st = o_token_stride; p.o_sh = o_head_stride;
+    p.cu = cu_seqlens; p.lens = seq_lens; p.table = page_table;
+    p.batch = batch; p.hkv = n_kv_heads; p.G = n_heads / n_kv_heads; p.ppr = pages_per_request; p.page_size = page_size;
+    p.piece = 128;
+    while (page_size % p.piece) p.piece >>= 1;
+    const int64_t cap = static_cast<int64_t>(pages_per_request) * page_size;
+    p.max_keys = static_cast<int>(cap < (1 << 30) ? cap : (1 << 30));
+    p.total = total; p.window = window; p.sinks = sinks;
+    p.ka = ka; p.kb = kb; p.ek = static_cast<const uint16_t*>(ek);
+    p.va = static_cast<const uint8_t*>(va); p.vb = static_cast<const uint8_t*>(vb); p.evs = v_scale;
+    p.counters = counters; p.parts = parts; p.status = status; p.others = others;
+    CUtensorMap vmap = {};
+    if (!vb) {   // a bf16 V: rows of the pool, boxes of 64 channels of a piece's keys
+        EncodeFn fn = encode_fn();
+        cuuint64_t dims[2] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(pool_rows)};
+        cuuint64_t strides[1] = {static_cast<cuuint64_t>(head_dim) * 2};
+        cuuint32_t box[2] = {64u, static_cast<cuuint32_t>(p.piece)};
+        cuuint32_t estr[2] = {1, 1};
+        if (!fn || fn(&vmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(va), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+            set_error("fold_chunk_sm100: cuTensorMapEncodeTiled failed");
+            return FOLD_ERR_LAUNCH;
+        }
+    }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (head_dim == 64) {
+        if (vb) return is_f16 ? launch<64, true, true>(p, vmap, ctas, st) : launch<64, true, false>(p, vmap, ctas, st);
+        return is_f16 ? launch<64, false, true>(p, vmap, ctas, st) : launch<64, false, false>(p, vmap, ctas, st);
+    }
+    if (vb) return is_f16 ? launch<128, true, true>(p, vmap, ctas, st) : launch<128, true, false>(p, vmap, ctas, st);
+    return is_f16 ? launch<128, false, true>(p, vmap, ctas, st) : launch<128, false, false>(p, vmap, ctas, st);
+}

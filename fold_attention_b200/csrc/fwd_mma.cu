@@ -45,6 +45,7 @@ __global__ void __launch_bounds__(128) fwd_mma_kernel(const FwdParams p) {
     if constexpr (EXT) {
         if (p.plan) {
             const int4 pl = p.plan[b];
+            if (pl.x < 0) return;   // another kernel's
             klen = pl.x;
             qoff = klen - len;
             kstart = pl.y;

@@ -228,6 +228,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
     if constexpr (EXT) {
         if (p.plan) {
             const int4 pl = p.plan[b];
+            if (pl.x < 0) return;   // another kernel's
             klen = pl.x;
             qoff = klen - len;
             kstart = pl.y;

@@ -15,6 +15,7 @@ takes prompts whole and then one token a request.
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -25,7 +26,8 @@ _lib.register("fold_build_tables", [P, P, I, P, I, I, I, P, I, P, P, P, P, P])
 _lib.register("fold_write_tokens", [P, P, I, L, L, L, L, P, L, I, I, I, P, P, P, P, P, F, P])
 _lib.register("fold_read_tokens", [P, L, I, I, I, P, P, P, P, P, F, P, P, I, P])
 _lib.register("fold_chunk_sums", [P, I, L, L, I, I, I, P, I, P, P, F, P, P, P])
-_lib.register("fold_chunk_gather", [P, P, I, P, I, I, I, I, I, I, P, P, P, P, P, F, I, I, P, P, P, P, P, P])
+_lib.register("fold_chunk_gather", [P, P, I, P, I, I, I, I, I, I, P, P, P, P, P, F, I, I, I, I, P, P, P, P, P, P])
+_lib.register("fold_chunk_sm100", [P, L, L, P, L, L, I, P, P, I, I, I, I, I, P, I, I, L, P, P, P, P, P, F, I, I, I, I, P, P, P, P])
 
 _HALF = (torch.bfloat16, torch.float16)
 _OUT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -156,33 +158,54 @@ def chunk_sums(v, cu_seqlens, lens_new, seq_lens, v_scale, vsum, vmean):
         )
 
 
-def chunk_attention(q, cu_seqlens, max_new, cap_tiles, seq_lens, page_table, page_size, ka, kb, va, vb, ek, v_scale, n_kv_heads,
-                    window, sinks, softmax_scale):
+SHORT_ROWS = 128     # new tokens x query heads a KV head that chunk_sm100.cu takes
+
+
+def chunk_attention(q, cu_seqlens, lens, cap_tiles, seq_lens, page_table, page_size, ka, kb, va, vb, ek, v_scale, n_kv_heads,
+                    window, sinks):
     """Attention of each request's last tokens over the pool: `q` `(total, H,
-    D)`, cut by `cu_seqlens`, at most `max_new` a request. `cap_tiles` is how many
-    128-key tiles the requests' visible keys fill, at most. Returns `(out, status)`."""
+    D)`, cut by `cu_seqlens`, `lens[b]` rows of request b. A request of up to
+    `SHORT_ROWS` query rows a KV head is attended straight from the codes; the
+    others' keys are dequantised first, `cap_tiles` 128-key tiles of them at
+    most. Returns `(out, status)`."""
     total, H, D = q.shape
     dev, dt = q.device, q.dtype
-    B = seq_lens.shape[0]
+    B, G = seq_lens.shape[0], H // n_kv_heads
+    f16, win = int(dt == torch.float16), window or 1 << 30
+    short = any(0 < n * G <= SHORT_ROWS for n in lens)
+    wide = max(lens) * G > SHORT_ROWS
     out = torch.empty((total, H, D), device=dev, dtype=dt)
-    work = torch.zeros(1 + 4 * B + 2 * cap_tiles + 3, device=dev, dtype=torch.int32)
-    status, plan, tiles = work[:1], work[4:4 + 4 * B], work[4 + 4 * B:4 + 4 * B + 2 * cap_tiles]
-    rows = cap_tiles * 128
-    kw = torch.empty((2, n_kv_heads, rows, D), device=dev, dtype=dt)
-    vw = kw[1]
-    win = window or 1 << 30
-    f16 = int(dt == torch.float16)
-    strides = (ctypes.c_int64 * 12)(0, q.stride(0), q.stride(1), 0, D, rows * D, 0, D, rows * D, 0, out.stride(0), out.stride(1))
-    args = (q.data_ptr(), kw.data_ptr(), vw.data_ptr(), out.data_ptr(), None, ctypes.addressof(strides), cu_seqlens.data_ptr(), B, H,
-            n_kv_heads, max_new, total, D, f16, softmax_scale, win, sinks, plan.data_ptr(), rows)
+    n_count = -(-B * n_kv_heads // 4) * 4 if short else 0
+    n_plan = 4 * B + 2 * cap_tiles if wide else 0
+    work = torch.zeros(4 + n_count + n_plan, device=dev, dtype=torch.int32)
+    status = work[:1]
+    pool = (page_table.data_ptr(), page_table.shape[1], int(page_size))
+    planes = (ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb), ek.data_ptr(), float(v_scale))
+    base = work.data_ptr()
     with torch.cuda.device(dev):
-        _lib.call(
-            "fold_chunk_gather", cu_seqlens.data_ptr(), seq_lens.data_ptr(), B, page_table.data_ptr(), page_table.shape[1], int(page_size),
-            n_kv_heads, D, win, sinks, ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb), ek.data_ptr(), float(v_scale),
-            f16, cap_tiles, plan.data_ptr(), tiles.data_ptr(), kw.data_ptr(), vw.data_ptr(), status.data_ptr(), _lib.stream(dev),
-        )
-        if _lib.lib.fold_fwd_sm100_supported(D, f16):
-            _lib.call("fold_fwd_window_sm100", *args, status.data_ptr(), _lib.stream(dev))
-        else:
-            _lib.call("fold_fwd_window", *args, _lib.stream(dev))
+        st = _lib.stream(dev)
+        if short:
+            ctas = torch.cuda.get_device_properties(dev).multi_processor_count
+            parts = torch.empty(2 * ctas * (128 * D + 256), device=dev, dtype=torch.float32)
+            _lib.call(
+                "fold_chunk_sm100", q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), f16,
+                cu_seqlens.data_ptr(), seq_lens.data_ptr(), B, total, H, n_kv_heads, D, *pool, ka.shape[0], *planes, win, sinks, int(wide),
+                ctas, base + 16, parts.data_ptr(), base, st,
+            )
+        if wide:
+            rows = cap_tiles * 128
+            kw = torch.empty((2, n_kv_heads, rows, D), device=dev, dtype=dt)
+            vw = kw.data_ptr() + kw.stride(0) * 2
+            plan = base + 16 + 4 * n_count
+            _lib.call(
+                "fold_chunk_gather", cu_seqlens.data_ptr(), seq_lens.data_ptr(), B, *pool, n_kv_heads, D, win, sinks, *planes, f16,
+                SHORT_ROWS if short else 0, G, cap_tiles, plan, plan + 16 * B, kw.data_ptr(), vw, base, st,
+            )
+            strides = (ctypes.c_int64 * 12)(0, q.stride(0), q.stride(1), 0, D, rows * D, 0, D, rows * D, 0, out.stride(0), out.stride(1))
+            args = (q.data_ptr(), kw.data_ptr(), vw, out.data_ptr(), None, ctypes.addressof(strides), cu_seqlens.data_ptr(), B, H,
+                    n_kv_heads, max(lens), total, D, f16, 1.0 / math.sqrt(D), win, sinks, plan, rows)
+            if _lib.lib.fold_fwd_sm100_supported(D, f16):
+                _lib.call("fold_fwd_window_sm100", *args, base, st)
+            else:
+                _lib.call("fold_fwd_window", *args, st)
     return out, status

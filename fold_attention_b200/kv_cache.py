@@ -371,8 +371,8 @@ class FoldKVCache:
         which waits for the device. Returns `(total, H, D)` in q's dtype.
 
         Captured in a CUDA graph (with `lens`), each replay appends and attends at the
-        lengths the device then holds, up to `max_len`: call `sync_lens` before
-        the next eager call. A shared pool's pages are taken by the replays too.
+        lengths the device then holds, up to `max_len`, with the counts it was
+        captured with: call `sync_lens` before the next eager call. A shared pool's pages are taken by the replays too.
         """
         lens = self._chunk_lens(cu_seqlens, lens)
         self._check_chunk_q(q, lens)     # before anything is written
@@ -420,14 +420,13 @@ class FoldKVCache:
         capturing = torch.cuda.is_current_stream_capturing()
         cap = 0
         for n, a in zip(lens, self.lens):
-            if capturing:
-                cap += -(-self.max_len // 128)
-            elif n:
-                first = max(0, a - n - (self.window or a) + 1) // 128
-                cap += -(-a // 128) - max(0, first - -(-self.sinks // 128))
+            if n * self.group > tokens.SHORT_ROWS:
+                end = self.max_len if capturing else a
+                first = 0 if capturing else max(0, a - n - (self.window or a) + 1) // 128
+                cap += -(-end // 128) - max(0, first - -(-self.sinks // 128))
         out, self._chunk_status = tokens.chunk_attention(
-            q, cu_seqlens, q.shape[0] if capturing else max(lens), cap, self.seq_lens, self.page_table, self.page_size, self.ka, self.kb, self.va,
-            self.vb, self.ek, self.v_scale, self.n_kv_heads, self.window, self.sinks, 1.0 / math.sqrt(self.head_dim),
+            q, cu_seqlens, lens, cap, self.seq_lens, self.page_table, self.page_size, self.ka, self.kb, self.va, self.vb, self.ek,
+            self.v_scale, self.n_kv_heads, self.window, self.sinks,
         )
         if self.check_range or self.check_status:
             check_status(self._chunk_status, "attend_chunk")

@@ -72,13 +72,29 @@ int fold_chunk_sums(const void* v, int is_f16, int64_t v_token_stride, int64_t v
 /* The keys and values that the last cu_seqlens[b + 1] - cu_seqlens[b] tokens of each request can see,
  * as 16-bit rows for fold_fwd_window: whole tiles of 128 keys, requests one after another, zeros past
  * a request's end. kw, vw [n_kv_heads][cap_tiles * 128][head_dim] in bf16, or fp16 (is_f16,
- * saturating); plan int32[4 * batch]; tiles int32[2 * cap_tiles]. Requests that do not fit cap_tiles
- * see no key and raise *status (FOLD_ERR_ARGUMENT). */
+ * saturating); plan int32[4 * batch]; tiles int32[2 * cap_tiles]. Requests whose new tokens times
+ * `group` (query heads a KV head) are no more than rows_over are left out, by the attention too. Requests
+ * that do not fit cap_tiles see no key and raise *status (FOLD_ERR_ARGUMENT). */
 int fold_chunk_gather(const int32_t* cu_seqlens, const int32_t* seq_lens, int batch, const int32_t* page_table,
                       int pages_per_request, int page_size, int n_kv_heads, int head_dim, int window, int sinks,
                       const int8_t* ka, const int8_t* kb, const void* va, const void* vb, const void* ek,
-                      float v_scale, int is_f16, int cap_tiles, int32_t* plan, int32_t* tiles, void* kw, void* vw,
-                      int32_t* status, void* stream);
+                      float v_scale, int is_f16, int rows_over, int group, int cap_tiles, int32_t* plan,
+                      int32_t* tiles, void* kw, void* vw, int32_t* status, void* stream);
+
+/* Attention of each request's last cu_seqlens[b + 1] - cu_seqlens[b] tokens over the pool, for requests
+ * whose new tokens times query heads a KV head are 128 at most, straight from the codes on tcgen05
+ * tensor cores: causal, under `window` and `sinks`, softmax scale 1 / sqrt(head_dim). Requests with more
+ * rows are left alone when `others` is set and raise *status (FOLD_ERR_ARGUMENT) when it is not.
+ * q, o (total, n_heads, head_dim) bf16 or fp16 with element strides; pool_rows rows in the planes;
+ * pages of a multiple of 16 keys; `ctas` persistent CTAs (one an SM); counters int32[batch *
+ * n_kv_heads], zero; parts fp32[2 * ctas][128 * head_dim + 256]. */
+int fold_chunk_sm100(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* o,
+                     int64_t o_token_stride, int64_t o_head_stride, int is_f16, const int32_t* cu_seqlens,
+                     const int32_t* seq_lens, int batch, int total, int n_heads, int n_kv_heads, int head_dim,
+                     const int32_t* page_table, int pages_per_request, int page_size, int64_t pool_rows,
+                     const int8_t* ka, const int8_t* kb, const void* va, const void* vb, const void* ek,
+                     float v_scale, int window, int sinks, int others, int ctas, int32_t* counters, float* parts,
+                     int32_t* status, void* stream);
 
 /* ---- Path B: cache writes ------------------------------------------------ */
 
