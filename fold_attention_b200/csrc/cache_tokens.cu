@@ -252,6 +252,8 @@ constexpr int CP_THREADS = 256;
 __global__ void __launch_bounds__(CP_THREADS) chunk_plan_kernel(const int* __restrict__ cu, const int* __restrict__ lens, int batch, int max_keys,
                                                                 int window, int sinks, int rows_over, int group, int cap_tiles, int4* plan, int2* tiles, int* status) {
     __shared__ int s_warp[CP_THREADS / 32];
+    if (rows_over == 0 && threadIdx.x == 0) *status = 0;    // no other kernel of the call has a say in it
+    __syncthreads();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ns = (sinks + 127) / 128;
     int base = 0;

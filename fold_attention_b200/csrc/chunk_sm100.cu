@@ -16,14 +16,15 @@
 // Few rows would leave most of the 128 TMEM lanes, and three of the four softmax warps, without work:
 // a group of up to 32 (64) rows is stacked four (two) times, each copy's warp takes a quarter (half)
 // of a tile's keys, with zeros in P for the others, and the copies' sums meet in the epilogue.
+// Between two (request, head)s the next one's Q and first tiles are on their way while O is written out.
 //
 // Work is one list of 128-key tiles, request by request and head by head, cut evenly over one
 // persistent CTA per SM: a (request, head) spans neighbouring CTAs at most where their ranges meet.
 // Each leaves its piece (m, l, O) in the workspace and the last to arrive adds the pieces in list
 // order, so the bits do not depend on who that is.
 //
-// Warps: 0 K producer (both planes, scales), 3 V producer, 1 MMA issuer, 2 V's dead rows (bf16 V),
-// 4-7 Q, softmax and epilogue, 8-11 V's conversion (8-bit V). Every wait is bounded.
+// Warps: 0 K producer (both planes, scales), 3 V producer, 1 MMA issuer, 2 Q and V's dead rows (bf16 V),
+// 4-7 softmax and epilogue, 2 (8-bit V) or 8 (bf16 V) joins pieces, 8-11 V's conversion (8-bit V). Every wait is bounded.
 #include <cuda.h>
 
 #include <type_traits>
@@ -37,30 +38,39 @@ namespace csm100 {
 constexpr int BN = 128;
 constexpr long long WAIT_CYCLES = 1ll << 31;
 constexpr float LAZY = 8.0f;
+constexpr int SLOTS = 4;         // a CTA's pieces: of the item it starts in, of the one it ends in, two for the items between
 constexpr int MIN_TILES = 4;     // tiles a CTA takes at least: its fixed costs are two or three tiles' time
+// What a (request, head) costs a CTA beside its tiles, in tiles: its first tile's way through the pipeline and
+// its last one's, and its O. Each item is that much longer in the list that the shares are cut from
+// (without it the CTA that met ten short requests finished a third later than the others).
+constexpr int ITEM_TILES = 5;
+
+constexpr int N_GEO = 6;         // requests a CTA keeps the lengths of (a share of a long list spans two or three)
 
 template <int D, bool V8>
 struct Lay {
     static constexpr int PLANE = 128 * D;                  // a tile of one 8-bit plane
-    static constexpr int NK = D == 128 ? 3 : 6, NV = D == 128 ? (V8 ? 2 : 3) : 5;
+    static constexpr int NK = D == 128 ? (V8 ? 2 : 3) : (V8 ? 5 : 6), NV = D == 128 ? (V8 ? 2 : 3) : 5;
     static constexpr int KSLOT = 2 * PLANE, VSLOT = 2 * PLANE;
-    static constexpr int SM_Q = 0;                         // plane A, plane B; between items the copies' sums
-    static constexpr int SM_V16 = 2 * PLANE;               // the converted tile (8-bit V)
-    static constexpr int SM_K = SM_V16 + (V8 ? 2 * PLANE : 0);
+    static constexpr int SM_Q = 0;                         // plane A, plane B
+    static constexpr int SM_V16 = 2 * PLANE;               // two converted tiles (8-bit V)
+    static constexpr int SM_K = SM_V16 + (V8 ? 4 * PLANE : 0);
     static constexpr int SM_V = SM_K + NK * KSLOT;
     static constexpr int SM_EK = SM_V + NV * VSLOT;        // [NK][128] bf16
-    static constexpr int SM_ROW = SM_EK + NK * 256;        // eq, m, l [128] f32
-    static constexpr int SM_BAR = SM_ROW + 3 * 512;
-    static constexpr int SM_MISC = SM_BAR + 256;           // scan [12], walk [4], flags [2], TMEM address
-    static constexpr int USED = SM_MISC + 128;
+    static constexpr int SM_ROW = SM_EK + NK * 256;        // m, l [128] f32
+    static constexpr int SM_BAR = SM_ROW + 2 * 512;
+    static constexpr int SM_MISC = SM_BAR + 304;           // scan [12], walk [4], flags [2], TMEM address
+    static constexpr int SM_GEO = SM_MISC + 80;            // the share's first requests
+    static constexpr int USED = SM_GEO + N_GEO * 28;
     static constexpr int SLACK = 232448 - USED < 1024 ? 232448 - USED : 1024;   // room to align the base
     static constexpr int BYTES = USED + SLACK;
-    static constexpr int NTHREADS = V8 ? 384 : 256;
+    static constexpr int W_JOIN = V8 ? 2 : 8, N_JOIN = V8 ? 1 : 4;   // the warps that join pieces
+    static constexpr int NTHREADS = 384;
     static_assert(SLACK >= 0, "shared memory");
 };
 
-// barriers: [6] K slots, [5] V slots, then one each
-enum { B_KFULL = 0, B_KEMPTY = 6, B_VFULL = 12, B_VEMPTY = 17, B_VREADY = 22, B_SFULL = 27, B_SEMPTY = 28, B_PREADY = 29, B_ODONE = 30, B_QREADY = 31 };
+// barriers: [6] K slots, [5] V slots, [2] converted tiles, then one each
+enum { B_KFULL = 0, B_KEMPTY = 6, B_VFULL = 12, B_VEMPTY = 17, B_VREADY = 22, B_CEMPTY = 27, B_SFULL = 29, B_SEMPTY = 30, B_PREADY = 31, B_ODONE = 32, B_QFULL = 33, B_QEMPTY = 34, B_PIECE = 35, B_JOINED = 36 };
 
 constexpr uint32_t T_S1 = 0, T_S2 = 128, T_P = 256, T_P2 = 320, T_O = 384;   // TMEM columns: 128, 128, 64, 64, D
 
@@ -146,6 +156,11 @@ __device__ __forceinline__ float ex2f(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
@@ -181,6 +196,9 @@ __host__ __device__ constexpr uint32_t instr_desc(int c_fmt, int a_fmt, int b_fm
 struct Params {
     const uint16_t* q;
     int64_t q_st, q_sh;     // token, head
+    int8_t* qa;             // Q's planes and scales / 256 by (request, KV head, row), from chunk_q_kernel
+    int8_t* qb;
+    float* eq;
     uint16_t* o;
     int64_t o_st, o_sh;
     const int* cu;
@@ -195,19 +213,20 @@ struct Params {
     const uint8_t* vb;
     float evs;
     int* counters;          // [batch * hkv], zero
-    float* parts;           // [2 * CTAs][128 * D + 256]: O, then m and l
+    float* parts;           // [SLOTS * CTAs][128 * D + 256]: pieces, O, then m and l
     int* status;
     int others;             // whether another kernel takes the requests with more rows
 };
 
 // One request as this kernel sees it; nt = 0: not its (no new tokens, or more rows than 128).
 struct Geo {
-    int n, L, first, shift, nt;
-    bool wide;      // more rows than the kernel takes
+    int tok0, n, L, first, shift, nt;
+    int wide;       // more rows than the kernel takes
 };
 __device__ __forceinline__ Geo geo_of(const Params& p, int b) {
     Geo g;
     const int t0 = __ldg(p.cu + b), t1 = __ldg(p.cu + b + 1);
+    g.tok0 = t0;
     g.n = t0 < 0 || t1 > p.total ? 0 : t1 - t0;
     g.L = max(0, min(__ldg(p.lens + b), p.max_keys));
     g.first = g.L - g.n;                       // position of the first new token
@@ -217,28 +236,38 @@ __device__ __forceinline__ Geo geo_of(const Params& p, int b) {
     g.nt = g.n <= 0 || g.wide ? 0 : max(1, (g.L + BN - 1) / BN - g.shift);
     return g;
 }
-// A CTA's walk over its share of the list, a segment (tiles [t0, t1) of one (request, head)) at a time.
+// A CTA's walk over its share of the list, a segment (tiles [t0, t1) of one (request, head)) at a time. In
+// the list an item is ITEM_TILES + nt long, its tiles last.
 struct Walk {
-    int b, h, t;
+    int b, h, v;        // the next place: request, head, place in the item
     int left;
     Geo g;
     int t0, t1, segment;
+    int64_t start;      // the item's first place in the list
+    const Geo* kept;    // requests [b0, b0 + N_GEO)
+    int b0;
     __device__ __forceinline__ bool next(const Params& p) {
-        if (left <= 0) return false;
-        if (t < 0) {                           // the next item
-            t = 0;
-            if (++h == p.hkv) {
-                h = 0;
-                do {
-                    if (++b >= p.batch) { left = 0; return false; }
-                    g = geo_of(p, b);
-                } while (g.nt == 0);
+        for (;;) {
+            if (left <= 0) return false;
+            if (v < 0) {                           // the next item
+                v = 0;
+                start += ITEM_TILES + g.nt;
+                if (++h == p.hkv) {
+                    h = 0;
+                    do {
+                        if (++b >= p.batch) { left = 0; return false; }
+                        if (b - b0 < N_GEO) g = kept[b - b0];
+                        else g = geo_of(p, b);
+                    } while (g.nt == 0);
+                }
             }
+            const int v1 = min(ITEM_TILES + g.nt, v + left);
+            t0 = max(0, v - ITEM_TILES);
+            t1 = max(0, v1 - ITEM_TILES);
+            left -= v1 - v;
+            v = v1 == ITEM_TILES + g.nt ? -1 : v1;
+            if (t1 > t0) break;                    // (a share may end before an item's tiles begin)
         }
-        t0 = t;
-        t1 = min(g.nt, t + left);
-        left -= t1 - t0;
-        t = t1 == g.nt ? -1 : t1;
         ++segment;
         return true;
     }
@@ -247,9 +276,54 @@ struct Walk {
     }
 };
 
-// first CTA-independent tile of CTA c's share, and whose share tile x is
-__device__ __forceinline__ int share_start(int64_t total, int n, int c) { return static_cast<int>(total * c / n); }
+__device__ __forceinline__ int copies_of(int R) { return R <= 32 ? 4 : R <= 64 ? 2 : 1; }
+
+// the first place of CTA c's share of the list, and whose share place x is in
+__device__ __forceinline__ int64_t share_start(int64_t total, int n, int c) { return total * c / n; }
 __device__ __forceinline__ int share_of(int64_t total, int n, int64_t x) { return static_cast<int>(((x + 1) * n - 1) / total); }
+
+// Q's planes and scales, laid out as the attention's CTAs load them: row (token i, head g of the group) of
+// (request b, KV head h) at cu[b] H + h n G + i G + g, its 16-byte units swizzled for the tensor core. A
+// row costs a load and two thousand cycles of latency, which every CTA that meets the (request, head)
+// would pay between its tiles; here all rows pay it at once (the first form did: 16 thousand cycles a
+// (request, head) of which Q was half). Also zeroes the counters and the status word, in place of a memset.
+template <int D, bool F16>
+__global__ void __launch_bounds__(NT) chunk_q_kernel(const Params p, int heads, int64_t n_rows) {
+    constexpr int TPR = D / 16, RPB = NT / TPR;
+    const int64_t gt = static_cast<int64_t>(blockIdx.x) * NT + threadIdx.x;
+    for (int64_t i = gt; i < static_cast<int64_t>(p.batch) * p.hkv; i += static_cast<int64_t>(gridDim.x) * NT) p.counters[i] = 0;
+    if (gt == 0) *p.status = 0;
+    const int lane = threadIdx.x % TPR;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / TPR;
+    const int64_t rr = row < n_rows ? row : 0;
+    const int tok = static_cast<int>(rr / heads), hd = static_cast<int>(rr % heads);
+    float x[16];
+    uint4 raw[2];
+    load16<F16>(p.q + static_cast<int64_t>(tok) * p.q_st + static_cast<int64_t>(hd) * p.q_sh + lane * 16, x, raw);
+    int lo = 0, hi = p.batch;      // the last request that starts at or before the token
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(p.cu + mid) <= tok) lo = mid;
+        else hi = mid;
+    }
+    const int t0 = __ldg(p.cu + lo), t1 = __ldg(p.cu + lo + 1), n = t1 - t0;
+    const bool ok = row < n_rows && tok >= t0 && tok < t1 && t1 <= p.total && static_cast<int64_t>(n) * p.G <= 128;
+    const float qscale = D == 64 ? 0.18033688011112042f : 0.12751743082459868f;   // log2(e) / sqrt(D)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = __fmul_rn(x[i], qscale);
+    rotate16<TPR>(x, lane, D == 64 ? 0.125f : 0.08838834764831845f);
+    const float e = __fmul_rn(fmaxf(row_amax16<TPR>(x), 1e-30f), INV127);
+    uint4 wa, wb;
+    int8_planes16(x, e, wa, wb);
+    if (ok) {
+        const int r = (tok - t0) * p.G + hd % p.G;
+        const int64_t at = static_cast<int64_t>(t0) * heads + static_cast<int64_t>(hd / p.G) * n * p.G + r;
+        const int64_t unit = at * D + ((lane ^ (D == 128 ? r & 7 : (r >> 1) & 3)) << 4);
+        *reinterpret_cast<uint4*>(p.qa + unit) = wa;
+        *reinterpret_cast<uint4*>(p.qb + unit) = wb;
+        if (lane == 0) p.eq[at] = e * 0.00390625f;
+    }
+}
 
 template <int D, bool V8, bool F16>
 __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(const Params p, const __grid_constant__ CUtensorMap vmap) {
@@ -288,7 +362,12 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
         mbar_init(bar(B_SEMPTY), 128);
         mbar_init(bar(B_PREADY), 128);
         mbar_init(bar(B_ODONE), 1);
-        mbar_init(bar(B_QREADY), 128);
+        mbar_init(bar(B_QFULL), 1);
+        mbar_init(bar(B_QEMPTY), 1);
+        mbar_init(bar(B_PIECE), 128);
+        mbar_init(bar(B_JOINED), L::N_JOIN);
+        mbar_init(bar(B_CEMPTY), 1);
+        mbar_init(bar(B_CEMPTY + 1), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -298,18 +377,23 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
     }
     // ---- this CTA's share of the list: a block scan over the requests, twice (the total, then the place) ----
     int64_t total = 0;
-    int n_cta = 1, g0 = 0, g1 = 0;
+    int n_cta = 1;
+    int64_t g0 = 0, g1 = 0;
+    Geo mg = {};
+    int64_t mine = 0;
     for (int pass = 0; pass < 2; ++pass) {
         int64_t run = 0;
         for (int b0 = 0; b0 < p.batch; b0 += L::NTHREADS) {
             const int b = b0 + tid;
-            int mine = 0;
-            if (b < p.batch) {
-                const Geo g = geo_of(p, b);
-                mine = g.nt * p.hkv;
-                if (g.wide && !p.others) atomicExch(p.status, FOLD_ERR_ARGUMENT);   // counts the host did not plan for
+            if (pass == 0 || p.batch > L::NTHREADS) {
+                mine = 0;
+                if (b < p.batch) {
+                    mg = geo_of(p, b);
+                    mine = mg.nt ? static_cast<int64_t>(mg.nt + ITEM_TILES) * p.hkv : 0;
+                    if (mg.wide && !p.others) atomicExch(p.status, FOLD_ERR_ARGUMENT);   // counts the host did not plan for
+                }
             }
-            int x = mine;
+            int x = static_cast<int>(mine);      // (a request's places fit 31 bits: 2^30 keys are 2^23 tiles, of 128 heads)
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int y = __shfl_up_sync(0xffffffffu, x, o);
@@ -318,40 +402,46 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
             __syncthreads();
             if (lane == 31) s_scan[warp] = x;
             __syncthreads();
-            int before = 0, sum = 0;
-            for (int w = 0; w < L::NTHREADS / 32; ++w) {
-                if (w < warp) before += s_scan[w];
-                sum += s_scan[w];
+            int64_t before = 0, sum = 0;
+            for (int wi = 0; wi < L::NTHREADS / 32; ++wi) {
+                if (wi < warp) before += s_scan[wi];
+                sum += s_scan[wi];
             }
             const int64_t at = run + before + x - mine;
             if (pass == 1 && mine > 0 && g0 >= at && g0 < at + mine && g0 < g1) {
-                const int nt = mine / p.hkv, off = static_cast<int>(g0 - at);
+                const int per = mg.nt + ITEM_TILES, off = static_cast<int>(g0 - at);
                 s_walk[0] = b;
-                s_walk[1] = off / nt;
-                s_walk[2] = off % nt;
+                s_walk[1] = off / per;
+                s_walk[2] = off % per;
             }
             run += sum;
         }
         total = run;
         if (pass == 0) {
-            n_cta = static_cast<int>(max(static_cast<int64_t>(1), min(static_cast<int64_t>(gridDim.x), (total + MIN_TILES - 1) / MIN_TILES)));
+            n_cta = static_cast<int>(max(static_cast<int64_t>(1), min(static_cast<int64_t>(gridDim.x), (total + MIN_TILES + ITEM_TILES - 1) / (MIN_TILES + ITEM_TILES))));
             if (static_cast<int>(blockIdx.x) < n_cta) {
                 g0 = share_start(total, n_cta, blockIdx.x);
                 g1 = share_start(total, n_cta, blockIdx.x + 1);
             }
         }
     }
+    __syncthreads();
+    Walk w;
+    w.b = w.b0 = s_walk[0];
+    w.h = s_walk[1];
+    w.v = s_walk[2];
+    w.left = w.b < 0 ? 0 : static_cast<int>(g1 - g0);
+    w.segment = -1;
+    w.kept = reinterpret_cast<const Geo*>(smem + L::SM_GEO);
+    w.start = g0 - w.v;
+    if (w.left > 0) {
+        w.g = geo_of(p, w.b);
+        if (tid < N_GEO && w.b + tid < p.batch) reinterpret_cast<Geo*>(smem + L::SM_GEO)[tid] = geo_of(p, w.b + tid);
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *s_tmem;
-    Walk w;
-    w.b = s_walk[0];
-    w.h = s_walk[1];
-    w.t = s_walk[2];
-    w.left = w.b < 0 ? 0 : g1 - g0;
-    w.segment = -1;
-    if (w.left > 0) w.g = geo_of(p, w.b);
 
     const int np = BN / p.piece;
     // Whether any new token sees a key of [a, a + len): what is loaded; the rest of a tile's rows are masked in
@@ -360,6 +450,76 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
     auto pool_row = [&](const Walk& x, int pos) -> int64_t {
         const int pg = __ldg(p.table + static_cast<int64_t>(x.b) * p.ppr + pos / p.page_size);
         return (static_cast<int64_t>(pg) * p.hkv + x.h) * p.page_size + pos % p.page_size;
+    };
+
+    // A segment's piece: whole items alternate between two slots, the item the share starts in and the one it
+    // ends in keep theirs for whoever joins them. A whole item of 128-row groups needs none. A piece is
+    // [D / 4 units][128 rows] of four channels, so that a warp's store is 512 bytes in a row, then m and l.
+    auto is_whole = [&](const Walk& x) { return x.t0 == 0 && x.t1 == x.g.nt; };
+    auto slot_of = [&](int c, int k) { return p.parts + (static_cast<int64_t>(SLOTS) * c + k) * (128 * D + 256); };
+    // Join a (request, head)'s pieces: a row's pieces (each the copies' plain sums under one reference) are added
+    // in list order and copies within, by this CTA for an item of its own, by the last CTA to get here for
+    // one that several share.
+    auto join = [&](const Walk& x, int& joins) {
+        const int R = x.g.n * p.G, copies = copies_of(R), rows = 128 / copies;
+        const bool whole = is_whole(x);
+        if (whole && copies == 1) return;
+        const int jl = (warp - L::W_JOIN) * 32 + lane;
+        mbar_wait(bar(B_PIECE), joins & 1, abort_flag, p.status);
+        int c_first = blockIdx.x, c_last = blockIdx.x;
+        bool mine = true;
+        if (!whole) {
+            c_first = share_of(total, n_cta, x.start + ITEM_TILES);
+            c_last = share_of(total, n_cta, x.start + ITEM_TILES + x.g.nt - 1);
+            __threadfence();
+            if (jl == 0) *last_flag = atomicAdd(p.counters + static_cast<int64_t>(x.b) * p.hkv + x.h, 1) == c_last - c_first;
+            if (L::N_JOIN > 1) asm volatile("bar.sync 2, 128;" ::: "memory");
+            else __syncwarp();
+            mine = *last_flag != 0;
+            __threadfence();
+        }
+        if (mine) {
+            auto piece = [&](int c) { return whole ? slot_of(c, 2 + (joins & 1)) : slot_of(c, c == c_first ? 1 : 0); };
+            auto pk2 = [](float a, float b2) { return F16 ? pack_f16x2(a, b2) : pack_bf16x2(a, b2); };
+            const int n_work = R * (D / 8);
+            for (int i = jl; i < n_work; i += 32 * L::N_JOIN) {
+                const int row = i % R, u = i / R;      // 8 channels of a row
+                float mm = -INFINITY, ll = 0.f;
+                if (!whole) {
+                    for (int c = c_first; c <= c_last; ++c) mm = fmaxf(mm, __ldcg(piece(c) + 128 * D + row));
+                    if (mm == -INFINITY) mm = 0.f;
+                }
+                float4 a0 = make_float4(0.f, 0.f, 0.f, 0.f), a1 = a0;
+                for (int c = c_first; c <= c_last; ++c) {
+                    const float* pc = piece(c);
+                    const float4* src = reinterpret_cast<const float4*>(pc) + 2 * u * 128 + row;
+                    float4 v0[4], v1[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (k < copies) {
+                            v0[k] = __ldcg(src + k * rows);
+                            v1[k] = __ldcg(src + k * rows + 128);
+                        }
+                    const float lc = __ldcg(pc + 128 * D + 128 + row);
+                    const float fc = whole ? 1.f : ex2f(__ldcg(pc + 128 * D + row) - mm);
+                    ll = fmaf(lc, fc, ll);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (k < copies) {
+                            a0.x = fmaf(v0[k].x, fc, a0.x); a0.y = fmaf(v0[k].y, fc, a0.y); a0.z = fmaf(v0[k].z, fc, a0.z); a0.w = fmaf(v0[k].w, fc, a0.w);
+                            a1.x = fmaf(v1[k].x, fc, a1.x); a1.y = fmaf(v1[k].y, fc, a1.y); a1.z = fmaf(v1[k].z, fc, a1.z); a1.w = fmaf(v1[k].w, fc, a1.w);
+                        }
+                }
+                const float inv = ll > 0.f ? (V8 ? p.evs : 1.f) / ll : 0.f;
+                uint16_t* out = p.o + static_cast<int64_t>(x.g.tok0 + row / p.G) * p.o_st + static_cast<int64_t>(x.h * p.G + row % p.G) * p.o_sh + 8 * u;
+                *reinterpret_cast<uint4*>(out) = make_uint4(pk2(a0.x * inv, a0.y * inv), pk2(a0.z * inv, a0.w * inv),
+                                                            pk2(a1.x * inv, a1.y * inv), pk2(a1.z * inv, a1.w * inv));
+            }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_JOINED));
+        if (L::N_JOIN > 1 && !whole) asm volatile("bar.sync 2, 128;" ::: "memory");   // the flag has been read
+        ++joins;
     };
 
     if (warp == 0 || warp == 3) {
@@ -406,14 +566,14 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
             const uint64_t qa = smem_desc(base + L::SM_Q, 16, SBO, SW), qb = smem_desc(base + L::SM_Q + L::PLANE, 16, SBO, SW);
             int j = 0;
             while (w.next(p)) {
-                mbar_wait(bar(B_QREADY), w.segment & 1, abort_flag, p.status);
+                mbar_wait(bar(B_QFULL), w.segment & 1, abort_flag, p.status);
                 auto issue_pv = [&](int jj, bool acc) {
                     const int vs = jj % L::NV;
                     mbar_wait(bar(B_PREADY), jj & 1, abort_flag, p.status);
-                    if (V8) mbar_wait(bar(B_VREADY), jj & 1, abort_flag, p.status);
+                    if (V8) mbar_wait(bar(B_VREADY + (jj & 1)), (jj >> 1) & 1, abort_flag, p.status);
                     else mbar_wait(bar(B_VREADY + vs), (jj / L::NV) & 1, abort_flag, p.status);
                     tc_fence_after();
-                    const uint32_t vt = base + (V8 ? L::SM_V16 : L::SM_V + vs * L::VSLOT);
+                    const uint32_t vt = base + (V8 ? L::SM_V16 + (jj & 1) * 2 * L::PLANE : L::SM_V + vs * L::VSLOT);
 #pragma unroll
                     for (int ks = 0; ks < 8; ++ks)     // 16 keys per step
                         mma_ts(tmem + T_O, tmem + T_P + 8 * ks, smem_desc(vt + ks * 2048, 16384, 1024, 2), ID_PV, acc || ks > 0);
@@ -422,7 +582,7 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
                         for (int ks = 0; ks < 8; ++ks)
                             mma_ts(tmem + T_O, tmem + T_P2 + 8 * ks, smem_desc(vt + ks * 2048, 16384, 1024, 2), ID_PV, 1u);
                     }
-                    if (!V8) tc_commit(bar(B_VEMPTY + vs));
+                    tc_commit(bar(V8 ? B_CEMPTY + (jj & 1) : B_VEMPTY + vs));
                     tc_commit(bar(B_ODONE));
                 };
                 for (int t = w.t0; t < w.t1; ++t, ++j) {
@@ -440,25 +600,44 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
                     for (int ks = 0; ks < D / 32; ++ks) mma_i8(tmem + T_S2, qb + 2 * ks, ka + 2 * ks, ID_S, 1u);
                     tc_commit(bar(B_SFULL));
                     tc_commit(bar(B_KEMPTY + s));
+                    if (t + 1 == w.t1) tc_commit(bar(B_QEMPTY));   // the next item's Q may land
                     if (t > w.t0) issue_pv(j - 1, t - 1 > w.t0);
                 }
-                // the item's last product before the next item's Q may be laid down
+                // the item's last product: its epilogue waits for it
                 issue_pv(j - 1, w.t1 - w.t0 > 1);
             }
         }
     } else if (warp == 2) {
-        // ================= bf16 V: rows that no new token sees are zeroed in shared memory =================
-        if (!V8) {
-            int j = 0;
-            while (w.next(p)) {
+        // ================= Q of each item; bf16 V: rows that no new token sees are zeroed in shared memory; 8-bit V: pieces =================
+        [[maybe_unused]] int j = 0, joins = 0;
+        Walk before = w;
+        bool had = false;
+        while (w.next(p)) {
+            {
+                const int R = w.g.n * p.G, copies = copies_of(R), rows = 128 / copies;
+                const int64_t row0 = static_cast<int64_t>(w.g.tok0) * p.hkv * p.G + static_cast<int64_t>(w.h) * R;
+                if (lane == 0) {
+                    if (w.segment > 0) mbar_wait(bar(B_QEMPTY), (w.segment - 1) & 1, abort_flag, p.status);
+                    mbar_expect_tx(bar(B_QFULL), static_cast<uint32_t>(2 * copies * R * D));
+                }
+                __syncwarp();
+                if (lane < 2 * copies)
+                    bulk_load(base + L::SM_Q + (lane & 1) * L::PLANE + (lane >> 1) * rows * D, ((lane & 1) ? p.qb : p.qa) + row0 * D,
+                              static_cast<uint32_t>(R * D), bar(B_QFULL));
+            }
+            if constexpr (V8) {
+                if (had) join(before, joins);     // the item before, while this one's tiles run
+                before = w;
+                had = true;
+            } else {
                 for (int t = w.t0; t < w.t1; ++t, ++j) {
                     const int s = j % L::NV, pos = w.pos(p, t);
                     mbar_wait(bar(B_VFULL + s), (j / L::NV) & 1, abort_flag, p.status);
                     if (pos + BN > w.g.L || (pos <= w.g.first - p.window && pos + BN > p.sinks)) {
-                        for (int r = 0; r < BN; ++r) {
+                        for (int r = lane >> 4; r < BN; r += 2) {
                             if (wanted(w.g, pos + r, 1)) continue;
-                            if (lane < D / 8)
-                                sts128(base + L::SM_V + s * L::VSLOT + (lane >> 3) * 16384 + r * 128 + (lane & 7) * 16, make_uint4(0u, 0u, 0u, 0u));
+                            if ((lane & 15) < D / 8)
+                                sts128(base + L::SM_V + s * L::VSLOT + ((lane & 15) >> 3) * 16384 + r * 128 + (lane & 7) * 16, make_uint4(0u, 0u, 0u, 0u));
                         }
                         fence_async_smem();
                     }
@@ -467,129 +646,115 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
                 }
             }
         }
+        if constexpr (V8) {
+            if (had) join(before, joins);
+        }
+    } else if (!V8 && warp >= L::W_JOIN) {
+        int joins = 0;
+        while (w.next(p)) join(w, joins);
     } else if (warp < 8) {
         // ================= Q, softmax, epilogue: thread = TMEM lane =================
-        const int wq = warp - 4, m_row = 32 * wq + lane, t128 = tid - 128;
+        const int wq = warp - 4, m_row = 32 * wq + lane;
         const uint32_t lane_addr = static_cast<uint32_t>(32 * wq) << 16;
-        float* s_eq = reinterpret_cast<float*>(smem + L::SM_ROW);
-        float* s_m = s_eq + 128;
-        float* s_l = s_eq + 256;
-        int j = 0;
+        float* s_m = reinterpret_cast<float*>(smem + L::SM_ROW);
+        float* s_l = s_m + 128;
+        int j = 0, joins = 0;
+        auto scale_of = [&](const Walk& x) {
+            const int R = x.g.n * p.G, r = m_row & (128 / copies_of(R) - 1);
+            return r < R ? __ldg(p.eq + static_cast<int64_t>(x.g.tok0) * p.hkv * p.G + static_cast<int64_t>(x.h) * R + r) : 0.f;
+        };
+        float eq_next;
+        {
+            Walk x = w;
+            eq_next = x.next(p) ? scale_of(x) : 0.f;
+        }
         while (w.next(p)) {
             const Geo& g = w.g;
             const int R = g.n * p.G;
-            const int copies = R <= 32 ? 4 : R <= 64 ? 2 : 1;
+            const int copies = copies_of(R);
             const int rows = 128 / copies;                // a copy's lanes
             const int r = m_row & (rows - 1);             // the thread's query row: token r / G, head r % G of the group
             const int copy = m_row / rows;
-            // ---- Q's planes, for every copy ----
-            {
-                constexpr int TPR = D / 16, RPP = 128 / TPR;
-                const int ql = t128 % TPR;
-                for (int q0 = 0; q0 < rows; q0 += RPP) {
-                    const int qr = q0 + t128 / TPR;
-                    const bool ok = qr < R;
-                    const int tok = __ldg(p.cu + w.b) + (ok ? qr / p.G : 0), hd = w.h * p.G + (ok ? qr % p.G : 0);
-                    float x[16];
-                    uint4 raw16[2];
-                    load16<F16>(p.q + static_cast<int64_t>(tok) * p.q_st + static_cast<int64_t>(hd) * p.q_sh + ql * 16, x, raw16);
-                    const float qscale = D == 64 ? 0.18033688011112042f : 0.12751743082459868f;   // log2(e) / sqrt(D)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = ok ? __fmul_rn(x[i], qscale) : 0.f;
-                    rotate16<TPR>(x, ql, D == 64 ? 0.125f : 0.08838834764831845f);
-                    const float e = __fmul_rn(fmaxf(row_amax16<TPR>(x), 1e-30f), INV127);
-                    uint4 wa, wb;
-                    int8_planes16(x, e, wa, wb);
-                    if (qr < rows)
-                        for (int c = 0; c < copies; ++c) {
-                            const int mr = c * rows + qr;
-                            const uint32_t at = base + L::SM_Q + mr * D + ((ql ^ (D == 128 ? mr & 7 : (mr >> 1) & 3)) << 4);
-                            sts128(at, wa);
-                            sts128(at + L::PLANE, wb);
-                            if (ql == 0) s_eq[mr] = e * 0.00390625f;
-                        }
-                }
-                if (copies > 1) {       // P's columns of the other copies' keys stay zero
-                    uint32_t z[32];
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) z[i] = 0u;
-                    tmem_st32(tmem + lane_addr + T_P, z);
-                    tmem_st32(tmem + lane_addr + T_P + 32, z);
-                    if (TERMS == 2) {
-                        tmem_st32(tmem + lane_addr + T_P2, z);
-                        tmem_st32(tmem + lane_addr + T_P2 + 32, z);
-                    }
-                    tmem_wait_st();
-                }
-                fence_async_smem();
-                tc_fence_before();
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                mbar_arrive(bar(B_QREADY));
+            const bool live = r < R;
+            const float eq = eq_next;
+            {   // the next item's scale, while this one's tiles run
+                Walk x = w;
+                eq_next = x.next(p) ? scale_of(x) : 0.f;
             }
-            const float eq = s_eq[m_row];
             const int rpos = g.first + r / p.G;           // the row's position (rows past R: never written)
+            if (copies > 1) {       // P's columns of the other copies' keys stay zero
+                uint32_t z[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) z[i] = 0u;
+                tmem_st32(tmem + lane_addr + T_P, z);
+                tmem_st32(tmem + lane_addr + T_P + 32, z);
+                if (TERMS == 2) {
+                    tmem_st32(tmem + lane_addr + T_P2, z);
+                    tmem_st32(tmem + lane_addr + T_P2 + 32, z);
+                }
+                tmem_wait_st();
+            }
             float m_run = -INFINITY, l_run = 0.f;
             const int seg0 = j;
-            // one tile: NCH chunks of 32 keys from the copy's first
-            auto tile = [&](auto nch, int t) {
-                constexpr int NCH = decltype(nch)::value;
-                const int s = j % L::NK, pos = w.pos(p, t), k0 = copy * 32 * NCH;
+            // one tile: a copy's 32, 64 or 128 keys, 32 at a time
+            const int n_ch = 4 / copies;
+            auto tile = [&](auto one, int t) {
+                constexpr bool KEEP = decltype(one)::value;
+                const int nch = KEEP ? 1 : n_ch;
+                const int s = j % L::NK, pos = w.pos(p, t), k0 = copy * 32 * nch;
                 const bool need_mask = pos + BN - 1 > g.first || (pos <= g.L - 1 - p.window && pos + BN > p.sinks);
                 const int kmax = rpos - pos, kmin = rpos - p.window + 1 - pos, ksink = p.sinks - pos;
                 mbar_wait(bar(B_SFULL), j & 1, abort_flag, p.status);
                 tc_fence_after();
-                float x[32 * NCH];
-                float mx = -INFINITY;
-#pragma unroll
-                for (int c = 0; c < NCH; ++c) {
+                // Chunk c's logits over the row's scale, from S1, S2 and the keys' scales. One chunk is kept in
+                // registers; more would spill (168 a thread), and are made twice instead: for the maximum and for P.
+                auto logits = [&](int c, float (&x)[32]) {
                     uint32_t a[32], b2[32];
                     tmem_ld32(tmem + lane_addr + T_S1 + k0 + 32 * c, a);
                     tmem_ld32(tmem + lane_addr + T_S2 + k0 + 32 * c, b2);
-                    uint4 ew[4];
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) ew[u] = lds128(base + L::SM_EK + s * 256 + 2 * (k0 + 32 * c) + 16 * u);
+                    const uint4* es = reinterpret_cast<const uint4*>(smem + L::SM_EK + s * 256 + 2 * (k0 + 32 * c));
+                    const uint4 ew[4] = {es[0], es[1], es[2], es[3]};
                     tmem_wait_ld();
                     const uint32_t* ep = reinterpret_cast<const uint32_t*>(ew);
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
                         const float ekf = __uint_as_float((e & 1) ? (ep[e >> 1] & 0xFFFF0000u) : (ep[e >> 1] << 16));
-                        x[32 * c + e] = static_cast<float>(static_cast<int>(a[e]) * 256 + static_cast<int>(b2[e])) * ekf;
+                        x[e] = static_cast<float>(static_cast<int>(a[e]) * 256 + static_cast<int>(b2[e])) * ekf;
                     }
                     if (need_mask) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e) {
                             const int k = k0 + 32 * c + e;
-                            if (k > kmax || (k < kmin && k >= ksink)) x[32 * c + e] = -INFINITY;
+                            if (k > kmax || (k < kmin && k >= ksink)) x[e] = -INFINITY;
                         }
                     }
+                };
+                auto release = [&]() {                 // the logits are in registers: the next tile's may come
+                    tc_fence_before();
+                    mbar_arrive(bar(B_SEMPTY));
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(B_KEMPTY + s));
+                };
+                float x[32];
+                float mx = -INFINITY, mx1 = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < nch; ++c) {
+                    logits(c, x);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) mx = fmaxf(mx, x[32 * c + e]);
+                    for (int e = 0; e < 32; e += 4) {
+                        mx = max3f(mx, x[e], x[e + 1]);
+                        mx1 = max3f(mx1, x[e + 2], x[e + 3]);
+                    }
                 }
-                tc_fence_before();
-                mbar_arrive(bar(B_SEMPTY));            // the logits are in registers: the next tile's may come
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(B_KEMPTY + s));
-                const float m_cand = fmaxf(m_run, mx * eq);
+                if (KEEP) release();
+                const float m_cand = max3f(m_run, mx * eq, mx1 * eq);
                 const float m_new = m_cand > m_run + LAZY ? m_cand : m_run;
                 const float m_use = m_new == -INFINITY ? 0.f : m_new;
-                const float alpha = ex2f(m_run - m_use);
-                float sum = 0.f, sum2 = 0.f;
-                uint32_t pk[16 * NCH], pk2nd[TERMS == 2 ? 16 * NCH : 1];
-#pragma unroll
-                for (int e = 0; e < 32 * NCH; e += 2) {
-                    const float p0 = ex2f(fmaf(x[e], eq, -m_use)), p1 = ex2f(fmaf(x[e + 1], eq, -m_use));
-                    sum += p0;
-                    sum2 += p1;
-                    pk[e >> 1] = V8 ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1);
-                    if (TERMS == 2)
-                        pk2nd[e >> 1] = pack_bf16x2(p0 - __uint_as_float(pk[e >> 1] << 16), p1 - __uint_as_float(pk[e >> 1] & 0xFFFF0000u));
-                }
-                l_run = l_run * alpha + (sum + sum2);
-                m_run = m_new;
+                const float alpha = m_run == -INFINITY ? 1.f : ex2f(m_run - m_use);   // nothing summed yet: nothing to rescale
                 if (j > seg0) {                        // P's columns and O: the product before has read and written them
                     mbar_wait(bar(B_ODONE), (j - 1) & 1, abort_flag, p.status);
                     tc_fence_after();
-                    if (__any_sync(0xffffffffu, alpha != 1.0f)) {
+                    if (__any_sync(0xffffffffu, live && alpha != 1.0f)) {
 #pragma unroll
                         for (int c = 0; c < D / 32; ++c) {
                             uint32_t ov[32];
@@ -601,163 +766,102 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
                         }
                     }
                 }
-#pragma unroll
-                for (int c = 0; c < NCH; ++c) {
-                    uint32_t pc[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) pc[e] = pk[16 * c + e];
-                    tmem_st16(tmem + lane_addr + T_P + (k0 + 32 * c) / 2, pc);
-                    if (TERMS == 2) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) pc[e] = pk2nd[16 * c + e];
-                        tmem_st16(tmem + lane_addr + T_P2 + (k0 + 32 * c) / 2, pc);
+                float sum = 0.f, sum2 = 0.f;
+#pragma unroll 1
+                for (int c = 0; c < nch; ++c) {
+                    uint32_t pk[16], lo[16];
+                    if (!KEEP) {
+                        logits(c, x);
+                        if (c == nch - 1) release();
                     }
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float p0 = ex2f(fmaf(x[e], eq, -m_use)), p1 = ex2f(fmaf(x[e + 1], eq, -m_use));
+                        sum += p0;
+                        sum2 += p1;
+                        pk[e >> 1] = V8 ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1);
+                        if (TERMS == 2)
+                            lo[e >> 1] = pack_bf16x2(p0 - __uint_as_float(pk[e >> 1] << 16), p1 - __uint_as_float(pk[e >> 1] & 0xFFFF0000u));
+                    }
+                    tmem_st16(tmem + lane_addr + T_P + (k0 + 32 * c) / 2, pk);
+                    if (TERMS == 2) tmem_st16(tmem + lane_addr + T_P2 + (k0 + 32 * c) / 2, lo);
                 }
+                l_run = l_run * alpha + (sum + sum2);
+                m_run = m_new;
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(bar(B_PREADY));
             };
             for (int t = w.t0; t < w.t1; ++t, ++j) {
-                if (copies == 4) tile(std::integral_constant<int, 1>{}, t);
-                else if (copies == 2) tile(std::integral_constant<int, 2>{}, t);
-                else tile(std::integral_constant<int, 4>{}, t);
+                if (copies == 4) tile(std::true_type{}, t);
+                else tile(std::false_type{}, t);
             }
-            // ---- epilogue: the copies' sums together, then the output or this CTA's piece of it ----
+            // ---- epilogue: O out, or O and its statistics to a piece that another warp joins ----
             mbar_wait(bar(B_ODONE), (j - 1) & 1, abort_flag, p.status);
             tc_fence_after();
-            s_m[m_row] = m_run;
-            s_l[m_row] = l_run;
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            float mt = -INFINITY;
-            for (int c = 0; c < copies; ++c) mt = fmaxf(mt, s_m[c * rows + r]);
-            const float mu = mt == -INFINITY ? 0.f : mt;
-            float lt = 0.f;
-            for (int c = 0; c < copies; ++c) lt += s_l[c * rows + r] * ex2f(s_m[c * rows + r] - mu);
-            const float f = ex2f(m_run - mu);           // 0 for a copy that saw no key
-            // the item's place in the list: which CTAs share it
-            const int64_t gs = static_cast<int64_t>(g0) + (j - (w.t1 - w.t0)) - w.t0;   // its first tile (j counts this CTA's tiles)
-            const int c_first = share_of(total, n_cta, gs), c_last = share_of(total, n_cta, gs + g.nt - 1);
-            const bool whole = c_first == c_last;
-            float* part = p.parts + static_cast<int64_t>(2 * blockIdx.x + (w.t0 > 0 ? 0 : 1)) * (128 * D + 256);
-            // a row's 16-byte unit u of the sums in shared memory, swizzled so that a quarter warp's rows fall in other banks
-            auto sum_at = [&](int row, int u) { return base + L::SM_Q + row * (4 * D) + ((u ^ (row & 7)) << 4); };
-            const int tok0 = __ldg(p.cu + w.b);
-            auto out_at = [&](int row) { return p.o + static_cast<int64_t>(tok0 + row / p.G) * p.o_st + static_cast<int64_t>(w.h * p.G + row % p.G) * p.o_sh; };
-            auto pk2 = [](float a, float b2) { return F16 ? pack_f16x2(a, b2) : pack_bf16x2(a, b2); };
-            if (copies > 1) {
-                // each copy adds a column block of its own at a time, so nobody meets anybody
-                const int blocks = D / 32 / copies > 0 ? D / 32 / copies : 1;     // 32-column blocks per turn
-                for (int turn = 0; turn < copies; ++turn) {
-                    for (int k = 0; k < blocks; ++k) {
-                        const int blk = ((copy + turn) % copies) * blocks + k;
-                        if (blk < D / 32) {
-                            uint32_t ov[32];
-                            tmem_ld32(tmem + lane_addr + T_O + 32 * blk, ov);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int u = 0; u < 8; ++u) {
-                                float4 v = make_float4(__uint_as_float(ov[4 * u]) * f, __uint_as_float(ov[4 * u + 1]) * f,
-                                                       __uint_as_float(ov[4 * u + 2]) * f, __uint_as_float(ov[4 * u + 3]) * f);
-                                const uint32_t at = sum_at(r, 8 * blk + u);
-                                if (turn > 0) {
-                                    const float4 y = as_float4(lds128(at));
-                                    v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
-                                }
-                                sts128(at, as_uint4(v));
-                            }
-                        }
-                    }
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
-                }
-                if (copy == 0) {
-                    s_m[r] = mt;
-                    s_l[r] = lt;
-                }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                for (int i = t128; i < R * (D / 8); i += 128) {
-                    const int row = i / (D / 8), u = i % (D / 8);
-                    const float4 x = as_float4(lds128(sum_at(row, 2 * u))), y = as_float4(lds128(sum_at(row, 2 * u + 1)));
-                    if (whole) {
-                        const float l = s_l[row], inv = l > 0.f ? (V8 ? p.evs : 1.f) / l : 0.f;
-                        *reinterpret_cast<uint4*>(out_at(row) + 8 * u) =
-                            make_uint4(pk2(x.x * inv, x.y * inv), pk2(x.z * inv, x.w * inv), pk2(y.x * inv, y.y * inv), pk2(y.z * inv, y.w * inv));
-                    } else {
-                        float4* d = reinterpret_cast<float4*>(part + row * D + 8 * u);
-                        d[0] = x;
-                        d[1] = y;
-                    }
-                }
-                if (!whole && t128 < R) {
-                    part[128 * D + t128] = s_m[t128];
-                    part[128 * D + 128 + t128] = s_l[t128];
-                }
-            } else {
+            if (copies == 1 && is_whole(w)) {       // the whole row is this thread's
+                auto pk2 = [](float a, float b2) { return F16 ? pack_f16x2(a, b2) : pack_bf16x2(a, b2); };
                 const float inv = l_run > 0.f ? (V8 ? p.evs : 1.f) / l_run : 0.f;
-                uint16_t* orow = out_at(r < R ? r : 0);
-#pragma unroll
+                const int row = live ? r : 0;
+                uint16_t* orow = p.o + static_cast<int64_t>(g.tok0 + row / p.G) * p.o_st + static_cast<int64_t>(w.h * p.G + row % p.G) * p.o_sh;
+#pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
                     uint32_t ov[32];
                     tmem_ld32(tmem + lane_addr + T_O + 32 * c, ov);
                     tmem_wait_ld();
-                    if (r < R) {
-                        if (whole) {
+                    if (live) {
 #pragma unroll
-                            for (int u = 0; u < 4; ++u) {
-                                uint4 v;
-                                v.x = pk2(__uint_as_float(ov[8 * u]) * inv, __uint_as_float(ov[8 * u + 1]) * inv);
-                                v.y = pk2(__uint_as_float(ov[8 * u + 2]) * inv, __uint_as_float(ov[8 * u + 3]) * inv);
-                                v.z = pk2(__uint_as_float(ov[8 * u + 4]) * inv, __uint_as_float(ov[8 * u + 5]) * inv);
-                                v.w = pk2(__uint_as_float(ov[8 * u + 6]) * inv, __uint_as_float(ov[8 * u + 7]) * inv);
-                                *reinterpret_cast<uint4*>(orow + 32 * c + 8 * u) = v;
-                            }
-                        } else {
-                            uint4* d = reinterpret_cast<uint4*>(part + r * D + 32 * c);
-#pragma unroll
-                            for (int u = 0; u < 8; ++u) d[u] = make_uint4(ov[4 * u], ov[4 * u + 1], ov[4 * u + 2], ov[4 * u + 3]);
+                        for (int u = 0; u < 4; ++u) {
+                            uint4 v;
+                            v.x = pk2(__uint_as_float(ov[8 * u]) * inv, __uint_as_float(ov[8 * u + 1]) * inv);
+                            v.y = pk2(__uint_as_float(ov[8 * u + 2]) * inv, __uint_as_float(ov[8 * u + 3]) * inv);
+                            v.z = pk2(__uint_as_float(ov[8 * u + 4]) * inv, __uint_as_float(ov[8 * u + 5]) * inv);
+                            v.w = pk2(__uint_as_float(ov[8 * u + 6]) * inv, __uint_as_float(ov[8 * u + 7]) * inv);
+                            *reinterpret_cast<uint4*>(orow + 32 * c + 8 * u) = v;
                         }
                     }
                 }
-                if (!whole && r < R) {
-                    part[128 * D + r] = m_run;
-                    part[128 * D + 128 + r] = l_run;
+                tc_fence_before();
+                continue;
+            }
+            // the copies under one reference, so that a piece is plain sums
+            s_m[m_row] = m_run;
+            s_l[m_row] = l_run;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            float mt = -INFINITY, lt = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k < copies) mt = fmaxf(mt, s_m[k * rows + r]);
+            const float mu = mt == -INFINITY ? 0.f : mt;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k < copies) lt = fmaf(s_l[k * rows + r], ex2f(s_m[k * rows + r] - mu), lt);
+            const float f = ex2f(m_run - mu);
+            float* part = slot_of(blockIdx.x, is_whole(w) ? 2 + (joins & 1) : w.t0 > 0 ? 0 : 1);
+            if (live && copy == 0) {
+                part[128 * D + r] = mt;
+                part[128 * D + 128 + r] = lt;
+            }
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t ov[32];
+                tmem_ld32(tmem + lane_addr + T_O + 32 * c, ov);
+                tmem_wait_ld();
+                if (live) {
+                    uint4* d = reinterpret_cast<uint4*>(part) + 8 * c * 128 + m_row;
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        d[128 * u] = make_uint4(__float_as_uint(__uint_as_float(ov[4 * u]) * f), __float_as_uint(__uint_as_float(ov[4 * u + 1]) * f),
+                                          __float_as_uint(__uint_as_float(ov[4 * u + 2]) * f), __float_as_uint(__uint_as_float(ov[4 * u + 3]) * f));
                 }
             }
             tc_fence_before();
-            if (!whole) {
-                __threadfence();
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                if (t128 == 0) *last_flag = atomicAdd(p.counters + static_cast<int64_t>(w.b) * p.hkv + w.h, 1) == c_last - c_first;
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                if (*last_flag) {       // every piece is there: add them in list order
-                    __threadfence();
-                    auto piece = [&](int c) { return p.parts + static_cast<int64_t>(2 * c + (c == c_first ? 1 : 0)) * (128 * D + 256); };
-                    if (t128 < R) {
-                        float mm = -INFINITY, ll = 0.f;
-                        for (int c = c_first; c <= c_last; ++c) mm = fmaxf(mm, __ldcg(piece(c) + 128 * D + t128));
-                        if (mm == -INFINITY) mm = 0.f;
-                        for (int c = c_first; c <= c_last; ++c)
-                            ll += __ldcg(piece(c) + 128 * D + 128 + t128) * ex2f(__ldcg(piece(c) + 128 * D + t128) - mm);
-                        s_m[t128] = mm;
-                        s_l[t128] = ll > 0.f ? (V8 ? p.evs : 1.f) / ll : 0.f;
-                    }
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
-                    for (int i = t128; i < R * (D / 8); i += 128) {
-                        const int row = i / (D / 8), u = i % (D / 8);
-                        const float mm = s_m[row], inv = s_l[row];
-                        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-                        for (int c = c_first; c <= c_last; ++c) {
-                            const float fc = ex2f(__ldcg(piece(c) + 128 * D + row) - mm);
-                            const float4* src = reinterpret_cast<const float4*>(piece(c) + row * D + 8 * u);
-                            const float4 a = __ldcg(src), b2 = __ldcg(src + 1);
-                            x.x = fmaf(a.x, fc, x.x); x.y = fmaf(a.y, fc, x.y); x.z = fmaf(a.z, fc, x.z); x.w = fmaf(a.w, fc, x.w);
-                            y.x = fmaf(b2.x, fc, y.x); y.y = fmaf(b2.y, fc, y.y); y.z = fmaf(b2.z, fc, y.z); y.w = fmaf(b2.w, fc, y.w);
-                        }
-                        *reinterpret_cast<uint4*>(out_at(row) + 8 * u) =
-                            make_uint4(pk2(x.x * inv, x.y * inv), pk2(x.z * inv, x.w * inv), pk2(y.x * inv, y.y * inv), pk2(y.z * inv, y.w * inv));
-                    }
-                }
-            }
-            asm volatile("bar.sync 1, 128;" ::: "memory");   // the sums' memory is Q's again
+            // (the arrival releases the piece to the joining warps; what other CTAs see is their fence's matter)
+            // one piece at a time is handed over: the joining warp tells phases apart by their parity, and the slot
+            // of two pieces back is then free for the next
+            if (joins >= 1) mbar_wait(bar(B_JOINED), (joins - 1) & 1, abort_flag, p.status);
+            mbar_arrive(bar(B_PIECE));
+            ++joins;
         }
     } else {
         // ================= 8-bit V: two planes -> fp16 rows, MN-major, swizzled; dead rows are zeros =================
@@ -769,33 +873,42 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
                 const int s = j % L::NV, pos = w.pos(p, t);
                 const bool cut = pos + BN > w.g.L || (pos <= w.g.first - p.window && pos + BN > p.sinks);
                 mbar_wait(bar(B_VFULL + s), (j / L::NV) & 1, abort_flag, p.status);
-                if (j > 0) mbar_wait(bar(B_ODONE), (j - 1) & 1, abort_flag, p.status);   // the product before has read its rows
-                const uint32_t src = base + L::SM_V + s * L::VSLOT;
-#pragma unroll 4
-                for (int i = c0; i < BN * UPR; i += 128) {
-                    const int r = i / UPR, u = i % UPR;
-                    const uint4 a = lds128(src + r * D + u * 16), b2 = lds128(src + L::PLANE + r * D + u * 16);
-                    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b2.x, b2.y, b2.z, b2.w};
-                    uint32_t o[8];
-                    const bool live = !cut || wanted(w.g, pos + r, 1);
+                if (j > 1) mbar_wait(bar(B_CEMPTY + (j & 1)), ((j >> 1) - 1) & 1, abort_flag, p.status);   // the product two tiles back has read its rows
+                const uint4* src = reinterpret_cast<const uint4*>(smem + L::SM_V + s * L::VSLOT);
+                uint4* dst = reinterpret_cast<uint4*>(smem + L::SM_V16 + (j & 1) * 2 * L::PLANE);
+                // four units' loads at a time, then their arithmetic: one warp a scheduler has only its own
+                // instructions to hide a latency with
+                for (int i0 = c0; i0 < BN * UPR; i0 += 4 * 128) {
+                    uint4 a[4], b2[4];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        uint32_t ha, hb;
-                        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(ha) : "h"(static_cast<uint16_t>(aw[k >> 1] >> (16 * (k & 1)))));
-                        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hb) : "h"(static_cast<uint16_t>(bw[k >> 1] >> (16 * (k & 1)))));
-                        uint32_t x;
-                        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(x) : "r"(hb), "r"(0x30003000u), "r"(ha));   // a + b / 8
-                        o[k] = live ? x : 0u;
+                    for (int q = 0; q < 4; ++q) {
+                        a[q] = src[i0 + 128 * q];
+                        b2[q] = src[L::PLANE / 16 + i0 + 128 * q];
                     }
-                    const uint32_t dst = base + L::SM_V16 + (u >> 2) * 16384 + r * 128;
-                    const int ch = 2 * (u & 3);
-                    sts128(dst + ((ch ^ (r & 7)) << 4), make_uint4(o[0], o[1], o[2], o[3]));
-                    sts128(dst + (((ch + 1) ^ (r & 7)) << 4), make_uint4(o[4], o[5], o[6], o[7]));
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int i = i0 + 128 * q, r = i / UPR, u = i % UPR;
+                        const uint32_t aw[4] = {a[q].x, a[q].y, a[q].z, a[q].w}, bw[4] = {b2[q].x, b2[q].y, b2[q].z, b2[q].w};
+                        uint32_t o[8];
+                        const bool keep = !cut || wanted(w.g, pos + r, 1);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            uint32_t ha, hb, x;
+                            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(ha) : "h"(static_cast<uint16_t>(aw[k >> 1] >> (16 * (k & 1)))));
+                            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hb) : "h"(static_cast<uint16_t>(bw[k >> 1] >> (16 * (k & 1)))));
+                            asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(x) : "r"(hb), "r"(0x30003000u), "r"(ha));   // a + b / 8
+                            o[k] = keep ? x : 0u;
+                        }
+                        uint4* row = dst + (u >> 2) * 1024 + r * 8;
+                        const int ch = 2 * (u & 3);
+                        row[ch ^ (r & 7)] = make_uint4(o[0], o[1], o[2], o[3]);
+                        row[(ch + 1) ^ (r & 7)] = make_uint4(o[4], o[5], o[6], o[7]);
+                    }
                 }
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(bar(B_VREADY));
+                    mbar_arrive(bar(B_VREADY + (j & 1)));
                     mbar_arrive(bar(B_VEMPTY + s));
                 }
             }
@@ -832,9 +945,29 @@ EncodeFn encode_fn() {
     return fn;
 }
 
+// the workspace: pieces, Q's planes and scales, counters (bytes from its start, each on 16)
+struct Work {
+    int64_t parts, qa, qb, eq, counters, total;
+};
+Work chunk_work(int batch, int total, int heads, int hkv, int D, int ctas) {
+    auto up = [](int64_t x) { return (x + 15) / 16 * 16; };
+    const int64_t rows = static_cast<int64_t>(total) * heads;
+    Work w;
+    w.parts = 0;
+    w.qa = up(static_cast<int64_t>(csm100::SLOTS) * ctas * (128 * D + 256) * 4);
+    w.qb = up(w.qa + rows * D);
+    w.eq = up(w.qb + rows * D);
+    w.counters = up(w.eq + rows * 4);
+    w.total = up(w.counters + static_cast<int64_t>(batch) * hkv * 4);
+    return w;
+}
+
 template <int D, bool V8, bool F16>
 int launch(const csm100::Params& p, const CUtensorMap& vmap, int ctas, cudaStream_t st) {
     using L = csm100::Lay<D, V8>;
+    const int heads = p.hkv * p.G, rpb = NT / (D / 16);
+    const int64_t rows = static_cast<int64_t>(p.total) * heads;
+    csm100::chunk_q_kernel<D, F16><<<static_cast<unsigned>((rows + rpb - 1) / rpb), NT, 0, st>>>(p, heads, rows);
     auto kern = csm100::chunk_sm100_kernel<D, V8, F16>;
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
     kern<<<ctas, L::NTHREADS, L::BYTES, st>>>(p, vmap);
@@ -843,13 +976,18 @@ int launch(const csm100::Params& p, const CUtensorMap& vmap, int ctas, cudaStrea
 
 }  // namespace
 
+extern "C" int64_t fold_chunk_workspace_bytes(int batch, int total, int n_heads, int n_kv_heads, int head_dim, int ctas) {
+    if (batch <= 0 || total <= 0 || n_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 || ctas <= 0) return 0;
+    return chunk_work(batch, total, n_heads, n_kv_heads, head_dim, ctas).total;
+}
+
 extern "C" int fold_chunk_sm100(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* o, int64_t o_token_stride, int64_t o_head_stride,
                                 int is_f16, const int32_t* cu_seqlens, const int32_t* seq_lens, int batch, int total, int n_heads, int n_kv_heads,
                                 int head_dim, const int32_t* page_table, int pages_per_request, int page_size, int64_t pool_rows, const int8_t* ka,
                                 const int8_t* kb, const void* va, const void* vb, const void* ek, float v_scale, int window, int sinks, int others, int ctas,
-                                int32_t* counters, float* parts, int32_t* status, void* stream) {
+                                void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
     FOLD_CHECK_ARG(head_dim == 64 || head_dim == 128, "head_dim %d: the cache holds 64 or 128", head_dim);
-    FOLD_CHECK_ARG(q && o && cu_seqlens && seq_lens && page_table && ka && kb && va && ek && counters && parts && status, "fold_chunk_sm100: null pointer");
+    FOLD_CHECK_ARG(q && o && cu_seqlens && seq_lens && page_table && ka && kb && va && ek && workspace && status, "fold_chunk_sm100: null pointer");
     FOLD_CHECK_ARG(n_kv_heads > 0 && n_heads % n_kv_heads == 0 && n_heads / n_kv_heads <= 128, "fold_chunk_sm100: %d query heads over %d KV heads (128 a group at most)", n_heads, n_kv_heads);
     FOLD_CHECK_ARG(batch > 0 && total > 0 && pages_per_request > 0 && ctas > 0 && pool_rows > 0 && pool_rows < (1ll << 31),
                    "fold_chunk_sm100: %d requests, %d tokens, %d pages a request, %d CTAs, %lld pool rows", batch, total, pages_per_request, ctas, static_cast<long long>(pool_rows));
@@ -857,9 +995,15 @@ extern "C" int fold_chunk_sm100(const void* q, int64_t q_token_stride, int64_t q
     FOLD_CHECK_ARG(window > 0 && window <= FOLD_MAX_WINDOW && sinks >= 0 && sinks <= FOLD_MAX_WINDOW, "fold_chunk_sm100: a window of %d keys and %d sinks", window, sinks);
     FOLD_CHECK_ARG(q_token_stride % 8 == 0 && q_head_stride % 8 == 0 && o_token_stride % 8 == 0 && o_head_stride % 8 == 0 &&
                        reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(o) % 16 == 0 &&
-                       reinterpret_cast<uintptr_t>(parts) % 16 == 0 && reinterpret_cast<uintptr_t>(va) % 16 == 0,
+                       reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && reinterpret_cast<uintptr_t>(va) % 16 == 0,
                    "fold_chunk_sm100: rows must be 16-byte aligned");
+    const Work w = chunk_work(batch, total, n_heads, n_kv_heads, head_dim, ctas);
+    FOLD_CHECK_ARG(workspace_bytes >= w.total, "fold_chunk_sm100: a workspace of %lld bytes, %lld needed", static_cast<long long>(workspace_bytes),
+                   static_cast<long long>(w.total));
+    FOLD_CHECK_ARG((static_cast<int64_t>(total) * n_heads * head_dim / 16 + NT - 1) / NT < (1ll << 31), "fold_chunk_sm100: %d tokens of %d heads in one call", total, n_heads);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
     csm100::Params p;
+    p.qa = reinterpret_cast<int8_t*>(ws + w.qa); p.qb = reinterpret_cast<int8_t*>(ws + w.qb); p.eq = reinterpret_cast<float*>(ws + w.eq);
     p.q = static_cast<const uint16_t*>(q); p.q_st = q_token_stride; p.q_sh = q_head_stride;
     p.o = static_cast<uint16_t*>(o); p.o_st = o_token_stride; p.o_sh = o_head_stride;
     p.cu = cu_seqlens; p.lens = seq_lens; p.table = page_table;
@@ -871,7 +1015,7 @@ extern "C" int fold_chunk_sm100(const void* q, int64_t q_token_stride, int64_t q
     p.total = total; p.window = window; p.sinks = sinks;
     p.ka = ka; p.kb = kb; p.ek = static_cast<const uint16_t*>(ek);
     p.va = static_cast<const uint8_t*>(va); p.vb = static_cast<const uint8_t*>(vb); p.evs = v_scale;
-    p.counters = counters; p.parts = parts; p.status = status; p.others = others;
+    p.counters = reinterpret_cast<int*>(ws + w.counters); p.parts = reinterpret_cast<float*>(ws + w.parts); p.status = status; p.others = others;
     CUtensorMap vmap = {};
     if (!vb) {   // a bf16 V: rows of the pool, boxes of 64 channels of a piece's keys
         EncodeFn fn = encode_fn();

@@ -27,7 +27,8 @@ _lib.register("fold_write_tokens", [P, P, I, L, L, L, L, P, L, I, I, I, P, P, P,
 _lib.register("fold_read_tokens", [P, L, I, I, I, P, P, P, P, P, F, P, P, I, P])
 _lib.register("fold_chunk_sums", [P, I, L, L, I, I, I, P, I, P, P, F, P, P, P])
 _lib.register("fold_chunk_gather", [P, P, I, P, I, I, I, I, I, I, P, P, P, P, P, F, I, I, I, I, P, P, P, P, P, P])
-_lib.register("fold_chunk_sm100", [P, L, L, P, L, L, I, P, P, I, I, I, I, I, P, I, I, L, P, P, P, P, P, F, I, I, I, I, P, P, P, P])
+_lib.register("fold_chunk_sm100", [P, L, L, P, L, L, I, P, P, I, I, I, I, I, P, I, I, L, P, P, P, P, P, F, I, I, I, I, P, L, P, P])
+_lib.register("fold_chunk_workspace_bytes", [I, I, I, I, I, I], L)
 
 _HALF = (torch.bfloat16, torch.float16)
 _OUT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -175,9 +176,7 @@ def chunk_attention(q, cu_seqlens, lens, cap_tiles, seq_lens, page_table, page_s
     short = any(0 < n * G <= SHORT_ROWS for n in lens)
     wide = max(lens) * G > SHORT_ROWS
     out = torch.empty((total, H, D), device=dev, dtype=dt)
-    n_count = -(-B * n_kv_heads // 4) * 4 if short else 0
-    n_plan = 4 * B + 2 * cap_tiles if wide else 0
-    work = torch.zeros(4 + n_count + n_plan, device=dev, dtype=torch.int32)
+    work = torch.empty(4 + (4 * B + 2 * cap_tiles if wide else 0), device=dev, dtype=torch.int32)
     status = work[:1]
     pool = (page_table.data_ptr(), page_table.shape[1], int(page_size))
     planes = (ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb), ek.data_ptr(), float(v_scale))
@@ -186,17 +185,18 @@ def chunk_attention(q, cu_seqlens, lens, cap_tiles, seq_lens, page_table, page_s
         st = _lib.stream(dev)
         if short:
             ctas = torch.cuda.get_device_properties(dev).multi_processor_count
-            parts = torch.empty(2 * ctas * (128 * D + 256), device=dev, dtype=torch.float32)
+            nbytes = _lib.lib.fold_chunk_workspace_bytes(B, total, H, n_kv_heads, D, ctas)
+            space = torch.empty(nbytes, device=dev, dtype=torch.uint8)
             _lib.call(
                 "fold_chunk_sm100", q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), f16,
                 cu_seqlens.data_ptr(), seq_lens.data_ptr(), B, total, H, n_kv_heads, D, *pool, ka.shape[0], *planes, win, sinks, int(wide),
-                ctas, base + 16, parts.data_ptr(), base, st,
+                ctas, space.data_ptr(), nbytes, base, st,
             )
         if wide:
             rows = cap_tiles * 128
             kw = torch.empty((2, n_kv_heads, rows, D), device=dev, dtype=dt)
             vw = kw.data_ptr() + kw.stride(0) * 2
-            plan = base + 16 + 4 * n_count
+            plan = base + 16
             _lib.call(
                 "fold_chunk_gather", cu_seqlens.data_ptr(), seq_lens.data_ptr(), B, *pool, n_kv_heads, D, win, sinks, *planes, f16,
                 SHORT_ROWS if short else 0, G, cap_tiles, plan, plan + 16 * B, kw.data_ptr(), vw, base, st,

@@ -74,7 +74,8 @@ int fold_chunk_sums(const void* v, int is_f16, int64_t v_token_stride, int64_t v
  * a request's end. kw, vw [n_kv_heads][cap_tiles * 128][head_dim] in bf16, or fp16 (is_f16,
  * saturating); plan int32[4 * batch]; tiles int32[2 * cap_tiles]. Requests whose new tokens times
  * `group` (query heads a KV head) are no more than rows_over are left out, by the attention too. Requests
- * that do not fit cap_tiles see no key and raise *status (FOLD_ERR_ARGUMENT). */
+ * that do not fit cap_tiles see no key and raise *status (FOLD_ERR_ARGUMENT), which a call with
+ * rows_over 0 clears first. */
 int fold_chunk_gather(const int32_t* cu_seqlens, const int32_t* seq_lens, int batch, const int32_t* page_table,
                       int pages_per_request, int page_size, int n_kv_heads, int head_dim, int window, int sinks,
                       const int8_t* ka, const int8_t* kb, const void* va, const void* vb, const void* ek,
@@ -86,15 +87,16 @@ int fold_chunk_gather(const int32_t* cu_seqlens, const int32_t* seq_lens, int ba
  * tensor cores: causal, under `window` and `sinks`, softmax scale 1 / sqrt(head_dim). Requests with more
  * rows are left alone when `others` is set and raise *status (FOLD_ERR_ARGUMENT) when it is not.
  * q, o (total, n_heads, head_dim) bf16 or fp16 with element strides; pool_rows rows in the planes;
- * pages of a multiple of 16 keys; `ctas` persistent CTAs (one an SM); counters int32[batch *
- * n_kv_heads], zero; parts fp32[2 * ctas][128 * head_dim + 256]. */
+ * pages of a multiple of 16 keys; `ctas` persistent CTAs (one an SM); a workspace of
+ * fold_chunk_workspace_bytes bytes on a 16-byte boundary, whose contents do not matter. Sets *status. */
+int64_t fold_chunk_workspace_bytes(int batch, int total, int n_heads, int n_kv_heads, int head_dim, int ctas);
 int fold_chunk_sm100(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* o,
                      int64_t o_token_stride, int64_t o_head_stride, int is_f16, const int32_t* cu_seqlens,
                      const int32_t* seq_lens, int batch, int total, int n_heads, int n_kv_heads, int head_dim,
                      const int32_t* page_table, int pages_per_request, int page_size, int64_t pool_rows,
                      const int8_t* ka, const int8_t* kb, const void* va, const void* vb, const void* ek,
-                     float v_scale, int window, int sinks, int others, int ctas, int32_t* counters, float* parts,
-                     int32_t* status, void* stream);
+                     float v_scale, int window, int sinks, int others, int ctas, void* workspace,
+                     int64_t workspace_bytes, int32_t* status, void* stream);
 
 /* ---- Path B: cache writes ------------------------------------------------ */
 
