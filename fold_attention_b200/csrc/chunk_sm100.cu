@@ -59,7 +59,7 @@ struct Lay {
     static constexpr int SM_EK = SM_V + NV * VSLOT;        // [NK][128] bf16
     static constexpr int SM_ROW = SM_EK + NK * 256;        // m, l [128] f32
     static constexpr int SM_BAR = SM_ROW + 2 * 512;
-    static constexpr int SM_MISC = SM_BAR + 304;           // scan [12], walk [4], flags [2], TMEM address
+    static constexpr int SM_MISC = SM_BAR + 304;           // scan [12], walk [3] and the last piece's number, flags [2], TMEM address
     static constexpr int SM_GEO = SM_MISC + 80;            // the share's first requests
     static constexpr int USED = SM_GEO + N_GEO * 28;
     static constexpr int SLACK = 232448 - USED < 1024 ? 232448 - USED : 1024;   // room to align the base
@@ -246,28 +246,36 @@ struct Walk {
     int64_t start;      // the item's first place in the list
     const Geo* kept;    // requests [b0, b0 + N_GEO)
     int b0;
+    // the next segment; false, with the last one left standing, when the share is through
     __device__ __forceinline__ bool next(const Params& p) {
+        int nb = b, nh = h, nv = v, nleft = left;
+        int64_t ns = start;
+        Geo ng = g;
         for (;;) {
-            if (left <= 0) return false;
-            if (v < 0) {                           // the next item
-                v = 0;
-                start += ITEM_TILES + g.nt;
-                if (++h == p.hkv) {
-                    h = 0;
+            if (nleft <= 0) return false;
+            if (nv < 0) {                          // the next item
+                nv = 0;
+                ns += ITEM_TILES + ng.nt;
+                if (++nh == p.hkv) {
+                    nh = 0;
                     do {
-                        if (++b >= p.batch) { left = 0; return false; }
-                        if (b - b0 < N_GEO) g = kept[b - b0];
-                        else g = geo_of(p, b);
-                    } while (g.nt == 0);
+                        if (++nb >= p.batch) return false;
+                        if (nb - b0 < N_GEO) ng = kept[nb - b0];
+                        else ng = geo_of(p, nb);
+                    } while (ng.nt == 0);
                 }
             }
-            const int v1 = min(ITEM_TILES + g.nt, v + left);
-            t0 = max(0, v - ITEM_TILES);
-            t1 = max(0, v1 - ITEM_TILES);
-            left -= v1 - v;
-            v = v1 == ITEM_TILES + g.nt ? -1 : v1;
-            if (t1 > t0) break;                    // (a share may end before an item's tiles begin)
+            const int v1 = min(ITEM_TILES + ng.nt, nv + nleft);
+            const int n0 = max(0, nv - ITEM_TILES), n1 = max(0, v1 - ITEM_TILES);
+            nleft -= v1 - nv;
+            nv = v1 == ITEM_TILES + ng.nt ? -1 : v1;
+            if (n1 > n0) {                         // (a share may end before an item's tiles begin)
+                t0 = n0;
+                t1 = n1;
+                break;
+            }
         }
+        b = nb; h = nh; v = nv; left = nleft; start = ns; g = ng;
         ++segment;
         return true;
     }
@@ -460,12 +468,19 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
     // Join a (request, head)'s pieces: a row's pieces (each the copies' plain sums under one reference) are added
     // in list order and copies within, by this CTA for an item of its own, by the last CTA to get here for
     // one that several share.
-    auto join = [&](const Walk& x, int& joins) {
+    // `end`: the share's last item, which every thread of the CTA joins once nothing else is left to do.
+    auto join = [&](const Walk& x, int& joins, auto end) {
+        constexpr bool END = decltype(end)::value;
         const int R = x.g.n * p.G, copies = copies_of(R), rows = 128 / copies;
         const bool whole = is_whole(x);
         if (whole && copies == 1) return;
-        const int jl = (warp - L::W_JOIN) * 32 + lane;
-        mbar_wait(bar(B_PIECE), joins & 1, abort_flag, p.status);
+        const int jl = END ? tid : (warp - L::W_JOIN) * 32 + lane;
+        constexpr int NJ = END ? L::NTHREADS : 32 * L::N_JOIN;
+        if (!END) {
+            Walk y = x;
+            if (!y.next(p)) return;
+            mbar_wait(bar(B_PIECE), joins & 1, abort_flag, p.status);
+        }
         int c_first = blockIdx.x, c_last = blockIdx.x;
         bool mine = true;
         if (!whole) {
@@ -473,7 +488,8 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
             c_last = share_of(total, n_cta, x.start + ITEM_TILES + x.g.nt - 1);
             __threadfence();
             if (jl == 0) *last_flag = atomicAdd(p.counters + static_cast<int64_t>(x.b) * p.hkv + x.h, 1) == c_last - c_first;
-            if (L::N_JOIN > 1) asm volatile("bar.sync 2, 128;" ::: "memory");
+            if (END) __syncthreads();
+            else if (L::N_JOIN > 1) asm volatile("bar.sync 2, 128;" ::: "memory");
             else __syncwarp();
             mine = *last_flag != 0;
             __threadfence();
@@ -482,7 +498,7 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
             auto piece = [&](int c) { return whole ? slot_of(c, 2 + (joins & 1)) : slot_of(c, c == c_first ? 1 : 0); };
             auto pk2 = [](float a, float b2) { return F16 ? pack_f16x2(a, b2) : pack_bf16x2(a, b2); };
             const int n_work = R * (D / 8);
-            for (int i = jl; i < n_work; i += 32 * L::N_JOIN) {
+            for (int i = jl; i < n_work; i += NJ) {
                 const int row = i % R, u = i / R;      // 8 channels of a row
                 float mm = -INFINITY, ll = 0.f;
                 if (!whole) {
@@ -516,6 +532,7 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
                                                             pk2(a1.x * inv, a1.y * inv), pk2(a1.z * inv, a1.w * inv));
             }
         }
+        if (END) return;
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_JOINED));
         if (L::N_JOIN > 1 && !whole) asm volatile("bar.sync 2, 128;" ::: "memory");   // the flag has been read
@@ -626,7 +643,7 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
                               static_cast<uint32_t>(R * D), bar(B_QFULL));
             }
             if constexpr (V8) {
-                if (had) join(before, joins);     // the item before, while this one's tiles run
+                if (had) join(before, joins, std::false_type{});     // the item before, while this one's tiles run
                 before = w;
                 had = true;
             } else {
@@ -646,12 +663,9 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
                 }
             }
         }
-        if constexpr (V8) {
-            if (had) join(before, joins);
-        }
     } else if (!V8 && warp >= L::W_JOIN) {
         int joins = 0;
-        while (w.next(p)) join(w, joins);
+        while (w.next(p)) join(w, joins, std::false_type{});
     } else if (warp < 8) {
         // ================= Q, softmax, epilogue: thread = TMEM lane =================
         const int wq = warp - 4, m_row = 32 * wq + lane;
@@ -860,6 +874,7 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
             // one piece at a time is handed over: the joining warp tells phases apart by their parity, and the slot
             // of two pieces back is then free for the next
             if (joins >= 1) mbar_wait(bar(B_JOINED), (joins - 1) & 1, abort_flag, p.status);
+            if (m_row == 0) s_walk[3] = joins;    // (the share's last piece is found by it)
             mbar_arrive(bar(B_PIECE));
             ++joins;
         }
@@ -916,6 +931,11 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
     }
     tc_fence_before();
     __syncthreads();
+    while (w.next(p)) {}      // (the issuing warp's other lanes have not walked)
+    if (w.segment >= 0) {     // w is the share's last segment
+        int joins = s_walk[3];
+        join(w, joins, std::true_type{});
+    }
     if (warp == 1) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }

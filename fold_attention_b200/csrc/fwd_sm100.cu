@@ -22,6 +22,9 @@
 // schedule is this kernel's own).
 #include <cuda.h>
 
+#include <algorithm>
+#include <type_traits>
+
 #include "bwd_common.cuh"
 #include "common.cuh"
 #include "fold_b200.h"
@@ -176,33 +179,19 @@ struct Params {
     int B, H, HKV, G, S, causal;
     float scale;
     int* status;
-    // a build with EXT = true only (it is causal): a row sees the `window` newest keys up to its own
-    // position and the first `sinks` keys; with `plan` the queries are request b's last positions and its
-    // keys plan[b].x rows of (row, head) tensors from row plan[b].y on, without the plan[b].z tiles of 128
-    // keys between the sinks' tiles and the window's that no query of the chunk sees
+    // fwd_window_sm100_kernel's: a row sees the `window` newest keys up to its own position and the first
+    // `sinks` keys; with `plan` the queries are request b's last positions and its keys plan[b].x rows of
+    // (row, head) tensors from row plan[b].y on, without the plan[b].z tiles of 128 keys between the sinks'
+    // tiles and the window's that no query of the chunk sees
     int window, sinks;
     const int4* plan;
+    int n_work;      // work items: heads x blocks of 256 rows (dense), x slots of 256 packed rows and one per request
 };
 struct Maps {
     CUtensorMap q, k, v;   // (channel, row, head, batch), boxes (64, 128, 1, 1)
 };
 
-// The key tiles one CTA walks, in order: the tiles that hold sinks, then the window's, for both of
-// its query tiles; each query tile takes the ones it sees (`active`).
-struct TileList {
-    int ns, lo, n;          // tiles [0, ns), then [lo, lo + n - ns)
-    int end[2], low[2];     // query tile x sees tiles [low[x], end[x]) and the sinks'
-    int sinks;
-    __device__ __forceinline__ int tile(int j) const { return j < ns ? j : lo + j - ns; }
-    __device__ __forceinline__ bool active(int x, int j) const {
-        const int t = tile(j);
-        return j < n && t < end[x] && (t >= low[x] || t * BN < sinks);
-    }
-};
-
-// EXT: the build with a window, sinks and keys of another length than the queries. The causal and
-// full builds keep their own tile arithmetic (and their bits).
-template <bool F16, bool EXT>
+template <bool F16>
 __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, const __grid_constant__ Maps maps) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = static_cast<uint32_t>(__cvta_generic_to_shared(smem_raw));
@@ -224,50 +213,15 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
     if (m0 >= len) return;
     const int hkv = h / p.G;
     const int bb = p.cu ? 0 : b;
-    int klen = len, qoff = 0, kstart = start, kshift = 0;   // keys, and the first query's position among them
-    if constexpr (EXT) {
-        if (p.plan) {
-            const int4 pl = p.plan[b];
-            if (pl.x < 0) return;   // another kernel's
-            klen = pl.x;
-            qoff = klen - len;
-            kstart = pl.y;
-            kshift = pl.z;
-        }
-    }
     // key tiles each of the two query tiles meets (the second tile may lie past the sequence)
     int nt[2];
-    TileList tl{};
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int mx = m0 + x * BM;
-        if constexpr (EXT) {
-            const int kv_end = mx >= len ? 0 : max(0, min(klen, qoff + min(mx + BM, len)));
-            tl.end[x] = (kv_end + BN - 1) / BN;
-            tl.low[x] = max(0, qoff + mx - p.window + 1) / BN;
-        } else {
-            const int kv_end = mx >= len ? 0 : (p.causal ? min(len, mx + BM) : len);
-            nt[x] = (kv_end + BN - 1) / BN;
-        }
+        const int kv_end = mx >= len ? 0 : (p.causal ? min(len, mx + BM) : len);
+        nt[x] = (kv_end + BN - 1) / BN;
     }
-    if constexpr (EXT) {
-        tl.sinks = p.sinks;
-        tl.ns = (p.sinks + BN - 1) / BN;
-        tl.lo = tl.low[0];
-        if (tl.ns >= tl.lo) tl.ns = tl.lo = 0;   // the sinks' tiles run into the window's
-        tl.n = max(0, tl.ns + max(tl.end[0], tl.end[1]) - tl.lo);
-        const int st = (p.sinks + BN - 1) / BN;
-        for (int x = 0; x < 2; ++x)              // tiles each query tile takes
-            nt[x] = min(tl.end[x], st) + max(0, tl.end[x] - max(tl.low[x], st));
-    }
-    const int n_tiles = EXT ? tl.n : max(nt[0], nt[1]);
-    auto tile_of = [&](int j) { return EXT ? tl.tile(j) : j; };
-    // the tile's first row: tiles that the chunk leaves out have none
-    auto row_of = [&](int j) {
-        const int t = tile_of(j);
-        return kstart + (EXT && t * BN >= p.sinks ? t - kshift : t) * BN;
-    };
-    auto takes = [&](int x, int j) { return EXT ? tl.active(x, j) : j < nt[x]; };
+    const int n_tiles = max(nt[0], nt[1]);
 
     if (tid == 0) {
         *abort_flag = 0;
@@ -294,7 +248,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
     if (warp == 0) {
         // ================= TMA producer =================
         if (lane == 0) {
-            if (nt[0] > 0 || nt[1] > 0) mbar_expect_tx(bar(B_Q), nt[0] > 0 && nt[1] > 0 ? 65536 : 32768);
+            mbar_expect_tx(bar(B_Q), nt[1] > 0 ? 65536 : 32768);
             for (int x = 0; x < 2; ++x) {
                 if (nt[x] == 0) continue;
                 for (int c = 0; c < 2; ++c)
@@ -306,8 +260,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
                 const uint32_t st = base + SM_KV + s * STAGE;
                 mbar_expect_tx(bar(B_KVFULL + s), 65536);
                 for (int c = 0; c < 2; ++c) {
-                    tma_load_4d(st + c * 16384, &maps.k, 64 * c, row_of(j), hkv, bb, bar(B_KVFULL + s));
-                    tma_load_4d(st + 32768 + c * 16384, &maps.v, 64 * c, row_of(j), hkv, bb, bar(B_KVFULL + s));
+                    tma_load_4d(st + c * 16384, &maps.k, 64 * c, start + j * BN, hkv, bb, bar(B_KVFULL + s));
+                    tma_load_4d(st + 32768 + c * 16384, &maps.v, 64 * c, start + j * BN, hkv, bb, bar(B_KVFULL + s));
                 }
             }
         }
@@ -316,7 +270,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
         if (lane == 0) {
             constexpr uint32_t ID_S = instr_desc(F16 ? 0 : 1, 128, 128, 0, 0);    // Q (K-major) x K (K-major)
             constexpr uint32_t ID_PV = instr_desc(F16 ? 0 : 1, 128, 128, 0, 1);   // P (TMEM) x V (MN-major)
-            if (nt[0] > 0 || nt[1] > 0) mbar_wait(bar(B_Q), 0, abort_flag, p.status);
+            mbar_wait(bar(B_Q), 0, abort_flag, p.status);
             auto issue_s = [&](int x, int j) {
                 const int s = j & 1;
                 mbar_wait(bar(B_KVFULL + s), (j >> 1) & 1, abort_flag, p.status);
@@ -330,30 +284,23 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
                 tc_commit(bar(B_SFULL + x));
             };
             for (int x = 0; x < 2; ++x)
-                if (takes(x, 0)) issue_s(x, 0);
-            int done[2] = {0, 0};   // EXT: products issued so far (a query tile may sit a key tile out)
+                if (nt[x] > 0) issue_s(x, 0);
             for (int j = 0; j < n_tiles; ++j) {
                 const int s = j & 1;
                 const uint32_t vt = base + SM_KV + s * STAGE + 32768;
                 for (int x = 0; x < 2; ++x) {
-                    if (takes(x, j)) {
-                        const int it = EXT ? done[x] : j;
-                        mbar_wait(bar(B_PREADY + x), it & 1, abort_flag, p.status);
-                        tc_fence_after();
+                    if (j >= nt[x]) continue;
+                    mbar_wait(bar(B_PREADY + x), j & 1, abort_flag, p.status);
+                    tc_fence_after();
 #pragma unroll
-                        for (int ks = 0; ks < 8; ++ks)   // 16 keys per step: 8 TMEM columns of P, 2048 bytes of V per box
-                            mma_ts(tmem + T_O + 128 * x, tmem + T_S + 128 * x + 8 * ks, smem_desc(vt + ks * 2048, 16384, 1024), ID_PV,
-                                   (it > 0) || (ks > 0));
-                        tc_commit(bar(B_ODONE + x));
-                        if constexpr (EXT) ++done[x];
-                    }
+                    for (int ks = 0; ks < 8; ++ks)   // 16 keys per step: 8 TMEM columns of P, 2048 bytes of V per box
+                        mma_ts(tmem + T_O + 128 * x, tmem + T_S + 128 * x + 8 * ks, smem_desc(vt + ks * 2048, 16384, 1024), ID_PV,
+                               (j > 0) || (ks > 0));
+                    tc_commit(bar(B_ODONE + x));
                     // the next scores overwrite S (and the P just consumed): the tensor pipe runs a
-                    // thread's MMAs in the order it issued them. (Only ever the next key tile's: a later
-                    // one's stage is not free before this tile is done with it.)
-                    if (takes(x, j + 1)) issue_s(x, j + 1);
+                    // thread's MMAs in the order it issued them
+                    if (j + 1 < nt[x]) issue_s(x, j + 1);
                 }
-                // EXT: a tile that no product of this thread reads has still to land before its stage is filled again
-                if (EXT && !takes(0, j) && !takes(1, j)) mbar_wait(bar(B_KVFULL + s), (j >> 1) & 1, abort_flag, p.status);
                 tc_commit(bar(B_KVEMPTY + s));
             }
         }
@@ -365,30 +312,15 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
         const float c2 = p.scale * kLog2e;
         const uint64_t c2x2 = pack2(c2, c2);
         const int mx = m0 + x * BM;
-        const int qr = mx + r;                 // the query's row in its sequence
-        const int qi = qr + qoff;              // its position among the keys
+        const int qi = mx + r;                 // the row's position in its sequence
         const int my_tiles = nt[x];
         float m_run = -INFINITY, l_run = 0.f;  // running maximum (log2 domain) and sum
         const uint32_t ts = tmem + lane_addr + T_S + 128 * x;
         const uint32_t to = tmem + lane_addr + T_O + 128 * x;
-        int it = 0;
-        for (int jj = 0; jj < (EXT ? n_tiles : my_tiles); ++jj) {
-            if (EXT && !takes(x, jj)) continue;
-            const int j = EXT ? it++ : jj;     // the query tile's own count of key tiles
-            const int n0 = tile_of(jj) * BN;
-            bool need_mask;
-            int kmax, kmin = 0, ksink = 0;     // the key columns this row sees: kmin .. kmax, and those under ksink
-            if constexpr (EXT) {
-                const bool cuts = n0 <= qoff + mx + BM - 1 - p.window && n0 + BN > p.sinks;   // the tile's last row has moved past its first key
-                need_mask = n0 + BN > qoff + mx || n0 + BN > klen || cuts;
-                kmax = min(klen - 1, qi) - n0;
-                kmin = qi - p.window + 1 - n0;
-                ksink = p.sinks - n0;
-            } else {
-                need_mask = (p.causal && n0 + BN > mx) || (n0 + BN > len);
-                kmax = min(len - 1, p.causal ? qi : len - 1) - n0;   // last key column this row may see
-            }
-            auto hidden = [&](int e) { return e > kmax || (EXT && e < kmin && e >= ksink); };
+        for (int j = 0; j < my_tiles; ++j) {
+            const int n0 = j * BN;
+            const bool need_mask = (p.causal && n0 + BN > mx) || (n0 + BN > len);
+            const int kmax = min(len - 1, p.causal ? qi : len - 1) - n0;   // last key column this row may see
             mbar_wait(bar(B_SFULL + x), j & 1, abort_flag, p.status);
             tc_fence_after();
             // pass 1: the row's maximum over the tile
@@ -401,7 +333,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
                 if (need_mask) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
-                        if (hidden(32 * c + e)) sv[e] = 0xff800000u;   // -inf
+                        if (32 * c + e > kmax) sv[e] = 0xff800000u;   // -inf
                 }
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) mxv = max3f(mxv, __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
@@ -433,8 +365,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
                     x0 = ex2f(x0);
                     x1 = ex2f(x1);
                     if (need_mask) {
-                        if (hidden(32 * c + e)) x0 = 0.f;
-                        if (hidden(32 * c + e + 1)) x1 = 0.f;
+                        if (32 * c + e > kmax) x0 = 0.f;
+                        if (32 * c + e + 1 > kmax) x1 = 0.f;
                     }
                     asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum2) : "l"(pack2(x0, x1)));   // even and odd columns apart
                     pp[e >> 1] = F16 ? pack_f16x2(x0, x1) : pack_bf16x2(x0, x1);
@@ -470,10 +402,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
             mbar_wait(bar(B_ODONE + x), (my_tiles - 1) & 1, abort_flag, p.status);
             tc_fence_after();
             // the warp's tcgen05.ld is collective: every lane reads, rows past the sequence store nothing
-            const bool row_ok = qr < len;
+            const bool row_ok = qi < len;
             auto pk2 = [](float a, float b2) { return F16 ? pack_f16x2(a, b2) : pack_bf16x2(a, b2); };
             const float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
-            uint16_t* orow = row_ptr<uint16_t>(p.o, b, start + (row_ok ? qr : 0), h);
+            uint16_t* orow = row_ptr<uint16_t>(p.o, b, start + (row_ok ? qi : 0), h);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 uint32_t ov[32];
@@ -491,17 +423,365 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
                     }
                 }
             }
-            if (row_ok && (!EXT || p.lse)) {
+            if (row_ok) {
                 const float lse = l_run > 0.f ? (m_run + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
-                p.lse[static_cast<int64_t>(b) * p.lse_sb + static_cast<int64_t>(h) * p.lse_sh + start + qr] = lse;
+                p.lse[static_cast<int64_t>(b) * p.lse_sb + static_cast<int64_t>(h) * p.lse_sh + start + qi] = lse;
             }
             tc_fence_before();
-        } else if (EXT && qr < len) {   // rows that see no key at all
-            uint16_t* orow = row_ptr<uint16_t>(p.o, b, start + qr, h);
-            for (int u = 0; u < 16; ++u) *reinterpret_cast<uint4*>(orow + 8 * u) = make_uint4(0u, 0u, 0u, 0u);
-            if (p.lse) p.lse[static_cast<int64_t>(b) * p.lse_sb + static_cast<int64_t>(h) * p.lse_sh + start + qr] = -INFINITY;
         }
     }
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+// ---- a sliding window with sinks, and keys of another length than the queries ------------------
+// The same tiles and the same softmax under another mask, as a persistent kernel: a window's CTA has ten
+// key tiles or so to walk, and what a CTA of its own costs each block (launch, TMEM, barriers, the first
+// loads, and the epilogue with nothing behind it) was half of its time. One CTA per SM walks the work items
+// in stride, and the next item's Q and first tiles are loaded, and its first scores issued, while the last
+// one's O is written. Barrier phases count key tiles and items since the CTA started.
+
+// What an item walks: key tiles [0, ns), then [lo, lo + n - ns); query tile x takes tiles
+// [low[x], end[x]) and those of the sinks (st of them).
+struct Item {
+    int m0, h, b, start, len, klen, qoff, kstart, kshift;
+    int ns, lo, n, st;
+    int end[2], low[2], nt[2];      // nt: key tiles that query tile x takes
+    __device__ __forceinline__ int tile(int j) const { return j < ns ? j : lo + j - ns; }
+    __device__ __forceinline__ bool takes(int e, int l, int j) const {
+        const int t = tile(j);
+        return j < n && t < e && (t >= l || t < st);
+    }
+    // the first row of the j-th tile (tiles that a chunk leaves out have none)
+    __device__ __forceinline__ int row(int j) const {
+        const int t = tile(j);
+        return kstart + (t < st ? t : t - kshift) * BN;
+    }
+};
+
+// Work item i, longest rows first in a dense call; false if it is empty.
+__device__ __forceinline__ bool load_item(const Params& p, int i, Item& w) {
+    const int blk = i / p.H;
+    w.h = i - blk * p.H;
+    if (p.cu) {
+        // packed: request b's blocks sit in slots from cu[b] / 256 + b on (at least as many as it needs)
+        const int slot = p.n_work / p.H - 1 - blk;
+        int lo = 0, hi = p.B;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (__ldg(p.cu + mid) / CTA_M + mid <= slot) lo = mid;
+            else hi = mid;
+        }
+        w.b = lo;
+        w.start = __ldg(p.cu + lo);
+        w.len = __ldg(p.cu + lo + 1) - w.start;
+        w.m0 = (slot - (w.start / CTA_M + lo)) * CTA_M;
+    } else {
+        const int nb = (p.S + CTA_M - 1) / CTA_M;
+        w.b = blk % p.B;
+        w.start = 0;
+        w.len = p.S;
+        w.m0 = (nb - 1 - blk / p.B) * CTA_M;
+    }
+    if (w.m0 < 0 || w.m0 >= w.len) return false;
+    w.klen = w.len;
+    w.qoff = w.kshift = 0;
+    w.kstart = w.start;
+    if (p.plan) {
+        const int4 pl = __ldg(p.plan + w.b);
+        if (pl.x < 0) return false;   // another kernel's
+        w.klen = pl.x;
+        w.qoff = pl.x - w.len;
+        w.kstart = pl.y;
+        w.kshift = pl.z;
+    }
+    w.st = w.ns = (p.sinks + BN - 1) / BN;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const int mx = w.m0 + x * BM;
+        const int kv_end = mx >= w.len ? 0 : max(0, min(w.klen, w.qoff + min(mx + BM, w.len)));
+        w.end[x] = (kv_end + BN - 1) / BN;
+        w.low[x] = max(0, w.qoff + mx - p.window + 1) / BN;
+        w.nt[x] = min(w.end[x], w.st) + max(0, w.end[x] - max(w.low[x], w.st));
+    }
+    w.lo = w.low[0];
+    if (w.ns >= w.lo) w.ns = w.lo = 0;   // the sinks' tiles run into the window's
+    w.n = max(0, w.ns + max(w.end[0], w.end[1]) - w.lo);
+    return true;
+}
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+template <bool F16>
+__global__ void __launch_bounds__(NTHREADS, 1) fwd_window_sm100_kernel(const Params p, const __grid_constant__ Maps maps) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = static_cast<uint32_t>(__cvta_generic_to_shared(smem_raw));
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    uint8_t* smem = smem_raw + (base - raw);
+    auto bar = [&](int i) { return base + SM_BAR + 8 * i; };
+    constexpr int B_QEMPTY = B_COUNT;      // the item's last scores are out of Q
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + SM_BAR + 8 * (B_COUNT + 1));
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM_BAR + 8 * (B_COUNT + 1) + 8);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        *abort_flag = 0;
+        mbar_init(bar(B_Q), 1);
+        mbar_init(bar(B_QEMPTY), 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar(B_KVFULL + i), 1);
+            mbar_init(bar(B_KVEMPTY + i), 1);
+            mbar_init(bar(B_SFULL + i), 1);
+            mbar_init(bar(B_PREADY + i), 128);
+            mbar_init(bar(B_ODONE + i), 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;"
+                     ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(tmem_slot))) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        // ================= TMA producer =================
+        if (lane == 0) {
+            int jk = 0, items = 0;         // key tiles, and items with any, so far
+            for (int i = blockIdx.x; i < p.n_work; i += gridDim.x) {
+                Item w;
+                if (!load_item(p, i, w) || w.nt[0] + w.nt[1] == 0) continue;
+                const int hkv = w.h / p.G, bb = p.cu ? 0 : w.b;
+                if (items > 0) mbar_wait(bar(B_QEMPTY), (items - 1) & 1, abort_flag, p.status);
+                mbar_expect_tx(bar(B_Q), w.nt[0] > 0 && w.nt[1] > 0 ? 65536 : 32768);
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    if (w.nt[x] > 0)
+                        for (int c = 0; c < 2; ++c)
+                            tma_load_4d(base + SM_Q + x * 32768 + c * 16384, &maps.q, 64 * c, w.start + w.m0 + x * BM, w.h, bb, bar(B_Q));
+                for (int j = 0; j < w.n; ++j, ++jk) {
+                    const int s = jk & 1;
+                    if (jk >= 2) mbar_wait(bar(B_KVEMPTY + s), ((jk >> 1) - 1) & 1, abort_flag, p.status);
+                    const uint32_t st = base + SM_KV + s * STAGE;
+                    mbar_expect_tx(bar(B_KVFULL + s), 65536);
+                    for (int c = 0; c < 2; ++c) {
+                        tma_load_4d(st + c * 16384, &maps.k, 64 * c, w.row(j), hkv, bb, bar(B_KVFULL + s));
+                        tma_load_4d(st + 32768 + c * 16384, &maps.v, 64 * c, w.row(j), hkv, bb, bar(B_KVFULL + s));
+                    }
+                }
+                ++items;
+            }
+        }
+    } else if (warp == 1) {
+        // ================= MMA issuer =================
+        if (lane == 0) {
+            constexpr uint32_t ID_S = instr_desc(F16 ? 0 : 1, 128, 128, 0, 0);    // Q (K-major) x K (K-major)
+            constexpr uint32_t ID_PV = instr_desc(F16 ? 0 : 1, 128, 128, 0, 1);   // P (TMEM) x V (MN-major)
+            int jk = 0, items = 0, done[2] = {0, 0};
+            for (int i = blockIdx.x; i < p.n_work; i += gridDim.x) {
+                Item w;
+                if (!load_item(p, i, w) || w.nt[0] + w.nt[1] == 0) continue;
+                mbar_wait(bar(B_Q), items & 1, abort_flag, p.status);
+                int left = w.nt[0] + w.nt[1];      // scores still to issue
+                auto issue_s = [&](int x, int j) {
+                    const int g = jk + j, s = g & 1;
+                    mbar_wait(bar(B_KVFULL + s), (g >> 1) & 1, abort_flag, p.status);
+                    tc_fence_after();
+                    const uint32_t kt = base + SM_KV + s * STAGE, qt = base + SM_Q + x * 32768;
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) {
+                        const uint32_t off = (ks >> 2) * 16384 + (ks & 3) * 32;
+                        mma_ss(tmem + T_S + 128 * x, smem_desc(qt + off, 16, 1024), smem_desc(kt + off, 16, 1024), ID_S, ks > 0);
+                    }
+                    tc_commit(bar(B_SFULL + x));
+                    if (--left == 0) tc_commit(bar(B_QEMPTY));
+                };
+                bool now[2], next[2], first[2] = {true, true};
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    next[x] = w.takes(w.end[x], w.low[x], 0);
+                    if (next[x]) issue_s(x, 0);
+                }
+                for (int j = 0; j < w.n; ++j) {
+                    const int s = (jk + j) & 1;
+                    const uint32_t vt = base + SM_KV + s * STAGE + 32768;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        now[x] = next[x];
+                        next[x] = w.takes(w.end[x], w.low[x], j + 1);
+                    }
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        if (now[x]) {
+                            mbar_wait(bar(B_PREADY + x), done[x] & 1, abort_flag, p.status);
+                            tc_fence_after();
+#pragma unroll
+                            for (int ks = 0; ks < 8; ++ks)   // 16 keys per step: 8 TMEM columns of P, 2048 bytes of V per box
+                                mma_ts(tmem + T_O + 128 * x, tmem + T_S + 128 * x + 8 * ks, smem_desc(vt + ks * 2048, 16384, 1024), ID_PV,
+                                       !first[x] || ks > 0);
+                            tc_commit(bar(B_ODONE + x));
+                            ++done[x];
+                            first[x] = false;
+                        }
+                        // the next scores overwrite S and the P just consumed: a thread's MMAs run in the order it issued
+                        // them. (Only ever the next key tile's: a later one's stage is not free before this tile is done with it.)
+                        if (next[x]) issue_s(x, j + 1);
+                    }
+                    // a tile that no product reads has still to land before its stage is filled again
+                    if (!now[0] && !now[1]) mbar_wait(bar(B_KVFULL + s), ((jk + j) >> 1) & 1, abort_flag, p.status);
+                    tc_commit(bar(B_KVEMPTY + s));
+                }
+                jk += w.n;
+                ++items;
+            }
+        }
+    } else if (warp >= 4) {
+        // ================= softmax: two groups, one per query tile; thread = query row = TMEM lane =================
+        const int x = (warp - 4) >> 2;
+        const int r = 32 * (warp & 3) + lane;
+        const uint32_t lane_addr = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+        const float c2 = p.scale * kLog2e;
+        const uint64_t c2x2 = pack2(c2, c2);
+        const uint32_t ts = tmem + lane_addr + T_S + 128 * x;
+        const uint32_t to = tmem + lane_addr + T_O + 128 * x;
+        int it = 0;                                // the query tile's key tiles so far
+        for (int i = blockIdx.x; i < p.n_work; i += gridDim.x) {
+            Item w;
+            if (!load_item(p, i, w)) continue;
+            const int mx = w.m0 + x * BM;
+            const int qr = mx + r;                 // the query's row in its sequence
+            const int qi = qr + w.qoff;            // its position among the keys
+            const int my_end = x ? w.end[1] : w.end[0], my_low = x ? w.low[1] : w.low[0], my_tiles = x ? w.nt[1] : w.nt[0];
+            float m_run = -INFINITY, l_run = 0.f;  // running maximum (log2 domain) and sum
+            bool first = true;
+            for (int j = 0; j < w.n; ++j) {
+                if (!w.takes(my_end, my_low, j)) continue;
+                const int n0 = w.tile(j) * BN;
+                // the tile's last row has moved past its first key, or its first row does not see the last
+                const bool need_mask = n0 + BN > w.qoff + mx || n0 + BN > w.klen || (n0 <= w.qoff + mx + BM - 1 - p.window && n0 + BN > p.sinks);
+                const int kmax = min(w.klen - 1, qi) - n0, kmin = qi - p.window + 1 - n0, ksink = p.sinks - n0;
+                // columns [32 c, 32 c + 32) that the row sees, as bits
+                auto seen = [&](int c) { return bits_below(kmax + 1 - 32 * c) & (~bits_below(kmin - 32 * c) | bits_below(ksink - 32 * c)); };
+                mbar_wait(bar(B_SFULL + x), it & 1, abort_flag, p.status);
+                tc_fence_after();
+                // pass 1: the row's maximum over the tile. The masked and the unmasked form are two pieces of code: left to
+                // itself the compiler evaluates this mask for every tile, at 1.6 times the kernel's time.
+                float mxv = -INFINITY;
+                auto row_max = [&](auto masked) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t sv[32];
+                        tmem_ld32(ts + 32 * c, sv);
+                        const uint32_t vis = decltype(masked)::value ? seen(c) : 0u;
+                        tmem_wait_ld();
+                        if (decltype(masked)::value) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (!(vis & (1u << e))) sv[e] = 0xff800000u;   // -inf
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) mxv = max3f(mxv, __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+                    }
+                };
+                if (need_mask) row_max(std::true_type{});
+                else row_max(std::false_type{});
+                // The reference point only moves when the row's maximum rose by more than 2^LAZY (fwd_sm100_kernel)
+                const float m_cand = fmaxf(m_run, mxv * c2);
+                const float m_new = m_cand > m_run + LAZY ? m_cand : m_run;
+                const float m_use = m_new == -INFINITY ? 0.f : m_new;     // a row that sees no key yet
+                const float alpha = m_run == -INFINITY ? 1.f : ex2f(m_run - m_use);   // (its O is zero: nothing to rescale)
+                uint64_t sum2 = 0ull;
+                const uint64_t nm2 = pack2(-m_use, -m_use);
+                auto weights = [&](auto masked) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t sv[32];
+                        tmem_ld32(ts + 32 * c, sv);
+                        const uint32_t vis = decltype(masked)::value ? seen(c) : 0u;
+                        tmem_wait_ld();
+                        uint32_t pp[16];
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            float x0, x1;
+                            fma2(x0, x1, __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]), c2x2, nm2);
+                            x0 = ex2f(x0);
+                            x1 = ex2f(x1);
+                            if (decltype(masked)::value) {
+                                if (!(vis & (1u << e))) x0 = 0.f;
+                                if (!(vis & (2u << e))) x1 = 0.f;
+                            }
+                            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum2) : "l"(pack2(x0, x1)));   // even and odd columns apart
+                            pp[e >> 1] = F16 ? pack_f16x2(x0, x1) : pack_bf16x2(x0, x1);
+                        }
+                        tmem_st16(ts + 16 * c, pp);
+                    }
+                };
+                if (need_mask) weights(std::true_type{});
+                else weights(std::false_type{});
+                float sum_e, sum_o;
+                asm("mov.b64 {%0, %1}, %2;" : "=f"(sum_e), "=f"(sum_o) : "l"(sum2));
+                l_run = l_run * alpha + (sum_e + sum_o);
+                m_run = m_new;
+                // O was last written by the product of the key tile before: rescale it where a row's maximum rose
+                if (!first && __any_sync(0xffffffffu, alpha != 1.0f)) {
+                    mbar_wait(bar(B_ODONE + x), (it - 1) & 1, abort_flag, p.status);
+                    tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t ov[32];
+                        tmem_ld32(to + 32 * c, ov);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+                        tmem_st32(to + 32 * c, ov);
+                    }
+                }
+                first = false;
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(bar(B_PREADY + x));
+                ++it;
+            }
+            // ---- epilogue: O / l -> 16-bit, LSE in nats ----
+            const bool row_ok = qr < w.len;
+            uint16_t* orow = row_ptr<uint16_t>(p.o, w.b, w.start + (row_ok ? qr : 0), w.h);
+            if (my_tiles > 0) {
+                mbar_wait(bar(B_ODONE + x), (it - 1) & 1, abort_flag, p.status);
+                tc_fence_after();
+                auto pk2 = [](float a, float b2) { return F16 ? pack_f16x2(a, b2) : pack_bf16x2(a, b2); };
+                const float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t ov[32];
+                    tmem_ld32(to + 32 * c, ov);
+                    tmem_wait_ld();
+                    if (row_ok) {
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            uint4 v;
+                            v.x = pk2(__uint_as_float(ov[8 * u]) * inv, __uint_as_float(ov[8 * u + 1]) * inv);
+                            v.y = pk2(__uint_as_float(ov[8 * u + 2]) * inv, __uint_as_float(ov[8 * u + 3]) * inv);
+                            v.z = pk2(__uint_as_float(ov[8 * u + 4]) * inv, __uint_as_float(ov[8 * u + 5]) * inv);
+                            v.w = pk2(__uint_as_float(ov[8 * u + 6]) * inv, __uint_as_float(ov[8 * u + 7]) * inv);
+                            *reinterpret_cast<uint4*>(orow + 32 * c + 8 * u) = v;
+                        }
+                    }
+                }
+                tc_fence_before();
+            } else if (row_ok) {   // rows that see no key at all
+                for (int u = 0; u < 16; ++u) *reinterpret_cast<uint4*>(orow + 8 * u) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            if (row_ok && p.lse) {
+                const float lse = l_run > 0.f ? (m_run + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
+                p.lse[static_cast<int64_t>(w.b) * p.lse_sb + static_cast<int64_t>(w.h) * p.lse_sh + w.start + qr] = lse;
+            }
+        }
+    }
+    tc_fence_before();
     __syncthreads();
     if (warp == 1) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
@@ -556,8 +836,7 @@ extern "C" int fold_fwd_sm100_supported(int head_dim, int is_f16) {
 
 namespace {
 
-// The causal and full forward (window 0, plan null), or the EXT build. `k_strides`-like entries of
-// `strides` are in elements: (batch, row, head) of q, k, v, o.
+// The causal and full forward, or (`ext`) the windowed one.
 int run_sm100(const char* what, const void* q, const void* k, const void* v, void* o, float* lse, const int64_t* strides,
               const int32_t* cu_seqlens, int batch, int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim,
               int causal, int is_f16, float softmax_scale, int ext, int window, int sinks, const int32_t* plan, int krows,
@@ -600,11 +879,26 @@ int run_sm100(const char* what, const void* q, const void* k, const void* v, voi
         set_error("%s: cuTensorMapEncodeTiled failed", what);
         return FOLD_ERR_LAUNCH;
     }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (ext) {
+        // packed: a slot per 256 rows and one per request (fsm100::load_item); dense: the blocks themselves
+        const int64_t blocks = cu_seqlens ? static_cast<int64_t>(total) / fsm100::CTA_M + batch
+                                          : static_cast<int64_t>((max_seqlen + fsm100::CTA_M - 1) / fsm100::CTA_M) * batch;
+        FOLD_CHECK_ARG(blocks * n_heads < (1ll << 31), "%s: %lld blocks of %d heads", what, static_cast<long long>(blocks), n_heads);
+        p.n_work = static_cast<int>(blocks * n_heads);
+        int dev = 0, sms = 1;
+        cudaGetDevice(&dev);
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        auto kern = f16 ? fsm100::fwd_window_sm100_kernel<true> : fsm100::fwd_window_sm100_kernel<false>;
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fsm100::SMEM_BYTES);
+        kern<<<std::min(p.n_work, sms), fsm100::NTHREADS, fsm100::SMEM_BYTES, st>>>(p, maps);
+        return check_launch(what);
+    }
+    p.n_work = 0;
     dim3 grid((max_seqlen + fsm100::CTA_M - 1) / fsm100::CTA_M, n_heads, batch);
-    auto kern = f16 ? (ext ? fsm100::fwd_sm100_kernel<true, true> : fsm100::fwd_sm100_kernel<true, false>)
-                    : (ext ? fsm100::fwd_sm100_kernel<false, true> : fsm100::fwd_sm100_kernel<false, false>);
+    auto kern = f16 ? fsm100::fwd_sm100_kernel<true> : fsm100::fwd_sm100_kernel<false>;
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fsm100::SMEM_BYTES);
-    kern<<<grid, fsm100::NTHREADS, fsm100::SMEM_BYTES, static_cast<cudaStream_t>(stream)>>>(p, maps);
+    kern<<<grid, fsm100::NTHREADS, fsm100::SMEM_BYTES, st>>>(p, maps);
     return check_launch(what);
 }
 
