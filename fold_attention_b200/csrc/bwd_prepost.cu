@@ -147,6 +147,132 @@ __global__ void __launch_bounds__(PRE_THREADS) bwd_preprocess_kernel(const BwdPa
     }
 }
 
+// The largest |x| of two 16-bit floats, kept in their own type (exact; NaN loses against a number, as
+// with fmaxf).
+template <bool F16>
+__device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t w) {
+    w &= 0x7FFF7FFFu;
+    if constexpr (F16) asm("max.f16x2 %0, %0, %1;" : "+r"(m) : "r"(w));
+    else asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w));
+    return m;
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t max_abs8(uint32_t m, uint4 w) {
+    return max_abs2<F16>(max_abs2<F16>(max_abs2<F16>(max_abs2<F16>(m, w.x), w.y), w.z), w.w);
+}
+template <bool F16>
+__device__ __forceinline__ float max_of2(uint32_t m) {
+    return fmaxf(half_bits_to_float<F16>(static_cast<uint16_t>(m & 0xFFFF)), half_bits_to_float<F16>(static_cast<uint16_t>(m >> 16)));
+}
+
+// The preprocess at head dim 128, which the general kernel above ran at the rate of its instructions (64 % of
+// the issue slots, 37 % of DRAM): half a warp a row, 16-byte accesses, the maxima of 16-bit values in 16 bits.
+// A lane holds what two neighbouring lanes of the general kernel hold, and the row sums add the same terms
+// in the same order, so Delta and the norms are the same bits.
+template <bool F16>
+__global__ void __launch_bounds__(PRE_THREADS, 4) bwd_preprocess128_kernel(const BwdParams p) {
+    constexpr int D = 128, NW = PRE_THREADS / 32, RB = 2;
+    const int mb = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+    const SeqInfo sq = seq_info(p, b);
+    const int len_r = (sq.len + ROW_PAD - 1) / ROW_PAD * ROW_PAD;
+    if (mb * PRE_ROWS >= len_r) return;
+    const int warp = threadIdx.x >> 5, half = (threadIdx.x >> 4) & 1, lane = threadIdx.x & 15;
+    const int hkv = h / p.G;
+    const bool kv_owner = (h % p.G) == 0;
+    const bool acc_stats = p.fold || p.sink_rows > 0;   // dK's and dV's grids are used
+    uint32_t mx_k = 0u, mx_v = 0u, mx_doc = 0u, mx_q = 0u;
+    float mx_dn = 0.f, mx_dl = 0.f;
+    const int64_t wbase = static_cast<int64_t>(h) * p.rows_p + sq.pstart;
+    int init = 0;
+    if (p.dq_bias) {   // the block's rows lie in one query tile: see the general kernel
+        const int tile = mb * PRE_ROWS / ROW_PAD, nkb = (sq.len + ROW_PAD - 1) / ROW_PAD;
+        unsigned n_part = static_cast<unsigned>(p.causal ? min(tile + 1, nkb) : nkb);
+        if (p.window > 0) {
+            const int lo = max(0, tile * ROW_PAD - p.window - (ROW_PAD - 2) + ROW_PAD - 1) / ROW_PAD;
+            n_part -= static_cast<unsigned>(lo - min(lo, (p.sinks + ROW_PAD - 1) / ROW_PAD));
+        }
+        init = static_cast<int>(0u - n_part * 0x4B400000u);
+    }
+#pragma unroll 1
+    for (int r0 = 2 * warp + half; r0 < PRE_ROWS; r0 += 2 * RB * NW) {
+        uint4 ow[RB], gw[RB], kw[RB], vw[RB], qw[RB];
+        float lraw[RB];
+#pragma unroll
+        for (int u = 0; u < RB; ++u) {
+            const int i = mb * PRE_ROWS + r0 + 2 * u * NW;
+            ow[u] = gw[u] = kw[u] = vw[u] = qw[u] = make_uint4(0u, 0u, 0u, 0u);
+            lraw[u] = 0.f;
+            if (i < sq.len) {
+                ow[u] = __ldg(reinterpret_cast<const uint4*>(row_ptr<const uint16_t>(p.o, b, sq.start + i, h)) + lane);
+                gw[u] = __ldg(reinterpret_cast<const uint4*>(row_ptr<const uint16_t>(p.dout, b, sq.start + i, h)) + lane);
+                if (acc_stats) qw[u] = __ldg(reinterpret_cast<const uint4*>(row_ptr<const uint16_t>(p.q, b, sq.start + i, h)) + lane);
+                if (kv_owner) {
+                    kw[u] = __ldg(reinterpret_cast<const uint4*>(row_ptr<const uint16_t>(p.k, b, sq.start + i, hkv)) + lane);
+                    vw[u] = __ldg(reinterpret_cast<const uint4*>(row_ptr<const uint16_t>(p.v, b, sq.start + i, hkv)) + lane);
+                }
+                lraw[u] = p.lse[b * p.lse_sb + h * p.lse_sh + sq.start + i];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < RB; ++u) {
+            const int i = mb * PRE_ROWS + r0 + 2 * u * NW;
+            float d2[2], n2[2];
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {      // the two lanes' terms
+                float o[4], g[4];
+                unpack4<F16>(v ? make_uint2(ow[u].z, ow[u].w) : make_uint2(ow[u].x, ow[u].y), o);
+                unpack4<F16>(v ? make_uint2(gw[u].z, gw[u].w) : make_uint2(gw[u].x, gw[u].y), g);
+                d2[v] = o[0] * g[0] + o[1] * g[1] + o[2] * g[2] + o[3] * g[3];
+                n2[v] = g[0] * g[0] + g[1] * g[1] + g[2] * g[2] + g[3] * g[3];
+            }
+            // the general kernel's butterfly: its offsets 16, 8, 4, 2 are 8, 4, 2, 1 here, its last one the thread's own
+#pragma unroll
+            for (int off = 8; off > 0; off >>= 1)
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    d2[v] += __shfl_xor_sync(0xffffffffu, d2[v], off);
+                    n2[v] += __shfl_xor_sync(0xffffffffu, n2[v], off);
+                }
+            const float delta = d2[0] + d2[1], norm2 = n2[0] + n2[1];
+            float lse2 = INFINITY;
+            if (i < sq.len) {
+                mx_dn = fmaxf(mx_dn, sqrtf(norm2));
+                mx_dl = fmaxf(mx_dl, fabsf(delta));
+                if (acc_stats) {
+                    mx_doc = max_abs8<F16>(mx_doc, gw[u]);
+                    mx_q = max_abs8<F16>(mx_q, qw[u]);
+                }
+                if (kv_owner) {
+                    mx_k = max_abs8<F16>(mx_k, kw[u]);
+                    mx_v = max_abs8<F16>(mx_v, vw[u]);
+                }
+                lse2 = (lraw[u] == -INFINITY) ? 0.f : lraw[u] * kLog2e;
+            }
+            if (lane == 0) {
+                p.dpsum[wbase + i] = i < sq.len ? delta : 0.f;
+                p.lse2[wbase + i] = lse2;
+            }
+            int4* acc = reinterpret_cast<int4*>(p.dq_acc + (wbase + i) * D) + lane;
+            acc[0] = make_int4(init, init, init, init);
+            acc[16] = make_int4(init, init, init, init);
+        }
+    }
+    __shared__ float s_red[6][NW];
+    const float m[6] = {warp_max(max_of2<F16>(mx_k)), warp_max(max_of2<F16>(mx_v)), warp_max(mx_dn), warp_max(mx_dl),
+                        warp_max(max_of2<F16>(mx_doc)), warp_max(max_of2<F16>(mx_q))};
+    if ((threadIdx.x & 31) == 0)
+        for (int i = 0; i < 6; ++i) s_red[i][warp] = m[i];
+    __syncthreads();
+    if (threadIdx.x < (acc_stats ? 6 : 4)) {
+        float r = s_red[threadIdx.x][0];
+        for (int w = 1; w < NW; ++w) r = fmaxf(r, s_red[threadIdx.x][w]);
+        constexpr int slots[6] = {ST_K, ST_V, ST_DO, ST_DELTA, ST_DOC, ST_Q};
+        if (threadIdx.x >= 2 || kv_owner)
+            atomicMax(reinterpret_cast<unsigned int*>(p.stats + (static_cast<int64_t>(b) * p.HKV + hkv) * N_STATS + slots[threadIdx.x]),
+                      __float_as_uint(r));
+    }
+}
+
 // element (row r, channel d) of a dQ accumulator tile of 128 rows
 __device__ __forceinline__ int64_t dq_tile_offset(int layout, int r, int d, int D) {
     if (layout == DQ_LAYOUT_ROW_MAJOR) return static_cast<int64_t>(r) * D + d;
@@ -211,10 +337,16 @@ int launch_bwd_preprocess(const BwdParams& p, cudaStream_t st) {
     }
     const int s_r = (p.S + ROW_PAD - 1) / ROW_PAD * ROW_PAD;
     dim3 grid(s_r / PRE_ROWS, p.H, p.B);
-    if (p.f16)
+    if (p.D == 128) {
+        if (p.f16)
+            bwd_preprocess128_kernel<true><<<grid, PRE_THREADS, 0, st>>>(p);
+        else
+            bwd_preprocess128_kernel<false><<<grid, PRE_THREADS, 0, st>>>(p);
+    } else if (p.f16) {
         bwd_preprocess_kernel<true><<<grid, PRE_THREADS, 0, st>>>(p);
-    else
+    } else {
         bwd_preprocess_kernel<false><<<grid, PRE_THREADS, 0, st>>>(p);
+    }
     bwd_finalize_l_kernel<<<dim3((s_r + 255) / 256, p.H, p.B), 256, 0, st>>>(p);
     return check_launch("bwd_preprocess");
 }

@@ -1044,6 +1044,7 @@ __global__ void __launch_bounds__(256) bwd_work_list_kernel(const BwdParams p, i
                                                             int sec, int tail_trip) {
     __shared__ int hist[WL_BINS];
     __shared__ int offs[WL_BINS];
+    __shared__ int part[8];
     // the last block sorts the merged tail (the last `tail_trip` triples as one section)
     const bool tail = blockIdx.x == gridDim.x - 1;
     const int body = n_trip - tail_trip;
@@ -1078,12 +1079,27 @@ __global__ void __launch_bounds__(256) bwd_work_list_kernel(const BwdParams p, i
         atomicAdd(&hist[min(w[7], WL_BINS - 1)], 1);
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        int at = 0;
-        for (int c = WL_BINS - 1; c >= 0; --c) {
-            offs[c] = at;
-            at += hist[c];
+    {   // where each cost's entries start, the longest first: four bins a thread, then a scan over the block
+        static_assert(WL_BINS == 4 * 256, "four bins a thread");
+        const int c0 = WL_BINS - 1 - 4 * threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        int own[4], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            own[i] = sum;
+            sum += hist[c0 - i];
         }
+        int x = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) part[warp] = x;
+        __syncthreads();
+        int at = x - sum;
+        for (int i = 0; i < warp; ++i) at += part[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) offs[c0 - i] = at + own[i];
     }
     __syncthreads();
     for (int li = threadIdx.x; li < count; li += blockDim.x) {
