@@ -7,6 +7,7 @@ command that builds it. Functions take raw device pointers
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -74,6 +75,18 @@ def call(name, *args):
 def ptr(t):
     """A tensor's device address, or NULL for None."""
     return None if t is None else t.data_ptr()
+
+
+_NOTHING = contextlib.nullcontext()
+_DEVICE = getattr(torch._C, "_cuda_getDevice", None)
+
+
+def on(device):
+    """A context in which `device` is the current CUDA device: the kernels
+    launch on the current one. Nothing to do, and nothing done, where it already is."""
+    if device.type != "cuda" or device.index is None or (_DEVICE is not None and _DEVICE() == device.index):
+        return _NOTHING
+    return torch.cuda.device(device)
 
 
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)

@@ -11,6 +11,7 @@ with no host synchronisation.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 
@@ -197,7 +198,7 @@ def prepare_backward(
         2 main loop, 4 postprocess; in that order), for callers that time them
         apart or look at the work list between them."""
         if window:
-            with torch.cuda.device(dev):
+            with _lib.on(dev):
                 _lib.call("fold_bwd_window", *args, int(phases), _lib.stream(dev))
         else:
             _lib.call("fold_bwd_run_phases", *args, int(phases), _lib.stream(dev))
@@ -279,7 +280,7 @@ def attention_forward(q, k, v, *, causal, softmax_scale=None, cu_seqlens=None, m
         status = torch.zeros(1, device=q.device, dtype=torch.int32)
         if window:
             del args[13]
-            with torch.cuda.device(q.device):
+            with _lib.on(q.device):
                 _lib.call("fold_fwd_window_sm100", *args, window, sinks, None, 0, status.data_ptr(), _lib.stream(q.device))
         else:
             _lib.call("fold_fwd_run_sm100", *args, status.data_ptr(), _lib.stream(q.device))
@@ -289,11 +290,89 @@ def attention_forward(q, k, v, *, causal, softmax_scale=None, cu_seqlens=None, m
         return o, lse
     if window:
         del args[13]
-        with torch.cuda.device(q.device):
+        with _lib.on(q.device):
             _lib.call("fold_fwd_window", *args, window, sinks, None, 0, _lib.stream(q.device))
     else:
         _lib.call("fold_fwd_run", *args, _lib.stream(q.device))
     return o, lse
+
+
+@functools.lru_cache(maxsize=1024)
+def _stride_array(*values):
+    """Element strides as the host int64 array a call reads (kept by their values)."""
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+@functools.lru_cache(maxsize=1024)
+def _window_workspace(*shape):
+    """Bytes of a windowed backward's workspace and its status word's offset, for `(B, H, H_KV, S, total, D, varlen, window, sinks)`."""
+    lay = (ctypes.c_int64 * 12)()
+    _lib.call("fold_bwd_window_layout", *shape, lay)
+    return lay[11], lay[5]
+
+
+def _packed_strides(ts, varlen):
+    """`(batch, row, head)` strides of `(B, S, H, D)` or packed `(total, H, D)` tensors."""
+    out = []
+    for t in ts:
+        st = t.stride()
+        out += (0, st[0], st[1]) if varlen else st[:3]
+    return _stride_array(*out)
+
+
+def window_forward(q, k, v, window, sinks, softmax_scale, cu_seqlens=None, max_seqlen=None):
+    """`attention_forward` under a window for tensors the public entry points
+    have checked: the same kernels with less on the host, which is what a small
+    call costs."""
+    varlen = cu_seqlens is not None
+    dev, f16 = q.device, int(q.dtype is torch.float16)
+    if varlen:
+        total, H, D = q.shape
+        B, S = cu_seqlens.shape[0] - 1, int(max_seqlen)
+        lse = torch.empty((H, total), device=dev, dtype=torch.float32)
+    else:
+        B, S, H, D = q.shape
+        total = B * S
+        lse = torch.empty((B, H, S), device=dev, dtype=torch.float32)
+    o = torch.empty(q.shape, device=dev, dtype=q.dtype)
+    strides = _packed_strides((q, k, v, o), varlen)
+    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), ctypes.addressof(strides),
+            _lib.ptr(cu_seqlens), B, H, k.shape[-2], S, total, D, f16, softmax_scale, window, sinks, None, 0)
+    with _lib.on(dev):
+        if D == 128 and _lib.lib.fold_fwd_sm100_supported(D, f16):
+            status = torch.zeros(1, device=dev, dtype=torch.int32)
+            _lib.call("fold_fwd_window_sm100", *args, status.data_ptr(), _lib.stream(dev))
+            attention_forward.last_status = status
+            if attention_forward.check_status:
+                check_status(status, "attention_forward")
+        else:
+            _lib.call("fold_fwd_window", *args, _lib.stream(dev))
+    return o, lse
+
+
+def window_backward(q, k, v, o, do, lse, window, sinks, softmax_scale, cu_seqlens=None, max_seqlen=None):
+    """dQ, dK and dV of `window_forward`'s call, and the status word: what
+    `prepare_backward(window=)` launches, once and in the caller's layout."""
+    varlen = cu_seqlens is not None
+    dev = q.device
+    if varlen:
+        total, H, D = q.shape
+        B, S = cu_seqlens.shape[0] - 1, int(max_seqlen)
+    else:
+        B, S, H, D = q.shape
+        total = B * S
+    HKV = k.shape[-2]
+    nbytes, at = _window_workspace(B, H, HKV, S, total, D, int(varlen), window, sinks)
+    work = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    strides = _packed_strides((q, k, v, o, do, dq, dk, dv), varlen)
+    with _lib.on(dev):
+        _lib.call(
+            "fold_bwd_window", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(), dq.data_ptr(),
+            dk.data_ptr(), dv.data_ptr(), ctypes.addressof(strides), _lib.ptr(cu_seqlens), B, H, HKV, S, total, D,
+            int(q.dtype is torch.float16), softmax_scale, work.data_ptr(), nbytes, 0, window, sinks, 15, _lib.stream(dev),
+        )
+    return dq, dk, dv, work[at:at + 4]
 
 
 # The tcgen05 forward's status word of the last call; with `check_status` set every call reads

@@ -52,7 +52,8 @@ WsLayout ws_layout(int B, int H, int HKV, int S, int total, int D, bool varlen, 
     w.dq_acc = off; off = align256(off + sizeof(int) * static_cast<size_t>(H) * w.rows_p * D);
     w.dpsum = off;  off = align256(off + sizeof(float) * static_cast<size_t>(H) * w.rows_p);
     w.lse2 = off;   off = align256(off + sizeof(float) * static_cast<size_t>(H) * w.rows_p);
-    // the maxima, then the status word, then the work list's two counters
+    // the maxima, then the status word, then the work list's two counters, then the dK and dV accumulators:
+    // one stretch of memory, zeroed in one go
     w.stats = off;  off = align256(off + sizeof(int) * (N_STATS * static_cast<size_t>(B) * HKV + 3));
     w.dk_acc = off; off = align256(off + 8 * acc);
     w.dv_acc = off; off = align256(off + (plan.dv_bits / 8) * acc);

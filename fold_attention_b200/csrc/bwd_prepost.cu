@@ -328,13 +328,14 @@ __global__ void __launch_bounds__(256) bwd_finalize_l_kernel(const BwdParams p) 
 }
 
 int launch_bwd_preprocess(const BwdParams& p, cudaStream_t st) {
-    // the maxima, the status word and the work list's two counters
-    cudaMemsetAsync(p.stats, 0, sizeof(int) * (N_STATS * p.B * p.HKV + 3), st);
-    const size_t acc_rows = p.fold ? p.rows_p : static_cast<size_t>(p.B) * p.sink_stride;
+    // the maxima, the status word and the work list's two counters, and the dK and dV accumulators,
+    // which follow them in the workspace
+    size_t zero = sizeof(int) * (N_STATS * static_cast<size_t>(p.B) * p.HKV + 3);
     if (p.fold || p.sink_rows > 0) {
-        cudaMemsetAsync(p.dk_acc, 0, 8 * static_cast<size_t>(p.HKV) * acc_rows * p.D, st);
-        cudaMemsetAsync(p.dv_acc, 0, (p.dv_bits / 8) * static_cast<size_t>(p.HKV) * acc_rows * p.D, st);
+        const size_t acc_rows = p.fold ? p.rows_p : static_cast<size_t>(p.B) * p.sink_stride;
+        zero = static_cast<uint8_t*>(p.dv_acc) - reinterpret_cast<uint8_t*>(p.stats) + (p.dv_bits / 8) * static_cast<size_t>(p.HKV) * acc_rows * p.D;
     }
+    cudaMemsetAsync(p.stats, 0, zero, st);
     const int s_r = (p.S + ROW_PAD - 1) / ROW_PAD * ROW_PAD;
     dim3 grid(s_r / PRE_ROWS, p.H, p.B);
     if (p.D == 128) {

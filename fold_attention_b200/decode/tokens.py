@@ -15,6 +15,7 @@ takes prompts whole and then one token a request.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -35,7 +36,7 @@ _OUT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 def _int32(name, t, shape, device):
-    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} is a contiguous int32 {tuple(shape)} on {device} (got {t.dtype} {tuple(t.shape)} on {t.device})")
 
 
@@ -74,7 +75,7 @@ def build_tables(cu_seqlens, seq_lens, page_table, page_size, total, *, free_pag
         _int32("taken", taken, (1,), dev)
     out = torch.empty(total + B + 1, device=dev, dtype=torch.int32)
     slots, lens, used = out[:total], out[total:total + B], out[total + B:]
-    with torch.cuda.device(dev):
+    with _lib.on(dev):
         _lib.call(
             "fold_build_tables", cu_seqlens.data_ptr(), seq_lens.data_ptr(), B, page_table.data_ptr(), page_table.shape[1], page_size,
             total, _lib.ptr(free_pages) or None, n_free, _lib.ptr(taken), slots.data_ptr(), lens.data_ptr(),
@@ -88,7 +89,7 @@ def _planes(D, ka, kb, va, vb, ek, dev):
     rows = ka.shape[0]
     vdt = torch.bfloat16 if vb is None else torch.float8_e4m3fn
     for name, t, dt in (("ka", ka, torch.int8), ("kb", kb, torch.int8), ("va", va, vdt), ("vb", vb, vdt)):
-        if t is not None and (t.dtype != dt or tuple(t.shape) != (rows, D) or t.device != dev or not t.is_contiguous()):
+        if t is not None and (t.dtype is not dt or t.shape != (rows, D) or t.device != dev or not t.is_contiguous()):
             raise ValueError(f"{name} is a contiguous {dt} ({rows}, {D}) on {dev} (got {t.dtype} {tuple(t.shape)} on {t.device})")
     if ek.dtype != torch.bfloat16 or tuple(ek.shape) != (rows,) or ek.device != dev or not ek.is_contiguous():
         raise ValueError(f"ek is a contiguous bf16 ({rows},) on {dev} (got {ek.dtype} {tuple(ek.shape)} on {ek.device})")
@@ -96,8 +97,8 @@ def _planes(D, ka, kb, va, vb, ek, dev):
 
 def _rows(t):
     """`t` with 16-byte rows the kernels can read in place, or a copy."""
-    ok = t.stride(-1) == 1 and all(s % 8 == 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0
-    return t if ok else t.contiguous()
+    a, b, c = t.stride()
+    return t if c == 1 and not (a | b) & 7 and not t.data_ptr() & 15 else t.contiguous()
 
 
 def write_tokens(k, v, slots, page_size, ka, kb, va, vb, ek, *, v_scale=1.0):
@@ -117,7 +118,7 @@ def write_tokens(k, v, slots, page_size, ka, kb, va, vb, ek, *, v_scale=1.0):
     _int32("slots", slots, (n,), dev)
     _planes(D, ka, kb, va, vb, ek, dev)
     k, v = _rows(k), _rows(v)
-    with torch.cuda.device(dev):
+    with _lib.on(dev):
         _lib.call(
             "fold_write_tokens", k.data_ptr(), v.data_ptr(), int(k.dtype == torch.float16), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
             slots.data_ptr(), n, HKV, D, int(page_size), ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb), ek.data_ptr(),
@@ -139,7 +140,7 @@ def read_tokens(slots, page_size, n_kv_heads, ka, kb, va, vb, ek, *, v_scale=1.0
     _planes(D, ka, kb, va, vb, ek, dev)
     k = torch.empty((n, HKV, D), device=dev, dtype=dtype)
     v = torch.empty_like(k)
-    with torch.cuda.device(dev):
+    with _lib.on(dev):
         _lib.call(
             "fold_read_tokens", slots.data_ptr(), n, HKV, D, int(page_size), ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb),
             ek.data_ptr(), float(v_scale), k.data_ptr(), v.data_ptr(), _OUT[dtype], _lib.stream(dev),
@@ -151,12 +152,17 @@ def chunk_sums(v, cu_seqlens, lens_new, seq_lens, v_scale, vsum, vmean):
     """The running V sums and means with a chunk's `v` added, and `seq_lens` set to `lens_new`."""
     n, HKV, D = v.shape
     v = _rows(v)
-    with torch.cuda.device(v.device):
+    with _lib.on(v.device):
         _lib.call(
             "fold_chunk_sums", v.data_ptr(), int(v.dtype == torch.float16), v.stride(0), v.stride(1), seq_lens.shape[0], HKV, D,
             cu_seqlens.data_ptr(), n, lens_new.data_ptr(), seq_lens.data_ptr(), float(v_scale), vsum.data_ptr(), vmean.data_ptr(),
             _lib.stream(v.device),
         )
+
+
+@functools.lru_cache(maxsize=None)
+def _sms(index):
+    return torch.cuda.get_device_properties(index).multi_processor_count
 
 
 SHORT_ROWS = 128     # new tokens x query heads a KV head that chunk_sm100.cu takes
@@ -181,10 +187,10 @@ def chunk_attention(q, cu_seqlens, lens, cap_tiles, seq_lens, page_table, page_s
     pool = (page_table.data_ptr(), page_table.shape[1], int(page_size))
     planes = (ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb), ek.data_ptr(), float(v_scale))
     base = work.data_ptr()
-    with torch.cuda.device(dev):
+    with _lib.on(dev):
         st = _lib.stream(dev)
         if short:
-            ctas = torch.cuda.get_device_properties(dev).multi_processor_count
+            ctas = _sms(dev.index)
             nbytes = _lib.lib.fold_chunk_workspace_bytes(B, total, H, n_kv_heads, D, ctas)
             space = torch.empty(nbytes, device=dev, dtype=torch.uint8)
             _lib.call(

@@ -15,7 +15,8 @@ import math
 
 import torch
 
-from .backward.launch import attention_forward, prepare_backward
+from .backward.launch import attention_forward, prepare_backward, window_backward, window_forward
+from .utils import check_status as read_status
 from .utils import check_window, require_sm100
 
 # Set to True to read the backward's device status word after every backward (one host
@@ -40,11 +41,23 @@ def _check_qkv(q, k, v, ndim):
     require_sm100(q.device)
 
 
+def _windowed_input(x):
+    """`x` as the windowed kernels read it in place, or a copy: a contiguous head
+    dim, rows on 16-byte boundaries, and no axis that a broadcast gave stride 0."""
+    st = x.stride()
+    ok = st[-1] == 1 and all(s and s % 8 == 0 for s in st[:-1]) and x.data_ptr() % 16 == 0
+    return x if ok else x.contiguous()
+
+
 class _FoldAttnFunc(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, softmax_scale, causal, window, sinks):
-        q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, v))
-        out, lse = attention_forward(q, k, v, causal=causal, softmax_scale=softmax_scale, window=window, sinks=sinks)
+        if window:
+            q, k, v = _windowed_input(q), _windowed_input(k), _windowed_input(v)
+            out, lse = window_forward(q, k, v, window, sinks, softmax_scale)
+        else:
+            q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, v))
+            out, lse = attention_forward(q, k, v, causal=causal, softmax_scale=softmax_scale)
         ctx.save_for_backward(q, k, v, out, lse)
         ctx.softmax_scale, ctx.causal, ctx.window, ctx.sinks = softmax_scale, causal, window, sinks
         return out
@@ -53,6 +66,11 @@ class _FoldAttnFunc(torch.autograd.Function):
     def backward(ctx, *grad_outputs):
         (dout,) = grad_outputs
         q, k, v, out, lse = ctx.saved_tensors
+        if ctx.window:
+            dq, dk, dv, status = window_backward(q, k, v, out, dout.contiguous(), lse, ctx.window, ctx.sinks, ctx.softmax_scale)
+            if check_status:
+                read_status(status.view(torch.int32), "fold_attn_func's backward")
+            return dq, dk, dv, None, None, None, None
         run = prepare_backward(
             q.transpose(1, 2),
             k.transpose(1, 2),
@@ -62,8 +80,6 @@ class _FoldAttnFunc(torch.autograd.Function):
             lse,
             causal=ctx.causal,
             softmax_scale=ctx.softmax_scale,
-            window=ctx.window,
-            sinks=ctx.sinks,
         )
         dq, dk, dv = run()
         if check_status:
@@ -74,11 +90,15 @@ class _FoldAttnFunc(torch.autograd.Function):
 class _FoldAttnVarlenFunc(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_seqlens, max_seqlen, softmax_scale, causal, window, sinks):
-        q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, v))
-        out, lse = attention_forward(
-            q, k, v, causal=causal, softmax_scale=softmax_scale,
-            cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, window=window, sinks=sinks,
-        )
+        if window:
+            q, k, v = _windowed_input(q), _windowed_input(k), _windowed_input(v)
+            out, lse = window_forward(q, k, v, window, sinks, softmax_scale, cu_seqlens, max_seqlen)
+        else:
+            q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, v))
+            out, lse = attention_forward(
+                q, k, v, causal=causal, softmax_scale=softmax_scale,
+                cu_seqlens=cu_seqlens, max_seqlen=max_seqlen,
+            )
         ctx.save_for_backward(q, k, v, out, lse, cu_seqlens)
         ctx.max_seqlen, ctx.softmax_scale, ctx.causal = max_seqlen, softmax_scale, causal
         ctx.window, ctx.sinks = window, sinks
@@ -88,6 +108,12 @@ class _FoldAttnVarlenFunc(torch.autograd.Function):
     def backward(ctx, *grad_outputs):
         (dout,) = grad_outputs
         q, k, v, out, lse, cu_seqlens = ctx.saved_tensors
+        if ctx.window:
+            dq, dk, dv, status = window_backward(
+                q, k, v, out, dout.contiguous(), lse, ctx.window, ctx.sinks, ctx.softmax_scale, cu_seqlens, ctx.max_seqlen)
+            if check_status:
+                read_status(status.view(torch.int32), "fold_attn_varlen_func's backward")
+            return dq, dk, dv, None, None, None, None, None, None
         run = prepare_backward(
             q,
             k,
@@ -99,8 +125,6 @@ class _FoldAttnVarlenFunc(torch.autograd.Function):
             softmax_scale=ctx.softmax_scale,
             cu_seqlens=cu_seqlens,
             max_seqlen=ctx.max_seqlen,
-            window=ctx.window,
-            sinks=ctx.sinks,
         )
         dq, dk, dv = run()
         if check_status:
@@ -126,7 +150,7 @@ def fold_attn_func(q, k, v, softmax_scale=None, causal=False, window=None, sinks
     if q.shape[1] != k.shape[1]:
         raise ValueError("self-attention needs equal query and key lengths")
     scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else float(softmax_scale)
-    return _FoldAttnFunc.apply(q, k, v, scale, bool(causal), window or None, sinks)
+    return _FoldAttnFunc.apply(q, k, v, scale, bool(causal), window, sinks)
 
 
 def fold_attn_varlen_func(
@@ -163,7 +187,7 @@ def fold_attn_varlen_func(
     if max_seqlen_k is not None and int(max_seqlen_k) != int(max_seqlen_q):
         raise ValueError("self-attention needs max_seqlen_k == max_seqlen_q")
     scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else float(softmax_scale)
-    return _FoldAttnVarlenFunc.apply(q, k, v, cu, int(max_seqlen_q), scale, bool(causal), window or None, sinks)
+    return _FoldAttnVarlenFunc.apply(q, k, v, cu, int(max_seqlen_q), scale, bool(causal), window, sinks)
 
 
 def fold_attn_with_kvcache(q, cache, k=None, v=None, cu_seqlens=None, lens=None):

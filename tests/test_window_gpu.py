@@ -196,3 +196,53 @@ def test_values_under_masks_of_all_sizes_stay_finite():
     # scores reach a few hundred: an fp32 product of 128 bf16 terms is off by 2^-24 of its terms' size, a
     # weight by that times the score; well inside the 16-bit roundings counted above
     check([x[0] for x in got], want, torch.bfloat16)
+
+
+@pytest.mark.parametrize("D", [128, 64])
+def test_broadcast_heads_and_odd_strides(D):
+    """One KV head's tensors expanded over four, queries in a view whose rows sit off the 16-byte boundary."""
+    import fold_attention_b200 as fa
+
+    S, window, sinks, dt = 300, 50, 2, torch.bfloat16
+    q, k, v, do = inputs(S, 4, 1, D, dt, seed=4)
+    wide = torch.zeros(1, S, 4, D + 3, device="cuda", dtype=dt)
+    wide[..., 3:] = q[None]
+    x = [wide[..., 3:].detach().requires_grad_(), k[None].clone().requires_grad_(), v[None].clone().requires_grad_()]
+    out = fa.fold_attn_func(x[0], x[1].expand(1, S, 4, D), x[2].expand(1, S, 4, D), causal=True, window=window, sinks=sinks)
+    got = (out.detach(), *torch.autograd.grad(out, x, do[None]))
+    # four heads' gradients are added up in 16 bits: three more roundings of a sum, each half a step
+    want = reference(q, k, v, do, window, sinks)
+    eps = half_step(dt)
+    for name, a, b, steps in zip(("out", "dq", "dk", "dv"), got, want, (1, 2, 5, 5)):
+        slack = {"dq": want[4], "dk": want[5]}.get(name)
+        tol = steps * eps * b.norm().item() + (0 if slack is None else slack.norm().item() * eps)
+        assert (a[0].double() - b).norm().item() <= tol, name
+
+
+def test_on_another_stream_and_captured_beside_an_eager_graph():
+    import fold_attention_b200 as fa
+
+    S, window, sinks = 500, 70, 3
+    q, k, v, do = (t[None] for t in inputs(S, 4, 2, 128, torch.bfloat16, seed=6))
+    want = run_dense(q, k, v, do, window, sinks)
+    x = [t.clone().requires_grad_() for t in (q, k, v)]
+    eager = fa.fold_attn_func(*x, causal=True, window=window, sinks=sinks)        # lives on while the graph is captured
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = [t.detach().clone().requires_grad_() for t in x]
+        other = fa.fold_attn_func(*y, causal=True, window=window, sinks=sinks)
+        grads = torch.autograd.grad(other, y, do)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((other, *grads), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            z = [t.detach().requires_grad_() for t in x]
+            out = fa.fold_attn_func(*z, causal=True, window=window, sinks=sinks)
+            captured = torch.autograd.grad(out, z, do)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((out, *captured), want))
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(eager, x, do), want[1:]))
