@@ -62,11 +62,17 @@ lib = _load()
 _ERRORS = {1: ValueError, 4: NotImplementedError}
 
 
+_FUNCTIONS = {}
+
+
 def call(name, *args):
     """Call an int-returning entry point; raise with the library's message on
     a non-zero status (bad argument -> ValueError, unsupported ->
     NotImplementedError, anything else -> FoldLibraryError)."""
-    rc = getattr(lib, name)(*args)
+    fn = _FUNCTIONS.get(name)
+    if fn is None:
+        fn = _FUNCTIONS[name] = getattr(lib, name)
+    rc = fn(*args)
     if rc != 0:
         msg = lib.fold_last_error().decode()
         raise _ERRORS.get(rc, FoldLibraryError)(f"{name}: {msg} (status {rc})")

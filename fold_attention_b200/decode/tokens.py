@@ -56,43 +56,60 @@ def build_tables(cu_seqlens, seq_lens, page_table, page_size, total, *, free_pag
     than the table are left as they are, so the same call gives the same
     answer. All tensors are int32 on one device; nothing waits on it.
     """
-    dev = seq_lens.device
-    if seq_lens.ndim != 1 or page_table.ndim != 2 or seq_lens.shape[0] < 1 or page_table.shape[1] < 1:
-        raise ValueError(f"seq_lens is (batch,) and page_table (batch, pages), got {tuple(seq_lens.shape)}, {tuple(page_table.shape)}")
-    B = seq_lens.shape[0]
-    _int32("seq_lens", seq_lens, (B,), dev)
-    _int32("cu_seqlens", cu_seqlens, (B + 1,), dev)
-    _int32("page_table", page_table, (B, page_table.shape[1]), dev)
     total, page_size = int(total), int(page_size)
+    B = seq_lens.numel()
+    if not (seq_lens.dtype is cu_seqlens.dtype is page_table.dtype is torch.int32 and seq_lens.ndim == 1 and page_table.ndim == 2
+            and cu_seqlens.shape == (B + 1,) and page_table.shape[0] == B and seq_lens.is_contiguous() and cu_seqlens.is_contiguous()
+            and page_table.is_contiguous() and cu_seqlens.get_device() == page_table.get_device() == seq_lens.get_device()
+            and B > 0 and page_table.shape[1] > 0):
+        _tables_refused(cu_seqlens, seq_lens, page_table)
     if total < 0 or page_size < 1:
         raise ValueError(f"{total} tokens, pages of {page_size} keys")
     if (free_pages is None) != (taken is None):
         raise ValueError("free_pages and taken are both given or both left out")
-    n_free = 0
+    dev = seq_lens.device
+    n_free, used = 0, None
     if free_pages is not None:
         n_free = free_pages.numel()
         _int32("free_pages", free_pages, (n_free,), dev)
         _int32("taken", taken, (1,), dev)
-    out = torch.empty(total + B + 1, device=dev, dtype=torch.int32)
-    slots, lens, used = out[:total], out[total:total + B], out[total + B:]
+        used = torch.empty_like(taken)
+    slots, lens = seq_lens.new_empty(total), torch.empty_like(seq_lens)
     with _lib.on(dev):
         _lib.call(
             "fold_build_tables", cu_seqlens.data_ptr(), seq_lens.data_ptr(), B, page_table.data_ptr(), page_table.shape[1], page_size,
-            total, _lib.ptr(free_pages) or None, n_free, _lib.ptr(taken), slots.data_ptr(), lens.data_ptr(),
-            used.data_ptr() if free_pages is not None else None, _lib.stream(dev),
+            total, _lib.ptr(free_pages) or None, n_free, _lib.ptr(taken), slots.data_ptr(), lens.data_ptr(), _lib.ptr(used), _lib.stream(dev),
         )
-    return slots, lens, used if free_pages is not None else None
+    return slots, lens, used
+
+
+def _tables_refused(cu_seqlens, seq_lens, page_table):
+    dev, B = seq_lens.device, seq_lens.numel()
+    if seq_lens.ndim != 1 or page_table.ndim != 2 or B < 1 or page_table.shape[1] < 1:
+        raise ValueError(f"seq_lens is (batch,) and page_table (batch, pages), got {tuple(seq_lens.shape)}, {tuple(page_table.shape)}")
+    _int32("seq_lens", seq_lens, (B,), dev)
+    _int32("cu_seqlens", cu_seqlens, (B + 1,), dev)
+    _int32("page_table", page_table, (B, page_table.shape[1]), dev)
 
 
 def _planes(D, ka, kb, va, vb, ek, dev):
     """The pool's planes, checked against each other: the kernels index all of them by one row."""
-    rows = ka.shape[0]
+    shape = (ka.shape[0], D)
+    ok = (ka.dtype is kb.dtype is torch.int8 and ek.dtype is torch.bfloat16 and ka.shape == kb.shape == va.shape == shape
+          and ek.shape == shape[:1] and ka.device == dev and kb.get_device() == va.get_device() == ek.get_device() == ka.get_device()
+          and ka.is_contiguous() and kb.is_contiguous() and va.is_contiguous() and ek.is_contiguous())
+    if vb is None:
+        ok = ok and va.dtype is torch.bfloat16
+    else:
+        ok = (ok and va.dtype is vb.dtype is torch.float8_e4m3fn and vb.shape == shape and vb.get_device() == ka.get_device()
+              and vb.is_contiguous())
+    if ok:
+        return
     vdt = torch.bfloat16 if vb is None else torch.float8_e4m3fn
-    for name, t, dt in (("ka", ka, torch.int8), ("kb", kb, torch.int8), ("va", va, vdt), ("vb", vb, vdt)):
-        if t is not None and (t.dtype is not dt or t.shape != (rows, D) or t.device != dev or not t.is_contiguous()):
-            raise ValueError(f"{name} is a contiguous {dt} ({rows}, {D}) on {dev} (got {t.dtype} {tuple(t.shape)} on {t.device})")
-    if ek.dtype != torch.bfloat16 or tuple(ek.shape) != (rows,) or ek.device != dev or not ek.is_contiguous():
-        raise ValueError(f"ek is a contiguous bf16 ({rows},) on {dev} (got {ek.dtype} {tuple(ek.shape)} on {ek.device})")
+    for name, t, dt, want in (("ka", ka, torch.int8, shape), ("kb", kb, torch.int8, shape), ("va", va, vdt, shape),
+                              ("vb", vb, vdt, shape), ("ek", ek, torch.bfloat16, shape[:1])):
+        if t is not None and (t.dtype is not dt or t.shape != want or t.device != dev or not t.is_contiguous()):
+            raise ValueError(f"{name} is a contiguous {dt} {want} on {dev} (got {t.dtype} {tuple(t.shape)} on {t.device})")
 
 
 def _rows(t):
@@ -118,9 +135,11 @@ def write_tokens(k, v, slots, page_size, ka, kb, va, vb, ek, *, v_scale=1.0):
     _int32("slots", slots, (n,), dev)
     _planes(D, ka, kb, va, vb, ek, dev)
     k, v = _rows(k), _rows(v)
+    k0, k1, _ = k.stride()
+    v0, v1, _ = v.stride()
     with _lib.on(dev):
         _lib.call(
-            "fold_write_tokens", k.data_ptr(), v.data_ptr(), int(k.dtype == torch.float16), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+            "fold_write_tokens", k.data_ptr(), v.data_ptr(), int(k.dtype is torch.float16), k0, k1, v0, v1,
             slots.data_ptr(), n, HKV, D, int(page_size), ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb), ek.data_ptr(),
             float(v_scale), _lib.stream(dev),
         )
@@ -138,7 +157,7 @@ def read_tokens(slots, page_size, n_kv_heads, ka, kb, va, vb, ek, *, v_scale=1.0
     n, HKV = slots.shape[0], int(n_kv_heads)
     _int32("slots", slots, (n,), dev)
     _planes(D, ka, kb, va, vb, ek, dev)
-    k = torch.empty((n, HKV, D), device=dev, dtype=dtype)
+    k = ka.new_empty((n, HKV, D), dtype=dtype)
     v = torch.empty_like(k)
     with _lib.on(dev):
         _lib.call(
@@ -168,19 +187,28 @@ def _sms(index):
 SHORT_ROWS = 128     # new tokens x query heads a KV head that chunk_sm100.cu takes
 
 
+# Where a batch holds wider requests too, its short ones get the second kernel only if that many 128-key tiles
+# (x KV heads) pay for it: nine requests of up to 1500 keys and two KV heads take 57 us dequantised together and 97 with
+# both kernels; a decode batch's long contexts read from the codes at a third of the bytes.
+MIXED_TILES = 1024
+
+
 def chunk_attention(q, cu_seqlens, lens, cap_tiles, seq_lens, page_table, page_size, ka, kb, va, vb, ek, v_scale, n_kv_heads,
                     window, sinks):
     """Attention of each request's last tokens over the pool: `q` `(total, H,
-    D)`, cut by `cu_seqlens`, `lens[b]` rows of request b. A request of up to
-    `SHORT_ROWS` query rows a KV head is attended straight from the codes; the
-    others' keys are dequantised first, `cap_tiles` 128-key tiles of them at
-    most. Returns `(out, status)`."""
+    D)`, cut by `cu_seqlens`, `lens[b]` rows of request b. `cap_tiles` is two
+    counts of 128-key tiles at most: of the requests with up to `SHORT_ROWS` query
+    rows a KV head, which are attended straight from the codes, and of the
+    others, whose keys are dequantised first. Returns `(out, status)`."""
     total, H, D = q.shape
     dev, dt = q.device, q.dtype
     B, G = seq_lens.shape[0], H // n_kv_heads
     f16, win = int(dt == torch.float16), window or 1 << 30
-    short = any(0 < n * G <= SHORT_ROWS for n in lens)
-    wide = max(lens) * G > SHORT_ROWS
+    short, wide = cap_tiles[0] > 0, cap_tiles[1] > 0
+    if short and wide and cap_tiles[0] * n_kv_heads < MIXED_TILES:
+        short, cap_tiles = False, sum(cap_tiles)
+    else:
+        cap_tiles = cap_tiles[1]
     out = torch.empty((total, H, D), device=dev, dtype=dt)
     work = torch.empty(4 + (4 * B + 2 * cap_tiles if wide else 0), device=dev, dtype=torch.int32)
     status = work[:1]

@@ -11,6 +11,7 @@ one power of two for the layer, fixed at prefill (`v_headroom`).
 from __future__ import annotations
 
 import math
+import operator
 
 import torch
 
@@ -411,19 +412,21 @@ class FoldKVCache:
         an 8-bit V. fp16 queries see K and V saturated to fp16's range."""
         lens = self._chunk_lens(cu_seqlens, lens)
         self._check_chunk_q(q, lens)
-        if any(n > a for n, a in zip(lens, self.lens)):
+        if any(map(operator.gt, lens, self.lens)):
             raise ValueError("a request has more query rows than tokens in the cache")
         if sum(lens) == 0:
             return torch.empty_like(q)
         q = tokens._rows(q)
         # a captured call is replayed on longer requests: it is laid out for the longest there can be
         capturing = torch.cuda.is_current_stream_capturing()
-        cap = 0
+        cap, st = [0, 0], -(-self.sinks // 128)
         for n, a in zip(lens, self.lens):
-            if n * self.group > tokens.SHORT_ROWS:
+            if n:
                 end = self.max_len if capturing else a
-                first = 0 if capturing else max(0, a - n - (self.window or a) + 1) // 128
-                cap += -(-end // 128) - max(0, first - -(-self.sinks // 128))
+                tiles = -(-end // 128)
+                if self.window:      # the sinks' tiles and those its window can touch, wherever it stands
+                    tiles = min(tiles, st + (n + self.window + 253) // 128)
+                cap[n * self.group > tokens.SHORT_ROWS] += tiles
         out, self._chunk_status = tokens.chunk_attention(
             q, cu_seqlens, lens, cap, self.seq_lens, self.page_table, self.page_size, self.ka, self.kb, self.va, self.vb, self.ek,
             self.v_scale, self.n_kv_heads, self.window, self.sinks,
@@ -456,7 +459,7 @@ class FoldKVCache:
             raise ValueError(f"cu_seqlens is int32 ({self.batch + 1},) on {self.seq_lens.device}")
         if lens is None:
             lens = torch.diff(cu_seqlens).tolist()
-        lens = [int(n) for n in lens]
+        lens = list(map(int, lens))
         if len(lens) != self.batch or min(lens) < 0:
             raise ValueError(f"{len(lens)} counts, the least {min(lens, default=0)}, for a batch of {self.batch}")
         return lens
