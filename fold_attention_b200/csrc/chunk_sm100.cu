@@ -24,7 +24,7 @@
 // order, so the bits do not depend on who that is.
 //
 // Warps: 0 K producer (both planes, scales), 3 V producer, 1 MMA issuer, 2 Q and V's dead rows (bf16 V),
-// 4-7 softmax and epilogue, 2 (8-bit V) or 8 (bf16 V) joins pieces, 8-11 V's conversion (8-bit V). Every wait is bounded.
+// 4-7 softmax and epilogue, 2 (8-bit V) or 8-11 (bf16 V) join pieces, 8-11 V's conversion (8-bit V). Every wait is bounded.
 #include <cuda.h>
 
 #include <type_traits>
@@ -769,7 +769,7 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
                     mbar_wait(bar(B_ODONE), (j - 1) & 1, abort_flag, p.status);
                     tc_fence_after();
                     if (__any_sync(0xffffffffu, live && alpha != 1.0f)) {
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < D / 32; ++c) {
                             uint32_t ov[32];
                             tmem_ld32(tmem + lane_addr + T_O + 32 * c, ov);
@@ -891,34 +891,31 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
                 if (j > 1) mbar_wait(bar(B_CEMPTY + (j & 1)), ((j >> 1) - 1) & 1, abort_flag, p.status);   // the product two tiles back has read its rows
                 const uint4* src = reinterpret_cast<const uint4*>(smem + L::SM_V + s * L::VSLOT);
                 uint4* dst = reinterpret_cast<uint4*>(smem + L::SM_V16 + (j & 1) * 2 * L::PLANE);
-                // four units' loads at a time, then their arithmetic: one warp a scheduler has only its own
-                // instructions to hide a latency with
-                for (int i0 = c0; i0 < BN * UPR; i0 += 4 * 128) {
-                    uint4 a[4], b2[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        a[q] = src[i0 + 128 * q];
-                        b2[q] = src[L::PLANE / 16 + i0 + 128 * q];
+                // One unit a turn, the next one's loads ahead of its arithmetic, and not unrolled: what the warps of a
+                // scheduler run must fit its instruction cache together (four units a turn took 94 us where this takes 84)
+                uint4 a = src[c0], b2 = src[L::PLANE / 16 + c0];
+#pragma unroll 1
+                for (int i = c0; i < BN * UPR; i += 128) {
+                    const int r = i / UPR, u = i % UPR;
+                    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b2.x, b2.y, b2.z, b2.w};
+                    if (i + 128 < BN * UPR) {
+                        a = src[i + 128];
+                        b2 = src[L::PLANE / 16 + i + 128];
                     }
+                    uint32_t o[8];
+                    const bool keep = !cut || wanted(w.g, pos + r, 1);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int i = i0 + 128 * q, r = i / UPR, u = i % UPR;
-                        const uint32_t aw[4] = {a[q].x, a[q].y, a[q].z, a[q].w}, bw[4] = {b2[q].x, b2[q].y, b2[q].z, b2[q].w};
-                        uint32_t o[8];
-                        const bool keep = !cut || wanted(w.g, pos + r, 1);
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            uint32_t ha, hb, x;
-                            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(ha) : "h"(static_cast<uint16_t>(aw[k >> 1] >> (16 * (k & 1)))));
-                            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hb) : "h"(static_cast<uint16_t>(bw[k >> 1] >> (16 * (k & 1)))));
-                            asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(x) : "r"(hb), "r"(0x30003000u), "r"(ha));   // a + b / 8
-                            o[k] = keep ? x : 0u;
-                        }
-                        uint4* row = dst + (u >> 2) * 1024 + r * 8;
-                        const int ch = 2 * (u & 3);
-                        row[ch ^ (r & 7)] = make_uint4(o[0], o[1], o[2], o[3]);
-                        row[(ch + 1) ^ (r & 7)] = make_uint4(o[4], o[5], o[6], o[7]);
+                    for (int k = 0; k < 8; ++k) {
+                        uint32_t ha, hb, x;
+                        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(ha) : "h"(static_cast<uint16_t>(aw[k >> 1] >> (16 * (k & 1)))));
+                        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hb) : "h"(static_cast<uint16_t>(bw[k >> 1] >> (16 * (k & 1)))));
+                        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(x) : "r"(hb), "r"(0x30003000u), "r"(ha));   // a + b / 8
+                        o[k] = keep ? x : 0u;
                     }
+                    uint4* row = dst + (u >> 2) * 1024 + r * 8;
+                    const int ch = 2 * (u & 3);
+                    row[ch ^ (r & 7)] = make_uint4(o[0], o[1], o[2], o[3]);
+                    row[(ch + 1) ^ (r & 7)] = make_uint4(o[4], o[5], o[6], o[7]);
                 }
                 fence_async_smem();
                 __syncwarp();
