@@ -186,6 +186,35 @@ __device__ __forceinline__ void store16(void* base, int64_t at, const float (&x)
     }
 }
 
+// A row's fp32 channels, 16 to a lane, stored by whole cache lines: within groups of four lanes the 4 x 4 matrix
+// of 16-byte units is transposed (lane l's unit t to lane t's unit l), so that a group's store is 64 bytes in a row.
+template <int TPR>
+__device__ __forceinline__ void store_f32(float* row, int lane, bool ok, const float (&x)[16]) {
+    float4 u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+    const int q = lane & 3;
+    auto swap = [](float4& a, float4& b, bool upper, int off) {     // exchange the lower lane's b with the upper lane's a
+        const float4 give = upper ? a : b;
+        float4 got;
+        got.x = __shfl_xor_sync(0xffffffffu, give.x, off);
+        got.y = __shfl_xor_sync(0xffffffffu, give.y, off);
+        got.z = __shfl_xor_sync(0xffffffffu, give.z, off);
+        got.w = __shfl_xor_sync(0xffffffffu, give.w, off);
+        if (upper) a = got;
+        else b = got;
+    };
+    swap(u[0], u[1], q & 1, 1);
+    swap(u[2], u[3], q & 1, 1);
+    swap(u[0], u[2], q & 2, 2);
+    swap(u[1], u[3], q & 2, 2);
+    // lane q now holds unit q of lanes 0..3 of its group
+    float4* d = reinterpret_cast<float4*>(row) + (lane & ~3) * 4 + q;
+    if (ok)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[4 * i] = u[i];
+}
+
 template <int D, bool V8, int OUT>
 __global__ void __launch_bounds__(NT) read_tokens_kernel(const int* __restrict__ slots, int64_t n_rows, int hkv, int page_size, const Planes p,
                                                          void* k, void* v) {
@@ -198,7 +227,12 @@ __global__ void __launch_bounds__(NT) read_tokens_kernel(const int* __restrict__
     const int64_t prow = slot_row(slot < 0 ? 0 : slot, page_size, hkv, static_cast<int>(rr % hkv), off);
     float xk[16], xv[16];
     load_row<D, V8>(p, prow, off, lane, slot >= 0, xk, xv);
-    if (r < n_rows) {
+    if (OUT == OUT_F32) {
+        // 64 bytes a lane: a row's lanes take turns so that each store is a stretch of memory, not 16 bytes of
+        // every 64 (TPR lanes: unit t of lane l goes out as unit l + TPR t of the row)
+        store_f32<TPR>(static_cast<float*>(k) + r * D, lane, r < n_rows, xk);
+        store_f32<TPR>(static_cast<float*>(v) + r * D, lane, r < n_rows, xv);
+    } else if (r < n_rows) {
         store16<OUT>(k, r * D + lane * 16, xk);
         store16<OUT>(v, r * D + lane * 16, xv);
     }
@@ -247,21 +281,24 @@ __global__ void __launch_bounds__(16 * D / 4) chunk_sums_kernel(const uint16_t* 
 //
 // chunk_plan_kernel (one CTA) lays them out: plan[b] = (keys, first row, tiles left out between the
 // sinks' tiles and the window's, last position before the first query's window); keys -1: the request is
-// another kernel's; and for each 128-row tile (request, tile in the request).
+// another kernel's; then each request's first block of 256 query rows and their count, and for each 128-row tile (request, tile
+// in the request).
 constexpr int CP_THREADS = 256;
 __global__ void __launch_bounds__(CP_THREADS) chunk_plan_kernel(const int* __restrict__ cu, const int* __restrict__ lens, int batch, int max_keys,
                                                                 int window, int sinks, int rows_over, int group, int cap_tiles, int4* plan, int2* tiles, int* status) {
-    __shared__ int s_warp[CP_THREADS / 32];
+    __shared__ int s_warp[CP_THREADS / 32], s_warpq[CP_THREADS / 32];
     if (rows_over == 0 && threadIdx.x == 0) *status = 0;    // no other kernel of the call has a say in it
     __syncthreads();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ns = (sinks + 127) / 128;
-    int base = 0;
+    int* qfirst = reinterpret_cast<int*>(plan + batch);
+    int base = 0, qbase = 0;
     for (int b0 = 0; b0 < batch; b0 += CP_THREADS) {
         const int b = b0 + tid;
-        int klen = 0, shift = 0, nt = 0, before = -1;
+        int klen = 0, shift = 0, nt = 0, before = -1, nq = 0;
         if (b < batch) {
             const int n = cu[b + 1] - cu[b], len = lens[b];
+            nq = n > 0 && static_cast<int64_t>(n) * group > rows_over ? (n + 255) / 256 : 0;
             if (static_cast<int64_t>(n) * group <= rows_over) {
                 klen = -1;                     // another kernel's
             } else if (n > 0 && len > 0) {
@@ -272,28 +309,41 @@ __global__ void __launch_bounds__(CP_THREADS) chunk_plan_kernel(const int* __res
                 nt = max(0, (klen + 127) / 128 - shift);
             }
         }
-        int x = nt;
+        int x = nt, xq = nq;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
+            const int y = __shfl_up_sync(0xffffffffu, x, o), yq = __shfl_up_sync(0xffffffffu, xq, o);
+            if (lane >= o) {
+                x += y;
+                xq += yq;
+            }
         }
-        if (lane == 31) s_warp[warp] = x;
+        if (lane == 31) {
+            s_warp[warp] = x;
+            s_warpq[warp] = xq;
+        }
         __syncthreads();
-        int add = base, sum = 0;
+        int add = base, sum = 0, addq = qbase, sumq = 0;
         for (int w = 0; w < CP_THREADS / 32; ++w) {
-            if (w < warp) add += s_warp[w];
+            if (w < warp) {
+                add += s_warp[w];
+                addq += s_warpq[w];
+            }
             sum += s_warp[w];
+            sumq += s_warpq[w];
         }
         if (b < batch) {
             const int first = add + x - nt;
             const bool fits = first + nt <= cap_tiles;
             if (!fits) atomicExch(status, FOLD_ERR_ARGUMENT);   // lengths the host did not plan for: the request sees nothing
+            qfirst[b] = addq + xq - nq;
             plan[b] = make_int4(fits || klen < 0 ? klen : 0, first * 128, shift, before);
         }
         base += sum;
+        qbase += sumq;
         __syncthreads();
     }
+    if (tid == 0) qfirst[batch] = qbase;
     for (int g = tid; g < cap_tiles; g += CP_THREADS) {
         int lo = 0, hi = batch;          // the last request that starts at or before tile g
         while (hi - lo > 1) {

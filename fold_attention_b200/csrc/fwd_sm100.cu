@@ -185,7 +185,7 @@ struct Params {
     // tiles and the window's that no query of the chunk sees
     int window, sinks;
     const int4* plan;
-    int n_work;      // work items: heads x blocks of 256 rows (dense), x slots of 256 packed rows and one per request
+    int blocks;      // blocks of 256 rows (dense), or slots of 256 packed rows and one per request; with `plan` its own count
 };
 struct Maps {
     CUtensorMap q, k, v;   // (channel, row, head, batch), boxes (64, 128, 1, 1)
@@ -449,6 +449,7 @@ struct Item {
     int m0, h, b, start, len, klen, qoff, kstart, kshift;
     int ns, lo, n, st;
     int end[2], low[2], nt[2];      // nt: key tiles that query tile x takes
+    bool half;                      // 128 rows: there is no second query tile
     __device__ __forceinline__ int tile(int j) const { return j < ns ? j : lo + j - ns; }
     __device__ __forceinline__ bool takes(int e, int l, int j) const {
         const int t = tile(j);
@@ -462,22 +463,44 @@ struct Item {
 };
 
 // Work item i, longest rows first in a dense call; false if it is empty.
-__device__ __forceinline__ bool load_item(const Params& p, int i, Item& w) {
+struct List {
+    int blocks;      // of 256 rows
+    int whole;       // blocks x heads, of which so many are walked whole and the others as two items of 128 rows
+    int items;       // so many in all
+    const int* first;   // with `plan`: each request's first block
+};
+__device__ __forceinline__ List list_of(const Params& p) {
+    List l;
+    l.first = p.plan ? reinterpret_cast<const int*>(p.plan + p.B) : nullptr;
+    l.blocks = p.plan ? __ldg(l.first + p.B) : p.blocks;
+    // The last wave: where at most half of the CTAs would have an item of 256 rows, it is walked as twice as many
+    // of 128: the 512 items of a 2 x 2048-token chunk are 3.46 waves of 148 (1658 -> 1624 us).
+    const int n = l.blocks * p.H, ctas = static_cast<int>(gridDim.x), rest = n % ctas;
+    l.whole = n > ctas && 2 * rest <= ctas ? n - rest : n;
+    l.items = l.whole + 2 * (n - l.whole);
+    return l;
+}
+__device__ __forceinline__ bool load_item(const Params& p, const List& l, int i, Item& w) {
+    w.half = i >= l.whole;
+    const int second = w.half ? (i - l.whole) & 1 : 0;
+    if (w.half) i = l.whole + ((i - l.whole) >> 1);
     const int blk = i / p.H;
     w.h = i - blk * p.H;
     if (p.cu) {
         // packed: request b's blocks sit in slots from cu[b] / 256 + b on (at least as many as it needs)
-        const int slot = p.n_work / p.H - 1 - blk;
+        // (a chunk's plan counts them exactly)
+        const int slot = l.blocks - 1 - blk;
+        auto first_of = [&](int b) { return l.first ? __ldg(l.first + b) : __ldg(p.cu + b) / CTA_M + b; };
         int lo = 0, hi = p.B;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (__ldg(p.cu + mid) / CTA_M + mid <= slot) lo = mid;
+            if (first_of(mid) <= slot) lo = mid;
             else hi = mid;
         }
         w.b = lo;
         w.start = __ldg(p.cu + lo);
         w.len = __ldg(p.cu + lo + 1) - w.start;
-        w.m0 = (slot - (w.start / CTA_M + lo)) * CTA_M;
+        w.m0 = (slot - first_of(lo)) * CTA_M;
     } else {
         const int nb = (p.S + CTA_M - 1) / CTA_M;
         w.b = blk % p.B;
@@ -485,7 +508,9 @@ __device__ __forceinline__ bool load_item(const Params& p, int i, Item& w) {
         w.len = p.S;
         w.m0 = (nb - 1 - blk / p.B) * CTA_M;
     }
-    if (w.m0 < 0 || w.m0 >= w.len) return false;
+    if (w.m0 < 0) return false;
+    w.m0 += second * BM;
+    if (w.m0 >= w.len) return false;
     w.klen = w.len;
     w.qoff = w.kshift = 0;
     w.kstart = w.start;
@@ -501,7 +526,7 @@ __device__ __forceinline__ bool load_item(const Params& p, int i, Item& w) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int mx = w.m0 + x * BM;
-        const int kv_end = mx >= w.len ? 0 : max(0, min(w.klen, w.qoff + min(mx + BM, w.len)));
+        const int kv_end = mx >= w.len || (x == 1 && w.half) ? 0 : max(0, min(w.klen, w.qoff + min(mx + BM, w.len)));
         w.end[x] = (kv_end + BN - 1) / BN;
         w.low[x] = max(0, w.qoff + mx - p.window + 1) / BN;
         w.nt[x] = min(w.end[x], w.st) + max(0, w.end[x] - max(w.low[x], w.st));
@@ -547,14 +572,15 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_window_sm100_kernel(const Par
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    const List list = list_of(p);
 
     if (warp == 0) {
         // ================= TMA producer =================
         if (lane == 0) {
             int jk = 0, items = 0;         // key tiles, and items with any, so far
-            for (int i = blockIdx.x; i < p.n_work; i += gridDim.x) {
+            for (int i = blockIdx.x; i < list.items; i += gridDim.x) {
                 Item w;
-                if (!load_item(p, i, w) || w.nt[0] + w.nt[1] == 0) continue;
+                if (!load_item(p, list, i, w) || w.nt[0] + w.nt[1] == 0) continue;
                 const int hkv = w.h / p.G, bb = p.cu ? 0 : w.b;
                 if (items > 0) mbar_wait(bar(B_QEMPTY), (items - 1) & 1, abort_flag, p.status);
                 mbar_expect_tx(bar(B_Q), w.nt[0] > 0 && w.nt[1] > 0 ? 65536 : 32768);
@@ -582,9 +608,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_window_sm100_kernel(const Par
             constexpr uint32_t ID_S = instr_desc(F16 ? 0 : 1, 128, 128, 0, 0);    // Q (K-major) x K (K-major)
             constexpr uint32_t ID_PV = instr_desc(F16 ? 0 : 1, 128, 128, 0, 1);   // P (TMEM) x V (MN-major)
             int jk = 0, items = 0, done[2] = {0, 0};
-            for (int i = blockIdx.x; i < p.n_work; i += gridDim.x) {
+            for (int i = blockIdx.x; i < list.items; i += gridDim.x) {
                 Item w;
-                if (!load_item(p, i, w) || w.nt[0] + w.nt[1] == 0) continue;
+                if (!load_item(p, list, i, w) || w.nt[0] + w.nt[1] == 0) continue;
                 mbar_wait(bar(B_Q), items & 1, abort_flag, p.status);
                 int left = w.nt[0] + w.nt[1];      // scores still to issue
                 auto issue_s = [&](int x, int j) {
@@ -649,9 +675,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_window_sm100_kernel(const Par
         const uint32_t ts = tmem + lane_addr + T_S + 128 * x;
         const uint32_t to = tmem + lane_addr + T_O + 128 * x;
         int it = 0;                                // the query tile's key tiles so far
-        for (int i = blockIdx.x; i < p.n_work; i += gridDim.x) {
+        for (int i = blockIdx.x; i < list.items; i += gridDim.x) {
             Item w;
-            if (!load_item(p, i, w)) continue;
+            if (!load_item(p, list, i, w) || (x == 1 && w.half)) continue;
             const int mx = w.m0 + x * BM;
             const int qr = mx + r;                 // the query's row in its sequence
             const int qi = qr + w.qoff;            // its position among the keys
@@ -884,17 +910,17 @@ int run_sm100(const char* what, const void* q, const void* k, const void* v, voi
         // packed: a slot per 256 rows and one per request (fsm100::load_item); dense: the blocks themselves
         const int64_t blocks = cu_seqlens ? static_cast<int64_t>(total) / fsm100::CTA_M + batch
                                           : static_cast<int64_t>((max_seqlen + fsm100::CTA_M - 1) / fsm100::CTA_M) * batch;
-        FOLD_CHECK_ARG(blocks * n_heads < (1ll << 31), "%s: %lld blocks of %d heads", what, static_cast<long long>(blocks), n_heads);
-        p.n_work = static_cast<int>(blocks * n_heads);
+        FOLD_CHECK_ARG(2 * blocks * n_heads < (1ll << 31), "%s: %lld blocks of %d heads", what, static_cast<long long>(blocks), n_heads);
+        p.blocks = static_cast<int>(blocks);
         int dev = 0, sms = 1;
         cudaGetDevice(&dev);
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
         auto kern = f16 ? fsm100::fwd_window_sm100_kernel<true> : fsm100::fwd_window_sm100_kernel<false>;
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fsm100::SMEM_BYTES);
-        kern<<<std::min(p.n_work, sms), fsm100::NTHREADS, fsm100::SMEM_BYTES, st>>>(p, maps);
+        kern<<<static_cast<int>(std::min<int64_t>(blocks * n_heads, sms)), fsm100::NTHREADS, fsm100::SMEM_BYTES, st>>>(p, maps);
         return check_launch(what);
     }
-    p.n_work = 0;
+    p.blocks = 0;
     dim3 grid((max_seqlen + fsm100::CTA_M - 1) / fsm100::CTA_M, n_heads, batch);
     auto kern = f16 ? fsm100::fwd_sm100_kernel<true> : fsm100::fwd_sm100_kernel<false>;
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fsm100::SMEM_BYTES);

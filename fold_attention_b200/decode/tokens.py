@@ -210,7 +210,8 @@ def chunk_attention(q, cu_seqlens, lens, cap_tiles, seq_lens, page_table, page_s
     else:
         cap_tiles = cap_tiles[1]
     out = torch.empty((total, H, D), device=dev, dtype=dt)
-    work = torch.empty(4 + (4 * B + 2 * cap_tiles if wide else 0), device=dev, dtype=torch.int32)
+    n_plan = -(-(5 * B + 1) // 2) * 2      # (the tile map sits on 8 bytes)
+    work = torch.empty(4 + (n_plan + 2 * cap_tiles if wide else 0), device=dev, dtype=torch.int32)
     status = work[:1]
     pool = (page_table.data_ptr(), page_table.shape[1], int(page_size))
     planes = (ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb), ek.data_ptr(), float(v_scale))
@@ -233,7 +234,7 @@ def chunk_attention(q, cu_seqlens, lens, cap_tiles, seq_lens, page_table, page_s
             plan = base + 16
             _lib.call(
                 "fold_chunk_gather", cu_seqlens.data_ptr(), seq_lens.data_ptr(), B, *pool, n_kv_heads, D, win, sinks, *planes, f16,
-                SHORT_ROWS if short else 0, G, cap_tiles, plan, plan + 16 * B, kw.data_ptr(), vw, base, st,
+                SHORT_ROWS if short else 0, G, cap_tiles, plan, plan + 4 * n_plan, kw.data_ptr(), vw, base, st,
             )
             strides = (ctypes.c_int64 * 12)(0, q.stride(0), q.stride(1), 0, D, rows * D, 0, D, rows * D, 0, out.stride(0), out.stride(1))
             args = (q.data_ptr(), kw.data_ptr(), vw, out.data_ptr(), None, ctypes.addressof(strides), cu_seqlens.data_ptr(), B, H,

@@ -72,7 +72,7 @@ int fold_chunk_sums(const void* v, int is_f16, int64_t v_token_stride, int64_t v
 /* The keys and values that the last cu_seqlens[b + 1] - cu_seqlens[b] tokens of each request can see,
  * as 16-bit rows for fold_fwd_window: whole tiles of 128 keys, requests one after another, zeros past
  * a request's end. kw, vw [n_kv_heads][cap_tiles * 128][head_dim] in bf16, or fp16 (is_f16,
- * saturating); plan int32[4 * batch]; tiles int32[2 * cap_tiles]. Requests whose new tokens times
+ * saturating); plan int32[5 * batch + 1]; tiles int32[2 * cap_tiles], on 8 bytes. Requests whose new tokens times
  * `group` (query heads a KV head) are no more than rows_over are left out, by the attention too. Requests
  * that do not fit cap_tiles see no key and raise *status (FOLD_ERR_ARGUMENT), which a call with
  * rows_over 0 clears first. */
