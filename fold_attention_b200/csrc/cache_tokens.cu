@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(TB_THREADS) build_tables_kernel(const int* __r
 template <int D, bool V8, bool F16>
 __global__ void __launch_bounds__(NT) write_tokens_kernel(const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int64_t k_st,
                                                           int64_t k_sh, int64_t v_st, int64_t v_sh, const int* __restrict__ slots,
-                                                          int64_t n_rows, int hkv, int page_size, int8_t* ka, int8_t* kb, void* va,
+                                                          int64_t n_rows, int hkv, int page_size, int64_t pool_rows, int8_t* ka, int8_t* kb, void* va,
                                                           void* vb, __nv_bfloat16* ek, float ievs) {
     constexpr int TPR = D / 16, RPB = NT / TPR;
     const int lane = threadIdx.x % TPR;
@@ -90,7 +90,8 @@ __global__ void __launch_bounds__(NT) write_tokens_kernel(const uint16_t* __rest
     const int64_t t = rr / hkv;
     const int h = static_cast<int>(rr % hkv);
     const int slot = slots[t];
-    const bool ok = r < n_rows && slot >= 0;
+    // a slot outside the pool is no place either (a page's rows end (hkv * page_size) after they begin)
+    const bool ok = r < n_rows && slot >= 0 && (static_cast<int64_t>(slot / page_size) + 1) * hkv * page_size <= pool_rows;
     float xk[16], xv[16];
     uint4 wk[2], wv[2];
     load16<F16>(k + t * k_st + h * k_sh + lane * 16, xk, wk);
@@ -216,17 +217,18 @@ __device__ __forceinline__ void store_f32(float* row, int lane, bool ok, const f
 }
 
 template <int D, bool V8, int OUT>
-__global__ void __launch_bounds__(NT) read_tokens_kernel(const int* __restrict__ slots, int64_t n_rows, int hkv, int page_size, const Planes p,
+__global__ void __launch_bounds__(NT) read_tokens_kernel(const int* __restrict__ slots, int64_t n_rows, int hkv, int page_size, int64_t pool_rows, const Planes p,
                                                          void* k, void* v) {
     constexpr int TPR = D / 16, RPB = NT / TPR;
     const int lane = threadIdx.x % TPR;
     const int64_t r = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / TPR;
     const int64_t rr = r < n_rows ? r : 0;
     const int slot = slots[rr / hkv];
+    const bool ok = slot >= 0 && (static_cast<int64_t>(slot / page_size) + 1) * hkv * page_size <= pool_rows;
     int off;
-    const int64_t prow = slot_row(slot < 0 ? 0 : slot, page_size, hkv, static_cast<int>(rr % hkv), off);
+    const int64_t prow = slot_row(ok ? slot : 0, page_size, hkv, static_cast<int>(rr % hkv), off);
     float xk[16], xv[16];
-    load_row<D, V8>(p, prow, off, lane, slot >= 0, xk, xv);
+    load_row<D, V8>(p, prow, off, lane, ok, xk, xv);
     if (OUT == OUT_F32) {
         // 64 bytes a lane: a row's lanes take turns so that each store is a stretch of memory, not 16 bytes of
         // every 64 (TPR lanes: unit t of lane l goes out as unit l + TPR t of the row)
@@ -404,8 +406,8 @@ extern "C" int fold_build_tables(const int32_t* cu_seqlens, const int32_t* seq_l
 }
 
 extern "C" int fold_write_tokens(const void* k, const void* v, int is_f16, int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
-                                 int64_t v_head_stride, const int32_t* slots, int64_t total, int n_kv_heads, int head_dim, int page_size, int8_t* ka,
-                                 int8_t* kb, void* va, void* vb, void* ek, float v_scale, void* stream) {
+                                 int64_t v_head_stride, const int32_t* slots, int64_t total, int n_kv_heads, int head_dim, int page_size, int64_t pool_rows,
+                                 int8_t* ka, int8_t* kb, void* va, void* vb, void* ek, float v_scale, void* stream) {
     FOLD_CHECK_ARG(head_dim == 64 || head_dim == 128, "head_dim %d: the cache writers take 64 or 128", head_dim);
     FOLD_CHECK_ARG(total >= 0 && n_kv_heads > 0 && page_size > 0, "fold_write_tokens: %lld tokens, %d heads, pages of %d", static_cast<long long>(total), n_kv_heads, page_size);
     if (total == 0) return FOLD_OK;
@@ -421,7 +423,7 @@ extern "C" int fold_write_tokens(const void* k, const void* v, int is_f16, int64
     const float ievs = 1.0f / v_scale;
 #define FOLD_WT(DD, VV, FF)                                                                                                       \
     write_tokens_kernel<DD, VV, FF><<<static_cast<unsigned>(grid), NT, 0, st>>>(kp, vp, k_token_stride, k_head_stride, v_token_stride, \
-        v_head_stride, slots, rows, n_kv_heads, page_size, ka, kb, va, vb, static_cast<__nv_bfloat16*>(ek), ievs)
+        v_head_stride, slots, rows, n_kv_heads, page_size, pool_rows, ka, kb, va, vb, static_cast<__nv_bfloat16*>(ek), ievs)
     if (head_dim == 64) {
         if (vb) { if (is_f16) FOLD_WT(64, true, true); else FOLD_WT(64, true, false); }
         else    { if (is_f16) FOLD_WT(64, false, true); else FOLD_WT(64, false, false); }
@@ -433,7 +435,7 @@ extern "C" int fold_write_tokens(const void* k, const void* v, int is_f16, int64
     return check_launch("fold_write_tokens");
 }
 
-extern "C" int fold_read_tokens(const int32_t* slots, int64_t total, int n_kv_heads, int head_dim, int page_size, const int8_t* ka, const int8_t* kb,
+extern "C" int fold_read_tokens(const int32_t* slots, int64_t total, int n_kv_heads, int head_dim, int page_size, int64_t pool_rows, const int8_t* ka, const int8_t* kb,
                                 const void* va, const void* vb, const void* ek, float v_scale, void* k, void* v, int out_dtype, void* stream) {
     FOLD_CHECK_ARG(head_dim == 64 || head_dim == 128, "head_dim %d: the cache holds 64 or 128", head_dim);
     FOLD_CHECK_ARG(total >= 0 && n_kv_heads > 0 && page_size > 0, "fold_read_tokens: %lld tokens, %d heads, pages of %d", static_cast<long long>(total), n_kv_heads, page_size);
@@ -446,7 +448,7 @@ extern "C" int fold_read_tokens(const int32_t* slots, int64_t total, int n_kv_he
     FOLD_CHECK_ARG(grid < (1ll << 31), "fold_read_tokens: %lld rows in one call", static_cast<long long>(rows));
     const Planes p = {ka, kb, static_cast<const uint16_t*>(ek), static_cast<const uint8_t*>(va), static_cast<const uint8_t*>(vb), v_scale};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define FOLD_RT(DD, VV, OO) read_tokens_kernel<DD, VV, OO><<<static_cast<unsigned>(grid), NT, 0, st>>>(slots, rows, n_kv_heads, page_size, p, k, v)
+#define FOLD_RT(DD, VV, OO) read_tokens_kernel<DD, VV, OO><<<static_cast<unsigned>(grid), NT, 0, st>>>(slots, rows, n_kv_heads, page_size, pool_rows, p, k, v)
 #define FOLD_RT3(DD, VV)                                    \
     do {                                                    \
         if (out_dtype == OUT_F32) FOLD_RT(DD, VV, OUT_F32); \

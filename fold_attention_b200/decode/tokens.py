@@ -24,8 +24,8 @@ from .. import _lib
 
 P, I, F, L = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_int64
 _lib.register("fold_build_tables", [P, P, I, P, I, I, I, P, I, P, P, P, P, P])
-_lib.register("fold_write_tokens", [P, P, I, L, L, L, L, P, L, I, I, I, P, P, P, P, P, F, P])
-_lib.register("fold_read_tokens", [P, L, I, I, I, P, P, P, P, P, F, P, P, I, P])
+_lib.register("fold_write_tokens", [P, P, I, L, L, L, L, P, L, I, I, I, L, P, P, P, P, P, F, P])
+_lib.register("fold_read_tokens", [P, L, I, I, I, L, P, P, P, P, P, F, P, P, I, P])
 _lib.register("fold_chunk_sums", [P, I, L, L, I, I, I, P, I, P, P, F, P, P, P])
 _lib.register("fold_chunk_gather", [P, P, I, P, I, I, I, I, I, I, P, P, P, P, P, F, I, I, I, I, P, P, P, P, P, P])
 _lib.register("fold_chunk_sm100", [P, L, L, P, L, L, I, P, P, I, I, I, I, I, P, I, I, L, P, P, P, P, P, F, I, I, I, I, P, L, P, P])
@@ -122,8 +122,8 @@ def write_tokens(k, v, slots, page_size, ka, kb, va, vb, ek, *, v_scale=1.0):
     """Quantise `k`, `v` `(total, H_KV, D)` (bf16 or fp16) into the pool at
     `slots`: the planes a prompt's write or a step's append puts there. `vb`
     None is a bf16 V; `v_scale` is an 8-bit V's power of two. The slots are
-    distinct, each within the pool (or negative: skipped); two tokens of one
-    call in one slot would leave a mixture."""
+    distinct (two tokens of one call in one slot would leave a mixture); a
+    token whose slot is negative or beyond the pool is skipped."""
     if k.ndim != 3 or v.shape != k.shape or k.dtype not in _HALF or v.dtype != k.dtype:
         raise ValueError(f"k and v are (total, H_KV, D) of one 16-bit type (got {k.dtype} {tuple(k.shape)}, {v.dtype} {tuple(v.shape)})")
     n, HKV, D = k.shape
@@ -140,15 +140,16 @@ def write_tokens(k, v, slots, page_size, ka, kb, va, vb, ek, *, v_scale=1.0):
     with _lib.on(dev):
         _lib.call(
             "fold_write_tokens", k.data_ptr(), v.data_ptr(), int(k.dtype is torch.float16), k0, k1, v0, v1,
-            slots.data_ptr(), n, HKV, D, int(page_size), ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb), ek.data_ptr(),
-            float(v_scale), _lib.stream(dev),
+            slots.data_ptr(), n, HKV, D, int(page_size), ka.shape[0], ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb),
+            ek.data_ptr(), float(v_scale), _lib.stream(dev),
         )
 
 
 def read_tokens(slots, page_size, n_kv_heads, ka, kb, va, vb, ek, *, v_scale=1.0, dtype=torch.bfloat16):
     """The tokens at `slots` as the values their codes stand for: `(k, v)`, each
     `(total, H_KV, D)` in `dtype` (float32, bfloat16 or float16, which
-    saturates), keys in their own basis. Slots may repeat; zeros at -1."""
+    saturates), keys in their own basis. Slots may repeat; zeros at a slot that
+    is negative or beyond the pool."""
     if dtype not in _OUT:
         raise ValueError(f"dtype is float32, bfloat16 or float16 (got {dtype})")
     dev, D = ka.device, ka.shape[-1]
@@ -161,7 +162,7 @@ def read_tokens(slots, page_size, n_kv_heads, ka, kb, va, vb, ek, *, v_scale=1.0
     v = torch.empty_like(k)
     with _lib.on(dev):
         _lib.call(
-            "fold_read_tokens", slots.data_ptr(), n, HKV, D, int(page_size), ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb),
+            "fold_read_tokens", slots.data_ptr(), n, HKV, D, int(page_size), ka.shape[0], ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb),
             ek.data_ptr(), float(v_scale), k.data_ptr(), v.data_ptr(), _OUT[dtype], _lib.stream(dev),
         )
     return k, v

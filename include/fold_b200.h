@@ -37,7 +37,8 @@ int fold_abi_version(void);
 /* ---- the paged cache a piece at a time --------------------------------------
  * No counterpart in the reference, which appends one token a request and whose tables are the
  * host's. A token's slot is page * page_size + offset, the same for every KV head and every layer
- * that shares the table; -1 stands for no place: writers skip it, readers return zeros. */
+ * that shares the table; -1 stands for no place: writers skip it, readers return zeros, and so they
+ * do for a slot whose page lies beyond the planes' pool_rows rows. */
 
 /* Block tables and the new tokens' slots from request lengths. Request b holds seq_lens[b] tokens
  * and brings cu_seqlens[b + 1] - cu_seqlens[b] more. With free_pages (n_free page numbers, of which
@@ -54,13 +55,13 @@ int fold_build_tables(const int32_t* cu_seqlens, const int32_t* seq_lens, int ba
  * would write. k, v (total, n_kv_heads, head_dim) 16-bit with element strides; vb NULL for a bf16 V. */
 int fold_write_tokens(const void* k, const void* v, int is_f16, int64_t k_token_stride, int64_t k_head_stride,
                       int64_t v_token_stride, int64_t v_head_stride, const int32_t* slots, int64_t total,
-                      int n_kv_heads, int head_dim, int page_size, int8_t* ka, int8_t* kb, void* va, void* vb,
-                      void* ek, float v_scale, void* stream);
+                      int n_kv_heads, int head_dim, int page_size, int64_t pool_rows, int8_t* ka, int8_t* kb,
+                      void* va, void* vb, void* ek, float v_scale, void* stream);
 
 /* The tokens at `slots` as the values their codes stand for, keys in their own basis: k, v
  * (total, n_kv_heads, head_dim) fp32 (out_dtype 0), bf16 (1) or fp16 (2, saturating). */
 int fold_read_tokens(const int32_t* slots, int64_t total, int n_kv_heads, int head_dim, int page_size,
-                     const int8_t* ka, const int8_t* kb, const void* va, const void* vb, const void* ek,
+                     int64_t pool_rows, const int8_t* ka, const int8_t* kb, const void* va, const void* vb, const void* ek,
                      float v_scale, void* k, void* v, int out_dtype, void* stream);
 
 /* A chunk's share of the running V sums and means (fp32 (batch * n_kv_heads, head_dim)), and the

@@ -157,3 +157,18 @@ def test_on_another_stream_and_from_a_graph():
     torch.cuda.synchronize()
     want = plain_tables([0, 3, 20], [16, 1], [[0, 0], [0, 0]], 16, 20, [6, 4, 2, 0], 0)
     assert (table.tolist(), slots.tolist(), after.tolist(), used.tolist()) == (want[0], want[1], want[2], [want[3]])
+
+
+def test_a_slot_beyond_the_pool_is_no_place():
+    from fold_attention_b200 import decode
+
+    HKV, D, page, pages = 3, 64, 16, 2
+    rows = pages * page * HKV
+    ka, kb = (torch.zeros(rows, D, device="cuda", dtype=torch.int8) for _ in range(2))
+    va, ek = torch.zeros(rows, D, device="cuda", dtype=torch.bfloat16), torch.zeros(rows, device="cuda", dtype=torch.bfloat16)
+    k = torch.randn(4, HKV, D, device="cuda").bfloat16()
+    slots = dev32([31, 32, 2 ** 31 - 1, -2 ** 31])        # the pool's last one, then three that it does not have
+    decode.write_tokens(k, k, slots, page, ka, kb, va, None, ek)
+    kr, vr = decode.read_tokens(slots, page, HKV, ka, kb, va, None, ek)
+    assert torch.equal(vr[0], k[0]) and not vr[1:].any() and not kr[1:].any()
+    assert int((ek != 0).sum()) == HKV
