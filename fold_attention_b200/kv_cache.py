@@ -438,8 +438,14 @@ class FoldKVCache:
     def sync_lens(self):
         """Read the lengths back from the device. A captured step moves them there
         on every replay; the host's copy, which the next eager call plans by, does
-        not follow by itself."""
-        self.lens = self.seq_lens.tolist()
+        not follow by itself. Raises if the replays ran past `max_len` or the
+        shared pool: the tokens beyond either were dropped."""
+        lens = self.seq_lens.tolist()
+        if max(lens) > self.max_len:
+            raise ValueError(f"a request was moved to {max(lens)} tokens, max_len={self.max_len}")
+        if self.taken is not None and int(self.taken) > self.n_pages:
+            raise ValueError(f"the requests wanted {int(self.taken)} pages, the pool has {self.n_pages}")
+        self.lens = lens
 
     def _attend_last(self, q):
         """A windowed layer's step: each request's newest token."""

@@ -303,3 +303,40 @@ def test_strided_queries_and_calls_without_lens():
     close(st.c.attend_chunk(q[[149, 168, 169]], cumulative([1, 2])), st.want(q[[149, 168, 169]], [1, 2]), st.dt)
     assert st.c.attend_chunk(q[:0], cumulative([0, 0])).shape == (0, 4, 128)
     assert st.c.extend(q[:0], k[:0], v[:0], cumulative([0, 0])).shape == (0, 4, 128)
+
+
+@pytest.mark.parametrize("v8", [False, True])
+def test_hundreds_of_requests(v8):
+    """More requests than the short chunks' kernel has threads, most of them without a new token."""
+    B = 450
+    st = Story(B, 4, 1, 64, 64, v8=v8, page_size=16, seed=5)
+    st.extend([b % 5 for b in range(B)])
+    st.extend([1 if b % 3 == 0 else 0 for b in range(B)])
+    st.extend([40 if b in (7, 440) else b % 2 for b in range(B)])
+
+
+def test_replays_past_the_end_are_told():
+    st = Story(2, 4, 2, 64, 40, page_size=16, pages=6, seed=5)
+    st.extend([30, 1])
+    q, k, v = (make([1, 1], h, 64, st.dt, st.g) for h in (4, 2, 2))
+    cu, graph, side = cumulative([1, 1]), torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            st.c.extend(q, k, v, cu, [1, 1])
+    for _ in range(9):
+        graph.replay()
+    st.c.sync_lens()
+    assert st.c.lens == [39, 10]
+    for _ in range(9):
+        graph.replay()
+    with pytest.raises(ValueError, match="max_len=40"):
+        st.c.sync_lens()
+
+
+def test_small_pages_and_one_key():
+    """A request of one key, alone: one visible key, whose value is the output to its rounding."""
+    st = Story(1, 8, 8, 128, 16, page_size=16, seed=1)
+    q, k, v = st.tokens([1])
+    got = st.c.extend(q, k, v, cumulative([1]), [1])
+    assert torch.equal(got, v)
