@@ -53,6 +53,10 @@ struct BwdParams {
     int sink_stride;    // and how many are laid out
 };
 
+// Whether each query of a sequence sees one key: P = 1 whatever its score, so dS = 0. dP - Delta would
+// leave the rounding of two sums there, and gradients that are zero throughout would come back as noise.
+__device__ __forceinline__ bool lone_keys(const BwdParams& p, int len) { return len == 1 || (p.window == 1 && p.sinks == 0); }
+
 // The longest a window's key block is walked before an item is cut, in the main loop's query blocks:
 // about what a block past the sinks walks, so the launch's longest items stay its ordinary ones. It
 // depends on the window alone: a sequence's bits do not depend on its neighbours.

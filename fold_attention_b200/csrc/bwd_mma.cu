@@ -49,6 +49,7 @@ __global__ void __launch_bounds__(NTHREADS, 2) bwd_main_mma_kernel(const BwdPara
     const int n0 = nb * BN;
     if (n0 >= sq.len) return;
     const bool sink = WIN && n0 < p.sinks;
+    const bool lone = WIN && lone_keys(p, sq.len);
     if (sink && rec * p.sink_record >= (sq.len + BM - 1) / BM) return;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int gid = lane >> 2, tq = lane & 3;
@@ -157,6 +158,7 @@ __global__ void __launch_bounds__(NTHREADS, 2) bwd_main_mma_kernel(const BwdPara
                     }
                     pv[e] = x;
                     ds[e] = x * (dp[nt][e] - de);
+                    if (WIN && lone) ds[e] = 0.f;
                 }
 #pragma unroll
                 for (int hlf = 0; hlf < 2; ++hlf) {

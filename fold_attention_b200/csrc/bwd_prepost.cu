@@ -318,6 +318,16 @@ __global__ void __launch_bounds__(256) bwd_postprocess_dq_kernel(const BwdParams
 __global__ void __launch_bounds__(256) bwd_finalize_l_kernel(const BwdParams p) {
     const int h = blockIdx.y, b = blockIdx.z;
     const SeqInfo sq = seq_info(p, b);
+    // rows behind the last sequence have no gradient (written here: the other kernels' loops are the long ones)
+    if (p.window > 0 && p.cu && b == p.B - 1)
+        for (int64_t t = max(sq.start + sq.len, 0) + static_cast<int64_t>(blockIdx.x * 8 + (threadIdx.x >> 5)); t < p.total; t += 8 * gridDim.x)
+            for (int c = threadIdx.x & 31; c < p.D / 2; c += 32) {
+                reinterpret_cast<uint32_t*>(row_ptr<uint16_t>(p.dq, 0, t, h))[c] = 0u;
+                if (h % p.G == 0) {
+                    reinterpret_cast<uint32_t*>(row_ptr<uint16_t>(p.dk, 0, t, h / p.G))[c] = 0u;
+                    reinterpret_cast<uint32_t*>(row_ptr<uint16_t>(p.dv, 0, t, h / p.G))[c] = 0u;
+                }
+            }
     const int len_r = (sq.len + ROW_PAD - 1) / ROW_PAD * ROW_PAD;
     const int i = blockIdx.x * 256 + threadIdx.x;
     if (i >= len_r) return;

@@ -668,6 +668,10 @@ bwd_main_sm100_kernel(const BwdParams p, const __grid_constant__ Maps maps) {
                 tc_fence_before();
                 mbar_arrive(sh.bar(B_P));
                 CNT_T(t_c);
+                if (WIN && lone_keys(p, it.sq.len)) {   // dS = 0 (from here on x serves dS alone)
+#pragma unroll
+                    for (int q = 0; q < QPW; ++q) x[q] = 0.f;
+                }
                 // ---- dS~^T = P~^T (dP^T - Delta) to shared, 16 queries at a time ----
                 // dP^T done means dO, and Delta with it, landed (the MMA thread waited for them)
                 mbar_wait<SLEEP_WORKER>(sh.bar(B_DP), t & 1, abort_flag, p.status);

@@ -21,6 +21,7 @@ struct FwdParams {
     // keys between the sinks' tiles and the window's that no query of the chunk sees
     int window, sinks;
     const int4* plan;
+    int total;       // packed rows
 };
 
 template <int D, bool F16, bool CAUSAL, bool EXT>
@@ -37,6 +38,11 @@ __global__ void __launch_bounds__(128) fwd_mma_kernel(const FwdParams p) {
         len = p.cu[b + 1] - start;
     }
     const int m0 = mb * 64;
+    if (EXT && p.cu && !p.plan && b == p.B - 1 && mb == 0)   // rows behind the last packed sequence: zeros
+        for (int64_t i = max(start + len, 0) + static_cast<int64_t>(threadIdx.x >> 5); i < p.total; i += 4) {
+            for (int c = threadIdx.x & 31; c < D / 2; c += 32) reinterpret_cast<uint32_t*>(row_ptr<uint16_t>(p.o, 0, i, h))[c] = 0u;
+            if ((threadIdx.x & 31) == 0 && p.lse) p.lse[h * p.lse_sh + i] = -INFINITY;
+        }
     if (m0 >= len) return;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tq = lane & 3;
     const int hkv = h / p.G;
@@ -236,6 +242,7 @@ static int fwd_run(const char* what, const void* q, const void* k, const void* v
     p.B = batch; p.H = n_heads; p.HKV = n_kv_heads; p.G = n_heads / n_kv_heads;
     p.S = max_seqlen; p.D = head_dim; p.causal = causal; p.f16 = is_f16; p.scale = softmax_scale;
     p.window = window; p.sinks = sinks; p.plan = reinterpret_cast<const int4*>(plan);
+    p.total = total;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (head_dim) {
         case 64: return fwd_launch_d<64>(p, st);

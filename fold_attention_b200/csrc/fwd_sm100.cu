@@ -185,6 +185,7 @@ struct Params {
     // tiles and the window's that no query of the chunk sees
     int window, sinks;
     const int4* plan;
+    int total;       // packed rows
     int blocks;      // blocks of 256 rows (dense), or slots of 256 packed rows and one per request; with `plan` its own count
 };
 struct Maps {
@@ -665,6 +666,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_window_sm100_kernel(const Par
                 ++items;
             }
         }
+    } else if (warp == 2) {
+        // rows behind the last packed sequence: zeros
+        if (p.cu && !p.plan)
+            for (int64_t i = max(__ldg(p.cu + p.B), 0) + static_cast<int64_t>(blockIdx.x); i < p.total; i += gridDim.x)
+                for (int h = 0; h < p.H; ++h) {
+                    if (lane < 16) *reinterpret_cast<uint4*>(row_ptr<uint16_t>(p.o, 0, i, h) + 8 * lane) = make_uint4(0u, 0u, 0u, 0u);
+                    if (lane == 0 && p.lse) p.lse[h * p.lse_sh + i] = -INFINITY;
+                }
     } else if (warp >= 4) {
         // ================= softmax: two groups, one per query tile; thread = query row = TMEM lane =================
         const int x = (warp - 4) >> 2;
@@ -912,6 +921,7 @@ int run_sm100(const char* what, const void* q, const void* k, const void* v, voi
                                           : static_cast<int64_t>((max_seqlen + fsm100::CTA_M - 1) / fsm100::CTA_M) * batch;
         FOLD_CHECK_ARG(2 * blocks * n_heads < (1ll << 31), "%s: %lld blocks of %d heads", what, static_cast<long long>(blocks), n_heads);
         p.blocks = static_cast<int>(blocks);
+        p.total = total;
         int dev = 0, sms = 1;
         cudaGetDevice(&dev);
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -920,7 +930,7 @@ int run_sm100(const char* what, const void* q, const void* k, const void* v, voi
         kern<<<static_cast<int>(std::min<int64_t>(blocks * n_heads, sms)), fsm100::NTHREADS, fsm100::SMEM_BYTES, st>>>(p, maps);
         return check_launch(what);
     }
-    p.blocks = 0;
+    p.blocks = p.total = 0;
     dim3 grid((max_seqlen + fsm100::CTA_M - 1) / fsm100::CTA_M, n_heads, batch);
     auto kern = f16 ? fsm100::fwd_sm100_kernel<true> : fsm100::fwd_sm100_kernel<false>;
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fsm100::SMEM_BYTES);

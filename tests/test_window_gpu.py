@@ -246,3 +246,36 @@ def test_on_another_stream_and_captured_beside_an_eager_graph():
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip((out, *captured), want))
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(eager, x, do), want[1:]))
+
+
+@pytest.mark.parametrize("D", [128, 64])
+def test_rows_behind_the_last_sequence_are_zeros(D):
+    import fold_attention_b200 as fa
+
+    lens, window, sinks, pad = [100, 0, 70], 20, 2, 37
+    q, k, v, do = inputs(sum(lens) + pad, 4, 2, D, torch.bfloat16, seed=11)
+    cu = torch.tensor([0, 100, 100, 170], device="cuda", dtype=torch.int32)
+    x = [t.clone().requires_grad_() for t in (q, k, v)]
+    torch.full((4 << 20,), float("nan"), device="cuda")        # what the allocator hands out next is not zero
+    out = fa.fold_attn_varlen_func(*x, cu, max_seqlen_q=100, causal=True, window=window, sinks=sinks)
+    got = (out.detach(), *torch.autograd.grad(out, x, do))
+    assert all(not t[170:].any() for t in got)
+    for sl in (slice(0, 100), slice(100, 170)):
+        check([t[sl] for t in got], reference(q[sl], k[sl], v[sl], do[sl], window, sinks), torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [128, 96])
+def test_one_visible_key_has_no_score_gradient(D, dtype):
+    """P is 1 whatever the score: dq and dk are zero, not the rounding of two sums that cancel."""
+    import fold_attention_b200 as fa
+
+    q, k, v, do = (t[None] for t in inputs(200, 4, 2, D, dtype, seed=3))
+    x = [t.clone().requires_grad_() for t in (q, k, v)]
+    dq, dk, dv = torch.autograd.grad(fa.fold_attn_func(*x, causal=True, window=1), x, do)
+    assert not dq.any() and not dk.any() and dv.any()
+    x = [t.clone().requires_grad_() for t in (q[0, :3], k[0, :3], v[0, :3])]
+    cu = torch.arange(4, device="cuda", dtype=torch.int32)                     # three sequences of one token
+    out = fa.fold_attn_varlen_func(*x, cu, max_seqlen_q=1, causal=True, window=50, sinks=2)
+    dq, dk, dv = torch.autograd.grad(out, x, do[0, :3])
+    assert not dq.any() and not dk.any() and dv.any()
