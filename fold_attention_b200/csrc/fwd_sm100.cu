@@ -705,7 +705,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_window_sm100_kernel(const Par
                 tc_fence_after();
                 // pass 1: the row's maximum over the tile. The masked and the unmasked form are two pieces of code: left to
                 // itself the compiler evaluates this mask for every tile, at 1.6 times the kernel's time.
-                float mxv = -INFINITY;
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // apart: one chain of 64 would be latency
                 auto row_max = [&](auto masked) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
@@ -719,11 +719,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_window_sm100_kernel(const Par
                                 if (!(vis & (1u << e))) sv[e] = 0xff800000u;   // -inf
                         }
 #pragma unroll
-                        for (int e = 0; e < 32; e += 2) mxv = max3f(mxv, __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+                        for (int e = 0; e < 32; e += 2)
+                            mx4[(e >> 1) & 3] = max3f(mx4[(e >> 1) & 3], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
                     }
                 };
                 if (need_mask) row_max(std::true_type{});
                 else row_max(std::false_type{});
+                const float mxv = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
                 // The reference point only moves when the row's maximum rose by more than 2^LAZY (fwd_sm100_kernel)
                 const float m_cand = fmaxf(m_run, mxv * c2);
                 const float m_new = m_cand > m_run + LAZY ? m_cand : m_run;
