@@ -24,13 +24,22 @@ struct FwdParams {
     int total;       // packed rows
 };
 
-template <int D, bool F16, bool CAUSAL, bool EXT>
-__global__ void __launch_bounds__(128) fwd_mma_kernel(const FwdParams p) {
+// KIND: the causal and full forward, a window, or a chunk. A chunk's blocks are few and their keys many, and
+// with four warps a block each scheduler has one, whose matrix instructions wait for one another: there two
+// groups of four warps take the key tiles in turn, and their sums meet at the end (9 requests of up to 300 new
+// tokens behind 1500, 6 heads: 46 -> 36 us).
+enum { KIND_PLAIN, KIND_WINDOW, KIND_CHUNK };
+
+template <int D, bool F16, bool CAUSAL, int KIND>
+__global__ void __launch_bounds__(KIND == KIND_CHUNK ? 256 : 128) fwd_mma_kernel(const FwdParams p) {
     constexpr int PITCH = D * 2 + 16, TILE = 64 * PITCH, NTO = D / 8;
+    constexpr bool EXT = KIND != KIND_PLAIN;
+    constexpr int GROUPS = KIND == KIND_CHUNK ? 2 : 1;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* sQ = smem;
-    uint8_t* sK = smem + TILE;
-    uint8_t* sV = smem + 2 * TILE;
+    const int grp = GROUPS == 2 ? threadIdx.x >> 7 : 0;
+    uint8_t* sK = smem + (1 + 2 * grp) * TILE;
+    uint8_t* sV = sK + TILE;
     const int mb = gridDim.x - 1 - blockIdx.x, h = blockIdx.y, b = blockIdx.z;
     int start = 0, len = p.S;
     if (p.cu) {
@@ -38,28 +47,26 @@ __global__ void __launch_bounds__(128) fwd_mma_kernel(const FwdParams p) {
         len = p.cu[b + 1] - start;
     }
     const int m0 = mb * 64;
-    if (EXT && p.cu && !p.plan && b == p.B - 1 && mb == 0)   // rows behind the last packed sequence: zeros
+    if (KIND == KIND_WINDOW && p.cu && b == p.B - 1 && mb == 0)   // rows behind the last packed sequence: zeros
         for (int64_t i = max(start + len, 0) + static_cast<int64_t>(threadIdx.x >> 5); i < p.total; i += 4) {
             for (int c = threadIdx.x & 31; c < D / 2; c += 32) reinterpret_cast<uint32_t*>(row_ptr<uint16_t>(p.o, 0, i, h))[c] = 0u;
             if ((threadIdx.x & 31) == 0 && p.lse) p.lse[h * p.lse_sh + i] = -INFINITY;
         }
     if (m0 >= len) return;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tq = lane & 3;
+    const int tid = threadIdx.x & 127, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tq = lane & 3;
     const int hkv = h / p.G;
     const float c2 = p.scale * kLog2e;
     int klen = len, qoff = 0, kstart = start, kshift = 0;   // keys, and the first query's position among them
-    if constexpr (EXT) {
-        if (p.plan) {
-            const int4 pl = p.plan[b];
-            if (pl.x < 0) return;   // another kernel's
-            klen = pl.x;
-            qoff = klen - len;
-            kstart = pl.y;
-            kshift = 128 * pl.z;
-        }
+    if constexpr (KIND == KIND_CHUNK) {
+        const int4 pl = p.plan[b];
+        if (pl.x < 0) return;   // another kernel's
+        klen = pl.x;
+        qoff = klen - len;
+        kstart = pl.y;
+        kshift = 128 * pl.z;
     }
 
-    load_tile_async<D, PITCH, 128>(sQ, row_ptr<const uint16_t>(p.q, b, start + m0, h), p.q.sr, 64, min(64, len - m0), tid);
+    load_tile_async<D, PITCH, 128 * GROUPS>(sQ, row_ptr<const uint16_t>(p.q, b, start + m0, h), p.q.sr, 64, min(64, len - m0), threadIdx.x);
     cp_async_commit();
 
     float o[NTO][4];
@@ -72,19 +79,26 @@ __global__ void __launch_bounds__(128) fwd_mma_kernel(const FwdParams p) {
     const int n_end = EXT ? max(0, min(klen, qoff + min(len, m0 + 64))) : CAUSAL ? min(len, m0 + 64) : len;
     // EXT: the first key tile of the block's window; between the sinks' tiles and it nothing is seen
     const int n_low = EXT ? max(0, qoff + m0 - p.window + 1) / 64 * 64 : 0;
-    for (int n0 = 0; n0 < n_end; n0 += 64) {
-        if (EXT && n0 >= p.sinks && n0 < n_low) {
-            n0 = n_low;
-            if (n0 >= n_end) break;
+    auto seen_from = [&](int n0) { return EXT && n0 >= p.sinks && n0 < n_low ? n_low : n0; };
+    int next = seen_from(0);
+    while (next < n_end) {
+        int n0 = next;
+        next = seen_from(n0 + 64);
+        if (GROUPS == 2) {
+            if (grp) n0 = next;
+            next = seen_from(next + 64);
         }
         __syncthreads();  // previous tile's reads are done
         const int kvalid = min(64, klen - n0);
         const int krow = kstart + (EXT && n0 >= (p.sinks + 127) / 128 * 128 ? n0 - kshift : n0);   // whole tiles of 128 keys are left out
-        load_tile_async<D, PITCH, 128>(sK, row_ptr<const uint16_t>(p.k, b, krow, hkv), p.k.sr, 64, kvalid, tid);
-        load_tile_async<D, PITCH, 128>(sV, row_ptr<const uint16_t>(p.v, b, krow, hkv), p.v.sr, 64, kvalid, tid);
+        if (GROUPS == 1 || n0 < n_end) {
+            load_tile_async<D, PITCH, 128>(sK, row_ptr<const uint16_t>(p.k, b, krow, hkv), p.k.sr, 64, kvalid, tid);
+            load_tile_async<D, PITCH, 128>(sV, row_ptr<const uint16_t>(p.v, b, krow, hkv), p.v.sr, 64, kvalid, tid);
+        }
         cp_async_commit();
         cp_async_wait<0>();
         __syncthreads();
+        if (GROUPS == 2 && n0 >= n_end) break;   // the second group's: the last tile is the first's
 
         float s[8][4];
 #pragma unroll
@@ -173,6 +187,37 @@ __global__ void __launch_bounds__(128) fwd_mma_kernel(const FwdParams p) {
         ls[r] += __shfl_xor_sync(0xffffffffu, ls[r], 1);
         ls[r] += __shfl_xor_sync(0xffffffffu, ls[r], 2);
     }
+    if constexpr (GROUPS == 2) {
+        float* part = reinterpret_cast<float*>(smem + TILE) + tid;   // over the key tiles: [4 NTO + 4][128]
+        __syncthreads();
+        if (grp) {
+#pragma unroll
+            for (int i = 0; i < NTO; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) part[(4 * i + e) * 128] = o[i][e];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                part[(4 * NTO + r) * 128] = mx[r];
+                part[(4 * NTO + 2 + r) * 128] = ls[r];
+            }
+        }
+        __syncthreads();
+        if (grp) return;
+        float f[2], g[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const float m2 = part[(4 * NTO + r) * 128], l2 = part[(4 * NTO + 2 + r) * 128], mm = fmaxf(mx[r], m2);
+            const float ms = mm == -INFINITY ? 0.f : mm;
+            f[r] = ex2_approx(mx[r] - ms);
+            g[r] = ex2_approx(m2 - ms);
+            ls[r] = ls[r] * f[r] + l2 * g[r];
+            mx[r] = mm;
+        }
+#pragma unroll
+        for (int i = 0; i < NTO; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] = o[i][e] * f[e >> 1] + part[(4 * i + e) * 128] * g[e >> 1];
+    }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         const int qi = m0 + 16 * warp + gid + 8 * r;
@@ -188,28 +233,34 @@ __global__ void __launch_bounds__(128) fwd_mma_kernel(const FwdParams p) {
     }
 }
 
-template <int D, bool F16, bool CAUSAL, bool EXT>
+template <int D, bool F16, bool CAUSAL, int KIND>
 static int fwd_launch_one(const FwdParams& p, cudaStream_t st) {
-    constexpr int BYTES = 3 * 64 * (D * 2 + 16);
-    auto kern = fwd_mma_kernel<D, F16, CAUSAL, EXT>;
+    constexpr int GROUPS = KIND == KIND_CHUNK ? 2 : 1;
+    constexpr int BYTES = (1 + 2 * GROUPS) * 64 * (D * 2 + 16);
+    auto kern = fwd_mma_kernel<D, F16, CAUSAL, KIND>;
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES);
     dim3 grid((p.S + 63) / 64, p.H, p.B);
-    kern<<<grid, 128, BYTES, st>>>(p);
+    kern<<<grid, 128 * GROUPS, BYTES, st>>>(p);
     return check_launch("fwd_mma");
 }
 
 template <int D>
 static int fwd_launch_d(const FwdParams& p, cudaStream_t st) {
-    if (p.window > 0) return p.f16 ? fwd_launch_one<D, true, true, true>(p, st) : fwd_launch_one<D, false, true, true>(p, st);
-    if (p.f16) return p.causal ? fwd_launch_one<D, true, true, false>(p, st) : fwd_launch_one<D, true, false, false>(p, st);
-    return p.causal ? fwd_launch_one<D, false, true, false>(p, st) : fwd_launch_one<D, false, false, false>(p, st);
+    if (p.plan) {
+        if constexpr (D == 64) return p.f16 ? fwd_launch_one<D, true, true, KIND_CHUNK>(p, st) : fwd_launch_one<D, false, true, KIND_CHUNK>(p, st);
+        set_error("head_dim %d: a plan comes with 64", D);
+        return FOLD_ERR_UNSUPPORTED;
+    }
+    if (p.window > 0) return p.f16 ? fwd_launch_one<D, true, true, KIND_WINDOW>(p, st) : fwd_launch_one<D, false, true, KIND_WINDOW>(p, st);
+    if (p.f16) return p.causal ? fwd_launch_one<D, true, true, KIND_PLAIN>(p, st) : fwd_launch_one<D, true, false, KIND_PLAIN>(p, st);
+    return p.causal ? fwd_launch_one<D, false, true, KIND_PLAIN>(p, st) : fwd_launch_one<D, false, false, KIND_PLAIN>(p, st);
 }
 
 }  // namespace fold
 
 using namespace fold;
 
-// The causal and full forward (window 0, plan null), or the EXT build.
+// The causal and full forward (window 0, plan null), a window's or a chunk's.
 static int fwd_run(const char* what, const void* q, const void* k, const void* v, void* o, float* lse,
                    const int64_t* strides, const int32_t* cu_seqlens, int batch, int n_heads, int n_kv_heads,
                    int max_seqlen, int total, int head_dim, int causal, int is_f16, float softmax_scale, int window,

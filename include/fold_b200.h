@@ -458,7 +458,8 @@ int fold_fwd_run_sm100(const void* q, const void* k, const void* v, void* o, flo
  * Arguments as fold_fwd_run / fold_fwd_run_sm100. With `plan` (fold_chunk_gather's) the keys and
  * values are the rows it laid out, (key_rows, head) tensors whose batch strides are not used, the
  * queries are each request's last positions (cu_seqlens, which must be given, cuts q and o alone)
- * and lse may be NULL. A row that sees no key gets zeros and an lse of -infinity. A window that no
+ * and lse may be NULL (head_dim 64 on the warp-level kernel, the caches' own, 128 on the other). A row that
+ * sees no key gets zeros and an lse of -infinity, and so do the rows behind the last sequence. A window that no
  * sequence fills is plain causal attention. No counterpart in the reference. */
 int fold_fwd_window(const void* q, const void* k, const void* v, void* o, float* lse,
                     const int64_t* strides /* host */, const int32_t* cu_seqlens, int batch,
