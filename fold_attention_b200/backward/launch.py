@@ -34,14 +34,14 @@ _lib.register(
 )
 _lib.register(
     "fold_bwd_window",
-    [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, P, Z, I, I, I, I, P],
+    [P, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, P, Z, I, I, I, I, P],
 )
 _lib.register("fold_bwd_window_layout", [I, I, I, I, I, I, I, I, I, P])
 _lib.register("fold_bwd_counters", [P, I])
 _lib.register("fold_wait_probe", [ctypes.c_longlong, P, P, P])
 _lib.register("fold_fwd_run", [P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, P])
-_lib.register("fold_fwd_window", [P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, I, P, I, P])
-_lib.register("fold_fwd_window_sm100", [P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, I, P, I, P, P])
+_lib.register("fold_fwd_window", [P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, I, P, I, P])
+_lib.register("fold_fwd_window_sm100", [P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, I, P, I, P, P])
 _lib.register("fold_fwd_sm100_supported", [I, I])
 _lib.register("fold_fwd_run_sm100", [P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, P, P])
 
@@ -183,8 +183,8 @@ def prepare_backward(
         plan.subgroup, plan.record,
     )
 
-    if window:   # the same arguments without the mask and the plan
-        args = (*args[:17], *args[18:23], window, sinks)
+    if window:   # the same arguments without the mask and the plan, and O as it was rounded
+        args = (*args[:4], None, *args[4:17], *args[18:23], window, sinks)
 
     def run():
         if window:
@@ -279,7 +279,8 @@ def attention_forward(q, k, v, *, causal, softmax_scale=None, cu_seqlens=None, m
     if can and kernel != "mma":
         status = torch.zeros(1, device=q.device, dtype=torch.int32)
         if window:
-            del args[13]
+            args[5:5] = [None]
+            del args[14]
             with _lib.on(q.device):
                 _lib.call("fold_fwd_window_sm100", *args, window, sinks, None, 0, status.data_ptr(), _lib.stream(q.device))
         else:
@@ -289,7 +290,8 @@ def attention_forward(q, k, v, *, causal, softmax_scale=None, cu_seqlens=None, m
             check_status(status, "attention_forward")
         return o, lse
     if window:
-        del args[13]
+        args[5:5] = [None]
+        del args[14]
         with _lib.on(q.device):
             _lib.call("fold_fwd_window", *args, window, sinks, None, 0, _lib.stream(q.device))
     else:
@@ -320,10 +322,20 @@ def _packed_strides(ts, varlen):
     return _stride_array(*out)
 
 
+# Delta = dO . O subtracts from dP of the same size where a query sees few keys, and O's rounding to 16 bits then shows
+# in dq and dk: 0.0036 of their norm in bf16 where every query sees 2 keys, 0.0026 at 8, 0.0024 from 64 on, against 0.0023 with
+# the exact O (the roundings of dS and of the results). Up to this many keys the forward leaves what its rounding took
+# as 16 bits more, and the backward adds it. With more it costs more than it gives (16384 tokens of 32 heads, window 128: 606 us
+# without, 664 with) but in a small call, where a sequence's first rows are many of its rows and a few bytes are nothing
+# beside the launches.
+REST_KEYS = 64
+REST_ELEMENTS = 1 << 22
+
+
 def window_forward(q, k, v, window, sinks, softmax_scale, cu_seqlens=None, max_seqlen=None):
     """`attention_forward` under a window for tensors the public entry points
     have checked: the same kernels with less on the host, which is what a small
-    call costs."""
+    call costs. Returns `(o, lse, o_rest)`."""
     varlen = cu_seqlens is not None
     dev, f16 = q.device, int(q.dtype is torch.float16)
     if varlen:
@@ -335,8 +347,9 @@ def window_forward(q, k, v, window, sinks, softmax_scale, cu_seqlens=None, max_s
         total = B * S
         lse = torch.empty((B, H, S), device=dev, dtype=torch.float32)
     o = torch.empty(q.shape, device=dev, dtype=q.dtype)
+    rest = torch.empty_like(o) if min(window + sinks, S) <= REST_KEYS or o.numel() <= REST_ELEMENTS else None
     strides = _packed_strides((q, k, v, o), varlen)
-    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), ctypes.addressof(strides),
+    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), _lib.ptr(rest), ctypes.addressof(strides),
             _lib.ptr(cu_seqlens), B, H, k.shape[-2], S, total, D, f16, softmax_scale, window, sinks, None, 0)
     with _lib.on(dev):
         if D == 128 and _lib.lib.fold_fwd_sm100_supported(D, f16):
@@ -347,10 +360,10 @@ def window_forward(q, k, v, window, sinks, softmax_scale, cu_seqlens=None, max_s
                 check_status(status, "attention_forward")
         else:
             _lib.call("fold_fwd_window", *args, _lib.stream(dev))
-    return o, lse
+    return o, lse, rest
 
 
-def window_backward(q, k, v, o, do, lse, window, sinks, softmax_scale, cu_seqlens=None, max_seqlen=None):
+def window_backward(q, k, v, o, rest, do, lse, window, sinks, softmax_scale, cu_seqlens=None, max_seqlen=None):
     """dQ, dK and dV of `window_forward`'s call, and the status word: what
     `prepare_backward(window=)` launches, once and in the caller's layout."""
     varlen = cu_seqlens is not None
@@ -368,8 +381,8 @@ def window_backward(q, k, v, o, do, lse, window, sinks, softmax_scale, cu_seqlen
     strides = _packed_strides((q, k, v, o, do, dq, dk, dv), varlen)
     with _lib.on(dev):
         _lib.call(
-            "fold_bwd_window", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(), lse.data_ptr(), dq.data_ptr(),
-            dk.data_ptr(), dv.data_ptr(), ctypes.addressof(strides), _lib.ptr(cu_seqlens), B, H, HKV, S, total, D,
+            "fold_bwd_window", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.ptr(rest), do.data_ptr(), lse.data_ptr(),
+            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ctypes.addressof(strides), _lib.ptr(cu_seqlens), B, H, HKV, S, total, D,
             int(q.dtype is torch.float16), softmax_scale, work.data_ptr(), nbytes, 0, window, sinks, 15, _lib.stream(dev),
         )
     return dq, dk, dv, work[at:at + 4]

@@ -71,7 +71,7 @@ extern "C" size_t fold_bwd_workspace_bytes(int batch, int n_heads, int n_kv_head
     return ws_layout(batch, n_heads, n_kv_heads, max_seqlen, total, head_dim, varlen != 0, plan, 0, 0).total;
 }
 
-static int bwd_run_phases(const void* q, const void* k, const void* v, const void* o,
+static int bwd_run_phases(const void* q, const void* k, const void* v, const void* o, const void* o_rest,
                           const void* dout, const float* lse, void* dq, void* dk, void* dv,
                           const int64_t* strides, const int32_t* cu_seqlens, int batch,
                           int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim,
@@ -111,6 +111,8 @@ static int bwd_run_phases(const void* q, const void* k, const void* v, const voi
                        "fold_bwd_run: rows of tensor %d must be 16-byte aligned", i);
     }
     p.lse = lse;
+    p.o_rest = o_rest;
+    FOLD_CHECK_ARG(reinterpret_cast<uintptr_t>(o_rest) % 16 == 0, "fold_bwd_run: o_rest must be 16-byte aligned");
     p.cu = cu_seqlens;
     if (varlen) {
         p.lse_sb = 0;
@@ -184,7 +186,7 @@ extern "C" int fold_bwd_run(const void* q, const void* k, const void* v, const v
                             int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim,
                             int causal, int is_f16, float softmax_scale, void* workspace,
                             size_t workspace_bytes, int kernel, int subgroup, int record, void* stream) {
-    return bwd_run_phases(q, k, v, o, dout, lse, dq, dk, dv, strides, cu_seqlens, batch, n_heads,
+    return bwd_run_phases(q, k, v, o, nullptr, dout, lse, dq, dk, dv, strides, cu_seqlens, batch, n_heads,
                           n_kv_heads, max_seqlen, total, head_dim, causal, is_f16, softmax_scale,
                           workspace, workspace_bytes, kernel, subgroup, record, 0, 0,
                           FOLD_BWD_PHASE_PRE | FOLD_BWD_PHASE_LIST | FOLD_BWD_PHASE_MAIN | FOLD_BWD_PHASE_POST, stream);
@@ -197,19 +199,19 @@ extern "C" int fold_bwd_run_phases(const void* q, const void* k, const void* v, 
                                    int head_dim, int causal, int is_f16, float softmax_scale,
                                    void* workspace, size_t workspace_bytes, int kernel, int subgroup,
                                    int record, int phases, void* stream) {
-    return bwd_run_phases(q, k, v, o, dout, lse, dq, dk, dv, strides, cu_seqlens, batch, n_heads,
+    return bwd_run_phases(q, k, v, o, nullptr, dout, lse, dq, dk, dv, strides, cu_seqlens, batch, n_heads,
                           n_kv_heads, max_seqlen, total, head_dim, causal, is_f16, softmax_scale,
                           workspace, workspace_bytes, kernel, subgroup, record, 0, 0, phases, stream);
 }
 
-extern "C" int fold_bwd_window(const void* q, const void* k, const void* v, const void* o,
+extern "C" int fold_bwd_window(const void* q, const void* k, const void* v, const void* o, const void* o_rest,
                                const void* dout, const float* lse, void* dq, void* dk, void* dv,
                                const int64_t* strides, const int32_t* cu_seqlens, int batch,
                                int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim,
                                int is_f16, float softmax_scale, void* workspace, size_t workspace_bytes,
                                int kernel, int window, int sinks, int phases, void* stream) {
     FOLD_CHECK_ARG(window > 0, "fold_bwd_window: a window of %d keys", window);
-    return bwd_run_phases(q, k, v, o, dout, lse, dq, dk, dv, strides, cu_seqlens, batch, n_heads,
+    return bwd_run_phases(q, k, v, o, o_rest, dout, lse, dq, dk, dv, strides, cu_seqlens, batch, n_heads,
                           n_kv_heads, max_seqlen, total, head_dim, 1, is_f16, softmax_scale,
                           workspace, workspace_bytes, kernel, 0, 0, window, sinks, phases, stream);
 }

@@ -18,6 +18,7 @@ struct TensorView {
 
 struct BwdParams {
     TensorView q, k, v, o, dout, dq, dk, dv;
+    const void* o_rest;    // what rounding took from o, laid out as o, or null: Delta then is dO's product with both
     const float* lse;      // natural log; dense (B, H, S), packed (H, total)
     int64_t lse_sb, lse_sh;
     const int* cu;         // (B + 1) int32 on the device, or null for dense

@@ -72,6 +72,12 @@ __global__ void __launch_bounds__(PRE_THREADS) bwd_preprocess_kernel(const BwdPa
                 unpack4<F16>(ow[u], o);
                 unpack4<F16>(gw[u], g);
                 float d = o[0] * g[0] + o[1] * g[1] + o[2] * g[2] + o[3] * g[3];
+                if (p.o_rest && active) {
+                    float z[4];
+                    const uint16_t* orow = row_ptr<const uint16_t>(p.o, b, sq.start + i, h) + lane * 4;
+                    unpack4<F16>(ldg8(static_cast<const uint16_t*>(p.o_rest) + (orow - static_cast<const uint16_t*>(p.o.ptr))), z);
+                    d += z[0] * g[0] + z[1] * g[1] + z[2] * g[2] + z[3] * g[3];
+                }
                 float n2 = g[0] * g[0] + g[1] * g[1] + g[2] * g[2] + g[3] * g[3];
                 d = warp_sum(d);
                 n2 = warp_sum(n2);
@@ -217,6 +223,11 @@ __global__ void __launch_bounds__(PRE_THREADS, 4) bwd_preprocess128_kernel(const
         for (int u = 0; u < RB; ++u) {
             const int i = mb * PRE_ROWS + r0 + 2 * u * NW;
             float d2[2], n2[2];
+            uint4 rw = make_uint4(0u, 0u, 0u, 0u);
+            if (p.o_rest && i < sq.len) {
+                const uint16_t* orow = row_ptr<const uint16_t>(p.o, b, sq.start + i, h);
+                rw = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.o_rest) + (orow - static_cast<const uint16_t*>(p.o.ptr))) + lane);
+            }
 #pragma unroll
             for (int v = 0; v < 2; ++v) {      // the two lanes' terms
                 float o[4], g[4];
@@ -224,6 +235,10 @@ __global__ void __launch_bounds__(PRE_THREADS, 4) bwd_preprocess128_kernel(const
                 unpack4<F16>(v ? make_uint2(gw[u].z, gw[u].w) : make_uint2(gw[u].x, gw[u].y), g);
                 d2[v] = o[0] * g[0] + o[1] * g[1] + o[2] * g[2] + o[3] * g[3];
                 n2[v] = g[0] * g[0] + g[1] * g[1] + g[2] * g[2] + g[3] * g[3];
+                if (p.o_rest) {
+                    unpack4<F16>(v ? make_uint2(rw.z, rw.w) : make_uint2(rw.x, rw.y), o);
+                    d2[v] += o[0] * g[0] + o[1] * g[1] + o[2] * g[2] + o[3] * g[3];
+                }
             }
             // the general kernel's butterfly: its offsets 16, 8, 4, 2 are 8, 4, 2, 1 here, its last one the thread's own
 #pragma unroll

@@ -22,6 +22,7 @@ struct FwdParams {
     int window, sinks;
     const int4* plan;
     int total;       // packed rows
+    void* o_rest;    // what rounding took from o, laid out as o, or null (a window's)
 };
 
 // KIND: the causal and full forward, a window, or a chunk. A chunk's blocks are few and their keys many, and
@@ -227,6 +228,16 @@ __global__ void __launch_bounds__(KIND == KIND_CHUNK ? 256 : 128) fwd_mma_kernel
 #pragma unroll
         for (int i = 0; i < NTO; ++i)
             *reinterpret_cast<uint32_t*>(orow + 8 * i + 2 * tq) = pack16x2<F16>(o[i][2 * r] * inv, o[i][2 * r + 1] * inv);
+        if (KIND == KIND_WINDOW && p.o_rest) {
+            uint16_t* rest = static_cast<uint16_t*>(p.o_rest) + (orow - static_cast<uint16_t*>(p.o.ptr));
+#pragma unroll
+            for (int i = 0; i < NTO; ++i) {
+                const float x = o[i][2 * r] * inv, y = o[i][2 * r + 1] * inv;
+                const uint32_t w = pack16x2<F16>(x, y);
+                *reinterpret_cast<uint32_t*>(rest + 8 * i + 2 * tq) =
+                    pack16x2<F16>(x - half_bits_to_float<F16>(static_cast<uint16_t>(w & 0xFFFFu)), y - half_bits_to_float<F16>(static_cast<uint16_t>(w >> 16)));
+            }
+        }
         if (tq == 0 && (!EXT || p.lse))
             p.lse[b * p.lse_sb + h * p.lse_sh + start + qi] =
                 ls[r] > 0.f ? (mx[r] + log2f(ls[r])) * 0.6931471805599453f : -INFINITY;
@@ -261,7 +272,7 @@ static int fwd_launch_d(const FwdParams& p, cudaStream_t st) {
 using namespace fold;
 
 // The causal and full forward (window 0, plan null), a window's or a chunk's.
-static int fwd_run(const char* what, const void* q, const void* k, const void* v, void* o, float* lse,
+static int fwd_run(const char* what, const void* q, const void* k, const void* v, void* o, float* lse, void* o_rest,
                    const int64_t* strides, const int32_t* cu_seqlens, int batch, int n_heads, int n_kv_heads,
                    int max_seqlen, int total, int head_dim, int causal, int is_f16, float softmax_scale, int window,
                    int sinks, const int32_t* plan, int krows, void* stream) {
@@ -293,7 +304,7 @@ static int fwd_run(const char* what, const void* q, const void* k, const void* v
     p.B = batch; p.H = n_heads; p.HKV = n_kv_heads; p.G = n_heads / n_kv_heads;
     p.S = max_seqlen; p.D = head_dim; p.causal = causal; p.f16 = is_f16; p.scale = softmax_scale;
     p.window = window; p.sinks = sinks; p.plan = reinterpret_cast<const int4*>(plan);
-    p.total = total;
+    p.total = total; p.o_rest = o_rest;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (head_dim) {
         case 64: return fwd_launch_d<64>(p, st);
@@ -309,11 +320,11 @@ extern "C" int fold_fwd_run(const void* q, const void* k, const void* v, void* o
                             int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim,
                             int causal, int is_f16, float softmax_scale, void* stream) {
     FOLD_CHECK_ARG(lse, "fold_fwd_run: null pointer");
-    return fwd_run("fold_fwd_run", q, k, v, o, lse, strides, cu_seqlens, batch, n_heads, n_kv_heads, max_seqlen, total,
+    return fwd_run("fold_fwd_run", q, k, v, o, lse, nullptr, strides, cu_seqlens, batch, n_heads, n_kv_heads, max_seqlen, total,
                    head_dim, causal, is_f16, softmax_scale, 0, 0, nullptr, 0, stream);
 }
 
-extern "C" int fold_fwd_window(const void* q, const void* k, const void* v, void* o, float* lse,
+extern "C" int fold_fwd_window(const void* q, const void* k, const void* v, void* o, float* lse, void* o_rest,
                                const int64_t* strides, const int32_t* cu_seqlens, int batch, int n_heads,
                                int n_kv_heads, int max_seqlen, int total, int head_dim, int is_f16,
                                float softmax_scale, int window, int sinks, const int32_t* plan, int key_rows,
@@ -321,6 +332,7 @@ extern "C" int fold_fwd_window(const void* q, const void* k, const void* v, void
     FOLD_CHECK_ARG(window > 0 && window <= FOLD_MAX_WINDOW && sinks >= 0 && sinks <= FOLD_MAX_WINDOW,
                    "fold_fwd_window: a window of %d keys and %d sinks (1 .. 2^30 and 0 .. 2^30)", window, sinks);
     FOLD_CHECK_ARG(!plan || key_rows > 0, "fold_fwd_window: %d key rows", key_rows);
-    return fwd_run("fold_fwd_window", q, k, v, o, lse, strides, cu_seqlens, batch, n_heads, n_kv_heads, max_seqlen, total,
+    FOLD_CHECK_ARG(reinterpret_cast<uintptr_t>(o_rest) % 16 == 0 && !(plan && o_rest), "fold_fwd_window: o_rest is 16-byte aligned, without a plan");
+    return fwd_run("fold_fwd_window", q, k, v, o, lse, o_rest, strides, cu_seqlens, batch, n_heads, n_kv_heads, max_seqlen, total,
                    head_dim, 1, is_f16, softmax_scale, window, sinks, plan, key_rows, stream);
 }

@@ -186,6 +186,7 @@ struct Params {
     int window, sinks;
     const int4* plan;
     int total;       // packed rows
+    void* o_rest;    // what rounding took from o, laid out as o, or null
     int blocks;      // blocks of 256 rows (dense), or slots of 256 packed rows and one per request; with `plan` its own count
 };
 struct Maps {
@@ -786,6 +787,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_window_sm100_kernel(const Par
             // ---- epilogue: O / l -> 16-bit, LSE in nats ----
             const bool row_ok = qr < w.len;
             uint16_t* orow = row_ptr<uint16_t>(p.o, w.b, w.start + (row_ok ? qr : 0), w.h);
+            uint16_t* rrow = static_cast<uint16_t*>(p.o_rest) + (orow - static_cast<uint16_t*>(p.o.ptr));
             if (my_tiles > 0) {
                 mbar_wait(bar(B_ODONE + x), (it - 1) & 1, abort_flag, p.status);
                 tc_fence_after();
@@ -805,6 +807,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_window_sm100_kernel(const Par
                             v.z = pk2(__uint_as_float(ov[8 * u + 4]) * inv, __uint_as_float(ov[8 * u + 5]) * inv);
                             v.w = pk2(__uint_as_float(ov[8 * u + 6]) * inv, __uint_as_float(ov[8 * u + 7]) * inv);
                             *reinterpret_cast<uint4*>(orow + 32 * c + 8 * u) = v;
+                            if (p.o_rest) {
+                                auto rest = [&](int e, uint32_t w) {
+                                    return pk2(__uint_as_float(ov[8 * u + e]) * inv - half_bits_to_float<F16>(static_cast<uint16_t>(w & 0xFFFFu)),
+                                               __uint_as_float(ov[8 * u + e + 1]) * inv - half_bits_to_float<F16>(static_cast<uint16_t>(w >> 16)));
+                                };
+                                *reinterpret_cast<uint4*>(rrow + 32 * c + 8 * u) = make_uint4(rest(0, v.x), rest(2, v.y), rest(4, v.z), rest(6, v.w));
+                            }
                         }
                     }
                 }
@@ -874,7 +883,7 @@ extern "C" int fold_fwd_sm100_supported(int head_dim, int is_f16) {
 namespace {
 
 // The causal and full forward, or (`ext`) the windowed one.
-int run_sm100(const char* what, const void* q, const void* k, const void* v, void* o, float* lse, const int64_t* strides,
+int run_sm100(const char* what, const void* q, const void* k, const void* v, void* o, float* lse, void* o_rest, const int64_t* strides,
               const int32_t* cu_seqlens, int batch, int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim,
               int causal, int is_f16, float softmax_scale, int ext, int window, int sinks, const int32_t* plan, int krows,
               int32_t* status, void* stream) {
@@ -894,6 +903,7 @@ int run_sm100(const char* what, const void* q, const void* k, const void* v, voi
     fsm100::Params p;
     p.o.ptr = o; p.o.sb = strides[9]; p.o.sr = strides[10]; p.o.sh = strides[11];
     p.lse = lse;
+    p.o_rest = o_rest;
     p.cu = cu_seqlens;
     if (cu_seqlens) {
         p.lse_sb = 0;
@@ -947,11 +957,11 @@ extern "C" int fold_fwd_run_sm100(const void* q, const void* k, const void* v, v
                                   int n_kv_heads, int max_seqlen, int total, int head_dim, int causal, int is_f16,
                                   float softmax_scale, int32_t* status, void* stream) {
     FOLD_CHECK_ARG(lse, "fold_fwd_run_sm100: null pointer");
-    return run_sm100("fold_fwd_run_sm100", q, k, v, o, lse, strides, cu_seqlens, batch, n_heads, n_kv_heads, max_seqlen, total,
+    return run_sm100("fold_fwd_run_sm100", q, k, v, o, lse, nullptr, strides, cu_seqlens, batch, n_heads, n_kv_heads, max_seqlen, total,
                      head_dim, causal, is_f16, softmax_scale, 0, 0, 0, nullptr, 0, status, stream);
 }
 
-extern "C" int fold_fwd_window_sm100(const void* q, const void* k, const void* v, void* o, float* lse,
+extern "C" int fold_fwd_window_sm100(const void* q, const void* k, const void* v, void* o, float* lse, void* o_rest,
                                      const int64_t* strides, const int32_t* cu_seqlens, int batch, int n_heads,
                                      int n_kv_heads, int max_seqlen, int total, int head_dim, int is_f16,
                                      float softmax_scale, int window, int sinks, const int32_t* plan, int key_rows,
@@ -959,6 +969,7 @@ extern "C" int fold_fwd_window_sm100(const void* q, const void* k, const void* v
     FOLD_CHECK_ARG(window > 0 && window <= FOLD_MAX_WINDOW && sinks >= 0 && sinks <= FOLD_MAX_WINDOW,
                    "fold_fwd_window_sm100: a window of %d keys and %d sinks (1 .. 2^30 and 0 .. 2^30)", window, sinks);
     FOLD_CHECK_ARG(!plan || key_rows > 0, "fold_fwd_window_sm100: %d key rows", key_rows);
-    return run_sm100("fold_fwd_window_sm100", q, k, v, o, lse, strides, cu_seqlens, batch, n_heads, n_kv_heads, max_seqlen, total,
+    FOLD_CHECK_ARG(reinterpret_cast<uintptr_t>(o_rest) % 16 == 0 && !(plan && o_rest), "fold_fwd_window_sm100: o_rest is 16-byte aligned, without a plan");
+    return run_sm100("fold_fwd_window_sm100", q, k, v, o, lse, o_rest, strides, cu_seqlens, batch, n_heads, n_kv_heads, max_seqlen, total,
                      head_dim, 1, is_f16, softmax_scale, 1, window, sinks, plan, key_rows, status, stream);
 }

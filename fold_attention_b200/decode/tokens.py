@@ -238,7 +238,7 @@ def chunk_attention(q, cu_seqlens, lens, cap_tiles, seq_lens, page_table, page_s
                 SHORT_ROWS if short else 0, G, cap_tiles, plan, plan + 4 * n_plan, kw.data_ptr(), vw, base, st,
             )
             strides = (ctypes.c_int64 * 12)(0, q.stride(0), q.stride(1), 0, D, rows * D, 0, D, rows * D, 0, out.stride(0), out.stride(1))
-            args = (q.data_ptr(), kw.data_ptr(), vw, out.data_ptr(), None, ctypes.addressof(strides), cu_seqlens.data_ptr(), B, H,
+            args = (q.data_ptr(), kw.data_ptr(), vw, out.data_ptr(), None, None, ctypes.addressof(strides), cu_seqlens.data_ptr(), B, H,
                     n_kv_heads, max(lens), total, D, f16, 1.0 / math.sqrt(D), win, sinks, plan, rows)
             if _lib.lib.fold_fwd_sm100_supported(D, f16):
                 _lib.call("fold_fwd_window_sm100", *args, base, st)

@@ -54,20 +54,21 @@ class _FoldAttnFunc(torch.autograd.Function):
     def forward(ctx, q, k, v, softmax_scale, causal, window, sinks):
         if window:
             q, k, v = _windowed_input(q), _windowed_input(k), _windowed_input(v)
-            out, lse = window_forward(q, k, v, window, sinks, softmax_scale)
+            out, lse, rest = window_forward(q, k, v, window, sinks, softmax_scale)
         else:
+            rest = None
             q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, v))
             out, lse = attention_forward(q, k, v, causal=causal, softmax_scale=softmax_scale)
-        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.save_for_backward(q, k, v, out, lse, rest)
         ctx.softmax_scale, ctx.causal, ctx.window, ctx.sinks = softmax_scale, causal, window, sinks
         return out
 
     @staticmethod
     def backward(ctx, *grad_outputs):
         (dout,) = grad_outputs
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, lse, rest = ctx.saved_tensors
         if ctx.window:
-            dq, dk, dv, status = window_backward(q, k, v, out, dout.contiguous(), lse, ctx.window, ctx.sinks, ctx.softmax_scale)
+            dq, dk, dv, status = window_backward(q, k, v, out, rest, dout.contiguous(), lse, ctx.window, ctx.sinks, ctx.softmax_scale)
             if check_status:
                 read_status(status.view(torch.int32), "fold_attn_func's backward")
             return dq, dk, dv, None, None, None, None
@@ -92,14 +93,15 @@ class _FoldAttnVarlenFunc(torch.autograd.Function):
     def forward(ctx, q, k, v, cu_seqlens, max_seqlen, softmax_scale, causal, window, sinks):
         if window:
             q, k, v = _windowed_input(q), _windowed_input(k), _windowed_input(v)
-            out, lse = window_forward(q, k, v, window, sinks, softmax_scale, cu_seqlens, max_seqlen)
+            out, lse, rest = window_forward(q, k, v, window, sinks, softmax_scale, cu_seqlens, max_seqlen)
         else:
+            rest = None
             q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, v))
             out, lse = attention_forward(
                 q, k, v, causal=causal, softmax_scale=softmax_scale,
                 cu_seqlens=cu_seqlens, max_seqlen=max_seqlen,
             )
-        ctx.save_for_backward(q, k, v, out, lse, cu_seqlens)
+        ctx.save_for_backward(q, k, v, out, lse, cu_seqlens, rest)
         ctx.max_seqlen, ctx.softmax_scale, ctx.causal = max_seqlen, softmax_scale, causal
         ctx.window, ctx.sinks = window, sinks
         return out
@@ -107,10 +109,10 @@ class _FoldAttnVarlenFunc(torch.autograd.Function):
     @staticmethod
     def backward(ctx, *grad_outputs):
         (dout,) = grad_outputs
-        q, k, v, out, lse, cu_seqlens = ctx.saved_tensors
+        q, k, v, out, lse, cu_seqlens, rest = ctx.saved_tensors
         if ctx.window:
             dq, dk, dv, status = window_backward(
-                q, k, v, out, dout.contiguous(), lse, ctx.window, ctx.sinks, ctx.softmax_scale, cu_seqlens, ctx.max_seqlen)
+                q, k, v, out, rest, dout.contiguous(), lse, ctx.window, ctx.sinks, ctx.softmax_scale, cu_seqlens, ctx.max_seqlen)
             if check_status:
                 read_status(status.view(torch.int32), "fold_attn_varlen_func's backward")
             return dq, dk, dv, None, None, None, None, None, None

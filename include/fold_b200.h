@@ -409,10 +409,13 @@ int fold_bwd_run_phases(const void* q, const void* k, const void* v, const void*
  * gradients are the same bits whatever it is packed with. fold_bwd_window_layout describes the
  * workspace as fold_bwd_workspace_layout does ([6], [7]: the sinks' accumulators
  * [n_kv_heads][batch][sinks rounded up to 128][head_dim]) with its size in bytes in out12[11].
+ * Delta_i is dout's product with o, or with o + o_rest where the forward's remainder is given: a row of few keys
+ * loses Delta to cancellation. dq and dk are zero where every query sees one key, and, as dv, behind the
+ * last packed sequence.
  * No counterpart in the reference. */
 int fold_bwd_window_layout(int batch, int n_heads, int n_kv_heads, int max_seqlen, int total,
                            int head_dim, int varlen, int window, int sinks, int64_t* out12);
-int fold_bwd_window(const void* q, const void* k, const void* v, const void* o, const void* dout,
+int fold_bwd_window(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* dout,
                     const float* lse, void* dq, void* dk, void* dv, const int64_t* strides /* host */,
                     const int32_t* cu_seqlens, int batch, int n_heads, int n_kv_heads, int max_seqlen,
                     int total, int head_dim, int is_f16, float softmax_scale, void* workspace,
@@ -460,13 +463,14 @@ int fold_fwd_run_sm100(const void* q, const void* k, const void* v, void* o, flo
  * queries are each request's last positions (cu_seqlens, which must be given, cuts q and o alone)
  * and lse may be NULL (head_dim 64 on the warp-level kernel, the caches' own, 128 on the other). A row that
  * sees no key gets zeros and an lse of -infinity, and so do the rows behind the last sequence. A window that no
- * sequence fills is plain causal attention. No counterpart in the reference. */
-int fold_fwd_window(const void* q, const void* k, const void* v, void* o, float* lse,
+ * sequence fills is plain causal attention. `o_rest` (or NULL; without a plan) receives what rounding to 16 bits
+ * took from o, itself in 16 bits and laid out as o: fold_bwd_window's Delta. No counterpart in the reference. */
+int fold_fwd_window(const void* q, const void* k, const void* v, void* o, float* lse, void* o_rest,
                     const int64_t* strides /* host */, const int32_t* cu_seqlens, int batch,
                     int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim, int is_f16,
                     float softmax_scale, int window, int sinks, const int32_t* plan, int key_rows,
                     void* stream);
-int fold_fwd_window_sm100(const void* q, const void* k, const void* v, void* o, float* lse,
+int fold_fwd_window_sm100(const void* q, const void* k, const void* v, void* o, float* lse, void* o_rest,
                           const int64_t* strides /* host */, const int32_t* cu_seqlens, int batch,
                           int n_heads, int n_kv_heads, int max_seqlen, int total, int head_dim,
                           int is_f16, float softmax_scale, int window, int sinks,

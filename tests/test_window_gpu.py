@@ -279,3 +279,28 @@ def test_one_visible_key_has_no_score_gradient(D, dtype):
     out = fa.fold_attn_varlen_func(*x, cu, max_seqlen_q=1, causal=True, window=50, sinks=2)
     dq, dk, dv = torch.autograd.grad(out, x, do[0, :3])
     assert not dq.any() and not dk.any() and dv.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [128, 96, 64])
+@pytest.mark.parametrize("lens,window,sinks", [([1000], 2, 0), ([3] * 100, 50, 0), ([300, 5], 3, 1)])
+def test_few_visible_keys_keep_their_gradients_precision(lens, window, sinks, D, dtype):
+    """Delta comes from the unrounded output: what is left is the rounding of dS and of the results. Each is at most half
+    a step, 0.58 of one in the root mean square, so two in a row make 0.82 of the gradient's norm where the terms' signs
+    are independent; 0.85 and 2^-15 for the softmax's fp32 are allowed. (O rounded to 16 bits would add 0.7 half steps at two keys a
+    query and 2 at sequences of three tokens.)"""
+    import fold_attention_b200 as fa
+
+    q, k, v, do = inputs(sum(lens), 4, 2, D, dtype, seed=5)
+    x = [t.clone().requires_grad_() for t in (q, k, v)]
+    cu = torch.tensor([0] + list(torch.tensor(lens).cumsum(0)), device="cuda", dtype=torch.int32)
+    out = fa.fold_attn_varlen_func(*x, cu, max_seqlen_q=max(lens), causal=True, window=window, sinks=sinks)
+    got = torch.autograd.grad(out, x, do)
+    at, want = 0, []
+    for n in lens:
+        sl = slice(at, at + n)
+        want.append(reference(q[sl], k[sl], v[sl], do[sl], window, sinks))
+        at += n
+    half = torch.finfo(dtype).eps / 2
+    for g, w in zip(got[:2], [torch.cat([r[i] for r in want]) for i in (1, 2)]):
+        assert (g.double() - w).norm() <= (0.85 * half + 2 ** -15) * w.norm()
