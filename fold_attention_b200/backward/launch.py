@@ -324,12 +324,12 @@ def _packed_strides(ts, varlen):
 
 # Delta = dO . O subtracts from dP of the same size where a query sees few keys, and O's rounding to 16 bits then shows
 # in dq and dk: 0.0036 of their norm in bf16 where every query sees 2 keys, 0.0026 at 8, 0.0024 from 64 on, against 0.0023 with
-# the exact O (the roundings of dS and of the results). Up to this many keys the forward leaves what its rounding took
-# as 16 bits more, and the backward adds it. With more it costs more than it gives (16384 tokens of 32 heads, window 128: 606 us
-# without, 664 with) but in a small call, where a sequence's first rows are many of its rows and a few bytes are nothing
-# beside the launches.
-REST_KEYS = 64
-REST_ELEMENTS = 1 << 22
+# the exact O (the roundings of dS and of the results); what counts is the keys that a row's weight sits on. Up to this
+# many visible keys the forward leaves what its rounding took as 16 bits more, and the backward adds it. That is a
+# tenth of the time of a large call (16384 tokens of 32 heads, window 128: 606 us without, 664 with; D=64 792 and 875), so
+# windows of many keys, whose rows seldom sit on a few of them, go without. The rule knows the window alone: a sequence's bits do
+# not depend on what it is packed with.
+REST_KEYS = 256
 
 
 def window_forward(q, k, v, window, sinks, softmax_scale, cu_seqlens=None, max_seqlen=None):
@@ -347,7 +347,7 @@ def window_forward(q, k, v, window, sinks, softmax_scale, cu_seqlens=None, max_s
         total = B * S
         lse = torch.empty((B, H, S), device=dev, dtype=torch.float32)
     o = torch.empty(q.shape, device=dev, dtype=q.dtype)
-    rest = torch.empty_like(o) if min(window + sinks, S) <= REST_KEYS or o.numel() <= REST_ELEMENTS else None
+    rest = torch.empty_like(o) if window + sinks <= REST_KEYS else None
     strides = _packed_strides((q, k, v, o), varlen)
     args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), _lib.ptr(rest), ctypes.addressof(strides),
             _lib.ptr(cu_seqlens), B, H, k.shape[-2], S, total, D, f16, softmax_scale, window, sinks, None, 0)

@@ -23,6 +23,12 @@
 // Each leaves its piece (m, l, O) in the workspace and the last to arrive adds the pieces in list
 // order, so the bits do not depend on who that is.
 //
+// Measured: 64 requests of up to 32768 keys, 8 KV heads, D=128, an 8-bit V, one token each under a window of 1024 with 4
+// sinks: 80-84 us of 41 that its bytes take at the copy's rate (3.3 TB/s): a CTA has some twenty tiles in three or four
+// (request, head)s, and what each of those costs beside its tiles is a quarter of its time; the conversion of V,
+// which the tensor core cannot take as stored, is most of the rest. 32 requests of up to 32768 keys, 3-8 tokens each, a
+// bf16 V: 290-300 us of 276 (6.2 TB/s); 370 in a loop of seconds, where the power cap holds the SMs at 1.4 GHz.
+//
 // Warps: 0 K producer (both planes, scales), 3 V producer, 1 MMA issuer, 2 Q and V's dead rows (bf16 V),
 // 4-7 softmax and epilogue, 2 (8-bit V) or 8-11 (bf16 V) join pieces, 8-11 V's conversion (8-bit V). Every wait is bounded.
 #include <cuda.h>

@@ -444,6 +444,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
 // loads, and the epilogue with nothing behind it) was half of its time. One CTA per SM walks the work items
 // in stride, and the next item's Q and first tiles are loaded, and its first scores issued, while the last
 // one's O is written. Barrier phases count key tiles and items since the CTA started.
+// Measured (D=128, 32 heads, 8 KV heads): 6 packed sequences of 16384 tokens in all, window 512: 240 us; 2 x 8192, window 1024,
+// 4 sinks: 360-390; chunks of 2 x 2048 behind 16384-24576 keys: 1660 (1.0 PFLOP/s). The tensor and the transcendental
+// pipe are busy 54 % of the time each: a tile's softmax waits for its scores and its product for the softmax, and two query
+// tiles a CTA cover one another in part. Taking the weights in one pass over the scores (the maximum found
+// on the way, a second pass where it rose) was slower, 2068 us for the chunks: the weights wait in registers for the verdict.
+// In a loop of seconds the power cap holds the SMs at 1.7 GHz and the chunks take 1850.
 
 // What an item walks: key tiles [0, ns), then [lo, lo + n - ns); query tile x takes tiles
 // [low[x], end[x]) and those of the sinks (st of them).

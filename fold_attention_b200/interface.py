@@ -145,7 +145,8 @@ def fold_attn_func(q, k, v, softmax_scale=None, causal=False, window=None, sinks
     `window` (with `causal=True`) is a sliding window: the query at position i
     sees the `window` newest keys up to its own, `i - window < j <= i`, and the
     sequence's first `sinks` keys. The work is the window's, not the
-    sequence's, and the gradients keep their order-free bits.
+    sequence's, and the gradients keep their order-free bits. Where every
+    query sees one key, dq and dk are zero.
     """
     window, sinks = check_window(window, sinks, causal)
     _check_qkv(q, k, v, 4)
@@ -175,7 +176,8 @@ def fold_attn_varlen_func(
     The keys are the queries' own sequences, so `cu_seqlens_k` and
     `max_seqlen_k` may be left out; if given they must match. A request's
     gradients are the same bits alone and packed with others. `window` and
-    `sinks` as for `fold_attn_func`, counted within each sequence.
+    `sinks` as for `fold_attn_func`, counted within each sequence; with a window,
+    rows behind the last sequence give zeros, and have zeros for gradients.
     """
     window, sinks = check_window(window, sinks, causal)
     _check_qkv(q, k, v, 3)
