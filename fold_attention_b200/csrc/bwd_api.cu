@@ -32,7 +32,7 @@ bool resolve_plan(int n_heads, int n_kv_heads, int max_seqlen, int subgroup, int
 }
 
 struct WsLayout {
-    size_t dq_acc, dpsum, lse2, stats, dk_acc, dv_acc, work, total;
+    size_t dq_acc, dpsum, lse2, stats, dk_acc, dv_acc, work, last, total;
     int64_t rows_p, n_items;
 };
 
@@ -58,6 +58,8 @@ WsLayout ws_layout(int B, int H, int HKV, int S, int total, int D, bool varlen, 
     w.dk_acc = off; off = align256(off + 8 * acc);
     w.dv_acc = off; off = align256(off + (plan.dv_bits / 8) * acc);
     w.work = off;   off = align256(off + 32 * static_cast<size_t>(w.n_items));
+    w.last = off;
+    if (window > 0 && varlen && D == 128) off = align256(off + sizeof(uint16_t) * 2 * static_cast<size_t>(B) * (H + HKV) * ROW_PAD * D);
     w.total = off;
     return w;
 }
@@ -166,6 +168,7 @@ static int bwd_run_phases(const void* q, const void* k, const void* v, const voi
         p.sink_rows = (n + tile - 1) / tile * tile;
         p.sink_record = sink_record_blocks(window, tile);
     }
+    p.last = window > 0 && varlen && sm100 ? reinterpret_cast<uint16_t*>(ws + w.last) : nullptr;
     p.dq_bias = (sm100 && bwd_sm100_biased()) ? 1 : 0;
     int rc = FOLD_OK;
     if (phases & FOLD_BWD_PHASE_PRE) rc = launch_bwd_preprocess(p, st);

@@ -50,6 +50,11 @@ struct BwdParams {
     // into records of `sink_record` query blocks and its dK, dV meet in the integer accumulators
     // (dk_acc, dv_acc), which then hold [HKV][B][sink_stride][D] for the sinks' blocks alone.
     int window, sinks, sink_record;
+    // Packed sequences under a window, on the tcgen05 main loop: each one's last block of 128 rows of Q, dO
+    // [B][H][128][D] and K, V [B][HKV][128][D], zeros past its end, or null. A tile that TMA takes from the
+    // tensor there holds the next sequence's first rows, or what lies behind the last one's, and a NaN among them would
+    // pass through the products' zeros.
+    uint16_t* last;
     int sink_rows;      // rows of a sequence whose dK, dV the accumulators hold: the sinks' whole key blocks
     int sink_stride;    // and how many are laid out
 };

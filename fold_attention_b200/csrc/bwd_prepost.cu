@@ -9,6 +9,8 @@
 // Postprocess: dQ = round16( float(acc) * (softmax_scale * 2^-s) ); and for folded
 //   dK, dV: dK = round16( float(acc) * (softmax_scale * 2^-s_dK) ), dV = round16( float(acc) * 2^-s_dV ).
 //   Reference: src/fold_attention/backward/postprocess.py:125-154,256-344.
+#include <climits>
+
 #include "bwd_common.cuh"
 
 namespace fold {
@@ -186,6 +188,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 4) bwd_preprocess128_kernel(const
     const int hkv = h / p.G;
     const bool kv_owner = (h % p.G) == 0;
     const bool acc_stats = p.fold || p.sink_rows > 0;   // dK's and dV's grids are used
+    const int cut = p.last && sq.len % ROW_PAD ? sq.len / ROW_PAD * ROW_PAD : INT_MAX;   // rows from here on go to p.last
     uint32_t mx_k = 0u, mx_v = 0u, mx_doc = 0u, mx_q = 0u;
     float mx_dn = 0.f, mx_dl = 0.f;
     const int64_t wbase = static_cast<int64_t>(h) * p.rows_p + sq.pstart;
@@ -211,7 +214,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 4) bwd_preprocess128_kernel(const
             if (i < sq.len) {
                 ow[u] = __ldg(reinterpret_cast<const uint4*>(row_ptr<const uint16_t>(p.o, b, sq.start + i, h)) + lane);
                 gw[u] = __ldg(reinterpret_cast<const uint4*>(row_ptr<const uint16_t>(p.dout, b, sq.start + i, h)) + lane);
-                if (acc_stats) qw[u] = __ldg(reinterpret_cast<const uint4*>(row_ptr<const uint16_t>(p.q, b, sq.start + i, h)) + lane);
+                if (acc_stats || i >= cut) qw[u] = __ldg(reinterpret_cast<const uint4*>(row_ptr<const uint16_t>(p.q, b, sq.start + i, h)) + lane);
                 if (kv_owner) {
                     kw[u] = __ldg(reinterpret_cast<const uint4*>(row_ptr<const uint16_t>(p.k, b, sq.start + i, hkv)) + lane);
                     vw[u] = __ldg(reinterpret_cast<const uint4*>(row_ptr<const uint16_t>(p.v, b, sq.start + i, hkv)) + lane);
@@ -266,6 +269,17 @@ __global__ void __launch_bounds__(PRE_THREADS, 4) bwd_preprocess128_kernel(const
             if (lane == 0) {
                 p.dpsum[wbase + i] = i < sq.len ? delta : 0.f;
                 p.lse2[wbase + i] = lse2;
+            }
+            if (i >= cut) {
+                constexpr int64_t TILE = ROW_PAD * D / 8;
+                uint4* last = reinterpret_cast<uint4*>(p.last) + static_cast<int64_t>(i - cut) * (D / 8) + lane;
+                last[(static_cast<int64_t>(b) * p.H + h) * TILE] = qw[u];
+                last[(static_cast<int64_t>(p.B + b) * p.H + h) * TILE] = gw[u];
+                if (kv_owner) {
+                    uint4* kv = last + 2 * static_cast<int64_t>(p.B) * p.H * TILE;
+                    kv[(static_cast<int64_t>(b) * p.HKV + hkv) * TILE] = kw[u];
+                    kv[(static_cast<int64_t>(p.B + b) * p.HKV + hkv) * TILE] = vw[u];
+                }
             }
             int4* acc = reinterpret_cast<int4*>(p.dq_acc + (wbase + i) * D) + lane;
             acc[0] = make_int4(init, init, init, init);

@@ -281,6 +281,7 @@ __host__ __device__ constexpr uint32_t instr_desc(int fmt, int M, int N, int a_m
 struct Maps {
     CUtensorMap q, dout, k, v;   // (channel, row, head, batch), boxes (64, 128, 1, 1)
     CUtensorMap dk, dv;          // the same view of the outputs, for the private exit's tile stores
+    CUtensorMap q_last, dout_last, k_last, v_last;   // the sequences' last blocks (p.last), as batches of 128 rows
     CUtensorMap dq;              // the int32 accumulator as (channel, head * padded row), boxes (32, 128)
 };
 
@@ -451,32 +452,36 @@ bwd_main_sm100_kernel(const BwdParams p, const __grid_constant__ Maps maps) {
                 __threadfence_block();
                 mbar_arrive(sh.bar(B_IFULL + sl));
                 if (idx < 0 || *abort_flag) break;
-                const int brow = it.sq.start + it.n0;
-                const int bb = p.cu ? 0 : it.b;
+                const bool last_k = WIN && p.last && it.n0 + BN > it.sq.len;
+                const int brow = last_k ? 0 : it.sq.start + it.n0;
+                const int bb = p.cu ? 0 : it.b, kb = last_k ? it.b : bb;
+                const CUtensorMap *mk = last_k ? &maps.k_last : &maps.k, *mv = last_k ? &maps.v_last : &maps.v;
                 // K and V: one buffer each, free when the item before has issued its last dQ~
                 if (j >= 1) mbar_wait<SLEEP_PRODUCER>(sh.bar(B_KVFREE), (j - 1) & 1, abort_flag, p.status);
                 mbar_expect_tx(sh.bar(B_KV), 2 * 32768);
                 for (int x = 0; x < 2; ++x) {
-                    tma_load_4d(base + SM_K + x * 16384, &maps.k, 64 * x, brow, it.hkv, bb, sh.bar(B_KV));
-                    tma_load_4d(base + SM_V + x * 16384, &maps.v, 64 * x, brow, it.hkv, bb, sh.bar(B_KV));
+                    tma_load_4d(base + SM_K + x * 16384, mk, 64 * x, brow, it.hkv, kb, sh.bar(B_KV));
+                    tma_load_4d(base + SM_V + x * 16384, mv, 64 * x, brow, it.hkv, kb, sh.bar(B_KV));
                 }
                 for (int i = 0; i < it.total; ++i, ++t) {
                     const int s = t % STAGES;
                     const int g = i / it.per_head, mb = it.m_first + i % it.per_head;
                     const int h = it.hkv * p.G + it.h0 + g;
-                    const int row = it.sq.start + mb * BM;
+                    const bool last_q = WIN && p.last && (mb + 1) * BM > it.sq.len;
+                    const int row = last_q ? 0 : it.sq.start + mb * BM, qb = last_q ? it.b : bb;
+                    const CUtensorMap *mq = last_q ? &maps.q_last : &maps.q, *mdo = last_q ? &maps.dout_last : &maps.dout;
                     const int64_t wrow = static_cast<int64_t>(h) * p.rows_p + it.sq.pstart + mb * BM;
                     // Q and L: two stages, free when dK of the tile two back has read Q
                     if (t >= STAGES) mbar_wait<SLEEP_PRODUCER>(sh.bar(B_QEMPTY + s), ((t / STAGES) - 1) & 1, abort_flag, p.status);
                     mbar_expect_tx(sh.bar(B_QFULL + s), 32768 + 512);
-                    for (int x = 0; x < 2; ++x) tma_load_4d(base + SM_Q + s * 32768 + x * 16384, &maps.q, 64 * x, row, h, bb, sh.bar(B_QFULL + s));
+                    for (int x = 0; x < 2; ++x) tma_load_4d(base + SM_Q + s * 32768 + x * 16384, mq, 64 * x, row, h, qb, sh.bar(B_QFULL + s));
                     bulk_load(base + SM_L + s * 512, p.lse2 + wrow, 512, sh.bar(B_QFULL + s));
                     // dO: one buffer, free when dV of the tile before has read it (three GEMMs ahead of
                     // the dP^T that wants the new one); Delta rides with it but alternates between two
                     // slots, because the compute warps may still be reading the last one
                     if (t >= 1) mbar_wait<SLEEP_PRODUCER>(sh.bar(B_OEMPTY), (t - 1) & 1, abort_flag, p.status);
                     mbar_expect_tx(sh.bar(B_OFULL), 32768 + 512);
-                    for (int x = 0; x < 2; ++x) tma_load_4d(base + SM_DO + x * 16384, &maps.dout, 64 * x, row, h, bb, sh.bar(B_OFULL));
+                    for (int x = 0; x < 2; ++x) tma_load_4d(base + SM_DO + x * 16384, mdo, 64 * x, row, h, qb, sh.bar(B_OFULL));
                     bulk_load(base + SM_DL + s * 512, p.dpsum + wrow, 512, sh.bar(B_OFULL));
                 }
             }
@@ -1212,6 +1217,18 @@ int launch_bwd_main_sm100(const BwdParams& p, bool build_list, bool run_main, cu
         !make_acc_map(&maps.dq, p)) {
         set_error("bwd_main_sm100: cuTensorMapEncodeTiled failed");
         return FOLD_ERR_LAUNCH;
+    }
+    maps.q_last = maps.q, maps.dout_last = maps.dout, maps.k_last = maps.k, maps.v_last = maps.v;
+    if (p.last) {
+        constexpr int64_t TILE = ROW_PAD * sm100::HD;
+        const int64_t nq = static_cast<int64_t>(p.B) * p.H * TILE, nk = static_cast<int64_t>(p.B) * p.HKV * TILE;
+        auto at = [&](int64_t off, int heads) { return TensorView{p.last + off, heads * TILE, sm100::HD, TILE}; };
+        if (!make_map(&maps.q_last, at(0, p.H), ROW_PAD, p.H, p.B, sm100::BM, f16) || !make_map(&maps.dout_last, at(nq, p.H), ROW_PAD, p.H, p.B, sm100::BM, f16) ||
+            !make_map(&maps.k_last, at(2 * nq, p.HKV), ROW_PAD, p.HKV, p.B, sm100::BN, f16) ||
+            !make_map(&maps.v_last, at(2 * nq + nk, p.HKV), ROW_PAD, p.HKV, p.B, sm100::BN, f16)) {
+            set_error("bwd_main_sm100: cuTensorMapEncodeTiled failed");
+            return FOLD_ERR_LAUNCH;
+        }
     }
     // The work list, then one persistent CTA per SM claiming from it. Sections: as many (request,
     // KV head, subgroup) triples as keep their Q, dO (16-bit) and dQ accumulator (int32) within a

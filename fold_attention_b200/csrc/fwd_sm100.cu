@@ -554,14 +554,16 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_window_sm100_kernel(const Par
     uint8_t* smem = smem_raw + (base - raw);
     auto bar = [&](int i) { return base + SM_BAR + 8 * i; };
     constexpr int B_QEMPTY = B_COUNT;      // the item's last scores are out of Q
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + SM_BAR + 8 * (B_COUNT + 1));
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM_BAR + 8 * (B_COUNT + 1) + 8);
+    constexpr int B_CUT = B_COUNT + 1;     // a sequence's last tile has landed, its V still with the rows behind it
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + SM_BAR + 8 * (B_COUNT + 2));
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM_BAR + 8 * (B_COUNT + 2) + 8);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
         *abort_flag = 0;
         mbar_init(bar(B_Q), 1);
         mbar_init(bar(B_QEMPTY), 1);
+        mbar_init(bar(B_CUT), 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(B_KVFULL + i), 1);
             mbar_init(bar(B_KVEMPTY + i), 1);
@@ -585,7 +587,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_window_sm100_kernel(const Par
     if (warp == 0) {
         // ================= TMA producer =================
         if (lane == 0) {
-            int jk = 0, items = 0;         // key tiles, and items with any, so far
+            int jk = 0, items = 0, cuts = 0;         // key tiles, items with any, and tiles cut short, so far
             for (int i = blockIdx.x; i < list.items; i += gridDim.x) {
                 Item w;
                 if (!load_item(p, list, i, w) || w.nt[0] + w.nt[1] == 0) continue;
@@ -601,10 +603,24 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_window_sm100_kernel(const Par
                     const int s = jk & 1;
                     if (jk >= 2) mbar_wait(bar(B_KVEMPTY + s), ((jk >> 1) - 1) & 1, abort_flag, p.status);
                     const uint32_t st = base + SM_KV + s * STAGE;
-                    mbar_expect_tx(bar(B_KVFULL + s), 65536);
+                    // A packed sequence's last tile holds rows behind its end: their scores are masked, but a NaN in V there
+                    // would pass through P's zeros, so V's are made zeros before the tile is handed on.
+                    const int live = max(0, w.klen - w.tile(j) * BN);
+                    const bool cut = p.cu && !p.plan && live < BN;
+                    const uint32_t full = bar(cut ? B_CUT : B_KVFULL + s);
+                    mbar_expect_tx(full, 65536);
                     for (int c = 0; c < 2; ++c) {
-                        tma_load_4d(st + c * 16384, &maps.k, 64 * c, w.row(j), hkv, bb, bar(B_KVFULL + s));
-                        tma_load_4d(st + 32768 + c * 16384, &maps.v, 64 * c, w.row(j), hkv, bb, bar(B_KVFULL + s));
+                        tma_load_4d(st + c * 16384, &maps.k, 64 * c, w.row(j), hkv, bb, full);
+                        tma_load_4d(st + 32768 + c * 16384, &maps.v, 64 * c, w.row(j), hkv, bb, full);
+                    }
+                    if (cut) {
+                        mbar_wait(full, cuts++ & 1, abort_flag, p.status);
+                        for (int c = 0; c < 2; ++c) {
+                            uint4* dead = reinterpret_cast<uint4*>(smem + SM_KV + s * STAGE + 32768 + c * 16384 + live * 128);
+                            for (int u = 0; u < 8 * (BN - live); ++u) dead[u] = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        mbar_arrive(bar(B_KVFULL + s));
                     }
                 }
                 ++items;

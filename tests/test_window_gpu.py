@@ -304,3 +304,28 @@ def test_few_visible_keys_keep_their_gradients_precision(lens, window, sinks, D,
     half = torch.finfo(dtype).eps / 2
     for g, w in zip(got[:2], [torch.cat([r[i] for r in want]) for i in (1, 2)]):
         assert (g.double() - w).norm() <= (0.85 * half + 2 ** -15) * w.norm()
+
+
+@pytest.mark.parametrize("where", ["tail", "neighbour"])
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("window,sinks", [(100, 3), (500, 0), (30, 200)])
+def test_what_lies_behind_a_sequence_does_not_reach_it(window, sinks, D, where):
+    """NaN and infinities in the rows behind a packed sequence, the next one's or nobody's: its results keep their bits."""
+    import fold_attention_b200 as fa
+
+    total = 470 + (60 if where == "tail" else 0)
+    live = 470 if where == "tail" else 300
+    cu = torch.tensor([0, 300, 470], device="cuda", dtype=torch.int32)
+    clean = inputs(total, 4, 2, D, torch.bfloat16, seed=4)
+
+    def run(q, k, v, do):
+        x = [t.clone().requires_grad_() for t in (q, k, v)]
+        out = fa.fold_attn_varlen_func(*x, cu, max_seqlen_q=300, causal=True, window=window, sinks=sinks)
+        return (out.detach(), *torch.autograd.grad(out, x, do))
+
+    want = run(*clean)
+    for n in range(4):
+        for value in (float("nan"), float("inf")):
+            bad = [t.clone() for t in clean]
+            bad[n][live:] = value
+            assert all(torch.equal(a[:live], b[:live]) for a, b in zip(want, run(*bad))), (n, value)
