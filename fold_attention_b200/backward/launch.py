@@ -332,10 +332,10 @@ def _packed_strides(ts, varlen):
 REST_KEYS = 256
 
 
-def window_forward(q, k, v, window, sinks, softmax_scale, cu_seqlens=None, max_seqlen=None):
+def window_forward(q, k, v, window, sinks, softmax_scale, cu_seqlens=None, max_seqlen=None, grad=True):
     """`attention_forward` under a window for tensors the public entry points
     have checked: the same kernels with less on the host, which is what a small
-    call costs. Returns `(o, lse, o_rest)`."""
+    call costs. Returns `(o, lse, o_rest)`; without `grad` no backward follows."""
     varlen = cu_seqlens is not None
     dev, f16 = q.device, int(q.dtype is torch.float16)
     if varlen:
@@ -347,7 +347,7 @@ def window_forward(q, k, v, window, sinks, softmax_scale, cu_seqlens=None, max_s
         total = B * S
         lse = torch.empty((B, H, S), device=dev, dtype=torch.float32)
     o = torch.empty(q.shape, device=dev, dtype=q.dtype)
-    rest = torch.empty_like(o) if window + sinks <= REST_KEYS else None
+    rest = torch.empty_like(o) if grad and window + sinks <= REST_KEYS else None
     strides = _packed_strides((q, k, v, o), varlen)
     args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), _lib.ptr(rest), ctypes.addressof(strides),
             _lib.ptr(cu_seqlens), B, H, k.shape[-2], S, total, D, f16, softmax_scale, window, sinks, None, 0)

@@ -54,7 +54,7 @@ class _FoldAttnFunc(torch.autograd.Function):
     def forward(ctx, q, k, v, softmax_scale, causal, window, sinks):
         if window:
             q, k, v = _windowed_input(q), _windowed_input(k), _windowed_input(v)
-            out, lse, rest = window_forward(q, k, v, window, sinks, softmax_scale)
+            out, lse, rest = window_forward(q, k, v, window, sinks, softmax_scale, grad=any(ctx.needs_input_grad))
         else:
             rest = None
             q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, v))
@@ -93,7 +93,8 @@ class _FoldAttnVarlenFunc(torch.autograd.Function):
     def forward(ctx, q, k, v, cu_seqlens, max_seqlen, softmax_scale, causal, window, sinks):
         if window:
             q, k, v = _windowed_input(q), _windowed_input(k), _windowed_input(v)
-            out, lse, rest = window_forward(q, k, v, window, sinks, softmax_scale, cu_seqlens, max_seqlen)
+            out, lse, rest = window_forward(
+                q, k, v, window, sinks, softmax_scale, cu_seqlens, max_seqlen, grad=any(ctx.needs_input_grad))
         else:
             rest = None
             q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k, v))
