@@ -395,6 +395,10 @@ __global__ void __launch_bounds__(NT) chunk_gather_kernel(const int4* __restrict
 
 using namespace fold;
 
+static bool planes_aligned(const void* ka, const void* kb, const void* va, const void* vb) {   // (16 bytes; vb may be null)
+    return ((reinterpret_cast<uintptr_t>(ka) | reinterpret_cast<uintptr_t>(kb) | reinterpret_cast<uintptr_t>(va) | reinterpret_cast<uintptr_t>(vb)) & 15) == 0;
+}
+
 extern "C" int fold_build_tables(const int32_t* cu_seqlens, const int32_t* seq_lens, int batch, int32_t* page_table, int pages_per_request,
                                  int page_size, int total, const int32_t* free_pages, int n_free, const int32_t* taken, int32_t* slots,
                                  int32_t* lens_out, int32_t* taken_out, void* stream) {
@@ -416,7 +420,7 @@ extern "C" int fold_write_tokens(const void* k, const void* v, int is_f16, int64
     if (total == 0) return FOLD_OK;
     FOLD_CHECK_ARG(k && v && slots && ka && kb && va && ek, "fold_write_tokens: null pointer");
     FOLD_CHECK_ARG(k_token_stride % 8 == 0 && k_head_stride % 8 == 0 && v_token_stride % 8 == 0 && v_head_stride % 8 == 0 &&
-                       reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0,
+                       reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0 && planes_aligned(ka, kb, va, vb),
                    "fold_write_tokens: rows must be 16-byte aligned");
     const int rpb = NT / (head_dim / 16);
     const int64_t rows = total * n_kv_heads, grid = (rows + rpb - 1) / rpb;
@@ -445,7 +449,7 @@ extern "C" int fold_read_tokens(const int32_t* slots, int64_t total, int n_kv_he
     FOLD_CHECK_ARG(out_dtype >= 0 && out_dtype <= 2, "fold_read_tokens: output type %d", out_dtype);
     if (total == 0) return FOLD_OK;
     FOLD_CHECK_ARG(slots && ka && kb && va && ek && k && v, "fold_read_tokens: null pointer");
-    FOLD_CHECK_ARG(reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0, "fold_read_tokens: rows must be 16-byte aligned");
+    FOLD_CHECK_ARG(reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0 && planes_aligned(ka, kb, va, vb), "fold_read_tokens: rows must be 16-byte aligned");
     const int rpb = NT / (head_dim / 16);
     const int64_t rows = total * n_kv_heads, grid = (rows + rpb - 1) / rpb;
     FOLD_CHECK_ARG(grid < (1ll << 31), "fold_read_tokens: %lld rows in one call", static_cast<long long>(rows));
@@ -492,6 +496,7 @@ extern "C" int fold_chunk_gather(const int32_t* cu_seqlens, const int32_t* seq_l
     FOLD_CHECK_ARG(batch > 0 && n_kv_heads > 0 && n_kv_heads <= 65535 && pages_per_request > 0 && page_size > 0 && cap_tiles > 0 && cap_tiles <= (1 << 24) &&
                        rows_over >= 0 && group > 0,
                    "fold_chunk_gather: %d requests, %d heads, %d pages of %d keys, %d tiles", batch, n_kv_heads, pages_per_request, page_size, cap_tiles);
+    FOLD_CHECK_ARG(planes_aligned(ka, kb, va, vb) && planes_aligned(kw, vw, plan, nullptr) && reinterpret_cast<uintptr_t>(tiles) % 8 == 0, "fold_chunk_gather: rows must be 16-byte aligned");
     FOLD_CHECK_ARG(window > 0 && window <= FOLD_MAX_WINDOW && sinks >= 0 && sinks <= FOLD_MAX_WINDOW, "fold_chunk_gather: a window of %d keys and %d sinks", window, sinks);
     const int64_t cap = static_cast<int64_t>(pages_per_request) * page_size;
     cudaStream_t st = static_cast<cudaStream_t>(stream);

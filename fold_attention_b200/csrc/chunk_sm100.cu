@@ -1018,7 +1018,8 @@ extern "C" int fold_chunk_sm100(const void* q, int64_t q_token_stride, int64_t q
     FOLD_CHECK_ARG(window > 0 && window <= FOLD_MAX_WINDOW && sinks >= 0 && sinks <= FOLD_MAX_WINDOW, "fold_chunk_sm100: a window of %d keys and %d sinks", window, sinks);
     FOLD_CHECK_ARG(q_token_stride % 8 == 0 && q_head_stride % 8 == 0 && o_token_stride % 8 == 0 && o_head_stride % 8 == 0 &&
                        reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(o) % 16 == 0 &&
-                       reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && reinterpret_cast<uintptr_t>(va) % 16 == 0,
+                       reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && reinterpret_cast<uintptr_t>(ka) % 16 == 0 && reinterpret_cast<uintptr_t>(kb) % 16 == 0 &&
+                       reinterpret_cast<uintptr_t>(va) % 16 == 0 && reinterpret_cast<uintptr_t>(vb) % 16 == 0 && reinterpret_cast<uintptr_t>(ek) % 16 == 0,
                    "fold_chunk_sm100: rows must be 16-byte aligned");
     const Work w = chunk_work(batch, total, n_heads, n_kv_heads, head_dim, ctas);
     FOLD_CHECK_ARG(workspace_bytes >= w.total, "fold_chunk_sm100: a workspace of %lld bytes, %lld needed", static_cast<long long>(workspace_bytes),

@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_sm100_kernel(const Params p, 
 // loads, and the epilogue with nothing behind it) was half of its time. One CTA per SM walks the work items
 // in stride, and the next item's Q and first tiles are loaded, and its first scores issued, while the last
 // one's O is written. Barrier phases count key tiles and items since the CTA started.
-// Measured (D=128, 32 heads, 8 KV heads): 6 packed sequences of 16384 tokens in all, window 512: 240 us; 2 x 8192, window 1024,
+// Measured (D=128, 32 heads, 8 KV heads): 6 packed sequences of 16384 tokens in all, window 512: 250 us; 2 x 8192, window 1024,
 // 4 sinks: 360-390; chunks of 2 x 2048 behind 16384-24576 keys: 1660 (1.0 PFLOP/s). The tensor and the transcendental
 // pipe are busy 54 % of the time each: a tile's softmax waits for its scores and its product for the softmax, and two query
 // tiles a CTA cover one another in part. Taking the weights in one pass over the scores (the maximum found

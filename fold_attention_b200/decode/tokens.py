@@ -115,7 +115,7 @@ def _planes(D, ka, kb, va, vb, ek, dev):
 def _rows(t):
     """`t` with 16-byte rows the kernels can read in place, or a copy."""
     a, b, c = t.stride()
-    return t if c == 1 and not (a | b) & 7 and not t.data_ptr() & 15 else t.contiguous()
+    return t if c == 1 and not (a | b) & 7 and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
 
 
 def write_tokens(k, v, slots, page_size, ka, kb, va, vb, ek, *, v_scale=1.0):

@@ -46,7 +46,7 @@ def _windowed_input(x):
     dim, rows on 16-byte boundaries, and no axis that a broadcast gave stride 0."""
     st = x.stride()
     ok = st[-1] == 1 and all(s and s % 8 == 0 for s in st[:-1]) and x.data_ptr() % 16 == 0
-    return x if ok else x.contiguous()
+    return x if ok else x.clone(memory_format=torch.contiguous_format)
 
 
 class _FoldAttnFunc(torch.autograd.Function):
@@ -68,7 +68,7 @@ class _FoldAttnFunc(torch.autograd.Function):
         (dout,) = grad_outputs
         q, k, v, out, lse, rest = ctx.saved_tensors
         if ctx.window:
-            dq, dk, dv, status = window_backward(q, k, v, out, rest, dout.contiguous(), lse, ctx.window, ctx.sinks, ctx.softmax_scale)
+            dq, dk, dv, status = window_backward(q, k, v, out, rest, _windowed_input(dout), lse, ctx.window, ctx.sinks, ctx.softmax_scale)
             if check_status:
                 read_status(status.view(torch.int32), "fold_attn_func's backward")
             return dq, dk, dv, None, None, None, None
@@ -113,7 +113,7 @@ class _FoldAttnVarlenFunc(torch.autograd.Function):
         q, k, v, out, lse, cu_seqlens, rest = ctx.saved_tensors
         if ctx.window:
             dq, dk, dv, status = window_backward(
-                q, k, v, out, rest, dout.contiguous(), lse, ctx.window, ctx.sinks, ctx.softmax_scale, cu_seqlens, ctx.max_seqlen)
+                q, k, v, out, rest, _windowed_input(dout), lse, ctx.window, ctx.sinks, ctx.softmax_scale, cu_seqlens, ctx.max_seqlen)
             if check_status:
                 read_status(status.view(torch.int32), "fold_attn_varlen_func's backward")
             return dq, dk, dv, None, None, None, None, None, None

@@ -209,3 +209,20 @@ def test_tables_and_tokens_are_checked():
         a.update(bad)
         with pytest.raises(ValueError):
             decode.read_tokens(**a)
+
+
+@pytest.mark.parametrize("plane", range(4))
+def test_pool_planes_off_a_16_byte_boundary_are_refused(plane):
+    """Before anything is launched: the addresses are never read."""
+    from fold_attention_b200 import _lib
+    from fold_attention_b200.decode import tokens  # noqa: F401 (declares the entry points)
+
+    planes = [0x1000] * 4
+    planes[plane] += 8
+    with pytest.raises(ValueError, match="16-byte aligned"):
+        _lib.call("fold_write_tokens", 0x1000, 0x1000, 0, 128, 64, 128, 64, 0x1000, 3, 2, 64, 16, 64, *planes, 0x1000, 1.0, None)
+    with pytest.raises(ValueError, match="16-byte aligned"):
+        _lib.call("fold_read_tokens", 0x1000, 3, 2, 64, 16, 64, *planes, 0x1000, 1.0, 0x1000, 0x1000, 1, None)
+    with pytest.raises(ValueError, match="16-byte aligned"):
+        _lib.call("fold_chunk_gather", 0x1000, 0x1000, 2, 0x1000, 4, 16, 2, 64, 1 << 30, 0, *planes, 0x1000, 1.0, 0, 0, 2, 4,
+                  0x1000, 0x1000, 0x1000, 0x1000, 0x1000, None)

@@ -172,3 +172,23 @@ def test_a_slot_beyond_the_pool_is_no_place():
     kr, vr = decode.read_tokens(slots, page, HKV, ka, kb, va, None, ek)
     assert torch.equal(vr[0], k[0]) and not vr[1:].any() and not kr[1:].any()
     assert int((ek != 0).sum()) == HKV
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_tokens_off_a_16_byte_boundary(dtype):
+    from fold_attention_b200 import decode
+
+    HKV, D, page, n = 2, 64, 16, 5
+    k, v = (torch.randn(n, HKV, D, device="cuda").to(dtype) for _ in range(2))
+    slots, pools = dev32([3, 17, 0, 30, 9]), []
+    for shift in (0, 1):
+        ka, kb = (torch.zeros(2 * page * HKV, D, device="cuda", dtype=torch.int8) for _ in range(2))
+        va, ek = torch.zeros_like(ka, dtype=torch.bfloat16), torch.zeros(2 * page * HKV, device="cuda", dtype=torch.bfloat16)
+        ins = []
+        for x in (k, v):
+            flat = torch.empty(x.numel() + shift, device="cuda", dtype=dtype)
+            flat[shift:] = x.flatten()
+            ins.append(flat[shift:].view(x.shape))
+        decode.write_tokens(*ins, slots, page, ka, kb, va, None, ek)
+        pools.append((ka, kb, va, ek))
+    assert all(torch.equal(a, b) for a, b in zip(*pools))

@@ -329,3 +329,22 @@ def test_what_lies_behind_a_sequence_does_not_reach_it(window, sinks, D, where):
             bad = [t.clone() for t in clean]
             bad[n][live:] = value
             assert all(torch.equal(a[:live], b[:live]) for a, b in zip(want, run(*bad))), (n, value)
+
+
+@pytest.mark.parametrize("D", [128, 64])
+def test_tensors_off_a_16_byte_boundary(D):
+    import fold_attention_b200 as fa
+
+    S, H, HKV, window, sinks = 200, 4, 2, 50, 2
+    t = [x[None] for x in inputs(S, H, HKV, D, torch.bfloat16, seed=8)]
+    want = run_dense(*t, window, sinks)
+    off = []
+    for x in t:
+        flat = torch.empty(x.numel() + 1, device="cuda", dtype=x.dtype)
+        flat[1:] = x.flatten()
+        off.append(flat[1:].view(x.shape))
+        assert off[-1].data_ptr() % 16
+    x = [y.detach().requires_grad_() for y in off[:3]]
+    out = fa.fold_attn_func(*x, causal=True, window=window, sinks=sinks)
+    got = (out.detach(), *torch.autograd.grad(out, x, off[3]))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
