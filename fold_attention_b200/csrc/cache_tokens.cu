@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(CP_THREADS) chunk_plan_kernel(const int* __res
                 klen = -1;                     // another kernel's
             } else if (n > 0 && len > 0) {
                 klen = min(len, max_keys);
-                before = len - n - window;
+                before = klen - n - window;    // (of the keys that the table holds: the attention counts its queries back from klen)
                 const int low = max(0, before + 1) / 128;
                 shift = max(0, low - ns);
                 nt = max(0, (klen + 127) / 128 - shift);

@@ -417,12 +417,14 @@ class FoldKVCache:
         if sum(lens) == 0:
             return torch.empty_like(q)
         q = tokens._rows(q)
-        # a captured call is replayed on longer requests: it is laid out for the longest there can be
+        # a captured call is replayed on longer requests: it is laid out for the longest there can be, which is the
+        # table's end (a request replayed past max_len would otherwise push the others out of the layout)
+        room = self.page_table.shape[1] * self.page_size
         capturing = torch.cuda.is_current_stream_capturing()
         cap, st = [0, 0], -(-self.sinks // 128)
         for n, a in zip(lens, self.lens):
             if n:
-                end = self.max_len if capturing else a
+                end = room if capturing else a
                 tiles = -(-end // 128)
                 if self.window:      # the sinks' tiles and those its window can touch, wherever it stands
                     tiles = min(tiles, st + (n + self.window + 253) // 128)
