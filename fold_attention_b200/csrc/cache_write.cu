@@ -136,7 +136,9 @@ __global__ void __launch_bounds__(NT) prompt_write_kernel(
 // CTAs [0, nq) quantise query rows (RPB rows each); CTAs [nq, nq + batch)
 // append one request's token for all KV heads, then move its length. One CTA
 // owns a request, so the length is read by every thread before one moves it
-// and `lens_out` may alias `lens_in`.
+// and `lens_out` may alias `lens_in`. A token past the end of its request's row of the
+// table has no place: it is dropped and the length moves on, which is how the host
+// learns of replays that ran past the end (every reader stops at the table's end).
 template <int D, bool V8, bool F16>
 __global__ void __launch_bounds__(NT) step_kernel(
     const void* __restrict__ q, int q_rows, int8_t* qa, int8_t* qb, float* eq,
@@ -170,6 +172,11 @@ __global__ void __launch_bounds__(NT) step_kernel(
     }
     const int b = blockIdx.x - nq;
     const int pos = lens_in[b];
+    if (pos < 0 || pos >= table_keys(ppr, page_size)) {
+        __syncthreads();
+        if (threadIdx.x == 0) lens_out[b] = pos + 1;
+        return;
+    }
     const int pg = __ldg(page_table + static_cast<int64_t>(b) * ppr + pos / page_size);
     const int off = pos % page_size;
     const float ievs = __fdiv_rn(1.0f, evs);
@@ -229,7 +236,7 @@ __global__ void __launch_bounds__(NT) tail_append_kernel(
     __shared__ float sY[16];
     const int kr = blockIdx.x, b = kr / hkv, h = kr % hkv, tid = threadIdx.x;
     const int pos = lens[b] - back;
-    if (pos < 0 || pos >= ppr * page_size) return;      // no appended token at this length: touch nothing
+    if (pos < 0 || pos >= table_keys(ppr, page_size)) return;      // no appended token at this length: touch nothing
     const int pg = __ldg(page_table + static_cast<int64_t>(b) * ppr + pos / page_size);
     const int off = pos % page_size;
     const int64_t prow = (static_cast<int64_t>(pg) * hkv + h) * page_size + off;

@@ -138,6 +138,8 @@ __device__ __forceinline__ int dk_scale_exp(const int* stats, float rows, float 
     float s = __fadd_rn(__fmul_rn(dn, __fmul_rn(v, cd)), dl);
     return pow2_scale_exp(__fmul_rn(rows, __fmul_rn(s, __int_as_float(stats[ST_Q]))), DKV_BITS);
 }
+// the keys that one request's row of a page table has room for
+__device__ __forceinline__ int64_t table_keys(int ppr, int page_size) { return static_cast<int64_t>(ppr) * page_size; }
 __device__ __forceinline__ float pow2f(int e) { return __int_as_float((e + 127) << 23); }
 // x * 2^e for any e in [-250, 250] without leaving fp32's exponent range half way
 __device__ __forceinline__ float scale_pow2(float x, int e) {

@@ -164,7 +164,8 @@ __global__ void __launch_bounds__(DEC_THREADS) decode_kernel(const DecodeParams 
     const int bhk = EX ? bh / p.gsub : bh;             // the KV head's row group in the cache's numbering
     const int breq = bhk / p.hkv, hkv = bhk % p.hkv;
     const int preq = (EX && p.req_map) ? p.req_map[breq] : breq;
-    const int slen = p.seq_lens[preq];
+    // (a length replayed past the table's end: the tokens beyond were dropped)
+    const int slen = static_cast<int>(min(static_cast<int64_t>(p.seq_lens[preq]), table_keys(p.ppr, p.page_size)));
     const int G = p.G, PS = p.page_size;
 
     // this split's tiles: interleaved (tile sp, sp + split, ...) or a fixed chunk
@@ -716,7 +717,7 @@ __global__ void __launch_bounds__(DEC_THREADS) mass_z_kernel(
     __shared__ int sClass[MASS_ROWS];   // 0 unused, 1 exact, 2 sample
     const int bh = blockIdx.x, bhk = bh / gsub, h = bhk % hkv, tid = threadIdx.x;
     const int breq = req_map ? req_map[bhk / hkv] : bhk / hkv;   // the row of page_table / seq_lens this group reads
-    const int n = seq_lens[breq];
+    const int n = static_cast<int>(min(static_cast<int64_t>(seq_lens[breq]), table_keys(ppr, PS)));
     for (int i = tid; i < G * D / 4; i += DEC_THREADS) {
         reinterpret_cast<uint32_t*>(&sQ[0][0][0])[i] = reinterpret_cast<const uint32_t*>(qa + static_cast<int64_t>(bh) * G * D)[i];
         reinterpret_cast<uint32_t*>(&sQ[1][0][0])[i] = reinterpret_cast<const uint32_t*>(qb + static_cast<int64_t>(bh) * G * D)[i];

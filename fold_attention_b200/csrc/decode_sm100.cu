@@ -421,7 +421,8 @@ __device__ __forceinline__ void decode_sm100_body(const Params& p, const CUtenso
     const int slot = blockIdx.x / p.split, sp = blockIdx.x % p.split;
     const int bh = p.order ? p.order[slot] : slot;
     const int breq = bh / p.hkv, hkv = bh % p.hkv;
-    const int slen = p.seq_lens[breq];
+    // (a length replayed past the table's end: the tokens beyond were dropped)
+    const int slen = static_cast<int>(min(static_cast<int64_t>(p.seq_lens[breq]), table_keys(p.ppr, p.page_size)));
     const int G = GC ? GC : p.G, PS = p.page_size;
 
     int lo, hi, tstep, n_tiles;

@@ -125,7 +125,8 @@ int fold_cache_write_prompt(const void* k, const void* v, int is_f16, const int3
 
 /* One decode step's writes: query planes (q != NULL) and/or one appended
  * token per request (k, v != NULL) at position lens_in[b]; lens_out[b] =
- * lens_in[b] + 1 (lens_out may alias lens_in).
+ * lens_in[b] + 1 (lens_out may alias lens_in). A token at or past pages_per_request *
+ * page_size is dropped: its length moves, and the decode reads up to the table's end.
  * Replaces: src/fold_attention/decode/write.py:380-440 (step_kernel),
  * :565-673 (prepare_step) and the append half of decode/front.py:255-471.
  *   q (batch*n_heads, head_dim); k, v (batch, n_kv_heads, head_dim)
