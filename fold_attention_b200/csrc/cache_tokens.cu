@@ -245,17 +245,23 @@ __global__ void __launch_bounds__(NT) read_tokens_kernel(const int* __restrict__
 // ------------------------------------------------------------- the sums ----
 // A chunk's share of the running V sums and means, and the lengths moved: one CTA per (KV head,
 // request). Token i goes to slot i % 16 and the slots are added in order, so the sum depends on the
-// chunk alone.
+// chunk alone. With the tokens' places (`slots`), those without one do not count. They are a request's last
+// (pages are handed out in order); where a page was missing the length stops at the last key that has a place, so that no
+// reader meets a page that is not there, and past the table's end (`room` keys), where every reader stops, it moves on.
 template <int D, bool F16>
 __global__ void __launch_bounds__(16 * D / 4) chunk_sums_kernel(const uint16_t* __restrict__ v, int64_t v_st, int64_t v_sh, int hkv,
-                                                                const int* __restrict__ cu, int total, const int* __restrict__ lens_new,
-                                                                int* lens, float evs, float* vsum, float* vmean) {
+                                                                const int* __restrict__ cu, int total, const int* __restrict__ slots, int64_t room,
+                                                                const int* __restrict__ lens_new, int* lens, float evs, float* vsum, float* vmean) {
     constexpr int TPR = D / 4;
     __shared__ float s_part[16][D];
+    __shared__ int s_placed[16];
     const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x % TPR, slot = threadIdx.x / TPR;
     const int t0 = max(cu[b], 0), t1 = min(cu[b + 1], total);
     float s[4] = {0.f, 0.f, 0.f, 0.f};
+    int placed = 0;
     for (int t = t0 + slot; t < t1; t += 16) {
+        if (slots && __ldg(slots + t) < 0) continue;
+        ++placed;
         const uint2 w = __ldg(reinterpret_cast<const uint2*>(v + t * v_st + h * v_sh + lane * 4));
         s[0] = __fadd_rn(s[0], half_bits_to_float<F16>(static_cast<uint16_t>(w.x & 0xFFFF)));
         s[1] = __fadd_rn(s[1], half_bits_to_float<F16>(static_cast<uint16_t>(w.x >> 16)));
@@ -264,17 +270,26 @@ __global__ void __launch_bounds__(16 * D / 4) chunk_sums_kernel(const uint16_t* 
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) s_part[slot][lane * 4 + i] = s[i];
+    if (lane == 0) s_placed[slot] = placed;
     __syncthreads();
-    if (threadIdx.x < D && t1 > t0) {
+    int len = lens_new[b], keys = len;
+    placed = 0;
+    for (int i = 0; i < 16; ++i) placed += s_placed[i];
+    if (slots) {
+        const int n = cu[b + 1] - cu[b], before = len - n;
+        if (placed < n && before + placed < room) len = before + placed;
+        keys = static_cast<int>(min(static_cast<int64_t>(len), room));
+    }
+    if (threadIdx.x < D && placed > 0) {
         const int64_t at = (static_cast<int64_t>(b) * hkv + h) * D + threadIdx.x;
         float acc = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc = __fadd_rn(acc, s_part[i][threadIdx.x]);
         acc = __fadd_rn(vsum[at], acc);
         vsum[at] = acc;
-        vmean[at] = __fdiv_rn(acc, __fmul_rn(static_cast<float>(lens_new[b]), evs));
+        vmean[at] = __fdiv_rn(acc, __fmul_rn(static_cast<float>(keys), evs));
     }
-    if (h == 0 && threadIdx.x == 0) lens[b] = lens_new[b];
+    if (h == 0 && threadIdx.x == 0) lens[b] = len;
 }
 
 // ------------------------------------------- a chunk's keys, dequantised ----
@@ -472,6 +487,13 @@ extern "C" int fold_read_tokens(const int32_t* slots, int64_t total, int n_kv_he
 extern "C" int fold_chunk_sums(const void* v, int is_f16, int64_t v_token_stride, int64_t v_head_stride, int batch, int n_kv_heads, int head_dim,
                                const int32_t* cu_seqlens, int total, const int32_t* lens_new, int32_t* lens, float v_scale, float* vsum, float* vmean,
                                void* stream) {
+    return fold_chunk_sums_placed(v, is_f16, v_token_stride, v_head_stride, batch, n_kv_heads, head_dim, cu_seqlens, total, nullptr, 0, lens_new, lens,
+                                  v_scale, vsum, vmean, stream);
+}
+
+extern "C" int fold_chunk_sums_placed(const void* v, int is_f16, int64_t v_token_stride, int64_t v_head_stride, int batch, int n_kv_heads, int head_dim,
+                                      const int32_t* cu_seqlens, int total, const int32_t* slots, int64_t room, const int32_t* lens_new, int32_t* lens,
+                                      float v_scale, float* vsum, float* vmean, void* stream) {
     FOLD_CHECK_ARG(head_dim == 64 || head_dim == 128, "head_dim %d: the cache writers take 64 or 128", head_dim);
     FOLD_CHECK_ARG(cu_seqlens && lens_new && lens && vsum && vmean && (v || total == 0), "fold_chunk_sums: null pointer");
     FOLD_CHECK_ARG(batch > 0 && batch <= 65535 && n_kv_heads > 0 && total >= 0, "fold_chunk_sums: %d requests, %d heads", batch, n_kv_heads);
@@ -480,7 +502,7 @@ extern "C" int fold_chunk_sums(const void* v, int is_f16, int64_t v_token_stride
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const uint16_t* vp = static_cast<const uint16_t*>(v);
 #define FOLD_CS(DD, FF) \
-    chunk_sums_kernel<DD, FF><<<grid, 16 * DD / 4, 0, st>>>(vp, v_token_stride, v_head_stride, n_kv_heads, cu_seqlens, total, lens_new, lens, v_scale, vsum, vmean)
+    chunk_sums_kernel<DD, FF><<<grid, 16 * DD / 4, 0, st>>>(vp, v_token_stride, v_head_stride, n_kv_heads, cu_seqlens, total, slots, room, lens_new, lens, v_scale, vsum, vmean)
     if (head_dim == 64) { if (is_f16) FOLD_CS(64, true); else FOLD_CS(64, false); }
     else                { if (is_f16) FOLD_CS(128, true); else FOLD_CS(128, false); }
 #undef FOLD_CS

@@ -138,7 +138,9 @@ __global__ void __launch_bounds__(NT) prompt_write_kernel(
 // owns a request, so the length is read by every thread before one moves it
 // and `lens_out` may alias `lens_in`. A token past the end of its request's row of the
 // table has no place: it is dropped and the length moves on, which is how the host
-// learns of replays that ran past the end (every reader stops at the table's end).
+// learns of replays that ran past the end (every reader stops at the table's end). A
+// token whose page is negative has none either: the shared pool ran out (which the
+// count of its pages tells), and the length stays at the last key that has a place.
 template <int D, bool V8, bool F16>
 __global__ void __launch_bounds__(NT) step_kernel(
     const void* __restrict__ q, int q_rows, int8_t* qa, int8_t* qb, float* eq,
@@ -172,12 +174,13 @@ __global__ void __launch_bounds__(NT) step_kernel(
     }
     const int b = blockIdx.x - nq;
     const int pos = lens_in[b];
-    if (pos < 0 || pos >= table_keys(ppr, page_size)) {
+    const bool inside = pos >= 0 && pos < table_keys(ppr, page_size);
+    const int pg = inside ? __ldg(page_table + static_cast<int64_t>(b) * ppr + pos / page_size) : -1;
+    if (pg < 0) {
         __syncthreads();
-        if (threadIdx.x == 0) lens_out[b] = pos + 1;
+        if (threadIdx.x == 0) lens_out[b] = inside ? pos : pos + 1;
         return;
     }
-    const int pg = __ldg(page_table + static_cast<int64_t>(b) * ppr + pos / page_size);
     const int off = pos % page_size;
     const float ievs = __fdiv_rn(1.0f, evs);
     const float n = __fmul_rn(static_cast<float>(pos + 1), evs);
@@ -238,6 +241,7 @@ __global__ void __launch_bounds__(NT) tail_append_kernel(
     const int pos = lens[b] - back;
     if (pos < 0 || pos >= table_keys(ppr, page_size)) return;      // no appended token at this length: touch nothing
     const int pg = __ldg(page_table + static_cast<int64_t>(b) * ppr + pos / page_size);
+    if (pg < 0) return;
     const int off = pos % page_size;
     const int64_t prow = (static_cast<int64_t>(pg) * hkv + h) * page_size + off;
     const int64_t blk = prow / 64;

@@ -27,6 +27,7 @@ _lib.register("fold_build_tables", [P, P, I, P, I, I, I, P, I, P, P, P, P, P])
 _lib.register("fold_write_tokens", [P, P, I, L, L, L, L, P, L, I, I, I, L, P, P, P, P, P, F, P])
 _lib.register("fold_read_tokens", [P, L, I, I, I, L, P, P, P, P, P, F, P, P, I, P])
 _lib.register("fold_chunk_sums", [P, I, L, L, I, I, I, P, I, P, P, F, P, P, P])
+_lib.register("fold_chunk_sums_placed", [P, I, L, L, I, I, I, P, I, P, L, P, P, F, P, P, P])
 _lib.register("fold_chunk_gather", [P, P, I, P, I, I, I, I, I, I, P, P, P, P, P, F, I, I, I, I, P, P, P, P, P, P])
 _lib.register("fold_chunk_sm100", [P, L, L, P, L, L, I, P, P, I, I, I, I, I, P, I, I, L, P, P, P, P, P, F, I, I, I, I, P, L, P, P])
 _lib.register("fold_chunk_workspace_bytes", [I, I, I, I, I, I], L)
@@ -51,8 +52,11 @@ def build_tables(cu_seqlens, seq_lens, page_table, page_size, total, *, free_pag
     stands as it is. Returns `(slots, lens, taken)`: each new token's slot
     (int32 `(total,)`), the lengths with the new tokens, and the pages then in
     use (None without `free_pages`). A token that its request's table row or
-    the pool has no page for, and a row that no request covers, gets slot -1;
-    `taken` past the list's end says that the pool ran out. The arguments other
+    the pool has no page for, or whose page in the table is negative, and a row
+    that no request covers, gets slot -1; `taken` past the list's end says that
+    the pool ran out. The entry of a page that the pool could not give stands as
+    it was, and calls on the longer lengths read it: a table over a pool that may
+    run out starts as -1 throughout. The arguments other
     than the table are left as they are, so the same call gives the same
     answer. All tensors are int32 on one device; nothing waits on it.
     """
@@ -168,14 +172,15 @@ def read_tokens(slots, page_size, n_kv_heads, ka, kb, va, vb, ek, *, v_scale=1.0
     return k, v
 
 
-def chunk_sums(v, cu_seqlens, lens_new, seq_lens, v_scale, vsum, vmean):
-    """The running V sums and means with a chunk's `v` added, and `seq_lens` set to `lens_new`."""
+def chunk_sums(v, cu_seqlens, slots, room, lens_new, seq_lens, v_scale, vsum, vmean):
+    """The running V sums and means with a chunk's `v` added, and `seq_lens` set to `lens_new`: of the tokens
+    whose `slots` are a place, and up to the first page that is missing of the `room` keys in the table."""
     n, HKV, D = v.shape
     v = _rows(v)
     with _lib.on(v.device):
         _lib.call(
-            "fold_chunk_sums", v.data_ptr(), int(v.dtype == torch.float16), v.stride(0), v.stride(1), seq_lens.shape[0], HKV, D,
-            cu_seqlens.data_ptr(), n, lens_new.data_ptr(), seq_lens.data_ptr(), float(v_scale), vsum.data_ptr(), vmean.data_ptr(),
+            "fold_chunk_sums_placed", v.data_ptr(), int(v.dtype == torch.float16), v.stride(0), v.stride(1), seq_lens.shape[0], HKV, D,
+            cu_seqlens.data_ptr(), n, slots.data_ptr(), room, lens_new.data_ptr(), seq_lens.data_ptr(), float(v_scale), vsum.data_ptr(), vmean.data_ptr(),
             _lib.stream(v.device),
         )
 

@@ -160,7 +160,8 @@ class FoldKVCache:
             pool = int(pages)
             if pool < 1:
                 raise ValueError(f"a pool of {pages} pages")
-            self.page_table = torch.zeros((batch, per), device=dev, dtype=torch.int32)
+            # -1: no page yet, and what a token that the pool has no page for finds (it is dropped)
+            self.page_table = torch.full((batch, per), -1, device=dev, dtype=torch.int32)
             self.free_pages = torch.arange(pool, device=dev, dtype=torch.int32)
             self.taken = torch.zeros(1, device=dev, dtype=torch.int32)
         self.n_pages = pool
@@ -279,6 +280,7 @@ class FoldKVCache:
         self._check_pool(lens)
         if self.free_pages is not None:      # every page is free again: the prompts replace what there was
             fresh = torch.zeros_like(self.seq_lens)
+            self.page_table.fill_(-1)
             self._take_pages(self._cu(lens), fresh, 0, torch.zeros_like(self.taken))
         self._v_scale = write.write_prompt(
             k, v, lens, self.page_table, self.page_size, self.ka, self.kb, self.va, self.vb,
@@ -401,7 +403,8 @@ class FoldKVCache:
             return
         slots, lens_new = self._take_pages(cu_seqlens, self.seq_lens, total)
         tokens.write_tokens(k, v, slots, self.page_size, self.ka, self.kb, self.va, self.vb, self.ek, v_scale=self.v_scale)
-        tokens.chunk_sums(v, cu_seqlens, lens_new, self.seq_lens, self.v_scale, self.vsum, self.vmean)
+        tokens.chunk_sums(v, cu_seqlens, slots, self.page_table.shape[1] * self.page_size, lens_new, self.seq_lens, self.v_scale,
+                          self.vsum, self.vmean)
         self.lens = after
 
     def attend_chunk(self, q, cu_seqlens, lens=None):
@@ -441,7 +444,9 @@ class FoldKVCache:
         """Read the lengths back from the device. A captured step moves them there
         on every replay; the host's copy, which the next eager call plans by, does
         not follow by itself. Raises if the replays ran past `max_len` or the
-        shared pool: the tokens beyond either were dropped."""
+        shared pool: the tokens beyond either were dropped, and what the replays returned
+        for their requests from there on is not their attention. The others are
+        as they should be; the cache goes on from new prompts."""
         lens = self.seq_lens.tolist()
         if max(lens) > self.max_len:
             raise ValueError(f"a request was moved to {max(lens)} tokens, max_len={self.max_len}")
@@ -759,13 +764,16 @@ class FoldKVCache:
             raise ValueError(f"k and v are ({self.batch}, {self.n_kv_heads}, {self.head_dim})")
         if qf is not None and qf.shape[0] != self.batch * self.n_heads:
             raise ValueError(f"q is ({self.batch}, {self.n_heads}, {self.head_dim})")
+        # where the tail finds the token: behind the lengths that the step moves, or, as a shared pool's step may
+        # drop a token and leave its length, at the lengths it met
+        at = (self.seq_lens.clone(), 0) if k is not None and self.tail is not None and self.free_pages is not None else (self.seq_lens, 1)
         write.step(
             qf, k, v, self.qa.view(-1, self.head_dim), self.qb.view(-1, self.head_dim),
             self.eq.view(-1), self.ek, self.page_table, self.page_size, self.seq_lens,
             self.ka, self.kb, self.va, self.vb, self.v_scale, self.vsum, self.vmean, self.seq_lens,
         )
         if k is not None and self.tail is not None:
-            write.tail_append(v, self.tail, self.ka, self.ek, self.page_table, self.page_size, self.seq_lens, 1)
+            write.tail_append(v, self.tail, self.ka, self.ek, self.page_table, self.page_size, *at)
         if q is not None:
             mass_z(self.qa, self.qb, self.eq, self.ka, self.ek, self.page_table, self.page_size,
                    self.seq_lens, self.n_kv_heads, self.z)

@@ -44,9 +44,11 @@ int fold_abi_version(void);
  * and brings cu_seqlens[b + 1] - cu_seqlens[b] more. With free_pages (n_free page numbers, of which
  * the first *taken are in use) the pages it grows by are taken in request order and written to its
  * row of page_table; without, the table stands. slots[total] gets each new token's slot (-1 past the
- * table's end, where the pool ran out, and for rows no request covers), lens_out[b] the lengths
- * moved, *taken_out the pages then in use (beyond n_free: the pool ran out). The outputs are other
- * tensors than the inputs. */
+ * table's end, where the pool ran out, where the table holds a negative page, and for rows no request
+ * covers), lens_out[b] the lengths moved, *taken_out the pages then in use (beyond n_free: the pool ran
+ * out). The outputs are other tensors than the inputs. Where the pool ran out the entry stands as it was,
+ * and a later call that reads it takes it for the request's page: a table over a pool that may run out
+ * starts as -1 throughout. */
 int fold_build_tables(const int32_t* cu_seqlens, const int32_t* seq_lens, int batch, int32_t* page_table,
                       int pages_per_request, int page_size, int total, const int32_t* free_pages, int n_free,
                       const int32_t* taken, int32_t* slots, int32_t* lens_out, int32_t* taken_out, void* stream);
@@ -69,6 +71,14 @@ int fold_read_tokens(const int32_t* slots, int64_t total, int n_kv_heads, int he
 int fold_chunk_sums(const void* v, int is_f16, int64_t v_token_stride, int64_t v_head_stride, int batch,
                     int n_kv_heads, int head_dim, const int32_t* cu_seqlens, int total, const int32_t* lens_new,
                     int32_t* lens, float v_scale, float* vsum, float* vmean, void* stream);
+
+/* The same for tokens of which some may have found no place: those with a negative slot do not count,
+ * and a length stops at its last key that has a place, unless that is the table's end (`room` =
+ * pages_per_request * page_size keys): past it the length moves on, and every reader stops there. */
+int fold_chunk_sums_placed(const void* v, int is_f16, int64_t v_token_stride, int64_t v_head_stride, int batch,
+                           int n_kv_heads, int head_dim, const int32_t* cu_seqlens, int total, const int32_t* slots,
+                           int64_t room, const int32_t* lens_new, int32_t* lens, float v_scale, float* vsum, float* vmean,
+                           void* stream);
 
 /* The keys and values that the last cu_seqlens[b + 1] - cu_seqlens[b] tokens of each request can see,
  * as 16-bit rows for fold_fwd_window: whole tiles of 128 keys, requests one after another, zeros past
@@ -126,7 +136,8 @@ int fold_cache_write_prompt(const void* k, const void* v, int is_f16, const int3
 /* One decode step's writes: query planes (q != NULL) and/or one appended
  * token per request (k, v != NULL) at position lens_in[b]; lens_out[b] =
  * lens_in[b] + 1 (lens_out may alias lens_in). A token at or past pages_per_request *
- * page_size is dropped: its length moves, and the decode reads up to the table's end.
+ * page_size is dropped: its length moves, and the decode reads up to the table's end. So is one whose
+ * page is negative: its length stays.
  * Replaces: src/fold_attention/decode/write.py:380-440 (step_kernel),
  * :565-673 (prepare_step) and the append half of decode/front.py:255-471.
  *   q (batch*n_heads, head_dim); k, v (batch, n_kv_heads, head_dim)
