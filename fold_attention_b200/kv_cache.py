@@ -336,6 +336,7 @@ class FoldKVCache:
 
     def append(self, k, v):
         """Write one token per request, `(batch, H_KV, D)` each, at its length."""
+        self._check_step(None, k, v)
         self._room_for_one()
         self._step(None, k, v)
         self.lens = [x + 1 for x in self.lens]
@@ -344,16 +345,20 @@ class FoldKVCache:
         """Attention of `q` `(batch, H, D)` over the cache as it stands."""
         if self.window:
             return self._attend_last(q)
+        self._check_step(q, None, None)
         self._step(q, None, None)
         return self._run(q, split)
 
     def decode(self, q, k, v, split=None):
         """One decode step: append `k`, `v` `(batch, H_KV, D)` and attend with
         `q` `(batch, H, D)`."""
-        self._room_for_one()
         if self.window:
             if q.shape != (self.batch, self.n_heads, self.head_dim):
                 raise ValueError(f"q is ({self.batch}, {self.n_heads}, {self.head_dim})")
+            self._check_chunk_q(q, [1] * self.batch)
+        self._check_step(None if self.window else q, k, v)     # before a page is taken or anything is written
+        self._room_for_one()
+        if self.window:
             self._step(None, k, v)
             self.lens = [x + 1 for x in self.lens]
             return self._attend_last(q)
@@ -756,14 +761,18 @@ class FoldKVCache:
             )
         return self._launches[key]
 
+    def _check_step(self, q, k, v):
+        """A step's tensors, as `write.step` takes them."""
+        if k is not None and (k.shape != (self.batch, self.n_kv_heads, self.head_dim) or v.shape != k.shape):
+            raise ValueError(f"k and v are ({self.batch}, {self.n_kv_heads}, {self.head_dim})")
+        if q is not None and q.numel() != self.batch * self.n_heads * self.head_dim:
+            raise ValueError(f"q is ({self.batch}, {self.n_heads}, {self.head_dim})")
+        write.check_step(q, k, v, self.seq_lens.device)
+
     def _step(self, q, k, v):
         """The step's front: Q's planes, the appended token, then each row's
         reference Z from the cache as it now stands."""
         qf = None if q is None else q.reshape(-1, self.head_dim)
-        if k is not None and (k.shape != (self.batch, self.n_kv_heads, self.head_dim) or v.shape != k.shape):
-            raise ValueError(f"k and v are ({self.batch}, {self.n_kv_heads}, {self.head_dim})")
-        if qf is not None and qf.shape[0] != self.batch * self.n_heads:
-            raise ValueError(f"q is ({self.batch}, {self.n_heads}, {self.head_dim})")
         # where the tail finds the token: behind the lengths that the step moves, or, as a shared pool's step may
         # drop a token and leave its length, at the lengths it met
         at = (self.seq_lens.clone(), 0) if k is not None and self.tail is not None and self.free_pages is not None else (self.seq_lens, 1)

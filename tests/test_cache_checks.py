@@ -1,0 +1,33 @@
+"""What a cache refuses, it refuses before it takes a page, moves a length or writes a key."""
+
+import pytest
+import torch
+
+import fold_attention_b200 as fa
+
+BF = torch.bfloat16
+
+
+def cache(**kw):
+    """A cache on the CPU, whose kernels cannot run: a call that is not refused first fails in another way."""
+    return fa.FoldKVCache(2, 4, 2, 64, 96, page_size=16, device="cpu", **kw)
+
+
+def state(c):
+    return list(c.lens), c.seq_lens.tolist(), c.page_table.tolist(), None if c.taken is None else c.taken.tolist()
+
+
+@pytest.mark.parametrize("kw", [{}, dict(pages=7), dict(pages=7, window=8), dict(pages=7, depth=9.0, tail=None)])
+def test_a_refused_step_leaves_the_cache_as_it_was(kw):
+    c = cache(**kw)
+    before = state(c)       # empty: the first token of each request would take a page
+    q, k = torch.zeros(2, 4, 64, dtype=BF), torch.zeros(2, 2, 64, dtype=BF)
+    for bk, bv in ((k[:1], k), (k, k[:, :1]), (k[..., :32], k[..., :32]), (k, k.half()), (k.float(), k.float()), (k.to("meta"), k)):
+        with pytest.raises(ValueError, match="k and v|same type|is on"):
+            c.append(bk, bv)
+        with pytest.raises(ValueError, match="k and v|same type|is on"):
+            c.decode(q, bk, bv)
+    for bq in (q[:1], q[:, :2], q[..., :32], q.float(), q.to("meta")):
+        with pytest.raises(ValueError, match="q is|same type"):
+            c.decode(bq, k, k)
+    assert state(c) == before
