@@ -28,6 +28,16 @@ def chunk_table(lens):
     return torch.tensor(first + rows, dtype=torch.int32), len(rows) // 4
 
 
+def check_prompt(k, v, lens):
+    """What `write_prompt` reads by `lens` and as one 16-bit type."""
+    if k.dtype not in (torch.bfloat16, torch.float16) or v.dtype != k.dtype:
+        raise ValueError("k and v must be bf16 or fp16")
+    if v.shape != k.shape:
+        raise ValueError(f"k and v are of one shape (got {tuple(k.shape)}, {tuple(v.shape)})")
+    if sum(lens) != k.shape[0]:
+        raise ValueError(f"lens sum to {sum(lens)} but k holds {k.shape[0]} tokens")
+
+
 def write_prompt(
     k, v, lens, page_table, page_size, ka, kb, va, vb, ek, vsum, vmean, *, v_headroom, v_scale
 ):
@@ -35,11 +45,8 @@ def write_prompt(
     the paged cache, each key's scale into the pool `ek`, and each row
     group's V sum and mean. Returns V's scale as a one-element device tensor;
     nothing here waits on the device."""
-    total, HKV, D = k.shape
-    if k.dtype not in (torch.bfloat16, torch.float16) or v.dtype != k.dtype:
-        raise ValueError("k and v must be bf16 or fp16")
-    if sum(lens) != total:
-        raise ValueError(f"lens sum to {sum(lens)} but k holds {total} tokens")
+    check_prompt(k, v, lens)
+    _, HKV, D = k.shape
     k, v = k.contiguous(), v.contiguous()
     dev = k.device
     meta, nc = chunk_table(lens)

@@ -277,6 +277,12 @@ class FoldKVCache:
             raise ValueError(f"{len(lens)} prompts for a batch of {self.batch}")
         if min(lens) < 1 or max(lens) > self.max_len:
             raise ValueError(f"prompt lengths {min(lens)}..{max(lens)} are not in 1..{self.max_len}")
+        # all of it before the pages are handed out anew: a refused prompt leaves the cache as it was
+        if k.ndim != 3 or k.shape[1:] != (self.n_kv_heads, self.head_dim) or v.shape != k.shape:
+            raise ValueError(f"k and v are (total, {self.n_kv_heads}, {self.head_dim}) (got {tuple(k.shape)}, {tuple(v.shape)})")
+        if k.device != self.seq_lens.device or v.device != self.seq_lens.device:
+            raise ValueError(f"k and v are on {k.device} and {v.device}, the cache on {self.seq_lens.device}")
+        write.check_prompt(k, v, lens)
         self._check_pool(lens)
         if self.free_pages is not None:      # every page is free again: the prompts replace what there was
             fresh = torch.zeros_like(self.seq_lens)

@@ -31,3 +31,23 @@ def test_a_refused_step_leaves_the_cache_as_it_was(kw):
         with pytest.raises(ValueError, match="q is|same type"):
             c.decode(bq, k, k)
     assert state(c) == before
+
+
+@pytest.mark.parametrize("kw", [{}, dict(pages=7), dict(pages=7, v8=True), dict(pages=7, window=8)])
+def test_a_refused_prompt_leaves_the_cache_as_it_was(kw):
+    c = cache(**kw)
+    before = state(c)
+    k, cu = torch.zeros(5, 2, 64, dtype=BF), torch.tensor([0, 3, 5], dtype=torch.int32)
+    for bk, bv, lens, match in (
+        (k, k[:4], [3, 2], "k and v"), (k, k[..., :32], [3, 2], "k and v"), (k[:, :1], k[:, :1], [3, 2], "k and v"),
+        (k.flatten(), k.flatten(), [3, 2], "k and v"), (k, k.half(), [3, 2], "bf16 or fp16"), (k.float(), k.float(), [3, 2], "bf16 or fp16"),
+        (k, k, [3, 3], "lens sum to 6"), (k, k, [5], "batch of 2"), (k, k, [5, 0], "not in 1..96"), (k, k, [97, 1], "not in 1..96"),
+        (k.to("meta"), k, [3, 2], "k and v are on"),
+    ):
+        with pytest.raises(ValueError, match=match):
+            c.write_prompt(bk, bv, cu, lens)
+    if c.taken is not None:
+        long = torch.zeros(120, 2, 64, dtype=BF)
+        with pytest.raises(ValueError, match="pool has 7"):
+            c.write_prompt(long, long, cu, [60, 60])
+    assert state(c) == before
