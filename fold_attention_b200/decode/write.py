@@ -5,6 +5,8 @@ mirrors `write_prompt` and `step` of the reference
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from .. import _lib
@@ -62,6 +64,20 @@ def write_prompt(
         float(v_headroom), vfix, _lib.stream(dev),
     )
     return scratch[-1:]
+
+
+def v_scale_for(v, headroom):
+    """The scale a prompt of these values would set: the least power of two at or
+    above their largest magnitude times `headroom` / 448 (NaN aside), in the prompt
+    kernel's fp32 steps; None for zeros. Waits for the device."""
+    top = torch.where(v.isnan(), 0, v.abs()).amax().float().cpu()
+    if not torch.isfinite(top):
+        raise ValueError("v holds an infinity: no 8-bit scale fits it")
+    if top == 0:
+        return None
+    t = (top * torch.tensor(headroom, dtype=torch.float32)) * torch.tensor(1.0 / 448.0, dtype=torch.float32)
+    m, e = math.frexp(max(float(t), 1e-30))      # t = m 2^e with m in [1/2, 1)
+    return math.ldexp(1.0, e - 1 if m == 0.5 else e)
 
 
 def check_step(q, k, v, device):

@@ -52,7 +52,7 @@ class FoldKVCache:
     keeps every key. The reference is each row's log-sum-exp, estimated every
     step from the cache and the step's query alone. `v8` stores V as two e4m3
     planes rather than bf16 under one power-of-two scale: `v_scale` if given,
-    otherwise set by the prefill from the batch's largest value.
+    otherwise set by the prefill (or the first chunk) from the batch's largest value.
     `refine_k`, `refine_v` and `weight_terms` trade accuracy for time and
     default to the reference's gates. `split` fixes the CTAs per row group and
     `chunk` the keys per split (a multiple of 64); with either, a request's
@@ -179,6 +179,7 @@ class FoldKVCache:
             raise ValueError(f"v_scale={v_scale} is not a power of two")
         self._fixed_v_scale = v_scale
         self._v_scale = float(v_scale) if (self.v8 and v_scale is not None) else 1.0
+        self._v_unset = self.v8 and v_scale is None      # until a prompt or a chunk has set it
         self.seq_lens = torch.zeros((batch,), device=dev, dtype=torch.int32)
         self.lens = [0] * batch
         self.order = torch.arange(self.n_groups * self._gsub, device=dev, dtype=torch.int32)
@@ -293,6 +294,7 @@ class FoldKVCache:
             self.ek, self.vsum, self.vmean, v_headroom=self.v_headroom,
             v_scale=self._fixed_v_scale if self.v8 else None,
         )
+        self._v_unset = False
         self.seq_lens.copy_(torch.tensor(lens, dtype=torch.int32), non_blocking=True)
         self.lens = list(lens)
         if self.tail is not None:
@@ -396,7 +398,9 @@ class FoldKVCache:
     def append_chunk(self, k, v, cu_seqlens, lens=None):
         """`extend`'s first half: the new tokens quantised into the cache, in the
         format of a prompt's, and the lengths moved. An 8-bit V keeps the scale
-        of the prompt, or the one the cache was given."""
+        of the prompt, or the one the cache was given; without either the first chunk
+        whose V is not all zeros sets it as a prompt would, which waits for the
+        device once and cannot be captured."""
         lens = self._chunk_lens(cu_seqlens, lens)
         total = sum(lens)
         shape = (total, self.n_kv_heads, self.head_dim)
@@ -412,11 +416,22 @@ class FoldKVCache:
         self._check_pool(after)
         if total == 0:
             return
+        if self._v_unset:
+            self._fit_v_scale(v)
         slots, lens_new = self._take_pages(cu_seqlens, self.seq_lens, total)
         tokens.write_tokens(k, v, slots, self.page_size, self.ka, self.kb, self.va, self.vb, self.ek, v_scale=self.v_scale)
         tokens.chunk_sums(v, cu_seqlens, slots, self.page_table.shape[1] * self.page_size, lens_new, self.seq_lens, self.v_scale,
                           self.vsum, self.vmean)
         self.lens = after
+
+    def _fit_v_scale(self, v):
+        """V's scale from the first chunk. (Zeros are stored alike at any scale, so they leave it open.)"""
+        if v.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise ValueError("the first chunk of an 8-bit V sets its scale, which the host reads: not in a capture (or give v_scale)")
+        scale = write.v_scale_for(v, self.v_headroom)
+        if scale is not None:
+            self._v_scale, self._v_unset = scale, False
+            self._launches.clear()
 
     def attend_chunk(self, q, cu_seqlens, lens=None):
         """`extend`'s second half: attention of the last tokens of each request,
@@ -782,6 +797,8 @@ class FoldKVCache:
         # where the tail finds the token: behind the lengths that the step moves, or, as a shared pool's step may
         # drop a token and leave its length, at the lengths it met
         at = (self.seq_lens.clone(), 0) if k is not None and self.tail is not None and self.free_pages is not None else (self.seq_lens, 1)
+        if k is not None:
+            self._v_unset = False
         write.step(
             qf, k, v, self.qa.view(-1, self.head_dim), self.qb.view(-1, self.head_dim),
             self.eq.view(-1), self.ek, self.page_table, self.page_size, self.seq_lens,

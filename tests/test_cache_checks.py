@@ -51,3 +51,14 @@ def test_a_refused_prompt_leaves_the_cache_as_it_was(kw):
         with pytest.raises(ValueError, match="pool has 7"):
             c.write_prompt(long, long, cu, [60, 60])
     assert state(c) == before
+
+
+def test_an_8_bit_scale_that_chunks_set():
+    from fold_attention_b200.decode.write import v_scale_for
+
+    v = torch.tensor([[1.0, -3.5, float("nan")]], dtype=BF)
+    assert v_scale_for(v, 2.0) == 2.0 ** -6                       # 7 / 448 is a power of two itself
+    assert v_scale_for(v * 1.01, 2.0) == 2.0 ** -5
+    assert v_scale_for(v * 0, 2.0) is None
+    with pytest.raises(ValueError, match="infinity"):
+        v_scale_for(v * float("inf"), 2.0)

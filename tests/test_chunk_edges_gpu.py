@@ -1,0 +1,53 @@
+"""Chunks over the cache where they can go wrong: an 8-bit V's scale, NaN, what a request is batched with."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from test_chunk_gpu import Story, close, cumulative, make  # noqa: E402
+
+
+@pytest.mark.parametrize("size", [1e-3, 1.0, 3e3])
+@pytest.mark.parametrize("D", [64, 128])
+def test_pieces_of_a_prompt_set_the_8_bit_scale_that_the_prompt_would(size, D):
+    """An empty 8-bit cache without v_scale, filled by chunks. With a power of two above V's largest value a plane's
+    rounding is half a step of e4m3 (2^-4 of the value) and the second plane's 2^-4 of that remainder, 2^-8 in all, down to
+    values 2^-9 of the scale's unit, of which a normal V this size has few: the norm is within 2^-8."""
+    import fold_attention_b200 as fa
+    from fold_attention_b200 import decode
+
+    g = torch.Generator(device="cuda").manual_seed(4)
+    n = [200, 1, 77]
+    k, v = make(n, 2, D, torch.bfloat16, g), make(n, 2, D, torch.bfloat16, g, scale=size)
+    a, b = (fa.FoldKVCache(3, 4, 2, D, 300, v8=True, page_size=64) for _ in range(2))
+    a.write_prompt(k, v, cumulative(n), n)
+    zeros = torch.zeros(1, 2, D, device="cuda", dtype=torch.bfloat16)
+    b.append_chunk(zeros, zeros, cumulative([0, 1, 0]), [0, 1, 0])          # zeros say nothing about the scale
+    at = [0, 200, 201]
+    first = torch.cat([torch.arange(at[0], 200), torch.arange(at[2], 278)]).cuda()
+    b.append_chunk(k[first], v[first], cumulative([200, 0, 77]), [200, 0, 77])
+    assert b.v_scale == decode.write.v_scale_for(v[first], 2.0)
+    assert a.v_scale == decode.write.v_scale_for(v, 2.0)
+    slots = (b.page_table[0, torch.arange(200, device="cuda") // 64] * 64 + torch.arange(200, device="cuda") % 64).int()
+    _, back = decode.read_tokens(slots, 64, 2, b.ka, b.kb, b.va, b.vb, b.ek, v_scale=b.v_scale, dtype=torch.float32)
+    assert (back.double() - v[:200].double()).norm() <= 2.0 ** -8 * v[:200].double().norm()
+    kept = b.v_scale                                                           # and later chunks keep it
+    b.append_chunk(k[:3], v[:3] * 0.01, cumulative([1, 1, 1]), [1, 1, 1])
+    assert b.v_scale == kept
+
+
+def test_a_captured_first_chunk_of_an_8_bit_cache_is_refused():
+    import fold_attention_b200 as fa
+
+    c = fa.FoldKVCache(1, 4, 2, 64, 64, v8=True, page_size=16, pages=4)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    q, k, v = (make([3], h, 64, torch.bfloat16, g) for h in (4, 2, 2))
+    cu, graph, side = cumulative([3]), torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError, match="v_scale"):
+        with torch.cuda.stream(side):
+            with torch.cuda.graph(graph, stream=side):
+                c.extend(q, k, v, cu, [3])
+    assert c.lens == [0] and c.seq_lens.tolist() == [0] and c.taken.tolist() == [0]
+    c.extend(q, k, v, cu, [3])
