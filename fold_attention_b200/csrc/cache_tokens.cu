@@ -169,6 +169,12 @@ __device__ __forceinline__ void load_row(const Planes& p, int64_t prow, int off,
 
 enum { OUT_F32 = 0, OUT_BF16 = 1, OUT_F16 = 2 };
 
+__device__ __forceinline__ float to_f16_range(float x) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-65504.f));
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(65504.f));
+    return x;
+}
+
 template <int OUT>
 __device__ __forceinline__ void store16(void* base, int64_t at, const float (&x)[16]) {
     if constexpr (OUT == OUT_F32) {
@@ -180,8 +186,8 @@ __device__ __forceinline__ void store16(void* base, int64_t at, const float (&x)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             if constexpr (OUT == OUT_BF16) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
-            // the pool holds bf16's range: fp16 takes what it can
-            else w[i] = pack_f16x2(fminf(fmaxf(x[2 * i], -65504.f), 65504.f), fminf(fmaxf(x[2 * i + 1], -65504.f), 65504.f));
+            // the pool holds bf16's range: fp16 takes what it can, and a NaN stays one
+            else w[i] = pack_f16x2(to_f16_range(x[2 * i]), to_f16_range(x[2 * i + 1]));
         }
         uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + at);
         d[0] = make_uint4(w[0], w[1], w[2], w[3]);

@@ -335,7 +335,8 @@ __global__ void __launch_bounds__(NT) chunk_q_kernel(const Params p, int heads, 
         const int64_t unit = at * D + ((lane ^ (D == 128 ? r & 7 : (r >> 1) & 3)) << 4);
         *reinterpret_cast<uint4*>(p.qa + unit) = wa;
         *reinterpret_cast<uint4*>(p.qb + unit) = wb;
-        if (lane == 0) p.eq[at] = e * 0.00390625f;
+        // codes hold neither NaN nor infinity: the row's scale does (the rotation has spread a NaN over the row)
+        if (lane == 0) p.eq[at] = x[0] == x[0] && e < INFINITY ? e * 0.00390625f : NAN;
     }
 }
 

@@ -438,7 +438,9 @@ class FoldKVCache:
         which the cache already holds, over the cache. `q` `(total, H, D)` packed by
         `cu_seqlens`, as many rows of a request as it has tokens at most. Every
         key counts in full, whatever the cache's `depth`: both planes of K and of
-        an 8-bit V. fp16 queries see K and V saturated to fp16's range."""
+        an 8-bit V. fp16 queries of more than 128 rows a KV head see K and V saturated to
+        fp16's range. A row whose query holds a NaN or an infinity gives NaN, and so does one
+        that sees a NaN in a bf16 V; a key's codes, and an 8-bit V's, hold none."""
         lens = self._chunk_lens(cu_seqlens, lens)
         self._check_chunk_q(q, lens)
         if any(map(operator.gt, lens, self.lens)):

@@ -51,3 +51,47 @@ def test_a_captured_first_chunk_of_an_8_bit_cache_is_refused():
                 c.extend(q, k, v, cu, [3])
     assert c.lens == [0] and c.seq_lens.tolist() == [0] and c.taken.tolist() == [0]
     c.extend(q, k, v, cu, [3])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_nan_in_v_stays_one_in_fp16(D):
+    import fold_attention_b200 as fa
+    from fold_attention_b200 import decode
+
+    dt, g = torch.float16, torch.Generator(device="cuda").manual_seed(4)
+    c = fa.FoldKVCache(1, 2, 2, D, 640, page_size=16)
+    q, k, v = (make([300], 2, D, dt, g) for _ in range(3))
+    v[7] = float("nan")
+    out = c.extend(q, k, v, cumulative([300]), [300])              # more than 128 rows: dequantised to fp16
+    assert torch.isnan(out[8:]).all()
+    assert torch.isnan(c.attend_chunk(q[-2:], cumulative([2]), [2])).all()
+    slots = torch.tensor([6, 7], device="cuda", dtype=torch.int32)
+    for t in (torch.float16, torch.bfloat16, torch.float32):
+        _, back = decode.read_tokens(slots, 16, 2, c.ka, c.kb, c.va, c.vb, c.ek, dtype=t)
+        assert torch.isnan(back[1]).all() and torch.isfinite(back[0]).all()
+    c.va.fill_(1e30)                                               # beyond fp16: the largest it has
+    c.va[0] = -1e30
+    _, back = decode.read_tokens(slots - 6, 16, 2, c.ka, c.kb, c.va, c.vb, c.ek, dtype=torch.float16)
+    assert (back[1] == 65504).all() and (back[0, 0] == -65504).all()
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("v8", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_query_that_is_no_number_gives_none(value, v8, dtype):
+    """In the short chunks' kernel as in the long ones': the row alone, and nothing beside it."""
+    import fold_attention_b200 as fa
+
+    g = torch.Generator(device="cuda").manual_seed(4)
+    c = fa.FoldKVCache(2, 8, 2, 128, 2000, page_size=64, v8=v8, v_scale=0.25 if v8 else None)
+    n = [1500, 200]
+    c.append_chunk(*(make(n, 2, 128, dtype, g) for _ in range(2)), cumulative(n), n)
+    for rows in ([3, 1], [20, 30], [200, 150]):
+        q = make(rows, 8, 128, dtype, g)
+        want = c.attend_chunk(q, cumulative(rows), rows)
+        bad = q.clone()
+        bad[rows[0] - 1, 5, 17] = value
+        got = c.attend_chunk(bad, cumulative(rows), rows)
+        assert torch.isnan(got[rows[0] - 1, 5]).all()
+        got[rows[0] - 1, 5] = want[rows[0] - 1, 5]
+        assert torch.equal(got, want), rows
