@@ -56,7 +56,8 @@ class FoldKVCache:
     `refine_k`, `refine_v` and `weight_terms` trade accuracy for time and
     default to the reference's gates. `split` fixes the CTAs per row group and
     `chunk` the keys per split (a multiple of 64); with either, a request's
-    output depends on the request alone.
+    output of `decode` and `attend` depends on the request alone. (Chunks of new
+    tokens are cut by the batch: see `attend_chunk`.)
 
     `kernel` (not a reference argument) picks the split-KV kernel: "mma" is
     the warp-level one, which takes every shape; "sm100" the tcgen05 one
@@ -85,7 +86,9 @@ class FoldKVCache:
     `window` and `sinks` (not reference arguments) make it a sliding-window
     layer's cache: a token at position i attends keys j with `i - window < j <= i`
     or `j < sinks`, in `prefill`, `extend` and `decode` alike. Every key it sees
-    counts (`depth=None`), and its step runs the chunk's kernels. `pages` is
+    counts (`depth=None`), in full, and its step runs the chunk's kernels: `split` and
+    `chunk` are refused, and `kernel`, `refine_k`, `refine_v` and `weight_terms`,
+    which are the other decode's, have no say. `pages` is
     the size of a pool that the requests share: pages are handed out on the
     device as requests grow, instead of `max_len` keys' worth to each.
     """
@@ -134,6 +137,8 @@ class FoldKVCache:
         self.window = window or None
         if window and depth is not None:
             raise NotImplementedError("a windowed cache attends every key its window holds: depth=None")
+        if window and (split is not None or chunk is not None):
+            raise NotImplementedError("split and chunk cut the decode's keys: a windowed cache's step is attend_chunk's, cut by the batch")
         # the split-KV kernel (not a reference argument): "mma", "sm100" or "auto"
         self.kernel = kernel
         self.mix_kernels = False
@@ -352,6 +357,7 @@ class FoldKVCache:
     def attend(self, q, split=None):
         """Attention of `q` `(batch, H, D)` over the cache as it stands."""
         if self.window:
+            self._no_split(split)
             return self._attend_last(q)
         self._check_step(q, None, None)
         self._step(q, None, None)
@@ -361,6 +367,7 @@ class FoldKVCache:
         """One decode step: append `k`, `v` `(batch, H_KV, D)` and attend with
         `q` `(batch, H, D)`."""
         if self.window:
+            self._no_split(split)
             if q.shape != (self.batch, self.n_heads, self.head_dim):
                 raise ValueError(f"q is ({self.batch}, {self.n_heads}, {self.head_dim})")
             self._check_chunk_q(q, [1] * self.batch)
@@ -686,6 +693,10 @@ class FoldKVCache:
     def _no_window(self, what):
         if self.window:
             raise NotImplementedError(f"{what} runs the decode over whole requests: a windowed cache's step is attend_chunk's")
+
+    def _no_split(self, split):
+        if split is not None:
+            raise NotImplementedError("split cuts the decode's keys: a windowed cache's step is attend_chunk's, cut by the batch")
 
     def _set_order(self):
         """Which row group each grid slot takes; it changes no bit. Without a

@@ -62,3 +62,14 @@ def test_an_8_bit_scale_that_chunks_set():
     assert v_scale_for(v * 0, 2.0) is None
     with pytest.raises(ValueError, match="infinity"):
         v_scale_for(v * float("inf"), 2.0)
+
+
+def test_a_windowed_cache_refuses_the_splits_it_would_not_keep():
+    for kw in (dict(split=2), dict(chunk=64)):
+        with pytest.raises(NotImplementedError, match="windowed"):
+            cache(window=8, **kw)
+    c, q, k = cache(window=8), torch.zeros(2, 4, 64, dtype=BF), torch.zeros(2, 2, 64, dtype=BF)
+    for call in (lambda: c.attend(q, split=2), lambda: c.decode(q, k, k, split=2)):
+        with pytest.raises(NotImplementedError, match="windowed"):
+            call()
+    assert state(c)[0] == [0, 0]
