@@ -195,7 +195,8 @@ SHORT_ROWS = 128     # new tokens x query heads a KV head that chunk_sm100.cu ta
 
 # Where a batch holds wider requests too, its short ones get the second kernel only if that many 128-key tiles
 # (x KV heads) pay for it: nine requests of up to 1500 keys and two KV heads take 57 us dequantised together and 97 with
-# both kernels; a decode batch's long contexts read from the codes at a third of the bytes.
+# both kernels; a decode batch's long contexts read from the codes at a third of the bytes. It is a rule on the batch: a short
+# request's keys are exact from the codes in one batch and rounded to q's 16 bits in another.
 MIXED_TILES = 1024
 
 

@@ -445,7 +445,13 @@ class FoldKVCache:
         which the cache already holds, over the cache. `q` `(total, H, D)` packed by
         `cu_seqlens`, as many rows of a request as it has tokens at most. Every
         key counts in full, whatever the cache's `depth`: both planes of K and of
-        an 8-bit V. fp16 queries of more than 128 rows a KV head see K and V saturated to
+        an 8-bit V.
+
+        The same call gives the same bits. A request's bits are its batch's, though: where its
+        keys are cut is a matter of the whole batch, and so is, for a request of up to
+        128 query rows a KV head, whether it is attended from the codes or with
+        the wider ones, whose keys are rounded to q's type first (`decode/tokens.py`,
+        `MIXED_TILES`). The difference is within the rounding of 16 bits. fp16 queries of more than 128 rows a KV head see K and V saturated to
         fp16's range. A row whose query holds a NaN or an infinity gives NaN, and so does one
         that sees a NaN in a bf16 V; a key's codes, and an 8-bit V's, hold none."""
         lens = self._chunk_lens(cu_seqlens, lens)

@@ -95,3 +95,14 @@ def test_a_query_that_is_no_number_gives_none(value, v8, dtype):
         assert torch.isnan(got[rows[0] - 1, 5]).all()
         got[rows[0] - 1, 5] = want[rows[0] - 1, 5]
         assert torch.equal(got, want), rows
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_short_request_is_as_right_beside_a_wide_one(D, dtype):
+    """Alone it is attended from the codes, beside a wide one or among many its keys may be rounded or cut
+    elsewhere: other bits, within the same tolerance."""
+    for others in ([], [600], [600, 3, 1], [2] * 40):
+        st = Story(1 + len(others), 8, 2, D, 1600, dtype=dtype, page_size=64, v8=True, seed=D)
+        st.extend([901] + [max(n, 30) for n in others])
+        st.extend([3] + others)
