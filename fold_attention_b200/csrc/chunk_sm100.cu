@@ -233,7 +233,7 @@ __device__ __forceinline__ Geo geo_of(const Params& p, int b) {
     Geo g;
     const int t0 = __ldg(p.cu + b), t1 = __ldg(p.cu + b + 1);
     g.tok0 = t0;
-    g.n = t0 < 0 || t1 > p.total ? 0 : t1 - t0;
+    g.n = t0 < 0 || t1 > p.total ? -1 : t1 - t0;     // (negative: counts that q has no rows for)
     g.L = max(0, min(__ldg(p.lens + b), p.max_keys));
     g.first = g.L - g.n;                       // position of the first new token
     const int ns = (p.sinks + BN - 1) / BN;
@@ -405,7 +405,7 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
                 if (b < p.batch) {
                     mg = geo_of(p, b);
                     mine = mg.nt ? static_cast<int64_t>(mg.nt + ITEM_TILES) * p.hkv : 0;
-                    if (mg.wide && !p.others) atomicExch(p.status, FOLD_ERR_ARGUMENT);   // counts the host did not plan for
+                    if (mg.n < 0 || (mg.wide && !p.others)) atomicExch(p.status, FOLD_ERR_ARGUMENT);   // counts the host did not plan for
                 }
             }
             int x = static_cast<int>(mine);      // (a request's places fit 31 bits: 2^30 keys are 2^23 tiles, of 128 heads)

@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(KIND == KIND_CHUNK ? 256 : 128) fwd_mma_kernel
     int klen = len, qoff = 0, kstart = start, kshift = 0;   // keys, and the first query's position among them
     if constexpr (KIND == KIND_CHUNK) {
         const int4 pl = p.plan[b];
-        if (pl.x < 0) return;   // another kernel's
+        if (pl.x < 0 || start < 0 || len > p.total - start) return;   // another kernel's, or counts that q has no rows for
         klen = pl.x;
         qoff = klen - len;
         kstart = pl.y;

@@ -519,6 +519,10 @@ __device__ __forceinline__ bool load_item(const Params& p, const List& l, int i,
     if (w.m0 < 0) return false;
     w.m0 += second * BM;
     if (w.m0 >= w.len) return false;
+    if (p.plan && (w.start < 0 || w.len > p.total - w.start)) {   // counts that q has no rows for
+        atomicExch(p.status, FOLD_ERR_ARGUMENT);
+        return false;
+    }
     w.klen = w.len;
     w.qoff = w.kshift = 0;
     w.kstart = w.start;

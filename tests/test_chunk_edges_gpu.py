@@ -106,3 +106,25 @@ def test_a_short_request_is_as_right_beside_a_wide_one(D, dtype):
         st = Story(1 + len(others), 8, 2, D, 1600, dtype=dtype, page_size=64, v8=True, seed=D)
         st.extend([901] + [max(n, 30) for n in others])
         st.extend([3] + others)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("counts,lens", [([1, 260], [1, 200]), ([3, 9], [3, 4]), ([40, 5], [40, 2])])
+def test_counts_that_q_has_no_rows_for_touch_no_row(D, counts, lens):
+    """cu_seqlens says more than the host's counts and q's rows: the request is left alone, the others are answered,
+    and where the kernel has a status word it is raised."""
+    st = Story(2, 8, 2, D, 600, page_size=64, seed=2)
+    st.extend([90, 300])
+    q, k, v = st.tokens(lens)
+    st.c.append_chunk(k, v, cumulative(lens), lens)
+    room = torch.zeros(sum(counts) + 8, 8, D, device="cuda", dtype=st.dt)          # (what lies behind q is this test's)
+    room[:sum(lens)] = q
+    out = st.c.attend_chunk(room[:sum(lens)], cumulative(counts), lens)
+    close(out[:lens[0]], st.want(q, lens)[:lens[0]], st.dt)
+    if D == 128 or max(lens) <= 32:
+        assert st.c._chunk_status.item() == 1
+        st.c.check_status = True
+        from fold_attention_b200._lib import FoldLibraryError
+
+        with pytest.raises(FoldLibraryError):
+            st.c.attend_chunk(room[:sum(lens)], cumulative(counts), lens)
