@@ -56,13 +56,14 @@ def write_prompt(
     scratch = torch.empty(nc * HKV * (D + 1) + 1, device=dev, dtype=torch.float32)
     v8 = vb is not None
     vfix = (float(v_scale) if v_scale is not None else 0.0) if v8 else 1.0
-    _lib.call(
-        "fold_cache_write_prompt", k.data_ptr(), v.data_ptr(), int(k.dtype == torch.float16),
-        meta.data_ptr(), nc, len(lens), page_table.data_ptr(), page_table.shape[1],
-        int(page_size), HKV, D, ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb),
-        ek.data_ptr(), vsum.data_ptr(), vmean.data_ptr(), scratch.data_ptr(),
-        float(v_headroom), vfix, _lib.stream(dev),
-    )
+    with _lib.on(dev):
+        _lib.call(
+            "fold_cache_write_prompt", k.data_ptr(), v.data_ptr(), int(k.dtype == torch.float16),
+            meta.data_ptr(), nc, len(lens), page_table.data_ptr(), page_table.shape[1],
+            int(page_size), HKV, D, ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb),
+            ek.data_ptr(), vsum.data_ptr(), vmean.data_ptr(), scratch.data_ptr(),
+            float(v_headroom), vfix, _lib.stream(dev),
+        )
     return scratch[-1:]
 
 
@@ -109,13 +110,14 @@ def step(
         q = q.contiguous()
     if k is not None:
         k, v = k.contiguous(), v.contiguous()
-    _lib.call(
-        "fold_step_append", _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), int(x.dtype == torch.float16),
-        B, heads, HKV, D, page_table.data_ptr(), page_table.shape[1], int(page_size),
-        lens.data_ptr(), lens_out.data_ptr(), _lib.ptr(qa), _lib.ptr(qb), _lib.ptr(eq),
-        ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb), ek.data_ptr(), float(v_scale),
-        vsum.data_ptr(), vmean.data_ptr(), _lib.stream(x.device),
-    )
+    with _lib.on(x.device):
+        _lib.call(
+            "fold_step_append", _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), int(x.dtype == torch.float16),
+            B, heads, HKV, D, page_table.data_ptr(), page_table.shape[1], int(page_size),
+            lens.data_ptr(), lens_out.data_ptr(), _lib.ptr(qa), _lib.ptr(qb), _lib.ptr(eq),
+            ka.data_ptr(), kb.data_ptr(), va.data_ptr(), _lib.ptr(vb), ek.data_ptr(), float(v_scale),
+            vsum.data_ptr(), vmean.data_ptr(), _lib.stream(x.device),
+        )
 
 
 def tail_append(v, tail, ka, ek, page_table, page_size, lens, back):
@@ -126,9 +128,10 @@ def tail_append(v, tail, ka, ek, page_table, page_size, lens, back):
         raise ValueError(f"v must be bf16 or fp16 (it is {v.dtype})")
     B, HKV, D = v.shape
     v = v.contiguous()
-    _lib.call(
-        "fold_tail_append", v.data_ptr(), int(v.dtype == torch.float16), B, HKV, D, page_table.data_ptr(),
-        page_table.shape[1], int(page_size), lens.data_ptr(), int(back), ka.data_ptr(), ek.data_ptr(),
-        _lib.ptr(tail.u), _lib.ptr(tail.vr), tail.vsum.data_ptr(), _lib.ptr(tail.ysum), tail.rows.data_ptr(),
-        tail.rank, _lib.stream(v.device),
-    )
+    with _lib.on(v.device):
+        _lib.call(
+            "fold_tail_append", v.data_ptr(), int(v.dtype == torch.float16), B, HKV, D, page_table.data_ptr(),
+            page_table.shape[1], int(page_size), lens.data_ptr(), int(back), ka.data_ptr(), ek.data_ptr(),
+            _lib.ptr(tail.u), _lib.ptr(tail.vr), tail.vsum.data_ptr(), _lib.ptr(tail.ysum), tail.rows.data_ptr(),
+            tail.rank, _lib.stream(v.device),
+        )

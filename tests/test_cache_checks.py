@@ -73,3 +73,32 @@ def test_a_windowed_cache_refuses_the_splits_it_would_not_keep():
         with pytest.raises(NotImplementedError, match="windowed"):
             call()
     assert state(c)[0] == [0, 0]
+
+
+@pytest.mark.parametrize("kw", [dict(window=8), dict(pages=7)])
+def test_a_caches_writes_run_on_its_own_device(kw, monkeypatch):
+    """Whatever the current one is: each launch happens inside `_lib.on` of the cache's device (faked, as is the launch)."""
+    import contextlib
+
+    from fold_attention_b200 import _lib
+
+    inside, seen = [], []
+
+    @contextlib.contextmanager
+    def on(device):
+        inside.append(device)
+        yield
+        inside.pop()
+
+    monkeypatch.setattr(_lib, "on", on)
+    monkeypatch.setattr(_lib, "call", lambda name, *a: seen.append((name, list(inside))))
+    monkeypatch.setattr(_lib, "stream", lambda device: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    c, k = cache(**kw), torch.zeros(2, 2, 64, dtype=BF)
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32)
+    c.write_prompt(k, k, cu, [1, 1])
+    c._v_scale = 1.0               # (nothing ran: there is no scale to read)
+    c.append(k, k)
+    c.append_chunk(k, k, cu, [1, 1])
+    assert {"fold_cache_write_prompt", "fold_step_append", "fold_write_tokens", "fold_chunk_sums_placed"} <= {n for n, _ in seen}
+    assert all(where == [torch.device("cpu")] for _, where in seen), seen
