@@ -44,6 +44,10 @@ namespace csm100 {
 constexpr int BN = 128;
 constexpr long long WAIT_CYCLES = 1ll << 31;
 constexpr float LAZY = 8.0f;
+// An 8-bit V's weights are fp16, whose least step is 2^-24: they and their sum carry 2^LIFT, which O / l cancels. At most
+// 2^(LAZY + LIFT) of 65504, and a row's weights lose 2^-32 each of its largest at most instead of 2^-25, which a million keys
+// far under one would have added up to 3 % of the row.
+constexpr float LIFT = 7.0f;
 constexpr int SLOTS = 4;         // a CTA's pieces: of the item it starts in, of the one it ends in, two for the items between
 constexpr int MIN_TILES = 4;     // tiles a CTA takes at least: its fixed costs are two or three tiles' time
 // What a (request, head) costs a CTA beside its tiles, in tiles: its first tile's way through the pipeline and
@@ -787,6 +791,7 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
                         }
                     }
                 }
+                const float m_ref = V8 ? m_use - LIFT : m_use;
                 float sum = 0.f, sum2 = 0.f;
 #pragma unroll 1
                 for (int c = 0; c < nch; ++c) {
@@ -797,7 +802,7 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
                     }
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        const float p0 = ex2f(fmaf(x[e], eq, -m_use)), p1 = ex2f(fmaf(x[e + 1], eq, -m_use));
+                        const float p0 = ex2f(fmaf(x[e], eq, -m_ref)), p1 = ex2f(fmaf(x[e + 1], eq, -m_ref));
                         sum += p0;
                         sum2 += p1;
                         pk[e >> 1] = V8 ? pack_f16x2(p0, p1) : pack_bf16x2(p0, p1);

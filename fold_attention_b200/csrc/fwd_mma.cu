@@ -36,6 +36,9 @@ __global__ void __launch_bounds__(KIND == KIND_CHUNK ? 256 : 128) fwd_mma_kernel
     constexpr int PITCH = D * 2 + 16, TILE = 64 * PITCH, NTO = D / 8;
     constexpr bool EXT = KIND != KIND_PLAIN;
     constexpr int GROUPS = KIND == KIND_CHUNK ? 2 : 1;
+    // a chunk's fp16 weights (1 at most, of rows that may see millions of keys) and their sums carry 2^14, which
+    // O / l cancels: fp16's least step is then 2^-38 of a row's largest weight
+    constexpr float LIFT = KIND == KIND_CHUNK && F16 ? 14.f : 0.f;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* sQ = smem;
     const int grp = GROUPS == 2 ? threadIdx.x >> 7 : 0;
@@ -146,7 +149,7 @@ __global__ void __launch_bounds__(KIND == KIND_CHUNK ? 256 : 128) fwd_mma_kernel
             const float ms = mnew[r] == -INFINITY ? 0.f : mnew[r];
             corr[r] = ex2_approx(mx[r] - ms);
             mx[r] = mnew[r];
-            mnew[r] = ms;
+            mnew[r] = LIFT > 0.f ? ms - LIFT : ms;
         }
         float rsum[2] = {0.f, 0.f};
 #pragma unroll
@@ -240,7 +243,7 @@ __global__ void __launch_bounds__(KIND == KIND_CHUNK ? 256 : 128) fwd_mma_kernel
         }
         if (tq == 0 && (!EXT || p.lse))
             p.lse[b * p.lse_sb + h * p.lse_sh + start + qi] =
-                ls[r] > 0.f ? (mx[r] + log2f(ls[r])) * 0.6931471805599453f : -INFINITY;
+                ls[r] > 0.f ? ((LIFT > 0.f ? mx[r] - LIFT : mx[r]) + log2f(ls[r])) * 0.6931471805599453f : -INFINITY;
     }
 }
 

@@ -710,6 +710,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_window_sm100_kernel(const Par
         const uint64_t c2x2 = pack2(c2, c2);
         const uint32_t ts = tmem + lane_addr + T_S + 128 * x;
         const uint32_t to = tmem + lane_addr + T_O + 128 * x;
+        // A chunk's fp16 weights, of rows that may see millions of keys, and their sums carry 2^7, which O / l cancels: up to
+        // 2^(LAZY + 7) of 65504, and a weight loses 2^-32 of its row's largest at most instead of 2^-25
+        const float lift = F16 && p.plan ? 7.0f : 0.0f;
         int it = 0;                                // the query tile's key tiles so far
         for (int i = blockIdx.x; i < list.items; i += gridDim.x) {
             Item w;
@@ -759,7 +762,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_window_sm100_kernel(const Par
                 const float m_use = m_new == -INFINITY ? 0.f : m_new;     // a row that sees no key yet
                 const float alpha = m_run == -INFINITY ? 1.f : ex2f(m_run - m_use);   // (its O is zero: nothing to rescale)
                 uint64_t sum2 = 0ull;
-                const uint64_t nm2 = pack2(-m_use, -m_use);
+                const uint64_t nm2 = pack2(lift - m_use, lift - m_use);
                 auto weights = [&](auto masked) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
@@ -848,7 +851,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_window_sm100_kernel(const Par
                 for (int u = 0; u < 16; ++u) *reinterpret_cast<uint4*>(orow + 8 * u) = make_uint4(0u, 0u, 0u, 0u);
             }
             if (row_ok && p.lse) {
-                const float lse = l_run > 0.f ? (m_run + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
+                const float lse = l_run > 0.f ? (m_run - lift + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
                 p.lse[static_cast<int64_t>(w.b) * p.lse_sb + static_cast<int64_t>(w.h) * p.lse_sh + w.start + qr] = lse;
             }
         }

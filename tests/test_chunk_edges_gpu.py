@@ -128,3 +128,39 @@ def test_counts_that_q_has_no_rows_for_touch_no_row(D, counts, lens):
 
         with pytest.raises(FoldLibraryError):
             st.c.attend_chunk(room[:sum(lens)], cumulative(counts), lens)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("v8", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows", [1, 200])
+@pytest.mark.parametrize("gap", [16.0, 17.6])
+def test_many_weights_far_below_one(gap, rows, D, v8, dtype):
+    """N keys of logit 0 under one of `gap`: the one's value is 0, the others' 1, so the output is their share w / (1 + w)
+    with w = N e^-gap, 0.6 % at 17.6. Each of their weights may lose 2^-32 of the largest to fp16's least step, so N 2^-32 in
+    all, beside the roundings of a weight and of the output, half a step each, and fp32's of a sum of N terms in
+    128s: 2^-24 (128 + N / 128) of it at most."""
+    import math
+
+    import fold_attention_b200 as fa
+    from fold_attention_b200 import decode
+
+    N = 1 << 18
+    c = fa.FoldKVCache(1, 1, 1, D, N, v8=v8, v_scale=0.25 if v8 else None, page_size=256)
+    k = torch.zeros(N, 1, D, device="cuda", dtype=dtype)
+    v = torch.ones_like(k)
+    v[0], k[0, 0, 0] = 0, 16.0
+    c.append_chunk(k, v, cumulative([N]), [N])
+    q = torch.zeros(rows, 1, D, device="cuda", dtype=dtype)
+    q[:, 0, 0] = gap * math.sqrt(D) / 16.0
+    one = torch.zeros(1, device="cuda", dtype=torch.int32)
+    key, _ = decode.read_tokens(one, 256, 1, c.ka, c.kb, c.va, c.vb, c.ek, v_scale=c.v_scale, dtype=torch.float32)
+    x = (q[0, 0].double() @ key[0, 0].double()).item() / math.sqrt(D)
+    # logits of fp32 and codes of 16 bits: 2^-15 of x either way; the wide path rounds the key to 16 bits too
+    half = torch.finfo(dtype).eps / 2
+    slack = x * (2.0 ** -15 + (half if rows > 128 else 0))
+    seen = torch.arange(N - rows, N, device="cuda", dtype=torch.float64)
+    share = seen * math.exp(-x) / (1 + seen * math.exp(-x))
+    got = c.attend_chunk(q, cumulative([rows]), [rows])[:, 0].double()
+    tol = share * (2 * half + 2.0 ** -24 * (128 + N / 128) + math.expm1(slack)) + N * 2.0 ** -32
+    assert ((got - share[:, None]).abs() <= tol[:, None]).all(), ((got - share[:, None]).abs().max(1).values / tol).max()
