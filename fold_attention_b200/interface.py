@@ -192,7 +192,7 @@ def fold_attn_varlen_func(
     if max_seqlen_k is not None and int(max_seqlen_k) != int(max_seqlen_q):
         raise ValueError("self-attention needs max_seqlen_k == max_seqlen_q")
     scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else float(softmax_scale)
-    return _FoldAttnVarlenFunc.apply(q, k, v, cu, int(max_seqlen_q), scale, bool(causal), window, sinks)
+    return _FoldAttnVarlenFunc.apply(q, k, v, cu.contiguous(), int(max_seqlen_q), scale, bool(causal), window, sinks)
 
 
 def fold_attn_with_kvcache(q, cache, k=None, v=None, cu_seqlens=None, lens=None):

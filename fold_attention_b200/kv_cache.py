@@ -509,8 +509,9 @@ class FoldKVCache:
         return torch.tensor(out, dtype=torch.int32).to(self.seq_lens.device, non_blocking=True)
 
     def _chunk_lens(self, cu_seqlens, lens):
-        if cu_seqlens.dtype != torch.int32 or cu_seqlens.shape != (self.batch + 1,) or cu_seqlens.device != self.seq_lens.device:
-            raise ValueError(f"cu_seqlens is int32 ({self.batch + 1},) on {self.seq_lens.device}")
+        if (cu_seqlens.dtype != torch.int32 or cu_seqlens.shape != (self.batch + 1,) or cu_seqlens.device != self.seq_lens.device
+                or not cu_seqlens.is_contiguous()):
+            raise ValueError(f"cu_seqlens is a contiguous int32 ({self.batch + 1},) on {self.seq_lens.device}")
         if lens is None:
             lens = torch.diff(cu_seqlens).tolist()
         lens = list(map(int, lens))

@@ -102,3 +102,13 @@ def test_a_caches_writes_run_on_its_own_device(kw, monkeypatch):
     c.append_chunk(k, k, cu, [1, 1])
     assert {"fold_cache_write_prompt", "fold_step_append", "fold_write_tokens", "fold_chunk_sums_placed"} <= {n for n, _ in seen}
     assert all(where == [torch.device("cpu")] for _, where in seen), seen
+
+
+def test_strided_cumulative_lengths_are_refused():
+    """Every other entry of a longer list: the kernels would read the ones between."""
+    c, k, q = cache(), torch.zeros(2, 2, 64, dtype=BF), torch.zeros(2, 4, 64, dtype=BF)
+    cu = torch.tensor([0, 7, 1, 7, 2, 7], dtype=torch.int32)[::2]
+    c.lens = [1, 1]
+    for call in (lambda: c.append_chunk(k, k, cu, [1, 1]), lambda: c.attend_chunk(q, cu, [1, 1]), lambda: c.extend(q, k, k, cu, [1, 1])):
+        with pytest.raises(ValueError, match="contiguous"):
+            call()

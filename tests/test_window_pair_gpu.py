@@ -42,3 +42,19 @@ def test_a_remainder_that_does_not_fit_is_refused():
     for bad in (rest[:, :2], rest.contiguous(), rest.half(), rest.cpu()):
         with pytest.raises(ValueError, match="laid out as o"):
             prepare_backward(*args, lse, causal=True, window=3, o_rest=bad)
+
+
+@pytest.mark.parametrize("window", [None, 30])
+def test_strided_cumulative_lengths_are_the_sequences_they_say(window):
+    import fold_attention_b200 as fa
+
+    q, k, v, do = inputs(300, 4, 2, 64, torch.bfloat16, seed=5)
+    cu = torch.tensor([0, 9, 120, 9, 300, 9], device="cuda", dtype=torch.int32)[::2]
+
+    def run(cu):
+        x = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+        out = fa.fold_attn_varlen_func(*x, cu, max_seqlen_q=180, causal=True, window=window)
+        return (out.detach(), *torch.autograd.grad(out, x, do))
+
+    want = run(torch.tensor([0, 120, 300], device="cuda", dtype=torch.int32))
+    assert all(torch.equal(a, b) for a, b in zip(run(cu), want))
