@@ -43,6 +43,7 @@ namespace csm100 {
 
 constexpr int BN = 128;
 constexpr long long WAIT_CYCLES = 1ll << 31;
+constexpr long long DRAIN_CYCLES = 1ll << 22;    // two milliseconds: a copy takes microseconds
 constexpr float LAZY = 8.0f;
 // An 8-bit V's weights are fp16, whose least step is 2^-24: they and their sum carry 2^LIFT, which O / l cancels. At most
 // 2^(LAZY + LIFT) of 65504, and a row's weights lose 2^-32 each of its largest at most instead of 2^-25, which a million keys
@@ -558,7 +559,7 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
             for (int t = w.t0; t < w.t1; ++t, ++j) {
                 const int s = j % (is_k ? L::NK : L::NV), round = j / (is_k ? L::NK : L::NV);
                 const int pos = w.pos(p, t) + lane * p.piece;
-                const bool mine = lane < np && wanted(w.g, pos, p.piece);
+                const bool mine = lane < np && wanted(w.g, pos, p.piece) && !*abort_flag;   // (nothing new once a wait ran out)
                 const int64_t row = mine ? pool_row(w, pos) : 0;
                 const int count = __popc(__ballot_sync(0xffffffffu, mine));
                 const uint32_t full = bar((is_k ? B_KFULL : B_VFULL) + s);
@@ -644,12 +645,12 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
             {
                 const int R = w.g.n * p.G, copies = copies_of(R), rows = 128 / copies;
                 const int64_t row0 = static_cast<int64_t>(w.g.tok0) * p.hkv * p.G + static_cast<int64_t>(w.h) * R;
-                if (lane == 0) {
-                    if (w.segment > 0) mbar_wait(bar(B_QEMPTY), (w.segment - 1) & 1, abort_flag, p.status);
-                    mbar_expect_tx(bar(B_QFULL), static_cast<uint32_t>(2 * copies * R * D));
-                }
+                if (lane == 0 && w.segment > 0) mbar_wait(bar(B_QEMPTY), (w.segment - 1) & 1, abort_flag, p.status);
                 __syncwarp();
-                if (lane < 2 * copies)
+                const bool go = !__any_sync(0xffffffffu, *abort_flag != 0);
+                if (lane == 0 && go) mbar_expect_tx(bar(B_QFULL), static_cast<uint32_t>(2 * copies * R * D));
+                __syncwarp();
+                if (lane < 2 * copies && go)
                     bulk_load(base + L::SM_Q + (lane & 1) * L::PLANE + (lane >> 1) * rows * D, ((lane & 1) ? p.qb : p.qa) + row0 * D,
                               static_cast<uint32_t>(R * D), bar(B_QFULL));
             }
@@ -940,6 +941,11 @@ __global__ void __launch_bounds__(Lay<D, V8>::NTHREADS, 1) chunk_sm100_kernel(co
     }
     tc_fence_before();
     __syncthreads();
+    if (*abort_flag) {        // a wait ran out: what was under way lands before this memory is another CTA's
+        const long long t0 = clock64();
+        while (clock64() - t0 < DRAIN_CYCLES) {}
+        __syncthreads();
+    }
     while (w.next(p)) {}      // (the issuing warp's other lanes have not walked)
     if (w.segment >= 0) {     // w is the share's last segment
         int joins = s_walk[3];

@@ -36,6 +36,7 @@ constexpr int BM = 128, BN = 128;   // a query tile, a key tile
 constexpr int CTA_M = 2 * BM;       // a CTA owns two query tiles
 constexpr int NTHREADS = 384;
 constexpr long long WAIT_CYCLES = 1ll << 31;
+constexpr long long DRAIN_CYCLES = 1ll << 22;   // two milliseconds: a copy takes microseconds
 constexpr float LAZY = 8.0f;        // log2 of how far a row's maximum may pass its softmax reference before the reference moves
 
 // shared memory map (1024-aligned base)
@@ -595,6 +596,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_window_sm100_kernel(const Par
             for (int i = blockIdx.x; i < list.items; i += gridDim.x) {
                 Item w;
                 if (!load_item(p, list, i, w) || w.nt[0] + w.nt[1] == 0) continue;
+                if (*abort_flag) break;
                 const int hkv = w.h / p.G, bb = p.cu ? 0 : w.b;
                 if (items > 0) mbar_wait(bar(B_QEMPTY), (items - 1) & 1, abort_flag, p.status);
                 mbar_expect_tx(bar(B_Q), w.nt[0] > 0 && w.nt[1] > 0 ? 65536 : 32768);
@@ -606,6 +608,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_window_sm100_kernel(const Par
                 for (int j = 0; j < w.n; ++j, ++jk) {
                     const int s = jk & 1;
                     if (jk >= 2) mbar_wait(bar(B_KVEMPTY + s), ((jk >> 1) - 1) & 1, abort_flag, p.status);
+                    if (*abort_flag) break;    // nothing new once a wait ran out
                     const uint32_t st = base + SM_KV + s * STAGE;
                     // A packed sequence's last tile holds rows behind its end: their scores are masked, but a NaN in V there
                     // would pass through P's zeros, so V's are made zeros before the tile is handed on.
@@ -858,6 +861,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) fwd_window_sm100_kernel(const Par
     }
     tc_fence_before();
     __syncthreads();
+    if (*abort_flag) {        // a wait ran out: what was under way lands before this memory is another CTA's
+        const long long t0 = clock64();
+        while (clock64() - t0 < DRAIN_CYCLES) {}
+        __syncthreads();
+    }
     if (warp == 1) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
