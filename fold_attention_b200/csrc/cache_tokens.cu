@@ -175,24 +175,20 @@ __device__ __forceinline__ float to_f16_range(float x) {
     return x;
 }
 
+// A row's channels as 16-bit values, 16 to a lane.
 template <int OUT>
 __device__ __forceinline__ void store16(void* base, int64_t at, const float (&x)[16]) {
-    if constexpr (OUT == OUT_F32) {
-        float4* d = reinterpret_cast<float4*>(static_cast<float*>(base) + at);
+    static_assert(OUT != OUT_F32, "fp32 rows are store_f32's");
+    uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-    } else {
-        uint32_t w[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (OUT == OUT_BF16) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
-            // the pool holds bf16's range: fp16 takes what it can, and a NaN stays one
-            else w[i] = pack_f16x2(to_f16_range(x[2 * i]), to_f16_range(x[2 * i + 1]));
-        }
-        uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + at);
-        d[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        d[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (OUT == OUT_BF16) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+        // the pool holds bf16's range: fp16 takes what it can, and a NaN stays one
+        else w[i] = pack_f16x2(to_f16_range(x[2 * i]), to_f16_range(x[2 * i + 1]));
     }
+    uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + at);
+    d[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    d[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
 // A row's fp32 channels, 16 to a lane, stored by whole cache lines: within groups of four lanes the 4 x 4 matrix
@@ -237,9 +233,7 @@ __global__ void __launch_bounds__(NT) read_tokens_kernel(const int* __restrict__
     const int64_t prow = slot_row(ok ? slot : 0, page_size, hkv, static_cast<int>(rr % hkv), off);
     float xk[16], xv[16];
     load_row<D, V8>(p, prow, off, lane, ok, xk, xv);
-    if (OUT == OUT_F32) {
-        // 64 bytes a lane: a row's lanes take turns so that each store is a stretch of memory, not 16 bytes of
-        // every 64 (TPR lanes: unit t of lane l goes out as unit l + TPR t of the row)
+    if constexpr (OUT == OUT_F32) {      // 64 bytes a lane, by whole lines (with every lane of the warp, for its shuffles)
         store_f32<TPR>(static_cast<float*>(k) + r * D, lane, r < n_rows, xk);
         store_f32<TPR>(static_cast<float*>(v) + r * D, lane, r < n_rows, xv);
     } else if (r < n_rows) {

@@ -25,8 +25,9 @@
 //
 // Measured: 64 requests of up to 32768 keys, 8 KV heads, D=128, an 8-bit V, one token each under a window of 1024 with 4
 // sinks: 80-84 us of 41 that its bytes take at the copy's rate (3.3 TB/s): a CTA has some twenty tiles in three or four
-// (request, head)s, and what each of those costs beside its tiles is a quarter of its time; the conversion of V,
-// which the tensor core cannot take as stored, is most of the rest. 32 requests of up to 32768 keys, 3-8 tokens each, a
+// (request, head)s, and what each of those costs beside its tiles is a quarter of its time; the conversion of V's
+// two planes to fp16 is most of the rest. (The decode kernel feeds them to kind::f8f6f4 as stored, its weights as four E5M2
+// terms; P in such terms has not been tried here.) 32 requests of up to 32768 keys, 3-8 tokens each, a
 // bf16 V: 290-300 us of 276 (6.2 TB/s); 370 in a loop of seconds, where the power cap holds the SMs at 1.4 GHz.
 //
 // Warps: 0 K producer (both planes, scales), 3 V producer, 1 MMA issuer, 2 Q and V's dead rows (bf16 V),
