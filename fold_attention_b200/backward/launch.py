@@ -340,7 +340,7 @@ def _packed_strides(ts, varlen):
 # many visible keys the forward leaves what its rounding took as 16 bits more, and the backward adds it. That is a
 # tenth of the time of a large call (16384 tokens of 32 heads, window 128: 606 us without, 664 with; D=64 792 and 875), so
 # windows of many keys, whose rows seldom sit on a few of them, go without. The rule knows the window alone: a sequence's bits do
-# not depend on what it is packed with, and a window that hides nothing is plain causal attention's. Sequences of a few
+# not depend on what it is packed with, and a larger window that hides nothing is plain causal attention. Sequences of a few
 # tokens under a larger window go without too, as they do without a window: 0.0036-0.0039 of dq's and dk's norm in bf16.
 REST_KEYS = 256
 

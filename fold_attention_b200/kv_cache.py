@@ -486,8 +486,8 @@ class FoldKVCache:
         on every replay; the host's copy, which the next eager call plans by, does
         not follow by itself. Raises if the replays ran past `max_len` or the
         shared pool: the tokens beyond either were dropped, and what the replays returned
-        for their requests from there on is not their attention. The others are
-        as they should be; the cache goes on from new prompts."""
+        for their requests from there on is not their attention. No other request's keys
+        are touched; the cache goes on from new prompts."""
         lens = self.seq_lens.tolist()
         if max(lens) > self.max_len:
             raise ValueError(f"a request was moved to {max(lens)} tokens, max_len={self.max_len}")
