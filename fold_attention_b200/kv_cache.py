@@ -451,9 +451,11 @@ class FoldKVCache:
         keys are cut is a matter of the whole batch, and so is, for a request of up to
         128 query rows a KV head, whether it is attended from the codes or with
         the wider ones, whose keys are rounded to q's type first (`decode/tokens.py`,
-        `MIXED_TILES`). The difference is within the rounding of 16 bits. fp16 queries of more than 128 rows a KV head see K and V saturated to
-        fp16's range. A row whose query holds a NaN or an infinity gives NaN, and so does one
-        that sees a NaN in a bf16 V; a key's codes, and an 8-bit V's, hold none."""
+        `MIXED_TILES`). The difference is within the rounding of 16 bits.
+
+        fp16 queries attended that second way see K and V saturated to fp16's range. A
+        row whose query holds a NaN or an infinity gives NaN, and so does one that
+        sees a NaN in a bf16 V; a key's codes, and an 8-bit V's, hold none."""
         lens = self._chunk_lens(cu_seqlens, lens)
         self._check_chunk_q(q, lens)
         if any(map(operator.gt, lens, self.lens)):
